@@ -37,7 +37,12 @@ extern "C" {
 
 typedef void* skv_stream_t; /* a hipStream_t */
 
-enum skv_dtype { SKV_F32 = 0, SKV_BF16 = 1 };
+enum skv_dtype {
+  SKV_F32 = 0,
+  SKV_BF16 = 1,
+  SKV_MXFP4 = 2, /* block-scaled E2M1 cache storage, skv_q_* only */
+  SKV_MXFP8 = 3  /* block-scaled E4M3 cache storage, skv_q_* only */
+};
 
 enum skv_status {
   SKV_OK = 0,
@@ -263,6 +268,93 @@ int skv_append_prefill_attn(void* out, const void* q, void* k_cache, void* v_cac
                             const int32_t* n_new, int B, int C, int H_q, int H_kv, int D,
                             int T_cap, float scale, int n_splits, void* ws, size_t ws_bytes,
                             int cache_dt, int in_dt, int q_dt, int out_dt, skv_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Block-scaled caches (fmt SKV_MXFP4 or SKV_MXFP8; no counterpart in the
+ * reference, whose caches are fp32).
+ *
+ * 32 consecutive elements of a head's row share a scale 2^e, one byte e + 127,
+ * and are E2M1 numbers (0, .5, 1, 1.5, 2, 3, 4, 6 with a sign; two to a byte,
+ * the even element in the low half) or E4M3 numbers (a byte each, largest
+ * 448). e is the smallest integer with max|x| <= T 2^e, T = 7 (E2M1) or 464
+ * (E4M3), clamped to [-100, 125] or [-100, 119]; elements are x 2^-e rounded to
+ * nearest even, saturating. A group that holds a NaN or an infinity is stored
+ * as scale byte 255 and zero codes and reads back as NaN. The stored bytes do
+ * not depend on the entry point or the input's type, and every value a cache
+ * can hold is exact in bf16.
+ *
+ * Layout: codes [B, H_kv, T_cap, D * bits / 8], scales [B, H_kv, T_cap,
+ * D / 32] (head-major, unlike the plain caches: a head's rows lie end to end).
+ * With block_table (int32 [B, max_blocks]) the cache is a pool of pages
+ * [pages, H_kv, block_size, ...], block_size a power of two, and token t of
+ * sequence b is row t % block_size of page block_table[b, t / block_size];
+ * T_cap is not used. block_table NULL: contiguous. D: multiples of 32 up to
+ * 256. The codes, inputs and outputs are 16-byte aligned.
+ * ------------------------------------------------------------------------ */
+
+/* skv_append for a block-scaled cache: row k_new[b] (and v_new[b]), [B, H_kv,
+ * D] of in_dt, quantised into position lens[b], then lens[b]++; a full
+ * sequence is left as it is. */
+int skv_q_append(void* k, void* k_scale, void* v, void* v_scale, const void* k_new,
+                 const void* v_new, int32_t* lens, const int32_t* block_table, int max_blocks,
+                 int block_size, int B, int H_kv, int D, int T_cap, int fmt, int in_dt,
+                 skv_stream_t stream);
+
+/* skv_append_chunk for a block-scaled cache: rows i < n_new[b] (NULL: C) of
+ * k_new[b], [B, C, H_kv, D] of in_dt, to positions lens[b] + i; rows past the
+ * capacity are not written, lens is not advanced. Paged caches too. */
+int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale, const void* k_new,
+                       const void* v_new, const int32_t* lens, const int32_t* n_new,
+                       const int32_t* block_table, int max_blocks, int block_size, int B, int C,
+                       int H_kv, int D, int T_cap, int fmt, int in_dt, skv_stream_t stream);
+
+/* Rows back: k_out[b, i], v_out[b, i] ([B, C, H_kv, D] of out_dt, exact in
+ * either type) = position start[b] + i (start NULL: start_const + i), or zeros
+ * outside [0, lens[b]). */
+int skv_q_read(void* k_out, void* v_out, const void* k, const void* k_scale, const void* v,
+               const void* v_scale, const int32_t* lens, const int32_t* start, int start_const,
+               const int32_t* block_table, int max_blocks, int block_size, int B, int C, int H_kv,
+               int D, int T_cap, int fmt, int out_dt, skv_stream_t stream);
+
+/* Split sizing of skv_q_decode_attn (host-only): chunk_tokens (a multiple of
+ * 128) of one kv head per workgroup and n_chunks = ceil(max_len / chunk_tokens).
+ * total_len: filled tokens over the batch (<= 0: B * max_len). chunk_hint > 0
+ * forces the chunk size (rounded up). */
+int skv_q_decode_plan(int B, int H_kv, int max_len, long long total_len, int chunk_hint,
+                      int* chunk_tokens /* host */, int* n_chunks /* host */);
+
+/* Bytes of workspace skv_q_decode_attn needs for n_chunks > 1: fp32 partials
+ * (o[D], m, l) per (sequence, query head, chunk). No contents are expected. */
+size_t skv_q_decode_workspace_bytes(int B, int H_q, int D, int n_chunks);
+
+/* skv_decode_attn over a block-scaled cache: q, out [B, H_q, D] of q_dt /
+ * out_dt, G = H_q / H_kv from 1 to 16. lens[b] == 0 gives zeros. Products are
+ * of fp32 accuracy where q or out is fp32; with both bf16, K, V and q are
+ * exact and the probabilities carry 17 bits. A sequence longer than
+ * chunk_tokens * n_chunks gets NaN outputs.
+ * new_k, new_v ([B, H_kv, D] of in_dt; both or neither): exactly skv_q_append
+ * before the attention, which then covers the new token, with lens advanced
+ * after it; the plan covers the lengths after the append. */
+int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scale, void* v, void* v_scale,
+                      const void* new_k, const void* new_v, int32_t* lens,
+                      const int32_t* block_table, int max_blocks, int block_size, int B, int H_q,
+                      int H_kv, int D, int T_cap, float scale, int chunk_tokens, int n_chunks,
+                      void* ws, size_t ws_bytes, int fmt, int in_dt, int q_dt, int out_dt,
+                      skv_stream_t stream);
+
+/* skv_append_prefill_attn for a block-scaled cache (contiguous or paged):
+ * skv_q_append_chunk, causal attention of the chunk's queries over prefix +
+ * chunk, and the fills advanced, in one call. q, out [B, C, H_q, D] of q_dt /
+ * out_dt; H_q / H_kv in {1, 2, 4, 8}; n_splits and ws as in skv_prefill_attn
+ * (skv_prefill_plan, skv_prefill_workspace_bytes). Q and the probabilities
+ * enter the matrix cores as bf16, K and V exactly, as over a bf16 cache that
+ * holds the same values. */
+int skv_q_append_prefill_attn(void* out, const void* q, void* k, void* k_scale, void* v,
+                              void* v_scale, const void* k_new, const void* v_new, int32_t* lens,
+                              const int32_t* n_new, const int32_t* block_table, int max_blocks,
+                              int block_size, int B, int C, int H_q, int H_kv, int D, int T_cap,
+                              float scale, int n_splits, void* ws, size_t ws_bytes, int fmt,
+                              int in_dt, int q_dt, int out_dt, skv_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Decode-step ops of the model around the cache (fp32). They replace the

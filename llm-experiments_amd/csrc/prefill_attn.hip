@@ -48,22 +48,24 @@
 //    more than the 12 us merge pass.)
 //  * Rows i >= n_new[b] of the output are written as zeros by the workgroup
 //    that owns them (one split) or by the merge pass.
+//  * A block-scaled cache (quant.h, QF = 4 or 8 bits) runs the same kernel: its
+//    tiles go through registers, a thread converting one 32-element group (one
+//    scale) of K or V to bf16 on its way into the same LDS layout, so the
+//    products see what a bf16 cache of the same values would give them. A NaN
+//    group of V goes into LDS as zeros and its tile is marked: a masked
+//    probability of 0 would make it NaN for queries that do not attend the
+//    token; those that do get their NaN from the scales afterwards.
 #include <type_traits>
 
+#include "quant.h"
 #include "skv_common.h"
 
+// This file is three translation units: the plain caches' kernels and the C
+// entry points, and with SKV_PREFILL_QF = 4 or 8 the kernels of that
+// block-scaled format.
+
 namespace skv {
-namespace {
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-constexpr int kWaves = 8;                   // most wavefronts of a workgroup
-constexpr int kQB = 1;                      // 32-row query blocks per wavefront
-constexpr int kCUs = 256;                   // CUs of an MI355X
-constexpr int kBN = 64;                     // tokens per K/V tile
-constexpr int kXCD = 8;                     // XCDs of an MI355X
+namespace prefill {
 
 struct PrefillArgs {
   const void* q;
@@ -87,7 +89,30 @@ struct PrefillArgs {
   // them from there, advances the fills in adv (no separate advance launch)
   int32_t* snap;
   int32_t* adv;
+  quant::Cache c;  // a block-scaled cache (k and v are not used then)
 };
+
+// The kernel of a block-scaled cache at the padded head dim DK with W
+// wavefronts a workgroup; 0, or SKV_E_UNSUPPORTED without one.
+int launch_q4(const PrefillArgs& a, int DK, int G, int W, unsigned blocks, hipStream_t s);
+int launch_q8(const PrefillArgs& a, int DK, int G, int W, unsigned blocks, hipStream_t s);
+
+}  // namespace prefill
+
+namespace {
+
+using prefill::PrefillArgs;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kWaves = 8;                   // most wavefronts of a workgroup
+constexpr int kQB = 1;                      // 32-row query blocks per wavefront
+constexpr int kCUs = 256;                   // CUs of an MI355X
+constexpr int kBN = 64;                     // tokens per K/V tile
+constexpr int kXCD = 8;                     // XCDs of an MI355X
+
 
 // K and V tiles live in LDS row-major, [kBN tokens][D] bf16, two stages
 // each. The 16-byte chunks of a row are XOR-swizzled, physical chunk =
@@ -159,28 +184,31 @@ __device__ __forceinline__ void store4(void* out, size_t i, int dt, const float 
 // through registers, 16-byte loads (a.D % 8 == 0) or element loads.
 // W: wavefronts per workgroup (4 at D = 256, where a wavefront holds twice
 // the queries and accumulators, ~310 registers: one per SIMD).
-template <int D, int G, int LV, int W>
+// QF: 4 or 8 for a block-scaled cache of that many bits (PAGED: in pages), else 0.
+template <int D, int G, int LV, int W, int QF = 0, bool PAGED = false>
 __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(PrefillArgs a) {
   constexpr int KB = D / 16;  // k-blocks of the QK^T product
   constexpr int DB = D / 32;  // 32-row d blocks of O^T
   constexpr int BM = W * kQB * 32;  // query rows of the workgroup
   constexpr bool GEN = LV != 0;
+  constexpr bool REG = GEN || QF != 0;  // tiles go through registers
   const int RS = GEN ? a.D : D;  // row stride of q, out and the cache rows
   // LDS stages: register-staged tiles (GEN) share one struct; DMA-staged
   // tiles get one variable per stage, so the compiler sees that a stage's
   // reads cannot alias the DMA landing in the other one and does not make
   // them wait for it.
-  __shared__ Smem<GEN ? D : 16> sm;
-  __shared__ __attribute__((aligned(16))) uint16_t lds0[GEN ? 8 : 2 * kBN * D];
-  __shared__ __attribute__((aligned(16))) uint16_t lds1[GEN ? 8 : 2 * kBN * D];
+  __shared__ Smem<REG ? D : 16> sm;
+  __shared__ __attribute__((aligned(16))) uint16_t lds0[REG ? 8 : 2 * kBN * D];
+  __shared__ __attribute__((aligned(16))) uint16_t lds1[REG ? 8 : 2 * kBN * D];
+  __shared__ int s_nan[2];  // QF: the last tile staged with a NaN group of V, by LDS stage
   auto sk = [&](auto stage) -> uint16_t* {
     constexpr int s_ = decltype(stage)::value;
-    if constexpr (GEN) return sm.k[s_];
+    if constexpr (REG) return sm.k[s_];
     else return s_ == 0 ? lds0 : lds1;
   };
   auto sv = [&](auto stage) -> uint16_t* {
     constexpr int s_ = decltype(stage)::value;
-    if constexpr (GEN) return sm.v[s_];
+    if constexpr (REG) return sm.v[s_];
     else return (s_ == 0 ? lds0 : lds1) + kBN * D;
   };
 
@@ -230,7 +258,12 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       float v[8];
-      if constexpr (GEN) {  // element loads at clamped offsets, zeros past the head dim
+      if constexpr (GEN && QF != 0) {  // whole octets: the head dim is a multiple of 32
+        const int e = kb * 16 + g * 8;
+        load8_f32(a.q, qsafe + (e < RS ? e : 0), a.q_dt, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = e < RS ? v[j] : 0.f;
+      } else if constexpr (GEN) {  // element loads at clamped offsets, zeros past the head dim
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int e = kb * 16 + g * 8 + j;
@@ -271,14 +304,83 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
   // stop counting them in order: 552.2 -> 531.9 us per C4 chunk, same bits.)
   constexpr int RPK = 1024 / (D * 2);          // token rows per 1 KB
   constexpr int KPT = kBN * D * 2 / 1024;      // 1 KB pieces per tile and tensor
-  static_assert(GEN || KPT % W == 0, "tile pieces must split over the wavefronts");
+  static_assert(REG || KPT % W == 0, "tile pieces must split over the wavefronts");
   // Register-staged tiles (GEN): 16-byte chunk c of a tile is token row
   // c / (D/8), logical chunk c % (D/8), at the same swizzled LDS position as
   // the DMA form; chunks past the head dim are zeros.
   constexpr int NCH = kBN * D / 8;                             // chunks per tile and tensor
   constexpr int CPT = (NCH + W * 64 - 1) / (W * 64);  // chunks per thread
   uint4 rk[GEN ? CPT : 1], rv[GEN ? CPT : 1];
+  // Block-scaled tiles: unit u of a thread is EU elements (at most a group) of
+  // one row of K (the first half of the units) or V.
+  constexpr int QB = QF == 8 ? 8 : 4;
+  constexpr int EU = 2 * D / W < 32 ? 2 * D / W : 32;
+  constexpr int UPT = 2 * D / W / EU;
+  constexpr int UPR = D / EU;             // units per row
+  constexpr int QW = EU * QB / 32;        // words per unit
+  uint32_t qw[UPT][QW], qs[UPT];
+  int qblk[UPT];  // PAGED: the page of the unit's row in the next tile to load
+  const int cb = a.c.D * QB / 8, sb = a.c.D / quant::kGroup;
+  auto unit_row = [&](int u) { return ((tid + u * W * 64) % (kBN * UPR)) / UPR; };
+  auto unit_el = [&](int u) { return (tid + u * W * 64) % UPR * EU; };
+  auto unit_isv = [&](int u) { return tid + u * W * 64 >= kBN * UPR; };
+  auto q_pages = [&](int T0) {
+    if constexpr (PAGED)
+#pragma unroll
+      for (int u = 0; u < UPT; ++u) {
+        const int t = min(T0 + unit_row(u), kv_end - 1);
+        qblk[u] = a.c.bt[(size_t)b * a.c.max_blocks + (t >> a.c.bs_shift)];
+      }
+  };
+  auto q_tile_load = [&](int T0) {
+#pragma unroll
+    for (int u = 0; u < UPT; ++u) {
+      const int t = min(T0 + unit_row(u), kv_end - 1);
+      const int e = unit_el(u) < a.c.D ? unit_el(u) : 0;  // past the head dim: group 0, unused
+      const bool isv = unit_isv(u);
+      size_t row;
+      if constexpr (PAGED)
+        row = (((size_t)qblk[u] * a.Hkv + hk) << a.c.bs_shift) + (t & ((1 << a.c.bs_shift) - 1));
+      else
+        row = ((size_t)b * a.Hkv + hk) * a.T_cap + t;
+      const uint8_t* p = (isv ? a.c.v : a.c.k) + row * cb + e * QB / 8;
+      if constexpr (QW >= 4) {
+#pragma unroll
+        for (int i = 0; i < QW / 4; ++i) {
+          const uint4 x = reinterpret_cast<const uint4*>(p)[i];
+          qw[u][4 * i] = x.x; qw[u][4 * i + 1] = x.y;
+          qw[u][4 * i + 2] = x.z; qw[u][4 * i + 3] = x.w;
+        }
+      } else if constexpr (QW == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        qw[u][0] = x.x; qw[u][1] = x.y;
+      } else {
+        qw[u][0] = *reinterpret_cast<const uint32_t*>(p);
+      }
+      qs[u] = (isv ? a.c.vs : a.c.ks)[row * sb + e / quant::kGroup];
+    }
+    q_pages(T0 + kBN);
+  };
+  // ... into LDS stage ST as tile it
+  auto q_tile_store = [&](int ST, int it) {
+#pragma unroll
+    for (int u = 0; u < UPT; ++u) {
+      const bool isv = unit_isv(u);
+      const bool zero = isv && qs[u] == 255u;
+      if (zero) s_nan[ST] = it;
+      const float sc_ = quant::scale_f32(qs[u]);
+      uint16_t* dst = isv ? sm.v[ST] : sm.k[ST];
+#pragma unroll
+      for (int i = 0; i < EU / 8; ++i) {
+        const quant::bf16x8 x = quant::decode8_bf16<QB>(&qw[u][i * (QB / 4)], sc_);
+        uint4 y = __builtin_bit_cast(uint4, x);
+        if (zero) y = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + swz<D>(unit_row(u), unit_el(u) / 8 + i)) = y;
+      }
+    }
+  };
   auto reg_tile_load = [&](int T0) {
+    if constexpr (QF != 0) return q_tile_load(T0);
 #pragma unroll
     for (int u = 0; u < CPT; ++u) {
       const int c = min(tid + u * W * 64, NCH - 1);  // threads past NCH repeat the last chunk
@@ -307,7 +409,8 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
       }
     }
   };
-  auto reg_tile_store = [&](int ST) {
+  auto reg_tile_store = [&](int ST, int it) {
+    if constexpr (QF != 0) return q_tile_store(ST, it);
 #pragma unroll
     for (int u = 0; u < CPT; ++u) {
       const int c = tid + u * W * 64;
@@ -319,8 +422,8 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
   };
   // Per lane, the byte offset of its 16-byte chunk within a tile (the same
   // for every tile): token row piece * RPK + lane / (D / 8), swizzled chunk.
-  uint32_t dma_off[GEN ? 1 : KPT / W];
-  if constexpr (!GEN) {
+  uint32_t dma_off[REG ? 1 : KPT / W];
+  if constexpr (!REG) {
 #pragma unroll
     for (int c = 0; c < KPT / W; ++c) {
       const int piece = wave * (KPT / W) + c;
@@ -330,7 +433,7 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
     }
   }
 #define SKV_DMA_TILE(T0, ST)                                                                 \
-  if constexpr (!GEN) {                                                                      \
+  if constexpr (!REG) {                                                                      \
     /* a buffer over the tile's rows that exist: rows past kv_end read zeros */             \
     const int rows_ = max(0, min(kv_end - (T0), kBN));                                       \
     const int nrec_ = rows_ > 0 ? (int)(((rows_ - 1) * row_stride + D) * 2) : 0;           \
@@ -347,10 +450,15 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
   }
 
   const int n_tiles = s1 > s0 ? (s1 - s0 + kBN - 1) / kBN : 0;
-  if constexpr (GEN) {
+  if constexpr (QF != 0) {
+    if (tid < 2) s_nan[tid] = -1;
+    __syncthreads();
+  }
+  if constexpr (REG) {
     if (n_tiles > 0) {
+      if constexpr (QF != 0) q_pages(s0);
       reg_tile_load(s0);
-      reg_tile_store(0);
+      reg_tile_store(0, 0);
     }
   } else {
     if (n_tiles > 0) SKV_DMA_TILE(s0, 0);
@@ -370,8 +478,8 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
     // now and their LDS stores after this tile's products
     // (At D = 256 the registers of a staged tile are not free during the
     // products: its loads wait until after them, see the end of the tile.)
-    if constexpr (GEN && D <= 128) reg_tile_load(t0 + kBN);
-    else if constexpr (!GEN) SKV_DMA_TILE(t0 + kBN, st ^ 1);
+    if constexpr (REG && D <= 128) reg_tile_load(t0 + kBN);
+    else if constexpr (!REG) SKV_DMA_TILE(t0 + kBN, st ^ 1);
 
     // S^T for the whole 64-token tile first (two independent accumulator
     // chains per query block), then one online-softmax update, then PV.
@@ -478,8 +586,24 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
           }
     }
 
-    if constexpr (GEN && D > 128) reg_tile_load(t0 + kBN);
-    if constexpr (GEN) reg_tile_store(st ^ 1);
+    if constexpr (QF != 0) {
+      // NaN groups of V (zeros in LDS) reach the queries that attend their
+      // token; group db of a row is d block db of O^T
+      if (s_nan[st] == it) {  // uniform over the workgroup
+#pragma unroll
+        for (int qb = 0; qb < kQB; ++qb) {
+          const int t_end = min(min(t0 + kBN, s1), P + qrow[qb] / G + 1);
+          for (int t = t0; t < t_end; ++t) {
+            const uint8_t* vs = a.c.vs + quant::row_of<PAGED>(a.c, b, hk, t) * sb;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+              if (db < sb && vs[db] == 255) o[qb][db] = f32x16{} + __builtin_nanf("");
+          }
+        }
+      }
+    }
+    if constexpr (REG && D > 128) reg_tile_load(t0 + kBN);
+    if constexpr (REG) reg_tile_store(st ^ 1, it + 1);
     // the next tile's DMA has landed in LDS before anyone reads it
     wait_all_memory();
     __syncthreads();
@@ -511,7 +635,9 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = valid ? v(db, r4, e) : 0.f;
-        if constexpr (GEN) {
+        if constexpr (GEN && QF != 0) {
+          if (d0 < RS) store4(a.out, orow * RS + d0, a.out_dt, x);
+        } else if constexpr (GEN) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (d0 + e < RS) store_elem(a.out, orow * RS + d0 + e, a.out_dt, x[e]);
@@ -553,6 +679,47 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
     }
   }
 }
+
+#ifdef SKV_PREFILL_QF
+
+}  // namespace
+
+// (LV = 8: rows of a runtime stride; a head dim is a multiple of 32 here)
+template <int QF>
+static int launch_q(const PrefillArgs& a, int DK, int G, int W, unsigned blocks, hipStream_t s) {
+#define SKV_PQ(DD, GG, WW)                                                                    \
+  if (DK == DD && G == GG && W == WW) {                                                       \
+    if (a.c.bt)                                                                               \
+      hipLaunchKernelGGL((k_prefill_mfma<DD, GG, 8, WW, QF, true>), dim3(blocks),             \
+                         dim3(WW * 64), 0, s, a);                                             \
+    else                                                                                      \
+      hipLaunchKernelGGL((k_prefill_mfma<DD, GG, 8, WW, QF, false>), dim3(blocks),            \
+                         dim3(WW * 64), 0, s, a);                                             \
+    return 0;                                                                                 \
+  }
+#define SKV_PQG(DD, WW) SKV_PQ(DD, 1, WW) SKV_PQ(DD, 2, WW) SKV_PQ(DD, 4, WW) SKV_PQ(DD, 8, WW)
+  SKV_PQG(32, 4) SKV_PQG(32, 8) SKV_PQG(64, 4) SKV_PQG(64, 8)
+  SKV_PQG(128, 4) SKV_PQG(128, 8) SKV_PQG(256, 4)
+#undef SKV_PQG
+#undef SKV_PQ
+  return SKV_E_UNSUPPORTED;
+}
+
+#if SKV_PREFILL_QF == 4
+int prefill::launch_q4(const PrefillArgs& a, int DK, int G, int W, unsigned blocks,
+                       hipStream_t s) {
+  return launch_q<4>(a, DK, G, W, blocks, s);
+}
+#else
+int prefill::launch_q8(const PrefillArgs& a, int DK, int G, int W, unsigned blocks,
+                       hipStream_t s) {
+  return launch_q<8>(a, DK, G, W, blocks, s);
+}
+#endif
+
+}  // namespace skv
+
+#else
 
 constexpr int kMergeBatch = 4;  // splits whose partials the merge loads in one round trip
 
@@ -726,19 +893,22 @@ namespace {
 // skv_prefill_attn's checks and launches. adv (split bf16 path only): the
 // merge pass advances these fills (skv_advance's rule) from the snapshot at
 // the end of ws. launch = false: the checks alone, nothing launched.
+// qc: a block-scaled cache (cache_dt is its format, k_cache and v_cache its
+// codes, T_cap its capacity; quant_cache_args has checked it), else NULL.
 int prefill_attn_impl(void* out, const void* q, const void* k_cache, const void* v_cache,
                       const int32_t* start, const int32_t* n_new, int B, int C, int H_q,
                       int H_kv, int D, int T_cap, float scale, int n_splits, void* ws,
                       size_t ws_bytes, int cache_dt, int q_dt, int out_dt, skv_stream_t stream,
-                      const char* fn, int32_t* adv, bool launch) {
+                      const char* fn, int32_t* adv, bool launch,
+                      const quant::Cache* qc = nullptr) {
   SKV_REQUIRE(out && q && k_cache && v_cache && start, SKV_E_INVALID, "%s: null pointer argument",
               fn);
   SKV_REQUIRE(B > 0 && C > 0 && H_q > 0 && H_kv > 0 && T_cap > 0, SKV_E_INVALID,
               "%s: dims must be > 0", fn);
   SKV_REQUIRE(H_q % H_kv == 0, SKV_E_INVALID, "%s: H_q=%d not a multiple of H_kv=%d", fn, H_q,
               H_kv);
-  SKV_REQUIRE(dt_ok(cache_dt) && dt_ok(q_dt) && dt_ok(out_dt), SKV_E_INVALID, "%s: bad dtype",
-              fn);
+  SKV_REQUIRE((qc ? is_quant(cache_dt) : dt_ok(cache_dt)) && dt_ok(q_dt) && dt_ok(out_dt),
+              SKV_E_INVALID, "%s: bad dtype", fn);
   SKV_REQUIRE(scale > 0.f, SKV_E_INVALID, "%s: scale must be > 0", fn);
   if (cache_dt == SKV_F32) {  // fp32 cache: the fp32 MFMA path, no split
     SKV_REQUIRE(q_dt == SKV_F32 && out_dt == SKV_F32, SKV_E_UNSUPPORTED,
@@ -806,6 +976,12 @@ int prefill_attn_impl(void* out, const void* q, const void* k_cache, const void*
   if (!launch) return SKV_OK;
   hipStream_t s = (hipStream_t)stream;
   const int LV = load_form(D);
+  if (qc) {
+    a.c = *qc;
+    const int rc = cache_dt == SKV_MXFP4 ? prefill::launch_q4(a, DK, G, W, (unsigned)blocks, s)
+                                         : prefill::launch_q8(a, DK, G, W, (unsigned)blocks, s);
+    if (rc) return set_error(rc, "%s: no kernel for head_dim %d, G=%d", fn, D, G);
+  } else {
 #define SKV_PF(DD, GG, LL, WW)                                                                \
   if (DK == DD && G == GG && LV == LL && W == WW)                                             \
     hipLaunchKernelGGL((k_prefill_mfma<DD, GG, LL, WW>), dim3((unsigned)blocks),              \
@@ -819,6 +995,7 @@ int prefill_attn_impl(void* out, const void* q, const void* k_cache, const void*
   SKV_PFG(256, 0, 4) SKV_PFG(256, 8, 4) SKV_PFG(256, 1, 4)
 #undef SKV_PFG
 #undef SKV_PF
+  }
   int rc = check_launch(fn);
   if (rc) return rc;
   if (n_splits > 1) {
@@ -868,3 +1045,32 @@ extern "C" int skv_append_prefill_attn(void* out, const void* q, void* k_cache, 
   if (cache_dt == SKV_BF16 && n_splits > 1) return SKV_OK;
   return skv_advance(lens, n_new, C, B, T_cap, stream);
 }
+
+extern "C" int skv_q_append_prefill_attn(void* out, const void* q, void* k, void* k_scale, void* v,
+                                         void* v_scale, const void* k_new, const void* v_new,
+                                         int32_t* lens, const int32_t* n_new,
+                                         const int32_t* block_table, int max_blocks,
+                                         int block_size, int B, int C, int H_q, int H_kv, int D,
+                                         int T_cap, float scale, int n_splits, void* ws,
+                                         size_t ws_bytes, int fmt, int in_dt, int q_dt, int out_dt,
+                                         skv_stream_t stream) {
+  const char* fn = "skv_q_append_prefill_attn";
+  quant::Cache c;
+  int rc = quant_cache_args(&c, k, k_scale, v, v_scale, block_table, max_blocks, block_size, B,
+                            H_kv, D, T_cap, fmt, fn);
+  if (rc) return rc;
+  // every check of the attention first, so that a rejected call changes nothing
+  rc = prefill_attn_impl(out, q, k, v, lens, n_new, B, C, H_q, H_kv, D, c.cap, scale, n_splits, ws,
+                         ws_bytes, fmt, q_dt, out_dt, stream, fn, lens, false, &c);
+  if (rc) return rc;
+  rc = skv_q_append_chunk(k, k_scale, v, v_scale, k_new, v_new, lens, n_new, block_table,
+                          max_blocks, block_size, B, C, H_kv, D, T_cap, fmt, in_dt, stream);
+  if (rc) return rc;
+  rc = prefill_attn_impl(out, q, k, v, lens, n_new, B, C, H_q, H_kv, D, c.cap, scale, n_splits, ws,
+                         ws_bytes, fmt, q_dt, out_dt, stream, fn, lens, true, &c);
+  if (rc) return rc;
+  if (n_splits > 1) return SKV_OK;  // the merge pass has advanced the fills
+  return skv_advance(lens, n_new, C, B, c.cap, stream);
+}
+
+#endif  // SKV_PREFILL_QF

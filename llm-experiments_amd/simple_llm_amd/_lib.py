@@ -20,7 +20,7 @@ PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(PKG_ROOT, "libskv.so")
 HEADER_PATH = os.path.join(os.path.dirname(PKG_ROOT), "include", "skv.h")
 
-F32, BF16 = 0, 1
+F32, BF16, MXFP4, MXFP8 = 0, 1, 2, 3
 SKV_E_INVALID, SKV_E_UNSUPPORTED, SKV_E_WORKSPACE, SKV_E_HIP = -22, -95, -28, -5
 
 _P = ctypes.c_void_p
@@ -46,6 +46,18 @@ _SIGNATURES = {
                               _I, _I, _I, _P]),
     "skv_append_prefill_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
                                      _F, _I, _P, _Z, _I, _I, _I, _I, _P]),
+    "skv_q_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "skv_q_append_chunk": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
+                                _I, _I, _P]),
+    "skv_q_read": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I,
+                        _I, _P]),
+    "skv_q_decode_plan": (_I, [_I, _I, _I, ctypes.c_longlong, _I, ctypes.POINTER(_I),
+                               ctypes.POINTER(_I)]),
+    "skv_q_decode_workspace_bytes": (_Z, [_I, _I, _I, _I]),
+    "skv_q_decode_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
+                               _F, _I, _I, _P, _Z, _I, _I, _I, _I, _P]),
+    "skv_q_append_prefill_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I,
+                                       _I, _I, _I, _I, _F, _I, _P, _Z, _I, _I, _I, _I, _P]),
     "skv_embed": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "skv_layernorm": (_I, [_P, _P, _P, _P, _I, _I, _F, _P]),
     "skv_linear": (_I, [_P, _P, _P, _P, _P, _P, _P, _F, _I, _I, _I, _I, _I, _P, _Z, _P]),
@@ -142,6 +154,10 @@ def dtype_code(dt: torch.dtype) -> int:
     if code is None:
         raise ValueError(f"unsupported dtype {dt} (float32 or bfloat16)")
     return code
+
+
+#: Storage dtypes of the block-scaled caches and their C codes.
+QUANT_FORMATS = {torch.float4_e2m1fn_x2: MXFP4, torch.float8_e4m3fn: MXFP8}
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -22,6 +22,7 @@ from .gpu_kv_cache import (
     kv_cache_append_attend,
     kv_cache_create,
     kv_cache_prefill,
+    kv_cache_read,
     kv_cache_reset,
     kv_cache_set_block_table,
     kv_cache_update,
@@ -79,6 +80,7 @@ __all__ = [
     "kv_cache_append",
     "kv_cache_append_attend",
     "kv_cache_prefill",
+    "kv_cache_read",
     "kv_cache_set_block_table",
     "decode_attention",
     "decode_plan",

@@ -15,8 +15,9 @@ Differences from the reference, all supersets of its behaviour:
     by the append kernel (see KVCache in gpu_types.py for the position rule);
   * decode attention has no length cap (the reference raises above
     attention_workgroup_size = 256, gpu_kv_cache.py:250-257);
-  * bf16 storage, grouped-query heads and a paged layout are options of
-    KVCacheConfig; the defaults reproduce the reference's fp32 MHA cache.
+  * bf16 and block-scaled 4- and 8-bit storage, grouped-query heads and a
+    paged layout are options of KVCacheConfig; the defaults reproduce the
+    reference's fp32 MHA cache. Every function here takes every storage.
 
 Extensions beyond the reference's four functions:
   kv_cache_append           append with per-sequence positions (no
@@ -24,6 +25,7 @@ Extensions beyond the reference's four functions:
   kv_cache_set_block_table  install the page table of a paged cache
   kv_cache_prefill          append a chunk of tokens (prefill), optionally
                             followed by causal attention over prefix + chunk
+  kv_cache_read             rows of a block-scaled cache back as fp32 or bf16
 """
 from __future__ import annotations
 
@@ -36,6 +38,7 @@ import numpy as np
 import torch
 
 from .. import _lib
+from . import gpu_kv_quant
 from .gpu_ops import batch_count, validate_buffer_shape_2d
 from .gpu_types import (
     GPUBuffer2D,
@@ -60,6 +63,7 @@ def kv_cache_create(ctx: GPUContext, config: KVCacheConfig) -> KVCache:
     b*max_blocks .. b*max_blocks + max_blocks - 1) when the pool is big
     enough; a smaller pool has no table until kv_cache_set_block_table
     installs one (appends and attention raise ValueError before that).
+    Block-scaled caches: KVCacheLayer has their layout.
     """
     if config.batch_size <= 0:
         raise ValueError(f"batch_size must be > 0, got {config.batch_size}")
@@ -74,8 +78,12 @@ def kv_cache_create(ctx: GPUContext, config: KVCacheConfig) -> KVCache:
     n_kv = config.n_kv_heads or config.n_heads
     if n_kv <= 0 or config.n_heads % n_kv != 0:
         raise ValueError(f"n_heads ({config.n_heads}) must be a multiple of n_kv_heads ({n_kv})")
-    if config.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"dtype must be torch.float32 or torch.bfloat16, got {config.dtype}")
+    quant = config.dtype in _lib.QUANT_FORMATS
+    if not quant and config.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("dtype must be torch.float32, torch.bfloat16, torch.float4_e2m1fn_x2 or "
+                         f"torch.float8_e4m3fn, got {config.dtype}")
+    if quant:
+        gpu_kv_quant.check_sizes(config.batch_size, config.n_heads, n_kv, config.head_dim)
 
     e_kv = n_kv * config.head_dim
     B = config.batch_size
@@ -97,13 +105,17 @@ def kv_cache_create(ctx: GPUContext, config: KVCacheConfig) -> KVCache:
     # A layer's fills, and after them (16-byte aligned, zero-filled together) the
     # workspace of its one-launch decode steps where the sizes can take those.
     step = 0
-    if (config.block_size <= 0 and _step_sizes(B, config.n_heads, n_kv, config.head_dim)
+    if (not quant and config.block_size <= 0 and _step_sizes(B, config.n_heads, n_kv, config.head_dim)
             and ctx.device.type == "cuda"):
         step = int(_lib.lib().skv_decode_direct_workspace_bytes(B, config.n_heads,
                                                                 config.head_dim, _STEP_SPLIT))
     at = -(-B // 4) * 4
     layers: List[KVCacheLayer] = []
     for _ in range(config.n_layers):
+        if quant:
+            layers.append(gpu_kv_quant.create_layer(ctx, B, rows * n_kv, config.head_dim,
+                                                    config.dtype))
+            continue
         k = torch.zeros((rows, e_kv), dtype=config.dtype, device=ctx.device)
         v = torch.zeros((rows, e_kv), dtype=config.dtype, device=ctx.device)
         state = torch.zeros(at + -(-step // 4), dtype=torch.int32, device=ctx.device)
@@ -162,6 +174,12 @@ def _check_max_len(max_len: int, fills: np.ndarray) -> None:
                          f"plan would not cover every filled position")
 
 
+def _capacity(cache: KVCache) -> int:
+    """Tokens a sequence can hold, as the kernels see it."""
+    return (cache.block_table.shape[1] * cache.block_size if cache.paged
+            else cache.max_seq_len)
+
+
 def _check_tensor(t: torch.Tensor, name: str, device: torch.device) -> None:
     # Kernels dereference these pointers on the GPU: host tensors never reach them.
     # Fast path first (get_device() is an int; t.device builds an object).
@@ -186,6 +204,10 @@ def _launch_append(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, k: torc
         _check_tensor(t, n, dev)
     if k.dtype != v.dtype:
         raise ValueError("new_k and new_v must share a dtype")
+    if cache.quantized:
+        gpu_kv_quant.append(cache, layer, k, v)
+        layer.host_lens = _fills_after_append(layer.host_lens, _capacity(cache))[0]
+        return
     L = _lib.lib()
     stream = _lib.stream_handle(dev)
     cdt, idt = _lib.dtype_code(cache.dtype), _lib.dtype_code(k.dtype)
@@ -396,6 +418,9 @@ def decode_attention(ctx: GPUContext, cache: KVCache, layer_idx: int, q: torch.T
         max_len = int(layer.host_lens.max())
     _check_max_len(max_len, layer.host_lens)
     total = int(np.minimum(layer.host_lens, max_len).sum())
+    if cache.quantized:
+        gpu_kv_quant.attend(ctx, cache, layer, q, out, scale, max_len, total)
+        return
     chunk, nchunks = _decode_plan_span(ctx, cache.batch_size, cache.n_heads, cache.n_kv_heads,
                                        max_len, total, cache.head_dim, cache.dtype)
     L = _lib.lib()
@@ -461,6 +486,10 @@ def kv_cache_append_attend(ctx: GPUContext, cache: KVCache, layer_idx: int, new_
         max_len = top
     elif max_len < top:
         _check_max_len(max_len, after)  # raises
+    if cache.quantized:
+        gpu_kv_quant.attend(ctx, cache, layer, q, out, scale, max_len, total, new_k, new_v)
+        layer.host_lens = after
+        return after.copy()
     L = _lib.lib()
     D, sc = cache.head_dim, float(scale) if scale is not None else 1.0 / math.sqrt(cache.head_dim)
     stream = _lib.stream_handle(dev)
@@ -552,15 +581,16 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
     flash_attention, gpu/gpu_kernels.py:695-701, shifted by the cached
     prefix). The layer's fills advance by n_new. Returns the new fills.
 
-    A bfloat16 cache runs the bf16 MFMA prefill; a float32 cache runs every
-    product with fp32 accuracy (float32 q and out).
+    A bfloat16 or block-scaled cache runs the bf16 MFMA prefill; a float32
+    cache runs every product with fp32 accuracy (float32 q and out). The
+    queries attend the chunk's rows as the cache stores them.
 
     Raises ValueError (before any GPU work) on a bad layer, shapes, a chunk
-    that would overflow a sequence ("Cache is full"), a paged cache, or a
-    float32 cache with non-float32 q/output.
+    that would overflow a sequence ("Cache is full"), a paged cache that is
+    not block-scaled, or a float32 cache with non-float32 q/output.
     """
     _check_layer(cache, layer_idx)
-    if cache.paged:
+    if cache.paged and not cache.quantized:
         raise ValueError("kv_cache_prefill: paged caches take single-token appends only")
     layer = cache.layers[layer_idx]
     dev = layer.lens.device
@@ -596,7 +626,16 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
                                              out.dtype != torch.float32):
             raise ValueError("kv_cache_prefill: attention over a float32 cache takes float32 "
                              "q and output")
+        if cache.quantized and Hq // Hkv not in (1, 2, 4, 8):
+            raise ValueError(f"kv_cache_prefill: no kernel for {Hq // Hkv} query heads per kv "
+                             "head (1, 2, 4 or 8)")
     batch_count(ctx)
+    if cache.quantized:
+        gpu_kv_quant.prefill(ctx, cache, layer, new_k, new_v, q, out,
+                             n_host if n_new is not None else None,
+                             int((start + n_host).max()), scale, n_splits)
+        layer.host_lens = np.minimum(start + n_host, T)
+        return layer.host_lens.copy()
     L = _lib.lib()
     stream = _lib.stream_handle(dev)
     cdt, idt = _lib.dtype_code(cache.dtype), _lib.dtype_code(new_k.dtype)
@@ -633,3 +672,43 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
         _lib.check(rc, "skv_advance")
     layer.host_lens = np.minimum(start + n_host, T)
     return layer.host_lens.copy()
+
+
+# ============================================================================
+# READING BACK (extension; block-scaled caches)
+# ============================================================================
+
+
+def kv_cache_read(ctx: GPUContext, cache: KVCache, layer_idx: int, k_out: torch.Tensor,
+                  v_out: torch.Tensor, start=None) -> None:
+    """Rows of a block-scaled cache back as values.
+
+    k_out, v_out: [batch_size, C, n_kv_heads, head_dim] device tensors (float32
+    or bfloat16; the values are exact in both). Row i of sequence b is position
+    start + i (start: one integer or batch_size of them; None: 0), zeros past
+    the fill. Raises ValueError on a bad layer, shapes, a negative start or a
+    cache that is not block-scaled (its buffers hold the values themselves).
+    """
+    _check_layer(cache, layer_idx)
+    if not cache.quantized:
+        raise ValueError("kv_cache_read: the cache is not block-scaled; its buffers hold the "
+                         "values themselves")
+    layer = cache.layers[layer_idx]
+    dev = layer.lens.device
+    B, Hkv, D = cache.batch_size, cache.n_kv_heads, cache.head_dim
+    for t, nm in ((k_out, "k_out"), (v_out, "v_out")):
+        _check_tensor(t, nm, dev)
+        if t.dim() != 4 or t.shape[0] != B or t.shape[2] != Hkv or t.shape[3] != D:
+            raise ValueError(f"{nm} must be [batch_size, C, n_kv_heads, head_dim] = "
+                             f"[{B}, C, {Hkv}, {D}], got {tuple(t.shape)}")
+    if k_out.shape != v_out.shape or k_out.dtype != v_out.dtype:
+        raise ValueError("k_out and v_out must share shape and dtype")
+    if k_out.shape[1] == 0:
+        raise ValueError("k_out must hold at least one row per sequence")
+    at = np.asarray(0 if start is None else start, dtype=np.int64)
+    if at.ndim and at.shape != (B,):
+        raise ValueError(f"start must be one integer or {B} of them, got shape {at.shape}")
+    if (at < 0).any() or (at > 2**31 - 1).any():
+        raise ValueError("start must lie in [0, 2^31)")
+    batch_count(ctx)
+    gpu_kv_quant.read(cache, layer, k_out, v_out, at)

@@ -1,0 +1,187 @@
+"""Block-scaled KV caches (torch.float4_e2m1fn_x2 and torch.float8_e4m3fn): the
+launches behind the functions of gpu_kv_cache, which have checked the
+arguments. The formats and layouts are in include/skv.h (skv_q_*).
+
+The split workspaces are allocated per call from torch's caching allocator,
+in stream order: calls on different streams, and captured calls, do not share
+one.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+import threading
+from typing import Optional
+
+import numpy as np
+import torch
+
+from .. import _lib
+from .gpu_types import GPUBuffer2D, GPUContext, KVCache, KVCacheLayer
+
+GROUP = 32  # elements that share a scale
+MAX_HEAD_DIM = 256
+MAX_GROUPS = 16  # query heads per kv head
+
+_BITS = {torch.float4_e2m1fn_x2: 4, torch.float8_e4m3fn: 8}
+
+
+def check_sizes(batch_size: int, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
+    if head_dim % GROUP or head_dim > MAX_HEAD_DIM:
+        raise ValueError(f"head_dim must be a multiple of {GROUP} up to {MAX_HEAD_DIM} in a "
+                         f"block-scaled cache, got {head_dim}")
+    if n_heads // n_kv_heads > MAX_GROUPS:
+        raise ValueError(f"a block-scaled cache takes up to {MAX_GROUPS} query heads per kv head, "
+                         f"got {n_heads // n_kv_heads}")
+    if batch_size > 65535 or n_kv_heads > 65535:
+        raise ValueError("a block-scaled cache takes up to 65535 sequences and kv heads, got "
+                         f"{batch_size} and {n_kv_heads}")
+
+
+def create_layer(ctx: GPUContext, batch_size: int, rows: int, head_dim: int,
+                 dtype: torch.dtype) -> KVCacheLayer:
+    """rows: head rows, [sequences or pages, kv heads, positions] flattened."""
+    def buf(width: int) -> GPUBuffer2D:
+        t = torch.zeros((rows, width), dtype=torch.uint8, device=ctx.device)
+        return GPUBuffer2D(buffer=t, shape=(rows, width), size=rows * width)
+
+    codes, scales = head_dim * _BITS[dtype] // 8, head_dim // GROUP
+    return KVCacheLayer(k_cache=buf(codes), v_cache=buf(codes),
+                        lens=torch.zeros(batch_size, dtype=torch.int32, device=ctx.device),
+                        host_lens=np.zeros(batch_size, dtype=np.int64),
+                        k_scale=buf(scales), v_scale=buf(scales))
+
+
+def _on(dev: torch.device):
+    """Launches go to the current device: make it the cache's."""
+    if torch.cuda.current_device() == (dev.index or 0):
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _storage(layer: KVCacheLayer) -> tuple:
+    return (layer.k_cache.buffer.data_ptr(), layer.k_scale.buffer.data_ptr(),
+            layer.v_cache.buffer.data_ptr(), layer.v_scale.buffer.data_ptr())
+
+
+def _pages(cache: KVCache) -> tuple:
+    """(block table, pages a sequence, page size)."""
+    if not cache.paged:
+        return None, 0, 0
+    return cache.block_table.data_ptr(), cache.block_table.shape[1], cache.block_size
+
+
+def append(cache: KVCache, layer: KVCacheLayer, k: torch.Tensor, v: torch.Tensor) -> None:
+    dev = layer.lens.device
+    with _on(dev):
+        rc = _lib.lib().skv_q_append(*_storage(layer), k.data_ptr(), v.data_ptr(),
+                                     layer.lens.data_ptr(), *_pages(cache), cache.batch_size,
+                                     cache.n_kv_heads, cache.head_dim, cache.max_seq_len,
+                                     _lib.QUANT_FORMATS[cache.dtype], _lib.dtype_code(k.dtype),
+                                     _lib.stream_handle(dev))
+    _lib.check(rc, "skv_q_append")
+
+
+def read(cache: KVCache, layer: KVCacheLayer, k_out: torch.Tensor, v_out: torch.Tensor,
+         start: np.ndarray) -> None:
+    dev = layer.lens.device
+    with _on(dev):
+        stream = _lib.stream_handle(dev)
+        at, first = None, int(start.flat[0])
+        if start.ndim and (start != first).any():
+            at = _lib.upload_i32(start, dev, stream)
+        rc = _lib.lib().skv_q_read(k_out.data_ptr(), v_out.data_ptr(), *_storage(layer),
+                                   layer.lens.data_ptr(), at.data_ptr() if at is not None else None,
+                                   first, *_pages(cache), cache.batch_size, k_out.shape[1],
+                                   cache.n_kv_heads, cache.head_dim, cache.max_seq_len,
+                                   _lib.QUANT_FORMATS[cache.dtype], _lib.dtype_code(k_out.dtype),
+                                   stream)
+    _lib.check(rc, "skv_q_read")
+
+
+_PLAN_OUT = threading.local()
+
+
+def plan(batch_size: int, n_kv_heads: int, max_len: int, total_len: int,
+         hint: int = 0) -> tuple[int, int]:
+    """(chunk_tokens, n_chunks) of skv_q_decode_plan."""
+    out = getattr(_PLAN_OUT, "refs", None)
+    if out is None:  # per thread: the call releases the GIL while it fills them
+        c, n = ctypes.c_int(), ctypes.c_int()
+        out = _PLAN_OUT.refs = (c, n, ctypes.byref(c), ctypes.byref(n))
+    rc = _lib.lib().skv_q_decode_plan(batch_size, n_kv_heads, max(int(max_len), 1), int(total_len),
+                                      int(hint), out[2], out[3])
+    if rc:
+        _lib.check(rc, "skv_q_decode_plan")
+    return out[0].value, out[1].value
+
+
+def attend(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, q: torch.Tensor,
+           out: torch.Tensor, scale: Optional[float], max_len: int, total: int,
+           new_k: Optional[torch.Tensor] = None, new_v: Optional[torch.Tensor] = None) -> None:
+    """decode_attention, after the append of new_k and new_v if given."""
+    dev = layer.lens.device
+    L = _lib.lib()
+    B, Hq, Hkv, D = cache.batch_size, cache.n_heads, cache.n_kv_heads, cache.head_dim
+    chunk, n = plan(B, Hkv, max_len, total, ctx.config.decode_chunk_tokens)
+    sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    nk = nv = None
+    idt = 0
+    if new_k is not None:
+        nk, nv, idt = new_k.data_ptr(), new_v.data_ptr(), _lib.dtype_code(new_k.dtype)
+    with _on(dev):
+        ws, need = None, 0
+        if n > 1:
+            need = int(L.skv_q_decode_workspace_bytes(B, Hq, D, n))
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = L.skv_q_decode_attn(out.data_ptr(), q.data_ptr(), *_storage(layer), nk, nv,
+                                 layer.lens.data_ptr(), *_pages(cache), B, Hq, Hkv, D,
+                                 cache.max_seq_len, sc, chunk, n,
+                                 ws.data_ptr() if ws is not None else None, need,
+                                 _lib.QUANT_FORMATS[cache.dtype], idt, _lib.dtype_code(q.dtype),
+                                 _lib.dtype_code(out.dtype), _lib.stream_handle(dev))
+    _lib.check(rc, "skv_q_decode_attn")
+
+
+def prefill(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, new_k: torch.Tensor,
+            new_v: torch.Tensor, q: Optional[torch.Tensor], out: Optional[torch.Tensor],
+            counts: Optional[np.ndarray], max_end: int, scale: Optional[float],
+            n_splits: int) -> None:
+    """kv_cache_prefill; counts: tokens per sequence, or None for whole chunks."""
+    dev = layer.lens.device
+    L = _lib.lib()
+    B, Hq, Hkv, D = cache.batch_size, cache.n_heads, cache.n_kv_heads, cache.head_dim
+    C = int(new_k.shape[1])
+    fmt, idt = _lib.QUANT_FORMATS[cache.dtype], _lib.dtype_code(new_k.dtype)
+    table, max_blocks, page = _pages(cache)
+    cap = max_blocks * page if table is not None else cache.max_seq_len
+    with _on(dev):
+        stream = _lib.stream_handle(dev)
+        n_dev = None
+        if counts is not None and int(counts.min()) < C:
+            n_dev = _lib.upload_i32(counts, dev, stream)
+        n_ptr = n_dev.data_ptr() if n_dev is not None else None
+        if q is None:
+            rc = L.skv_q_append_chunk(*_storage(layer), new_k.data_ptr(), new_v.data_ptr(),
+                                      layer.lens.data_ptr(), n_ptr, table, max_blocks, page, B, C,
+                                      Hkv, D, cache.max_seq_len, fmt, idt, stream)
+            _lib.check(rc, "skv_q_append_chunk")
+            rc = L.skv_advance(layer.lens.data_ptr(), n_ptr, C, B, cap, stream)
+            _lib.check(rc, "skv_advance")
+            return
+        ns = ctypes.c_int(int(n_splits))
+        if n_splits <= 0:
+            _lib.check(L.skv_prefill_plan(B, C, Hq, Hkv, max(max_end, 1), ctypes.byref(ns)),
+                       "skv_prefill_plan")
+        need = int(L.skv_prefill_workspace_bytes(B, C, Hq, D, ns.value))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+        rc = L.skv_q_append_prefill_attn(out.data_ptr(), q.data_ptr(), *_storage(layer),
+                                         new_k.data_ptr(), new_v.data_ptr(),
+                                         layer.lens.data_ptr(), n_ptr, table, max_blocks, page, B,
+                                         C, Hq, Hkv, D, cache.max_seq_len, sc, ns.value,
+                                         ws.data_ptr() if ws is not None else None, need, fmt, idt,
+                                         _lib.dtype_code(q.dtype), _lib.dtype_code(out.dtype),
+                                         stream)
+        _lib.check(rc, "skv_q_append_prefill_attn")

@@ -100,17 +100,27 @@ class KVCacheLayer:
 
     step_ws: workspace of the layer's one-launch decode steps (zero between
     calls), or None where the cache's sizes do not take them.
+
+    Block-scaled caches (see KVCacheConfig.dtype) are uint8 and head-major:
+    k_cache, v_cache hold the codes, [batch_size * n_kv_heads * max_seq_len,
+    head_dim * bits / 8] or, paged, [n_blocks * n_kv_heads * block_size, ...];
+    k_scale, v_scale the scale bytes, the same rows by head_dim / 32 (None in
+    other caches).
     """
 
     def __init__(self, k_cache: GPUBuffer2D, v_cache: GPUBuffer2D,
                  lens: Optional[torch.Tensor] = None,
                  host_lens: Optional[np.ndarray] = None,
-                 step_ws: Optional[torch.Tensor] = None):
+                 step_ws: Optional[torch.Tensor] = None,
+                 k_scale: Optional[GPUBuffer2D] = None,
+                 v_scale: Optional[GPUBuffer2D] = None):
         self.k_cache = k_cache
         self.v_cache = v_cache
         self.lens = lens
         self.host_lens = host_lens
         self.step_ws = step_ws
+        self.k_scale = k_scale
+        self.v_scale = v_scale
 
     def __repr__(self) -> str:
         return f"KVCacheLayer(k_cache={self.k_cache.shape}, v_cache={self.v_cache.shape})"
@@ -121,8 +131,8 @@ class KVCache:
 
     Fields of the reference: layers, batch_size, max_seq_len, current_len,
     n_heads, head_dim. Extensions (defaults reproduce the reference):
-    n_kv_heads (grouped-query attention), dtype (float32 or bfloat16
-    storage), block_size / n_blocks / block_table (paged layout).
+    n_kv_heads (grouped-query attention), dtype (float32, bfloat16 or
+    block-scaled storage, see KVCacheConfig), block_size / n_blocks / block_table (paged layout).
 
     current_len is the number of filled positions. Each layer tracks its own
     fill, so updating layers 0..L-1 once per token writes every layer at the
@@ -157,6 +167,11 @@ class KVCache:
         return self.block_size > 0
 
     @property
+    def quantized(self) -> bool:
+        """Whether the storage is block-scaled 4- or 8-bit."""
+        return self.layers[0].k_scale is not None
+
+    @property
     def current_len(self) -> int:
         return int(max(int(layer.host_lens.max()) for layer in self.layers))
 
@@ -184,7 +199,12 @@ class KVCacheConfig:
 
     The first five fields are the reference's. Extensions:
       n_kv_heads  kv heads for grouped-query attention (None: n_heads)
-      dtype       storage dtype, torch.float32 or torch.bfloat16
+      dtype       storage dtype: torch.float32, torch.bfloat16, or one of the
+                  block-scaled formats (32 elements of a head share a
+                  power-of-two scale, include/skv.h has the rule):
+                  torch.float4_e2m1fn_x2, 4.25 bits an element, or
+                  torch.float8_e4m3fn, 8.25. Those take head dims that are
+                  multiples of 32 up to 256 and up to 16 query heads per kv head
       block_size  > 0 selects the paged layout with pages of this many tokens
                   (a power of two); max_seq_len is then the per-sequence limit
       n_blocks    pages in the pool (0: batch_size * ceil(max_seq_len/block_size))

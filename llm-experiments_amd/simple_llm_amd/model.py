@@ -186,6 +186,9 @@ class TransformerModel:
                  params: Optional[dict] = None, kv_dtype: torch.dtype = torch.float32):
         self.ctx = ctx
         self.tm_params = tm_params
+        if kv_dtype in _lib.QUANT_FORMATS:
+            raise ValueError(f"kv_dtype {kv_dtype}: the model's steps take a float32 or bfloat16 "
+                             "cache")
         self.kv_dtype = kv_dtype
         d = tm_params.embedding_dim
         if d % tm_params.n_heads:

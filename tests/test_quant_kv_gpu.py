@@ -1,0 +1,591 @@
+"""Block-scaled caches on the GPU: the stored values against the oracle's bit
+for bit, attention against float64 over the stored values.
+
+Error bounds, by arithmetic (u = 2^-24, half an fp32 step). A score is a sum of
+D products, each rounding at most u of the running magnitude A = scale * sum
+|q k|, then scaled and shifted (three roundings): off by at most (D + 8) u A.
+Its exponential is off by that much (natural units) plus one step of the
+exponential unit, weights and their sum by twice it, and the sums over n tokens
+by u for each sequential addition (at most n / 16 + 64 with four lanes, four
+wavefronts and chunks in parallel). All of it multiplies sum p |v|. With bf16
+in and out the probabilities carry 17 bits (2^-17) in decode and 8 (2^-8) in
+prefill, fp32 queries of a prefill are rounded to bf16 (2^-8 A on a score), and
+a bf16 output rounds by 2^-8 of itself.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import banner
+from oracle import quant_oracle as qo
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp4": torch.float4_e2m1fn_x2, "fp8": torch.float8_e4m3fn}
+F32, BF16 = torch.float32, torch.bfloat16
+U = 2.0 ** -24
+
+
+def _np(t):
+    return t.detach().float().cpu().numpy().astype(np.float64)
+
+
+def _rows(rng, *shape):
+    """Key-like rows: channels of unlike size, some groups all zero."""
+    x = rng.standard_normal(shape) * np.exp(rng.standard_normal(shape[-1])) * 0.7
+    x[..., :qo.GROUP] *= rng.random(shape[:-1] + (1,)) > 0.1
+    return x.astype(np.float32)
+
+
+def _dev(x, dtype):
+    return torch.from_numpy(np.ascontiguousarray(x)).to("cuda:0").to(dtype)
+
+
+class Model:
+    """What the cache should hold: float64 values [B, T, Hkv, D] and fills."""
+
+    def __init__(self, B, T, H, D, fmt):
+        self.k = np.zeros((B, T, H, D))
+        self.v = np.zeros((B, T, H, D))
+        self.lens = np.zeros(B, np.int64)
+        self.fmt, self.cap = fmt, T
+
+    def append(self, k, v, n=None):
+        """k, v [B, C, H, D]; n: rows of each sequence."""
+        n = np.full(len(self.lens), k.shape[1]) if n is None else n
+        k, v = qo.round_trip(k, self.fmt), qo.round_trip(v, self.fmt)
+        for b, m in enumerate(n):
+            at = self.lens[b]
+            m = int(min(m, self.cap - at))
+            self.k[b, at:at + m] = k[b, :m]
+            self.v[b, at:at + m] = v[b, :m]
+            self.lens[b] = at + m
+
+
+def _make(ctx, B, T, Hkv, G, D, fmt, page=0, seed=0):
+    from simple_llm_amd.gpu import gpu
+
+    cache = gpu.kv_cache_create(ctx, gpu.KVCacheConfig(B, T, 1, Hkv * G, D, n_kv_heads=Hkv,
+                                                       dtype=DT[fmt], block_size=page))
+    cap = T
+    if page:
+        per = -(-T // page)
+        perm = np.random.default_rng(seed + 77).permutation(B * per).astype(np.int32)
+        gpu.kv_cache_set_block_table(cache, torch.from_numpy(perm.reshape(B, per)))
+        cap = per * page
+    return gpu, cache, Model(B, cap, Hkv, D, fmt)
+
+
+def _fill(gpu, ctx, cache, m, rng, counts, dtype=F32):
+    """counts[b] tokens of each sequence, as one ragged chunk."""
+    counts = np.asarray(counts)
+    C = int(counts.max())
+    if C == 0:
+        return
+    B, _, H, D = m.k.shape
+    k, v = (_dev(_rows(rng, B, C, H, D), dtype) for _ in range(2))
+    gpu.kv_cache_prefill(ctx, cache, 0, k, v, n_new=counts)
+    m.append(_np(k), _np(v), counts)
+
+
+def _check_stored(gpu, ctx, cache, m, start=0, C=None, dtype=F32):
+    B, T, H, D = m.k.shape
+    C = T - start if C is None else C
+    ko = torch.full((B, C, H, D), 7.0, dtype=dtype, device="cuda:0")
+    vo = torch.full_like(ko, 7.0)
+    gpu.kv_cache_read(ctx, cache, 0, ko, vo, start=start)
+    for got, want in ((ko, m.k), (vo, m.v)):
+        w = np.zeros((B, C, H, D))
+        for b, n in enumerate(m.lens):
+            hi = min(int(n), start + C)
+            if hi > start:
+                w[b, :hi - start] = want[b, start:hi]
+        np.testing.assert_array_equal(_np(got), w)
+    assert cache.layers[0].lens.cpu().tolist() == m.lens.tolist()
+    assert cache.seq_lens().tolist() == m.lens.tolist()
+
+
+def _check_attention(got, q, m, G, scale, exact32, out_bf16, rows=None, prefill=False, q_f32=False):
+    """got, q [B, rows, Hq, D]; the last row of sequence b sees its whole fill."""
+    got, q = _np(got), _np(q)
+    B, R, Hq, D = q.shape
+    n_rows = np.full(B, R) if rows is None else rows
+    for b in range(B):
+        n, r = int(m.lens[b]), int(n_rows[b])
+        assert not got[b, r:].any(), f"rows past the count of sequence {b} are not zeros"
+        last = n - r + np.arange(r)
+        for h in range(Hq):
+            want, mag, big = qo.attention(q[b, :r, h], m.k[b, :n, h // G], m.v[b, :n, h // G],
+                                          scale, last)
+            tol = 2 * (D + 8) * U * big + (n / 16 + 64) * U
+            if prefill:
+                tol = tol + 2.0 ** -8 + (2 * 2.0 ** -8 * big if q_f32 else 0.0)
+            elif not exact32:
+                tol = tol + 2.0 ** -17
+            bound = tol[:, None] * mag + (2.0 ** -8 * (np.abs(want) + tol[:, None] * mag)
+                                          if out_bf16 else 0.0) + 1e-37
+            err = np.abs(got[b, :r, h] - want)
+            assert not np.isnan(got[b, :r, h]).any()
+            assert (err <= bound).all(), (
+                f"sequence {b} head {h}: off by {(err / bound).max():.2f} of the bound")
+
+
+# ---- writing and reading ---------------------------------------------------
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+@pytest.mark.parametrize("B,H,D,C,page,dtype", [
+    (1, 1, 32, 1, 0, F32), (3, 5, 64, 7, 0, BF16), (2, 3, 96, 45, 4, F32), (4, 2, 128, 33, 16, BF16),
+    (2, 1, 160, 17, 1, F32), (1, 7, 224, 5, 0, BF16), (2, 2, 256, 40, 32, F32)])
+def test_chunk_append_and_read(gpu_ctx, fmt, B, H, D, C, page, dtype):
+    banner(f"quant chunk append {fmt} B={B} H={H} D={D} C={C} page={page} {dtype}")
+    rng = np.random.default_rng(D * 7 + C)
+    gpu, cache, m = _make(gpu_ctx, B, 2 * C + 3, H, 1, D, fmt, page)
+    counts = rng.integers(0, C + 1, B)
+    counts[0] = C
+    _fill(gpu, gpu_ctx, cache, m, rng, counts, dtype)
+    _fill(gpu, gpu_ctx, cache, m, rng, rng.integers(0, C + 1, B), dtype)
+    _check_stored(gpu, gpu_ctx, cache, m)
+    _check_stored(gpu, gpu_ctx, cache, m, start=C // 2, C=C, dtype=BF16)
+    at = rng.integers(0, C, B)  # a start of its own for each sequence
+    ko = torch.empty((B, 3, H, D), device="cuda:0")
+    vo = torch.empty_like(ko)
+    gpu.kv_cache_read(gpu_ctx, cache, 0, ko, vo, start=at)
+    for b in range(B):
+        n = max(0, min(3, int(m.lens[b] - at[b])))
+        np.testing.assert_array_equal(_np(ko)[b, :n], m.k[b, at[b]:at[b] + n])
+        assert not _np(ko)[b, n:].any() and not _np(vo)[b, n:].any()
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+@pytest.mark.parametrize("B,H,D,page", [(1, 1, 32, 0), (5, 3, 64, 8), (3, 16, 128, 0), (2, 9, 256, 2)])
+def test_token_append_until_full(gpu_ctx, fmt, B, H, D, page):
+    banner(f"quant token append {fmt} B={B} H={H} D={D} page={page}")
+    rng = np.random.default_rng(D + B)
+    gpu, cache, m = _make(gpu_ctx, B, 6, H, 1, D, fmt, page)
+    _fill(gpu, gpu_ctx, cache, m, rng, rng.integers(0, 5, B))
+    for i in range(9):  # past the capacity: full sequences stay as they are
+        k, v = (_dev(_rows(rng, B, H, D), BF16 if i % 2 else F32) for _ in range(2))
+        gpu.kv_cache_append(gpu_ctx, cache, 0, k, v)
+        m.append(_np(k)[:, None], _np(v)[:, None])
+    _check_stored(gpu, gpu_ctx, cache, m)
+    assert (m.lens == m.cap).all()
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+def test_stored_bytes_at_the_edges(gpu_ctx, fmt):
+    """Group maxima at, just below and just above every border of the scale rule,
+    ties, both clamps, subnormals, zeros of both signs: codes and scale bytes."""
+    banner(f"quant edges {fmt}")
+    top = 7.0 if fmt == "fp4" else 464.0
+    rng = np.random.default_rng(5)
+    peaks = []
+    for e in (-149, -140, -127, -126, -110, -103, -102, -101, -100, -50, -1, 0, 1, 60, 118, 119,
+              120, 124, 125, 126):
+        for base in (1.0, 1.5, 1.75, 1.8125, 1.99999988):
+            with np.errstate(over="ignore"):
+                p = np.float32(np.ldexp(base, e))
+            if np.isfinite(p):
+                peaks += [p, np.nextafter(p, np.float32(0)), np.nextafter(p, np.float32(np.inf))]
+    peaks += [np.float32(0), np.finfo(np.float32).max, np.float32(top), np.float32(top / 2)]
+    peaks = np.array([p for p in peaks if np.isfinite(p)], np.float32)
+    n = -(-len(peaks) // 8) * 8
+    x = rng.uniform(-1, 1, (n, 32)).astype(np.float32)
+    x[:len(peaks)] *= peaks[:, None]
+    x[np.arange(len(peaks)), rng.integers(0, 32, len(peaks))] = peaks
+    # exact midpoints of the grid under scale 1, both signs
+    g = qo.grid(fmt)
+    mids = np.concatenate([(g[1:] + g[:-1]) / 2, g])
+    ties = np.zeros((-(-len(mids) // 31), 32), np.float32)
+    for i, t in enumerate(mids):
+        ties[i // 31, i % 31] = t if i % 2 else -t
+    ties[:, 31] = g[-1]
+    x = np.concatenate([x, ties, -np.zeros((1, 32), np.float32)])
+    x = np.concatenate([x, np.zeros((-len(x) % 4, 32), np.float32)]).reshape(1, -1, 1, 128)
+    gpu, cache, m = _make(gpu_ctx, 1, x.shape[1], 1, 1, 128, fmt)
+    k = _dev(x, F32)
+    gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, -k)
+    code, byte = qo.quantise(x[0, :, 0], fmt)
+    lay = cache.layers[0]
+    np.testing.assert_array_equal(lay.k_scale.buffer.cpu().numpy(), byte)
+    np.testing.assert_array_equal(lay.v_scale.buffer.cpu().numpy(), byte)
+    np.testing.assert_array_equal(lay.k_cache.buffer.cpu().numpy(), qo.pack(code, fmt))
+    np.testing.assert_array_equal(lay.v_cache.buffer.cpu().numpy(),
+                                  qo.pack(code ^ (8 if fmt == "fp4" else 128), fmt))
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+def test_groups_that_are_not_finite(gpu_ctx, fmt):
+    banner(f"quant not finite {fmt}")
+    rng = np.random.default_rng(8)
+    x = _rows(rng, 1, 5, 2, 64)
+    x[0, 1, 0, 3] = np.nan
+    x[0, 2, 1, 40] = np.inf
+    x[0, 3, 0, 63] = -np.inf
+    x[0, 4, 1, 0], x[0, 4, 1, 1] = np.inf, np.nan
+    gpu, cache, m = _make(gpu_ctx, 1, 5, 2, 1, 64, fmt)
+    for dtype in (F32, BF16):
+        gpu.kv_cache_reset(cache)
+        m.lens[:] = 0
+        k = _dev(x, dtype)
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, k)
+        m.append(_np(k), _np(k))
+        _check_stored(gpu, gpu_ctx, cache, m)
+        _check_stored(gpu, gpu_ctx, cache, m, dtype=BF16)
+
+
+# ---- decode ----------------------------------------------------------------
+
+DECODE = [
+    # B, Hkv, G, D, lens, page, io
+    (1, 1, 1, 32, [1], 0, F32), (3, 2, 1, 64, [0, 31, 33], 0, F32),
+    (2, 3, 2, 64, [127, 129], 0, BF16), (4, 1, 3, 96, [5, 0, 200, 64], 8, F32),
+    (2, 2, 4, 128, [300, 17], 16, BF16), (3, 4, 1, 128, [511, 512, 513], 0, F32),
+    (2, 1, 5, 160, [90, 257], 1, F32), (1, 2, 8, 128, [1000], 64, F32),
+    (2, 1, 16, 256, [140, 31], 0, F32), (1, 1, 16, 64, [77], 2, BF16),
+    (2, 2, 1, 224, [65, 128], 0, BF16), (1, 3, 7, 192, [150], 32, F32),
+    (5, 12, 1, 64, [700, 1, 0, 350, 699], 0, F32), (2, 8, 4, 128, [2100, 900], 16, F32),
+    (1, 2, 1, 256, [400], 4, BF16),
+]
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+@pytest.mark.parametrize("B,Hkv,G,D,lens,page,io", DECODE)
+def test_decode_attention(gpu_ctx, fmt, B, Hkv, G, D, lens, page, io):
+    banner(f"quant decode {fmt} B={B} Hkv={Hkv} G={G} D={D} lens={lens} page={page} {io}")
+    rng = np.random.default_rng(B * 100 + D + G)
+    gpu, cache, m = _make(gpu_ctx, B, max(lens) + 2, Hkv, G, D, fmt, page)
+    _fill(gpu, gpu_ctx, cache, m, rng, lens)
+    q = _dev(rng.standard_normal((B, Hkv * G, D)).astype(np.float32), io)
+    outs = []
+    for hint in (0, 128, 4096):  # several chunks a row, and one
+        gpu_ctx.config.decode_chunk_tokens = hint
+        out = torch.full_like(q, 9.0)
+        gpu.decode_attention(gpu_ctx, cache, 0, q, out)
+        _check_attention(out[:, None], q[:, None], m, G, D ** -0.5, io == F32, io == BF16)
+        outs.append(out)
+    gpu_ctx.config.decode_chunk_tokens = 0
+    again = torch.empty_like(q)
+    gpu.decode_attention(gpu_ctx, cache, 0, q, again)
+    assert torch.equal(again, outs[0])
+    # types of their own for q and out, another scale
+    mixed = torch.empty(q.shape, dtype=BF16 if io == F32 else F32, device="cuda:0")
+    gpu.decode_attention(gpu_ctx, cache, 0, q, mixed, scale=0.05)
+    _check_attention(mixed[:, None], q[:, None], m, G, 0.05, True, io == F32)
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+@pytest.mark.parametrize("B,Hkv,G,D,lens,page,io", [
+    (1, 1, 1, 32, [0], 0, F32), (3, 2, 2, 64, [0, 127, 128], 0, F32),
+    (2, 4, 4, 128, [255, 40], 16, BF16), (2, 1, 8, 256, [3, 130], 4, F32),
+    (4, 12, 1, 64, [700, 0, 31, 352], 0, F32), (2, 3, 3, 96, [64, 9], 1, BF16)])
+def test_append_attend(gpu_ctx, fmt, B, Hkv, G, D, lens, page, io):
+    """The one call against append and attention apart, several steps, up to full
+    sequences: the same bytes, fills and bits."""
+    banner(f"quant append_attend {fmt} B={B} Hkv={Hkv} G={G} D={D} lens={lens} page={page} {io}")
+    rng = np.random.default_rng(D + G)
+    T = max(lens) + 3
+    gpu, cache, m = _make(gpu_ctx, B, T, Hkv, G, D, fmt, page)
+    _, twin, m2 = _make(gpu_ctx, B, T, Hkv, G, D, fmt, page)
+    if max(lens):
+        k, v = (_dev(_rows(rng, B, max(lens), Hkv, D), F32) for _ in range(2))
+        for c in (cache, twin):
+            gpu.kv_cache_prefill(gpu_ctx, c, 0, k, v, n_new=lens)
+        m.append(_np(k), _np(v), lens)
+    for _ in range(5):
+        k, v = (_dev(_rows(rng, B, Hkv, D), io) for _ in range(2))
+        q = _dev(rng.standard_normal((B, Hkv * G, D)).astype(np.float32), io)
+        out, want = torch.empty_like(q), torch.empty_like(q)
+        fills = gpu.kv_cache_append_attend(gpu_ctx, cache, 0, k, v, q, out)
+        gpu.kv_cache_append(gpu_ctx, twin, 0, k, v)
+        gpu.decode_attention(gpu_ctx, twin, 0, q, want)
+        m.append(_np(k)[:, None], _np(v)[:, None])
+        assert fills.tolist() == m.lens.tolist()
+        assert torch.equal(out, want)
+        _check_attention(out[:, None], q[:, None], m, G, D ** -0.5, io == F32, io == BF16)
+    _check_stored(gpu, gpu_ctx, cache, m)
+
+
+def test_update_and_attention_of_the_reference(gpu_ctx):
+    """The reference's pair, kv_cache_update and attention_with_kv_cache, 2-D buffers."""
+    banner("quant reference pair")
+    rng = np.random.default_rng(3)
+    B, H, D = 2, 4, 64
+    gpu, cache, m = _make(gpu_ctx, B, 40, H, 1, D, "fp8")
+    for _ in range(40):
+        k, v = _rows(rng, B, H, D), _rows(rng, B, H, D)
+        bk, bv = (gpu.gpu_buffer_2d_create(gpu_ctx, B, H * D, x.reshape(B, -1)) for x in (k, v))
+        gpu.kv_cache_update(gpu_ctx, cache, 0, bk, bv)
+        m.append(k[:, None], v[:, None])
+    q = rng.standard_normal((B, H * D)).astype(np.float32)
+    bq, out = gpu.gpu_buffer_2d_create(gpu_ctx, B, H * D, q), gpu.gpu_buffer_2d_create(gpu_ctx, B, H * D)
+    gpu.attention_with_kv_cache(gpu_ctx, cache, 0, bq, out)
+    _check_attention(out.buffer.reshape(B, 1, H, D), bq.buffer.reshape(B, 1, H, D), m, 1, D ** -0.5,
+                     True, False)
+    with pytest.raises(ValueError, match="Cache is full"):
+        gpu.kv_cache_update(gpu_ctx, cache, 0, bk, bv)
+
+
+def test_page_layout_does_not_change_the_bits(gpu_ctx):
+    banner("quant paged against contiguous")
+    rng = np.random.default_rng(4)
+    B, H, G, D, lens = 3, 2, 4, 128, [333, 64, 1]
+    k, v = (_dev(_rows(rng, B, 333, H, D), F32) for _ in range(2))
+    q = _dev(rng.standard_normal((B, H * G, D)).astype(np.float32), F32)
+    outs = []
+    for page in (0, 1, 16, 256):
+        gpu, cache, _ = _make(gpu_ctx, B, 340, H, G, D, "fp4", page)
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, n_new=lens)
+        out = torch.empty_like(q)
+        gpu.decode_attention(gpu_ctx, cache, 0, q, out)
+        outs.append(out)
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+def test_nan_group_reaches_its_heads_only(gpu_ctx):
+    banner("quant decode NaN")
+    rng = np.random.default_rng(6)
+    B, H, G, D = 2, 2, 2, 64
+    gpu, cache, m = _make(gpu_ctx, B, 200, H, G, D, "fp4")
+    k, v = _rows(rng, B, 200, H, D), _rows(rng, B, 200, H, D)
+    k[0, 50, 0, 3] = np.nan   # sequence 0, kv head 0: every element of its heads
+    v[1, 120, 1, 40] = np.inf  # sequence 1, kv head 1: elements 32..63 of its heads
+    gpu.kv_cache_prefill(gpu_ctx, cache, 0, _dev(k, F32), _dev(v, F32))
+    q = _dev(rng.standard_normal((B, H * G, D)).astype(np.float32), F32)
+    out = torch.empty_like(q)
+    gpu.decode_attention(gpu_ctx, cache, 0, q, out)
+    nan = torch.isnan(out).cpu().numpy()
+    want = np.zeros((B, H * G, D), bool)
+    want[0, :G] = True
+    want[1, G:, 32:] = True
+    np.testing.assert_array_equal(nan, want)
+
+
+def test_plan_that_does_not_cover_a_fill_gives_nan(gpu_ctx):
+    """A captured plan that a sequence outgrew: NaN rows, the others right, the
+    token of a fused append still stored."""
+    banner("quant outgrown plan")
+    rng = np.random.default_rng(9)
+    B, H, D = 2, 2, 64
+    gpu, cache, m = _make(gpu_ctx, B, 600, H, 1, D, "fp8")
+    _fill(gpu, gpu_ctx, cache, m, rng, [500, 100])
+    from simple_llm_amd.gpu import gpu_kv_quant as gq
+
+    layer = cache.layers[0]
+    q = _dev(rng.standard_normal((B, H, D)).astype(np.float32), F32)
+    k, v = (_dev(_rows(rng, B, H, D), F32) for _ in range(2))
+    for chunk in (128, 512):  # two chunks; one (no merge)
+        gpu_ctx.config.decode_chunk_tokens = chunk
+        out = torch.empty_like(q)
+        gq.attend(gpu_ctx, cache, layer, q, out, None, 150, 300, k, v)
+        m.append(_np(k)[:, None], _np(v)[:, None])
+        layer.host_lens = m.lens.copy()
+        tokens, n = gq.plan(B, H, 150, 300, chunk)
+        assert n == (2 if chunk == 128 else 1) and m.lens[1] <= tokens * n < m.lens[0]
+        assert torch.isnan(out[0]).all()
+        assert not torch.isnan(out[1]).any()
+    gpu_ctx.config.decode_chunk_tokens = 0
+    _check_stored(gpu, gpu_ctx, cache, m)
+
+
+# ---- prefill ---------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+@pytest.mark.parametrize("B,Hkv,G,D,lens,C,counts,page,io", [
+    (1, 1, 1, 32, [0], 1, None, 0, BF16), (2, 2, 1, 64, [0, 70], 33, [33, 5], 0, F32),
+    (2, 1, 2, 96, [129, 3], 40, None, 8, BF16), (3, 2, 4, 128, [0, 64, 200], 50, [50, 0, 17], 16, BF16),
+    (1, 4, 8, 128, [30], 70, None, 0, BF16), (2, 1, 1, 128, [1000, 40], 130, [7, 130], 64, F32),
+    (1, 2, 1, 160, [65], 31, None, 1, BF16), (2, 1, 2, 256, [100, 0], 66, None, 0, BF16),
+    (1, 1, 8, 256, [5], 20, [11], 4, F32), (1, 12, 1, 64, [300], 257, None, 0, BF16),
+    (4, 8, 8, 32, [60, 61, 62, 63], 90, None, 0, BF16)])
+def test_prefill(gpu_ctx, fmt, B, Hkv, G, D, lens, C, counts, page, io):
+    banner(f"quant prefill {fmt} B={B} Hkv={Hkv} G={G} D={D} lens={lens} C={C} {counts} page={page}")
+    rng = np.random.default_rng(C + D)
+    for splits in (0, 1, 3):
+        gpu, cache, m = _make(gpu_ctx, B, max(lens) + C + 1, Hkv, G, D, fmt, page)
+        _fill(gpu, gpu_ctx, cache, m, rng, lens)
+        k, v = (_dev(_rows(rng, B, C, Hkv, D), io) for _ in range(2))
+        q = _dev(rng.standard_normal((B, C, Hkv * G, D)).astype(np.float32), io)
+        out = torch.full_like(q, 9.0)
+        fills = gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out, n_new=counts, n_splits=splits)
+        m.append(_np(k), _np(v), counts)
+        assert fills.tolist() == m.lens.tolist()
+        _check_attention(out, q, m, G, D ** -0.5, False, io == BF16,
+                         np.asarray(counts) if counts else None, True, io == F32)
+        _check_stored(gpu, gpu_ctx, cache, m)
+
+
+def test_prefill_equals_a_bf16_cache_of_the_same_values(gpu_ctx):
+    """K and V enter as a bf16 cache holding the stored values would give them."""
+    banner("quant prefill against bf16 cache")
+    from simple_llm_amd.gpu import gpu as g
+
+    rng = np.random.default_rng(12)
+    B, H, G, D, C = 2, 2, 4, 128, 100
+    for fmt in ("fp4", "fp8"):
+        gpu, cache, m = _make(gpu_ctx, B, 400, H, G, D, fmt)
+        plain = g.kv_cache_create(gpu_ctx, g.KVCacheConfig(B, 400, 1, H * G, D, n_kv_heads=H,
+                                                           dtype=BF16))
+        for n in (250, C):
+            k, v = (_dev(_rows(rng, B, n, H, D), BF16) for _ in range(2))
+            sk, sv = (_dev(qo.round_trip(_np(x), fmt).astype(np.float32), BF16) for x in (k, v))
+            q = _dev(rng.standard_normal((B, n, H * G, D)).astype(np.float32), BF16)
+            out, want = torch.empty_like(q), torch.empty_like(q)
+            gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out)
+            g.kv_cache_prefill(gpu_ctx, plain, 0, sk, sv, q, want)
+            assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+def test_prefill_nan_stays_behind_the_mask(gpu_ctx, splits):
+    """A NaN group reaches the queries that attend its token, not earlier ones of
+    the same tile: K all elements, V its group's."""
+    banner(f"quant prefill NaN splits={splits}")
+    rng = np.random.default_rng(14)
+    B, H, D, C = 1, 2, 64, 150
+    gpu, cache, m = _make(gpu_ctx, B, 300, H, 1, D, "fp4")
+    _fill(gpu, gpu_ctx, cache, m, rng, [70])
+    k, v = _rows(rng, B, C, H, D), _rows(rng, B, C, H, D)
+    k[0, 60, 0, 3] = np.nan
+    v[0, 100, 1, 40] = np.nan
+    q = _dev(rng.standard_normal((B, C, H, D)).astype(np.float32), BF16)
+    out = torch.empty_like(q)
+    gpu.kv_cache_prefill(gpu_ctx, cache, 0, _dev(k, BF16), _dev(v, BF16), q, out, n_splits=splits)
+    want = np.zeros((B, C, H, D), bool)
+    want[0, 60:, 0] = True
+    want[0, 100:, 1, 32:] = True
+    np.testing.assert_array_equal(torch.isnan(out).cpu().numpy(), want)
+
+
+# ---- together, streams, graphs, far offsets --------------------------------
+
+@pytest.mark.parametrize("fmt,page", [("fp4", 0), ("fp8", 16)])
+def test_serving_run(gpu_ctx, fmt, page):
+    """A server's use: ragged prompts prefilled in two chunks, decode steps, a
+    finished sequence replaced, more steps."""
+    banner(f"quant serving run {fmt} page={page}")
+    rng = np.random.default_rng(21)
+    B, H, G, D, T = 3, 2, 2, 64, 160
+    gpu, cache, m = _make(gpu_ctx, B, T, H, G, D, fmt, page)
+
+    def prefill(C, counts):
+        k, v = (_dev(_rows(rng, B, C, H, D), BF16) for _ in range(2))
+        q = _dev(rng.standard_normal((B, C, H * G, D)).astype(np.float32), BF16)
+        out = torch.empty_like(q)
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out, n_new=counts)
+        m.append(_np(k), _np(v), counts)
+        _check_attention(out, q, m, G, D ** -0.5, False, True, np.asarray(counts), True)
+
+    def steps(n):
+        for _ in range(n):
+            k, v = (_dev(_rows(rng, B, H, D), F32) for _ in range(2))
+            q = _dev(rng.standard_normal((B, H * G, D)).astype(np.float32), F32)
+            out = torch.empty_like(q)
+            gpu.kv_cache_append_attend(gpu_ctx, cache, 0, k, v, q, out)
+            m.append(_np(k)[:, None], _np(v)[:, None])
+            _check_attention(out[:, None], q[:, None], m, G, D ** -0.5, True, False)
+
+    prefill(40, [40, 0, 13])
+    prefill(64, [20, 64, 1])
+    steps(6)
+    lay = cache.layers[0]
+    lay.lens[1] = 0  # sequence 1 is done; another takes its place
+    lay.host_lens[1] = 0
+    m.lens[1] = 0
+    prefill(30, [0, 30, 0])
+    steps(4)
+    _check_stored(gpu, gpu_ctx, cache, m)
+
+
+def test_captured_steps(gpu_ctx):
+    """Decode steps in a captured graph, replayed between eager calls of the same
+    cache: every replay equals the eager step."""
+    banner("quant captured steps")
+    rng = np.random.default_rng(31)
+    B, H, G, D, T = 2, 2, 4, 128, 700
+    gpu, cache, _ = _make(gpu_ctx, B, T, H, G, D, "fp4", 16)
+    _, twin, m = _make(gpu_ctx, B, T, H, G, D, "fp4", 16)
+    k0, v0 = (_dev(_rows(rng, B, 300, H, D), F32) for _ in range(2))
+    for c in (cache, twin):
+        gpu.kv_cache_prefill(gpu_ctx, c, 0, k0, v0, n_new=[300, 120])
+    k, v = (torch.zeros(B, H, D, device="cuda:0") for _ in range(2))
+    q = torch.zeros(B, H * G, D, device="cuda:0")
+    out = torch.empty_like(q)
+    lay = cache.layers[0]
+    lens0, host0 = lay.lens.clone(), lay.host_lens.copy()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):  # a step before the capture, undone
+        gpu.kv_cache_append_attend(gpu_ctx, cache, 0, k, v, q, out, max_len=600)
+    side.synchronize()
+    lay.lens.copy_(lens0)
+    lay.host_lens = host0.copy()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.kv_cache_append_attend(gpu_ctx, cache, 0, k, v, q, out, max_len=600)
+    lay.host_lens = host0.copy()
+    for i in range(6):
+        k.copy_(_dev(_rows(rng, B, H, D), F32))
+        v.copy_(_dev(_rows(rng, B, H, D), F32))
+        q.copy_(_dev(rng.standard_normal((B, H * G, D)).astype(np.float32), F32))
+        want = torch.empty_like(q)
+        gpu.kv_cache_append_attend(gpu_ctx, twin, 0, k, v, q, want, max_len=600)
+        graph.replay()
+        torch.cuda.synchronize()
+        lay.host_lens += 1
+        assert torch.allclose(out, want, rtol=0, atol=2e-5 * float(want.abs().max()))
+        assert lay.lens.cpu().tolist() == twin.layers[0].lens.cpu().tolist()
+        eager = torch.empty_like(q)  # over the graph's cache, its plan, between the replays
+        gpu.decode_attention(gpu_ctx, cache, 0, q, eager)
+        assert torch.allclose(out, eager, rtol=0, atol=2e-5 * float(want.abs().max()))
+    for a, b in ((lay.k_cache, twin.layers[0].k_cache), (lay.v_scale, twin.layers[0].v_scale)):
+        assert torch.equal(a.buffer, b.buffer)
+
+
+def test_two_streams_at_once(gpu_ctx):
+    """Calls of one context on two streams share no workspace."""
+    banner("quant two streams")
+    rng = np.random.default_rng(41)
+    runs = []
+    for fmt in ("fp4", "fp8"):
+        gpu, cache, m = _make(gpu_ctx, 2, 3000, 4, 1, 128, fmt)
+        _fill(gpu, gpu_ctx, cache, m, rng, [2900, 1500])
+        q = _dev(rng.standard_normal((2, 4, 128)).astype(np.float32), F32)
+        want = torch.empty_like(q)
+        gpu.decode_attention(gpu_ctx, cache, 0, q, want)
+        runs.append((cache, q, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(8):
+        for cache, q, want, s in runs:
+            with torch.cuda.stream(s):
+                out = torch.empty_like(q)
+                gpu.decode_attention(gpu_ctx, cache, 0, q, out)
+                outs.append((out, want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in outs)
+
+
+def test_offsets_past_32_bits(gpu_ctx):
+    """The last sequence's rows lie past 4 GiB of codes."""
+    banner("quant far offsets")
+    rng = np.random.default_rng(51)
+    B, H, G, D, T = 3, 16, 2, 128, 1 << 21
+    gpu, cache, _ = _make(gpu_ctx, B, T, H, G, D, "fp4")
+    assert cache.layers[0].k_cache.buffer.numel() > 2 ** 32
+    m = Model(B, 400, H, D, "fp4")
+    _fill(gpu, gpu_ctx, cache, m, rng, [3, 0, 300])
+    k, v = (_dev(_rows(rng, B, H, D), F32) for _ in range(2))
+    q = _dev(rng.standard_normal((B, H * G, D)).astype(np.float32), F32)
+    out = torch.empty_like(q)
+    gpu.kv_cache_append_attend(gpu_ctx, cache, 0, k, v, q, out)
+    m.append(_np(k)[:, None], _np(v)[:, None])
+    _check_attention(out[:, None], q[:, None], m, G, D ** -0.5, True, False)
+    C = 20
+    k, v = (_dev(_rows(rng, B, C, H, D), BF16) for _ in range(2))
+    q = _dev(rng.standard_normal((B, C, H * G, D)).astype(np.float32), BF16)
+    out = torch.empty_like(q)
+    gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out)
+    m.append(_np(k), _np(v))
+    _check_attention(out, q, m, G, D ** -0.5, False, True, None, True)
+    _check_stored(gpu, gpu_ctx, cache, m)
