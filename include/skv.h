@@ -309,29 +309,35 @@ int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale, const voi
                        int H_kv, int D, int T_cap, int fmt, int in_dt, skv_stream_t stream);
 
 /* Rows back: k_out[b, i], v_out[b, i] ([B, C, H_kv, D] of out_dt, exact in
- * either type) = position start[b] + i (start NULL: start_const + i), or zeros
- * outside [0, lens[b]). */
+ * either type) = position start[b] + i, or zeros outside [0, lens[b]). start
+ * holds n_start integers: B of them, or one for every sequence; it has been
+ * read when the call returns. */
 int skv_q_read(void* k_out, void* v_out, const void* k, const void* k_scale, const void* v,
-               const void* v_scale, const int32_t* lens, const int32_t* start, int start_const,
-               const int32_t* block_table, int max_blocks, int block_size, int B, int C, int H_kv,
+               const void* v_scale, const int32_t* lens, const int32_t* start /* host */,
+               int n_start, const int32_t* block_table, int max_blocks, int block_size, int B, int C, int H_kv,
                int D, int T_cap, int fmt, int out_dt, skv_stream_t stream);
 
 /* Split sizing of skv_q_decode_attn (host-only): chunk_tokens (a multiple of
- * 128) of one kv head per workgroup and n_chunks = ceil(max_len / chunk_tokens).
- * total_len: filled tokens over the batch (<= 0: B * max_len). chunk_hint > 0
- * forces the chunk size (rounded up). */
-int skv_q_decode_plan(int B, int H_kv, int max_len, long long total_len, int chunk_hint,
-                      int* chunk_tokens /* host */, int* n_chunks /* host */);
+ * 128) of one kv head per workgroup, n_chunks = ceil(max_len / chunk_tokens)
+ * and n_wg, the workgroups of a kv head. total_len: filled tokens over the
+ * batch (<= 0: B * max_len). covering != 0: n_wg serves any lengths up to
+ * max_len (B * n_chunks), else (B <= 256) those that sum to total_len.
+ * chunk_hint > 0 forces the chunk size (rounded up). */
+int skv_q_decode_plan(int B, int H_kv, int max_len, long long total_len, int covering,
+                      int chunk_hint, int* chunk_tokens /* host */, int* n_chunks /* host */,
+                      int* n_wg /* host */);
 
 /* Bytes of workspace skv_q_decode_attn needs for n_chunks > 1: fp32 partials
- * (o[D], m, l) per (sequence, query head, chunk). No contents are expected. */
+ * (o[D] and four words) per (sequence, query head, chunk). No contents are
+ * expected. */
 size_t skv_q_decode_workspace_bytes(int B, int H_q, int D, int n_chunks);
 
 /* skv_decode_attn over a block-scaled cache: q, out [B, H_q, D] of q_dt /
  * out_dt, G = H_q / H_kv from 1 to 16. lens[b] == 0 gives zeros. Products are
  * of fp32 accuracy where q or out is fp32; with both bf16, K, V and q are
  * exact and the probabilities carry 17 bits. A sequence longer than
- * chunk_tokens * n_chunks gets NaN outputs.
+ * chunk_tokens * n_chunks, or whose chunks do not fit in n_wg workgroups (in
+ * batch order), gets NaN outputs.
  * new_k, new_v ([B, H_kv, D] of in_dt; both or neither): exactly skv_q_append
  * before the attention, which then covers the new token, with lens advanced
  * after it; the plan covers the lengths after the append. */
@@ -339,7 +345,7 @@ int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scale, void* v,
                       const void* new_k, const void* new_v, int32_t* lens,
                       const int32_t* block_table, int max_blocks, int block_size, int B, int H_q,
                       int H_kv, int D, int T_cap, float scale, int chunk_tokens, int n_chunks,
-                      void* ws, size_t ws_bytes, int fmt, int in_dt, int q_dt, int out_dt,
+                      int n_wg, void* ws, size_t ws_bytes, int fmt, int in_dt, int q_dt, int out_dt,
                       skv_stream_t stream);
 
 /* skv_append_prefill_attn for a block-scaled cache (contiguous or paged):

@@ -38,11 +38,13 @@ def hipcc() -> str:
     return os.path.join(rocm, "bin", "hipcc")
 
 
-# Extra flags per source. The flash backward keeps its MFMA accumulators in
-# ordinary VGPRs (gfx950 MFMAs take either register file); the default
-# heuristic put them in AGPRs and copied them back and forth every step.
+# Extra flags per source. The flash backward and the decode over block-scaled
+# caches keep their MFMA accumulators in ordinary VGPRs (gfx950 MFMAs take
+# either register file); the default heuristic put them in AGPRs and copied
+# them back and forth every step.
 SOURCE_FLAGS = {"flash_fp32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                 "flash_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                "quant_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                 # the flash backward past a head dim of 128: the same source as its own
                 # translation unit, accumulators free to live in AGPRs
                 "flash_fp32.hip:wide_bwd": ["-DSKV_FLASH_WIDE_BWD=1"],

@@ -91,20 +91,26 @@ __device__ __forceinline__ void put8(void* out, size_t i, int out_dt, const uint
   }
 }
 
-// Rows back, grid (token tiles, H_kv, B): row i is position start[b] + i
-// (start NULL: start0 + i), or zeros outside [0, fill).
+// First positions of a read, as a kernel argument: no copy to the device, which
+// would be a launch of its own (or hold the host until it landed).
+constexpr int kStarts = 256;
+struct Starts {
+  int32_t v[kStarts];
+};
+
+// Rows back, grid (token tiles, H_kv, sequences b0 ..): row i is position
+// start.v[b - b0] + i, or zeros outside [0, fill).
 template <int BITS, bool PAGED>
 __global__ __launch_bounds__(256) void k_q_read(Cache c, void* __restrict__ ko,
                                                 void* __restrict__ vo, int out_dt,
-                                                const int32_t* __restrict__ lens,
-                                                const int32_t* __restrict__ start, int start0,
-                                                int C) {
-  const int b = blockIdx.z, h = blockIdx.y;
+                                                const int32_t* __restrict__ lens, Starts start,
+                                                int b0, int C) {
+  const int b = b0 + blockIdx.z, h = blockIdx.y;
   const int opr = c.D / 8, tpw = tokens_per_wg(c.D);
   const int r = threadIdx.x / opr, o = threadIdx.x - r * opr;
   const int i = blockIdx.x * tpw + r;
   if (r >= tpw || i >= C) return;
-  const long long pos = (long long)(start ? start[b] : start0) + i;
+  const long long pos = (long long)start.v[blockIdx.z] + i;
   const bool here = pos >= 0 && pos < min(max(lens[b], 0), c.cap);
   uint32_t wk[Fmt<BITS>::NW] = {}, wv[Fmt<BITS>::NW] = {};
   uint32_t sk = 0, sv = 0;
@@ -222,7 +228,7 @@ extern "C" int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale
 
 extern "C" int skv_q_read(void* k_out, void* v_out, const void* k, const void* k_scale,
                           const void* v, const void* v_scale, const int32_t* lens,
-                          const int32_t* start, int start_const, const int32_t* block_table,
+                          const int32_t* start, int n_start, const int32_t* block_table,
                           int max_blocks, int block_size, int B, int C, int H_kv, int D,
                           int T_cap, int fmt, int out_dt, skv_stream_t stream) {
   const char* fn = "skv_q_read";
@@ -231,12 +237,18 @@ extern "C" int skv_q_read(void* k_out, void* v_out, const void* k, const void* k
                             const_cast<void*>(v), const_cast<void*>(v_scale), block_table,
                             max_blocks, block_size, B, H_kv, D, T_cap, fmt, fn);
   if (rc) return rc;
-  SKV_REQUIRE(k_out && v_out && lens && C > 0, SKV_E_INVALID, "%s: bad arguments", fn);
+  SKV_REQUIRE(k_out && v_out && lens && start && C > 0 && (n_start == 1 || n_start == B),
+              SKV_E_INVALID, "%s: bad arguments", fn);
   SKV_REQUIRE(dt_ok(out_dt), SKV_E_INVALID, "%s: bad dtype", fn);
   SKV_REQUIRE(aligned16(k_out) && aligned16(v_out), SKV_E_INVALID,
               "%s: k_out and v_out must be 16-byte aligned", fn);
   const int tpw = tokens_per_wg(D);
-  SKV_Q_CASES(k_q_read, dim3((unsigned)(((long)C + tpw - 1) / tpw), H_kv, B), dim3(256), 0,
-              (hipStream_t)stream, c, k_out, v_out, out_dt, lens, start, start_const, C);
+  for (int b0 = 0; b0 < B; b0 += kStarts) {
+    const int nb = B - b0 < kStarts ? B - b0 : kStarts;
+    Starts st;
+    for (int i = 0; i < nb; ++i) st.v[i] = start[n_start == 1 ? 0 : b0 + i];
+    SKV_Q_CASES(k_q_read, dim3((unsigned)(((long)C + tpw - 1) / tpw), H_kv, nb), dim3(256), 0,
+                (hipStream_t)stream, c, k_out, v_out, out_dt, lens, st, b0, C);
+  }
   return check_launch(fn);
 }

@@ -6,8 +6,8 @@
 // attention_with_kv_cache of the reference
 // (simple-llm/src/gpu/gpu_kv_cache.py:194-289) over the 4- and 8-bit storage.
 //
-// Work split: workgroup (chunk, b, kv head) of four wavefronts takes `chunk`
-// consecutive tokens of one kv head for its G query heads (1 to 16), each
+// Work split: a workgroup of four wavefronts takes `chunk` consecutive tokens
+// of one kv head of one sequence for its G query heads (1 to 16), each
 // wavefront every fourth 32-token tile; the head-major cache makes a tile one
 // run of bytes (2 KB of 4-bit codes at head dim 128). The wavefronts merge
 // through LDS, and the chunks in a second launch, which also advances the
@@ -19,7 +19,6 @@
 //    contraction may take the elements in any order as long as q does too, so
 //    the eight-element pieces go to the matrix core as they lie, and a lane's
 //    piece has one scale. Converted to bf16 with the scale they are exact.
-//    Column c of the product is query head c.
 //  * Online softmax in fp32, each lane holding 8 of the 32 scores of its
 //    column. The running max moves lazily: only when a score passes it by 8
 //    (log2 units), which is also the only time the four lanes of a column
@@ -29,9 +28,16 @@
 //    eight tokens of a lane would have eight), row-major with XOR-swizzled
 //    16-byte chunks, and comes back transposed (ds_read_b64_tr_b16). The
 //    probabilities are already in the operand's token order.
-// Precision: K and V enter exactly. fp32 q is three bf16 parts (all of its
-// bits) and p three (2^-24 of p); bf16 q is one part and, the output being
-// bf16, p two (2^-17).
+// Precision: K and V enter exactly. With fp32 in or out, q and p are three bf16
+// parts (all bits of q, 2^-24 of p); with bf16 in and out q is one part and p
+// two (2^-17). The parts use the matrix core's columns that few heads leave
+// idle: column c is head c % HC, slot c / HC, HC = 16, 8 or (three parts
+// only) 4 being the smallest that holds G, and slot s takes part s (as the
+// plain grouped-query kernel's duplicated columns do); parts beyond the slots
+// are products of their own. Up to four heads cost the same at either
+// precision. A head's scores are summed over the slots by rotations of the
+// 16-lane row whose additions are symmetric, so every slot has the same bits
+// and splits the same p.
 // Tokens past the chunk reread its last row and get weight 0: no memory past
 // the fill is touched, none of it meets a zero weight.
 // No atomics: results are bitwise reproducible, and a paged cache gives the
@@ -57,11 +63,14 @@ struct QDecodeArgs {
   const void* q;
   const int32_t* lens;
   int B, Hq, G;
-  float qscale;  // softmax scale * log2(e)
+  // scores are qscale * ((qsign * q) . k), in log2 units: qscale = |softmax
+  // scale| * log2(e), qsign its sign (0 for a scale of 0, with qscale 1)
+  float qscale, qsign;
   int q_dt, out_dt;
-  int chunk, n_chunks;
+  int chunk, n_chunks;  // tokens a workgroup takes; chunks the workspace has room for
+  int n_wg;             // workgroups of a kv head
   float* ws_o;   // [B * Hq][n_chunks][D]
-  float* ws_ml;  // [B * Hq][n_chunks][2]
+  float* ws_ml;  // [B * Hq][n_chunks][4]: m, l, and in chunk 0 the number of chunks (int), 0
   const void* new_k;  // fused append, or NULL
   const void* new_v;
   int in_dt;
@@ -71,20 +80,23 @@ __device__ __forceinline__ bool appends(const QDecodeArgs& a, int len) {
   return a.new_k != nullptr && len >= 0 && len < a.c.cap;
 }
 
-// W words from p (aligned to min(4 W, 16) bytes), read once: non-temporal.
+// W words from p (aligned to min(4 W, 16) bytes). Ordinary loads: a wavefront's
+// loads of one cache line are spread over several instructions or quarters of
+// one, which the non-temporal ones that the plain caches use fetched again
+// (64 ragged sequences of 8-bit rows: 82 -> 66 us).
 template <int W>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   if constexpr (W >= 4) {
 #pragma unroll
     for (int i = 0; i < W / 4; ++i) {
-      const u32x4_t x = stream_load16(p + 16 * i);
+      const uint4 x = *reinterpret_cast<const uint4*>(p + 16 * i);
       w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
     }
   } else if constexpr (W == 2) {
-    const u32x2_t x = stream_load8(p);
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
     w[0] = x.x; w[1] = x.y;
   } else {
-    w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
@@ -94,15 +106,19 @@ __device__ __forceinline__ i16x4 lds_read_tr16(const uint16_t* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p));
 }
 
-// The swizzle of a bf16 V row in LDS: 16-byte chunk ch of token t lies at
-// chunk ch ^ key(t), so that the transposed reads (4 adjacent chunks of 4
-// consecutive rows per 32 lanes) hit distinct banks.
+// The swizzle of a bf16 V row in LDS (element offset of 16-byte chunk ch of
+// token t). Two patterns must each hit distinct banks of the 256-byte sweep: a
+// store takes chunks 4 g + i (one i) of 128 bytes of lanes, a transposed read
+// two adjacent chunks of 8 consecutive rows. (With a key that spread four
+// adjacent chunks of four rows instead, LDS was busy 76 % of the time over
+// 4 x 16 x 128 of 32000 tokens, two thirds of it conflicts.)
 template <int DP>
 __device__ __forceinline__ int v_at(int t, int ch) {
   int key;
-  if constexpr (DP >= 128) key = 4 * (t & 3) + ((t >> 2) & 3);
-  else if constexpr (DP == 64) key = 4 * ((t >> 1) & 1) + ((t >> 2) & 3);
-  else key = (t >> 2) & 3;
+  if constexpr (DP == 256) key = 2 * (t & 7) ^ 2 * (ch >> 4);
+  else if constexpr (DP == 128) key = 2 * (t & 7);
+  else if constexpr (DP == 64) key = 2 * ((t >> 1) & 3);
+  else key = 2 * ((t >> 2) & 1);
   return t * DP + ((ch ^ key) * 8);
 }
 
@@ -114,10 +130,176 @@ __device__ __forceinline__ void wave_lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// Where the rows of a tile lie. The address of a load is a base that is the
+// same for the whole wavefront (of a run of rows that lie end to end) plus a
+// 32-bit lane offset: with 64-bit rows per lane a quarter of the loop's
+// instructions computed addresses.
+enum Pages {
+  kContig = 0,      // no pages
+  kPages16 = 1,     // pages of at least 16 tokens: a half tile lies in one
+  kPagesSmall = 2,  // smaller ones: every lane looks its row up
+};
+
+// What is left of x after its first bf16 part (exact).
+__device__ __forceinline__ float rest(float x) { return x - (float)(__bf16)x; }
+
+// What this lane's slot takes of x: the part after the `slot` first ones
+// (after the conversion to bf16). f[i] is 1 where slot > i, else 0. Three parts
+// are all of an fp32 value, so a fourth slot takes 0.
+template <int SL>
+__device__ __forceinline__ float slot_part(float x, const float (&f)[3]) {
+#pragma unroll
+  for (int i = 0; i < SL - 1; ++i) x = fmaf(-f[i], (float)(__bf16)x, x);
+  return x;
+}
+
+// x + the same head's values of the other slots, the same bits in each (SL
+// slots of 16 / SL columns; rotations within the 16-lane row).
+template <int SL>
+__device__ __forceinline__ float slot_sum(float x) {
+  if constexpr (SL >= 2) x += dpp<0x128>(x);  // row_ror:8
+  if constexpr (SL >= 4) x += dpp<0x124>(x);  // row_ror:4
+  return x;
+}
+
+// Four consecutive outputs.
+__device__ __forceinline__ void store4_out(void* out, size_t i, int dt, f32x4 x) {
+  if (dt == SKV_BF16) {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) =
+        make_uint2((uint32_t)f32_to_bf16(x[0]) | ((uint32_t)f32_to_bf16(x[1]) << 16),
+                   (uint32_t)f32_to_bf16(x[2]) | ((uint32_t)f32_to_bf16(x[3]) << 16));
+  } else {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(out) + i) = x;
+  }
+}
+
+// The row of a fused append at position t: threads [0, 2 D / 8) of the
+// workgroup, all of them of its first wavefront.
+template <int BITS, bool PAGED>
+__device__ __forceinline__ void append_row(const QDecodeArgs& a, int b, int hk, int t, int tid) {
+  const int opr = a.c.D / 8;
+  if (tid >= 2 * opr) return;
+  const bool isv = tid >= opr;
+  const int o = isv ? tid - opr : tid;
+  float x[8];
+  load8_f32(isv ? a.new_v : a.new_k, ((size_t)b * a.c.Hkv + hk) * a.c.D + o * 8, a.in_dt, x);
+  uint32_t w[Fmt<BITS>::NW];
+  const uint32_t byte = quantise8<BITS>(x, w);
+  store8<BITS>(isv ? a.c.v : a.c.k, isv ? a.c.vs : a.c.ks, row_of<PAGED>(a.c, b, hk, t), a.c.D, o,
+               w, byte);
+}
+
+// Which sequence and chunk workgroup w of a kv head has, and what it needs to
+// know of the sequence.
+struct Piece {
+  int b, ci, len;
+  int n;     // chunks of the sequence
+  bool app;  // a fused append adds its token (len counts it)
+  bool cut;  // the grid does not hold all of its chunks
+};
+
+__device__ __forceinline__ int row_len(const QDecodeArgs& a, int fill, bool* app) {
+  *app = appends(a, fill);
+  return min(max(fill, 0), a.c.cap) + (*app ? 1 : 0);
+}
+
+// Chunks of a row: at least one (which stores an empty sequence's zeros), at
+// most what the workspace holds.
+__device__ __forceinline__ int n_pieces(const QDecodeArgs& a, int len) {
+  return min(max((len + a.chunk - 1) / a.chunk, 1), a.n_chunks);
+}
+
+// Batches of up to this many sequences run only the workgroups that have
+// tokens: each finds its place by a prefix sum over the sequences' chunk
+// counts. (With one for every chunk of the longest row, those of shorter rows
+// wait for a workgroup's LDS only to leave: 64 ragged sequences of 8 kv heads,
+// 146,000 tokens in 8 chunks of the longest, 45 us against 33 for equal ones.)
+constexpr int kMaxScan = 256;
+
+// Inclusive prefix sum over the wavefront (DPP row shifts and broadcasts).
+__device__ __forceinline__ int wave_scan(int x) {
+#define SKV_SCAN(CTRL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, true)
+  SKV_SCAN(0x111, 0xF);
+  SKV_SCAN(0x112, 0xF);
+  SKV_SCAN(0x114, 0xF);
+  SKV_SCAN(0x118, 0xF);
+  SKV_SCAN(0x142, 0xA);  // lane 15 of each row to the next row (rows 1, 3)
+  SKV_SCAN(0x143, 0xC);  // lane 31 to rows 2, 3
+#undef SKV_SCAN
+  return x;
+}
+
+// Uniform over the wavefront. b = a.B: no sequence.
+__device__ __forceinline__ Piece find_piece(const QDecodeArgs& a, int w, int lane) {
+  Piece p;
+  if (a.n_chunks == 1 || a.B > kMaxScan) {  // chunks slowest
+    p.ci = a.n_chunks == 1 ? 0 : w / a.B;
+    p.b = w - p.ci * a.B;
+    p.len = row_len(a, a.lens[p.b], &p.app);
+    p.n = n_pieces(a, p.len);
+    p.cut = false;
+    return p;
+  }
+  p.b = a.B;
+  p.ci = 0;
+  p.len = 0;
+  p.n = 0;
+  p.app = p.cut = false;
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    bool app;
+    const int len = row_len(a, a.lens[min(b, a.B - 1)], &app);
+    const int n = b < a.B ? n_pieces(a, len) : 0;
+    const int incl = base + wave_scan(n);
+    const int total = __builtin_amdgcn_readlane(incl, 63);
+    if (w < total) {
+      const int at = __popcll(__ballot(incl <= w));  // the first lane whose chunks pass w
+      p.b = b0 + at;
+      p.ci = w - __builtin_amdgcn_readlane(incl - n, at);
+      p.len = __builtin_amdgcn_readlane(len, at);
+      p.n = __builtin_amdgcn_readlane(n, at);
+      p.app = __builtin_amdgcn_readlane((int)app, at) != 0;
+      p.cut = __builtin_amdgcn_readlane(incl, at) > a.n_wg;
+      return p;
+    }
+    base = total;
+  }
+  return p;
+}
+
+// The last workgroup of a kv head also takes the sequences behind its own, which
+// exist only where the fills outgrew the plan: NaN rows (chunk 0 alone, l =
+// NaN), a fused append's token stored all the same.
+template <int BITS, bool PAGED>
+__device__ __forceinline__ void left_over(const QDecodeArgs& a, int hk, const Piece& pc, int tid) {
+  // a sequence's first chunk is its own workgroup: those after pc.b have none
+  for (int b = pc.b + 1; b < a.B; ++b) {
+    bool app;
+    const int len = row_len(a, a.lens[b], &app);
+    if (app) append_row<BITS, PAGED>(a, b, hk, len - 1, tid);
+    if (tid < a.G)
+      *reinterpret_cast<float4*>(
+          a.ws_ml + ((size_t)b * a.Hq + hk * a.G + tid) * a.n_chunks * 4) =
+          make_float4(0.f, __builtin_nanf(""), __int_as_float(1), 0.f);
+  }
+}
+
+// Wavefronts per SIMD the registers are kept for: as many as fit without
+// spilling. At head dim 128 four instead of three are worth 59 -> 52 us on
+// 4 x 16 x 128 over 32000 tokens.
+constexpr int min_waves(int DP, int BITS, int PG, int SL, bool F32) {
+  if (DP <= 64) return 4;
+  if (DP == 128 && !F32) return BITS == 8 && PG == kPagesSmall ? 3 : 4;
+  if (DP == 128) return SL == 4 ? (BITS == 4 ? 4 : 3) : 2;
+  return F32 && SL < 4 ? 1 : 2;
+}
+
 // DP: head dim padded to a power of two (elements past D: q is zero, rows of
-// O^T are not stored). NQ parts of q, NP of p.
-template <int DP, int BITS, bool PAGED, int NQ, int NP>
-__global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
+// O^T are not stored). SL slots of HC = 16 / SL heads; F32: fp32 products.
+template <int DP, int BITS, int PG, int SL, bool F32>
+__global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, PG, SL, F32)) void k_q_decode(
+    QDecodeArgs a) {
   constexpr int NW = Fmt<BITS>::NW;
   constexpr int KE = DP / 4;                     // elements of a K row per lane
   constexpr int KO = KE / 8;                     // ... in pieces of 8: MFMAs per half tile
@@ -126,78 +308,50 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
   constexpr int VR = VL == 1 ? kTile : 64 / VL;  // V rows a pass moves (head dim 32: half the lanes)
   constexpr int VP = kTile / VR;                 // passes
   constexpr int DB = DP / 16;
+  constexpr int HC = 16 / SL;
+  constexpr int QS = F32 ? (3 + SL - 1) / SL : 1;          // operand sets of q ...
+  constexpr int PS = ((F32 ? 3 : 2) + SL - 1) / SL;        // ... and of p
   __shared__ __attribute__((aligned(16))) uint16_t sv[kWaves][kTile * DP];
   __shared__ float sml[kWaves][kMaxG][2];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n_rows = a.B * a.c.Hkv;
-  const int ci = blockIdx.x / n_rows, bh = blockIdx.x - ci * n_rows;
-  const int b = bh / a.c.Hkv, hk = bh - b * a.c.Hkv;
+  const int hk = blockIdx.x;
+  const Piece pc = find_piece(a, blockIdx.y, lane);
   const int D = a.c.D, G = a.G;
-  const int fill = a.lens[b];
-  const bool app = appends(a, fill);
-  const int len = min(max(fill, 0), a.c.cap) + (app ? 1 : 0);
+  if (a.B <= kMaxScan && a.n_chunks > 1 && (int)blockIdx.y == a.n_wg - 1)
+    left_over<BITS, PG != kContig>(a, hk, pc, tid);
+  const int b = pc.b, ci = pc.ci, len = pc.len;
+  if (b >= a.B || ci >= pc.n) return;
+  const bool app = pc.app;
   const int start = ci * a.chunk;
   const int end = min(len, start + a.chunk);
   const size_t head0 = (size_t)b * a.Hq + hk * G;  // first query head's output row
+  // the plan does not cover the fill: NaN
+  const bool outgrown = (ci == a.n_chunks - 1 && len > end) || (ci == 0 && pc.cut);
 
-  if (start >= end) {
-    // Nothing to attend: chunk 0 of an empty sequence stands for a zero
-    // output (m = 0, l = 1, o = 0); others have no weight (l = 0, o unread).
-    const bool zero = ci == 0;
+  if (len == 0) {
+    // nothing to attend: a zero output (as a part: m = 0, l = 1, o = 0)
     for (int i = tid; i < G * D; i += kWaves * 64) {
       const int g = i / D, d = i - g * D;
       if (a.n_chunks == 1) store_elem(a.out, (head0 + g) * D + d, a.out_dt, 0.f);
-      else if (zero) a.ws_o[(head0 + g) * a.n_chunks * D + d] = 0.f;
+      else a.ws_o[(head0 + g) * a.n_chunks * D + d] = 0.f;
     }
     if (a.n_chunks > 1 && tid < G)
-      *reinterpret_cast<float2*>(a.ws_ml + ((head0 + tid) * a.n_chunks + ci) * 2) =
-          zero ? make_float2(0.f, 1.f) : make_float2(-INFINITY, 0.f);
+      *reinterpret_cast<float4*>(a.ws_ml + (head0 + tid) * a.n_chunks * 4) =
+          make_float4(0.f, 1.f, __int_as_float(1), 0.f);
     return;
   }
 
   // A fused append: the chunk that holds the new token writes its row first
-  // (one wavefront: 2 D / 8 <= 64 lanes), and the workgroup reads it back from
-  // the cache as any other.
-  const bool outgrown = ci == a.n_chunks - 1 && len > end;  // the plan does not cover the fill
+  // and the workgroup reads it back from the cache as any other.
   if (app && (end == len || outgrown)) {
-    const int opr = D / 8;
-    if (tid < 2 * opr) {
-      const bool isv = tid >= opr;
-      const int o = isv ? tid - opr : tid;
-      float x[8];
-      load8_f32(isv ? a.new_v : a.new_k, ((size_t)b * a.c.Hkv + hk) * D + o * 8, a.in_dt, x);
-      uint32_t w[NW];
-      const uint32_t byte = quantise8<BITS>(x, w);
-      store8<BITS>(isv ? a.c.v : a.c.k, isv ? a.c.vs : a.c.ks, row_of<PAGED>(a.c, b, hk, len - 1),
-                   D, o, w, byte);
-    }
+    append_row<BITS, PG != kContig>(a, b, hk, len - 1, tid);
     __builtin_amdgcn_s_waitcnt(0);  // the stores have completed
     __syncthreads();
   }
 
   const int cl = lane & 15, kb = lane >> 4;  // MFMA row/column, k block
-
-  // ---- queries, operand B: column cl is head cl, elements kb KE + 8 i ----
-  bf16x8 qf[NQ][KO];
-#pragma unroll
-  for (int i = 0; i < KO; ++i) {
-    const int e = kb * KE + 8 * i;
-    const bool used = cl < G && e < D;
-    float x[8];
-    load8_f32(a.q, (head0 + (cl < G ? cl : 0)) * D + (e < D ? e : 0), a.q_dt, x);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float r = used ? x[j] : 0.f;
-#pragma unroll
-      for (int p = 0; p < NQ; ++p) {
-        const __bf16 h = (__bf16)r;
-        qf[p][i][j] = h;
-        r -= (float)h;
-      }
-    }
-  }
 
   const int cb = D * BITS / 8, sb = D / kGroup;  // code and scale bytes of a row
   // this lane's place in a K row: code offset of each scale's run, scale index
@@ -214,23 +368,101 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
 
   constexpr int KWS = KO * NW / KS;  // words under one scale
   uint32_t kw[2][KO * NW], kscale[2][KS], vw[VP][4 * NW], vscale[VP];
+  // Pages of the two halves of the tile that load_tile takes next (kPages16).
+  int blk[2] = {0, 0};
+  auto pages_of = [&](int t0) {
+    if constexpr (PG == kPages16) {
+      typedef const __attribute__((address_space(4))) int32_t* cptr;  // scalar loads
+      const cptr bt = (cptr)(a.c.bt + (size_t)b * a.c.max_blocks);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int T = t0 + 16 * u < end ? t0 + 16 * u : min(t0, end - 1);
+        blk[u] = bt[T >> a.c.bs_shift];
+      }
+    }
+  };
   auto load_tile = [&](int t0) {
+    // first row of each half and its last row that may be read; a half wholly
+    // past the end rereads the first
+    size_t r0[2];
+    int lim[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const size_t row = row_of<PAGED>(a.c, b, hk, min(t0 + 16 * u + cl, end - 1));
+      const int T = t0 + 16 * u < end ? t0 + 16 * u : t0;
+      lim[u] = min(15, end - 1 - T);
+      if constexpr (PG == kPages16)
+        r0[u] = (((size_t)blk[u] * a.c.Hkv + hk) << a.c.bs_shift) +
+                (T & ((1 << a.c.bs_shift) - 1));
+      else
+        r0[u] = ((size_t)b * a.c.Hkv + hk) * a.c.T_cap + T;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      size_t base = r0[u];
+      uint32_t r = min(cl, lim[u]);
+      if constexpr (PG == kPagesSmall) {
+        base = row_of<true>(a.c, b, hk, min(t0 + 16 * u + cl, end - 1));
+        r = 0;
+      }
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
-        load_words<KWS>(a.c.k + row * cb + ko[i], &kw[u][i * KWS]);
-        kscale[u][i] = a.c.ks[row * sb + ks[i]];
+        load_words<KWS>(a.c.k + base * cb + (r * (uint32_t)cb + ko[i]), &kw[u][i * KWS]);
+        kscale[u][i] = (a.c.ks + base * sb)[r * (uint32_t)sb + ks[i]];
       }
     }
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
-      const size_t row = row_of<PAGED>(a.c, b, hk, min(t0 + p * VR + vr, end - 1));
-      load_words<4 * NW>(a.c.v + row * cb + vgl * (kGroup * BITS / 8), vw[p]);
-      vscale[p] = a.c.vs[row * sb + vgl];
+      size_t base;
+      uint32_t r;
+      if constexpr (PG == kPagesSmall) {
+        base = row_of<true>(a.c, b, hk, min(t0 + p * VR + vr, end - 1));
+        r = 0;
+      } else if constexpr (VR <= 16) {  // a pass lies in one half
+        const int u = p * VR / 16;
+        base = r0[u];
+        r = min(p * VR % 16 + vr, lim[u]);
+      } else if constexpr (PG == kContig) {  // the tile's rows lie end to end
+        base = r0[0];
+        r = min(vr, min(kTile - 1, end - 1 - t0));
+      } else {
+        base = vr < 16 ? r0[0] : r0[1];
+        r = min(vr & 15, vr < 16 ? lim[0] : lim[1]);
+      }
+      load_words<4 * NW>(a.c.v + base * cb + (r * (uint32_t)cb + vgl * (kGroup * BITS / 8)), vw[p]);
+      vscale[p] = (a.c.vs + base * sb)[r * (uint32_t)sb + vgl];
     }
+    pages_of(t0 + kWaves * kTile);
   };
+
+  // the first tile's codes, in flight while the queries are converted
+  int t0 = start + wave * kTile;
+  if (t0 < end) {
+    pages_of(t0);
+    load_tile(t0);
+  }
+
+  // ---- queries, operand B: column cl is head cl % HC, elements kb KE + 8 i ----
+  const int head = cl % HC, slot = cl / HC;
+  const float sf[3] = {slot > 0 ? 1.f : 0.f, slot > 1 ? 1.f : 0.f, slot > 2 ? 1.f : 0.f};
+  bf16x8 qf[QS][KO];
+#pragma unroll
+  for (int i = 0; i < KO; ++i) {
+    const int e = kb * KE + 8 * i;
+    const bool used = head < G && e < D;
+    float x[8];
+    load8_f32(a.q, (head0 + (head < G ? head : 0)) * D + (e < D ? e : 0), a.q_dt, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float r = used ? x[j] * a.qsign : 0.f;
+#pragma unroll
+      for (int t = 0; t < QS; ++t) {
+        // bf16: every slot takes q itself and has the whole score
+        qf[t][i][j] = (__bf16)(F32 ? slot_part<SL>(r, sf) : r);
+#pragma unroll
+        for (int k = 0; k < SL; ++k) r = rest(r);
+      }
+    }
+  }
 
   f32x4 o[DB];
 #pragma unroll
@@ -238,8 +470,6 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
   float m_run = -INFINITY, l_run = 0.f;
   uint16_t* svw = sv[wave];
 
-  int t0 = start + wave * kTile;
-  if (t0 < end) load_tile(t0);
   for (; t0 < end; t0 += kWaves * kTile) {
     // ---- scores of the two halves ----
     f32x4 sc[2];
@@ -250,9 +480,12 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
       for (int i = 0; i < KO; ++i) {
         const bf16x8 kf = decode8_bf16<BITS>(&kw[u][i * NW], scale_f32(kscale[u][i * KS / KO]));
 #pragma unroll
-        for (int p = 0; p < NQ; ++p)
-          sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[p][i], sc[u], 0, 0, 0);
+        for (int t = 0; t < QS; ++t)
+          sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][i], sc[u], 0, 0, 0);
       }
+      if constexpr (F32)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[u][j] = slot_sum<SL>(sc[u][j]);
     }
     // ---- V to LDS as bf16 ----
 #pragma unroll
@@ -263,21 +496,20 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
         *reinterpret_cast<bf16x8*>(svw + v_at<DP>(p * VR + vr, vg * 4 + i)) = x;
       }
     // the next tile's codes, in flight over the rest of this one
-    const bool mask = t0 + kTile > end;
     if (t0 + kWaves * kTile < end) load_tile(t0 + kWaves * kTile);
 
     // ---- softmax: lane (cl, kb) has tokens t0 + 16 u + 4 kb + j ----
-    float s[8];
+    if (t0 + kTile > end) {  // uniform
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = sc[u][j] * a.qscale;
-        s[4 * u + j] = mask && t0 + 16 * u + 4 * kb + j >= end ? -INFINITY : x;
-      }
-    float mt = s[0];
+        for (int j = 0; j < 4; ++j)
+          if (t0 + 16 * u + 4 * kb + j >= end) sc[u][j] = -INFINITY;
+    }
+    float mt = sc[0][0];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) mt = fmaxf(mt, s[j]);
+    for (int j = 1; j < 8; ++j) mt = fmaxf(mt, sc[j >> 2][j & 3]);
+    mt *= a.qscale;
     if (__ballot(mt > m_run + kLazy) != 0ull) {  // uniform
       mt = fmaxf(mt, __shfl_xor(mt, 16));
       mt = xor32_max(mt);
@@ -289,19 +521,20 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
       for (int db = 0; db < DB; ++db) o[db] *= al;
     }
     const float m_use = m_run == -INFINITY ? 0.f : m_run;  // every score so far is -inf
-    bf16x8 pf[NP];
+    bf16x8 pf[PS];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float r = fast_exp2(s[j] - m_use);
+      float r = fast_exp2(fmaf(sc[j >> 2][j & 3], a.qscale, -m_use));
       l_run += r;
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        const __bf16 h = (__bf16)r;
-        pf[p][j] = h;
-        r -= (float)h;
+      for (int t = 0; t < PS; ++t) {
+        pf[t][j] = (__bf16)slot_part<SL>(r, sf);
+        if (t + 1 < PS)
+#pragma unroll
+          for (int k = 0; k < SL; ++k) r = rest(r);
       }
     }
-    // ---- O^T += V^T P: slots 0-3 are tokens 4 kb + j, 4-7 are 16 + 4 kb + j ----
+    // ---- O^T += V^T P: elements 0-3 are tokens 4 kb + j, 4-7 are 16 + 4 kb + j ----
     wave_lds_order();
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
@@ -311,8 +544,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
       const bf16x8 va =
           __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
-        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pf[p], o[db], 0, 0, 0);
+      for (int t = 0; t < PS; ++t)
+        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pf[t], o[db], 0, 0, 0);
     }
     wave_lds_order();
   }
@@ -320,6 +553,10 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
   // ---- the wavefronts' parts merge through the V tiles' space ----
   float lt = l_run + __shfl_xor(l_run, 16);
   lt = xor32_sum(lt);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[db][j] = slot_sum<SL>(o[db][j]);
   __syncthreads();
   float* mo = reinterpret_cast<float*>(&sv[0][0]);  // [kWaves][G][DP]
   static_assert(sizeof(sv) >= (size_t)kWaves * kMaxG * DP * sizeof(float), "merge space");
@@ -333,9 +570,10 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
     }
   }
   __syncthreads();
-  const int vpr = D / 4;
-  for (int i = tid; i < G * vpr; i += kWaves * 64) {
-    const int g = i / vpr, d = (i - g * vpr) * 4;
+  constexpr int LN = DP / 4;  // four elements a thread
+  const int d = tid % LN * 4;
+  for (int g = tid / LN; g < G; g += kWaves * 64 / LN) {
+    if (d >= D) break;
     float M = sml[0][g][0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sml[w][g][0]);
@@ -350,13 +588,13 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
     }
     if (outgrown) L = __builtin_nanf("");
     if (a.n_chunks == 1) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        store_elem(a.out, (head0 + g) * D + d + e, a.out_dt, O[e] / L);
+      store4_out(a.out, (head0 + g) * D + d, a.out_dt, O * (1.f / L));
     } else {
-      const size_t slot = (head0 + g) * a.n_chunks + ci;
-      *reinterpret_cast<f32x4*>(a.ws_o + slot * D + d) = O;
-      if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + slot * 2) = make_float2(M, L);
+      const size_t at = (head0 + g) * a.n_chunks + ci;
+      *reinterpret_cast<f32x4*>(a.ws_o + at * D + d) = O;
+      if (d == 0)
+        *reinterpret_cast<float4*>(a.ws_ml + at * 4) =
+            make_float4(M, L, __int_as_float(pc.n), 0.f);
     }
   }
 }
@@ -364,7 +602,9 @@ __global__ __launch_bounds__(kWaves * 64) void k_q_decode(QDecodeArgs a) {
 // Merge of the chunks' partials, grid (H_q, B): DP / 4 lanes of four elements
 // by 1024 / DP streams of chunks, then the streams through LDS. adv (fused
 // append): the fills, each advanced by its sequence's first workgroup; nothing
-// else here reads them (a chunk without tokens left m = -inf, l = 0).
+// else here reads them (chunk 0 has the number of chunks). A chunk's (m, l) and
+// o are loaded together, before it is known whether the row has that chunk:
+// one round trip to memory instead of three.
 template <int DP>
 __global__ __launch_bounds__(256) void k_q_merge(QDecodeArgs a, int32_t* adv) {
   constexpr int LN = DP / 4, NS = 256 / LN;
@@ -373,21 +613,19 @@ __global__ __launch_bounds__(256) void k_q_merge(QDecodeArgs a, int32_t* adv) {
   const int h = blockIdx.x, b = blockIdx.y;
   const int D = a.c.D;
   const int li = threadIdx.x % LN, st = threadIdx.x / LN;
-  if (adv != nullptr && h == 0 && threadIdx.x == 0) {
-    const int fill = adv[b];
-    if (appends(a, fill)) adv[b] = fill + 1;
-  }
   const size_t row = (size_t)b * a.Hq + h;
-  const float* ml = a.ws_ml + row * a.n_chunks * 2;
-  const float* po = a.ws_o + row * a.n_chunks * D;
-  const bool here = li * 4 < D;
+  const float* ml = a.ws_ml + row * a.n_chunks * 4;
+  const float* po = a.ws_o + row * a.n_chunks * D + (li * 4 < D ? li * 4 : 0);
+  int n = a.n_chunks;
   float M = -INFINITY, L = 0.f;
   f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = st; s < a.n_chunks; s += NS) {
-    const float2 x = *reinterpret_cast<const float2*>(ml + 2 * s);
-    if (x.x == -INFINITY && x.y == 0.f) continue;  // no weight (and perhaps no o)
-    const f32x4 v = here ? *reinterpret_cast<const f32x4*>(po + (size_t)s * D + li * 4)
-                         : f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = st; s < n; s += NS) {
+    const float2 x = *reinterpret_cast<const float2*>(ml + 4 * s);
+    const f32x4 v = *reinterpret_cast<const f32x4*>(po + (size_t)s * D);
+    if (s == st) {
+      n = __float_as_int(ml[2]);
+      if (s >= n) break;
+    }
     const float mn = fmaxf(M, x.x);
     const float ref = mn == -INFINITY ? 0.f : mn;
     const float wa = fast_exp2(M - ref), wb = fast_exp2(x.x - ref);
@@ -395,26 +633,31 @@ __global__ __launch_bounds__(256) void k_q_merge(QDecodeArgs a, int32_t* adv) {
     O = O * wa + v * wb;
     M = mn;
   }
+  if (adv != nullptr && h == 0 && threadIdx.x == 0) {
+    const int fill = adv[b];
+    if (appends(a, fill)) adv[b] = fill + 1;
+  }
   *reinterpret_cast<f32x4*>(&so[st][li * 4]) = O;
   if (li == 0) {
     sml[st][0] = M;
     sml[st][1] = L;
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float MM = -INFINITY;
+  if (threadIdx.x * 4 >= D) return;
+  const int d = threadIdx.x * 4;
+  float MM = -INFINITY;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) MM = fmaxf(MM, sml[s][0]);
-    float LL = 0.f, OO = 0.f;
+  for (int s = 0; s < NS; ++s) MM = fmaxf(MM, sml[s][0]);
+  float LL = 0.f;
+  f32x4 OO = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const float ms = sml[s][0];
-      const float w = ms == -INFINITY ? 0.f : fast_exp2(ms - MM);
-      LL = fmaf(w, sml[s][1], LL);
-      OO = fmaf(w, so[s][d], OO);
-    }
-    store_elem(a.out, row * D + d, a.out_dt, OO / LL);
+  for (int s = 0; s < NS; ++s) {
+    const float ms = sml[s][0];
+    const float w = ms == -INFINITY ? 0.f : fast_exp2(ms - MM);
+    LL = fmaf(w, sml[s][1], LL);
+    OO += w * *reinterpret_cast<const f32x4*>(&so[s][d]);
   }
+  store4_out(a.out, row * D + d, a.out_dt, OO * (1.f / LL));
 }
 
 bool dt_ok(int dt) { return dt == SKV_F32 || dt == SKV_BF16; }
@@ -424,14 +667,16 @@ int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 constexpr int kCUs = 256;
 constexpr int kStep = kWaves * kTile;  // tokens a workgroup takes at a time
 
-template <int DP, int BITS, bool PAGED>
-void launch_decode(const QDecodeArgs& a, unsigned blocks, bool exact32, hipStream_t s) {
-  if (exact32)
-    hipLaunchKernelGGL((k_q_decode<DP, BITS, PAGED, 3, 3>), dim3(blocks), dim3(kWaves * 64), 0, s,
-                       a);
-  else
-    hipLaunchKernelGGL((k_q_decode<DP, BITS, PAGED, 1, 2>), dim3(blocks), dim3(kWaves * 64), 0, s,
-                       a);
+template <int DP, int BITS, int PG>
+void launch_decode(const QDecodeArgs& a, bool f32, hipStream_t s) {
+  const dim3 grid(a.c.Hkv, a.n_wg), block(kWaves * 64);
+#define SKV_QS(SL, F) hipLaunchKernelGGL((k_q_decode<DP, BITS, PG, SL, F>), grid, block, 0, s, a)
+  if (f32 && a.G <= 4) SKV_QS(4, true);
+  else if (f32 && a.G <= 8) SKV_QS(2, true);
+  else if (f32) SKV_QS(1, true);
+  else if (a.G <= 8) SKV_QS(2, false);
+  else SKV_QS(1, false);
+#undef SKV_QS
 }
 
 }  // namespace
@@ -439,34 +684,41 @@ void launch_decode(const QDecodeArgs& a, unsigned blocks, bool exact32, hipStrea
 
 using namespace skv;
 
-extern "C" int skv_q_decode_plan(int B, int H_kv, int max_len, long long total_len,
-                                 int chunk_hint, int* chunk_tokens, int* n_chunks) {
+extern "C" int skv_q_decode_plan(int B, int H_kv, int max_len, long long total_len, int covering,
+                                 int chunk_hint, int* chunk_tokens, int* n_chunks, int* n_wg) {
   const char* fn = "skv_q_decode_plan";
-  SKV_REQUIRE(chunk_tokens && n_chunks, SKV_E_INVALID, "%s: null output", fn);
-  SKV_REQUIRE(B > 0 && H_kv > 0 && max_len > 0, SKV_E_INVALID,
-              "%s: dims must be > 0 (B=%d H_kv=%d max_len=%d)", fn, B, H_kv, max_len);
+  SKV_REQUIRE(chunk_tokens && n_chunks && n_wg, SKV_E_INVALID, "%s: null output", fn);
+  SKV_REQUIRE(B > 0 && B <= 65535 && H_kv > 0 && max_len > 0, SKV_E_INVALID,
+              "%s: bad dims (B=%d H_kv=%d max_len=%d)", fn, B, H_kv, max_len);
   if (total_len <= 0 || total_len > (long long)B * max_len) total_len = (long long)B * max_len;
   long long chunk = chunk_hint;
   if (chunk <= 0) chunk = total_len * H_kv / (4 * kCUs);
+  const long long most = ((long long)max_len + kStep - 1) / kStep * kStep;
+  const long long n_most = 65535 / B;  // chunks a row that the grid holds
+  const long long least = (max_len + n_most - 1) / n_most;
+  if (chunk < least) chunk = least;
   chunk = (chunk + kStep - 1) / kStep * kStep;
   if (chunk < kStep) chunk = kStep;
-  const long long most = ((long long)max_len + kStep - 1) / kStep * kStep;
   if (chunk > most) chunk = most;
+  const long long n = (max_len + chunk - 1) / chunk;
+  // sum of ceil(len / chunk) <= total / chunk + B
+  const long long some = total_len / chunk + B;
   *chunk_tokens = (int)chunk;
-  *n_chunks = (int)((max_len + chunk - 1) / chunk);
+  *n_chunks = (int)n;
+  *n_wg = (int)(covering || B > kMaxScan || some > B * n ? B * n : some);
   return SKV_OK;
 }
 
 extern "C" size_t skv_q_decode_workspace_bytes(int B, int H_q, int D, int n_chunks) {
   if (B <= 0 || H_q <= 0 || D <= 0 || n_chunks <= 0) return 0;
-  return (size_t)B * H_q * n_chunks * (size_t)(D + 2) * sizeof(float);
+  return (size_t)B * H_q * n_chunks * (size_t)(D + 4) * sizeof(float);
 }
 
 extern "C" int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scale, void* v,
                                  void* v_scale, const void* new_k, const void* new_v,
                                  int32_t* lens, const int32_t* block_table, int max_blocks,
                                  int block_size, int B, int H_q, int H_kv, int D, int T_cap,
-                                 float scale, int chunk_tokens, int n_chunks, void* ws,
+                                 float scale, int chunk_tokens, int n_chunks, int n_wg, void* ws,
                                  size_t ws_bytes, int fmt, int in_dt, int q_dt, int out_dt,
                                  skv_stream_t stream) {
   const char* fn = "skv_q_decode_attn";
@@ -489,9 +741,16 @@ extern "C" int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scal
   SKV_REQUIRE(chunk_tokens > 0 && chunk_tokens % kStep == 0 && n_chunks >= 1, SKV_E_INVALID,
               "%s: chunk_tokens=%d must be a positive multiple of %d, n_chunks=%d positive", fn,
               chunk_tokens, kStep, n_chunks);
-  const long long blocks = (long long)B * H_kv * n_chunks;
-  SKV_REQUIRE(blocks < (1LL << 31) && (long long)chunk_tokens * n_chunks < (1LL << 31),
-              SKV_E_UNSUPPORTED, "%s: grid too large", fn);
+  SKV_REQUIRE((long long)chunk_tokens * n_chunks < (1LL << 31) &&
+                  (long long)B * H_q * n_chunks < (1LL << 31),
+              SKV_E_UNSUPPORTED, "%s: plan too large", fn);
+  // every chunk of every sequence, unless a batch small enough to be scanned
+  // needs fewer workgroups
+  const long long all = (long long)B * n_chunks;
+  SKV_REQUIRE(n_wg == all || (B <= kMaxScan && n_wg >= B && n_wg < all), SKV_E_INVALID,
+              "%s: n_wg=%d for %d sequences of %d chunks", fn, n_wg, B, n_chunks);
+  SKV_REQUIRE(n_wg <= 65535, SKV_E_UNSUPPORTED, "%s: grid too large (%d workgroups a head)", fn,
+              n_wg);
   const bool parts = n_chunks > 1;
   SKV_REQUIRE(!parts || (ws && ws_bytes >= skv_q_decode_workspace_bytes(B, H_q, D, n_chunks)),
               SKV_E_WORKSPACE, "%s: workspace %zu bytes < %zu required", fn, ws_bytes,
@@ -502,23 +761,26 @@ extern "C" int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scal
   a.B = B;
   a.Hq = H_q;
   a.G = H_q / H_kv;
-  a.qscale = scale * LOG2E;
+  a.qscale = scale == 0.f ? 1.f : fabsf(scale) * LOG2E;
+  a.qsign = scale == 0.f ? 0.f : copysignf(1.f, scale);
   a.q_dt = q_dt;
   a.out_dt = out_dt;
   a.chunk = chunk_tokens;
   a.n_chunks = n_chunks;
+  a.n_wg = n_wg;
   a.ws_o = static_cast<float*>(ws);
   a.ws_ml = parts ? a.ws_o + (size_t)B * H_q * n_chunks * D : nullptr;
   a.new_k = new_k;
   a.new_v = new_v;
   a.in_dt = in_dt;
-  const bool exact32 = q_dt == SKV_F32 || out_dt == SKV_F32;
+  const bool f32 = q_dt == SKV_F32 || out_dt == SKV_F32;
   const int DP = padded(D), bits = fmt == SKV_MXFP4 ? 4 : 8;
   hipStream_t s = (hipStream_t)stream;
 #define SKV_QD(DD, BB)                                                                          \
   if (DP == DD && bits == BB) {                                                                 \
-    if (a.c.bt) launch_decode<DD, BB, true>(a, (unsigned)blocks, exact32, s);                    \
-    else launch_decode<DD, BB, false>(a, (unsigned)blocks, exact32, s);                          \
+    if (!a.c.bt) launch_decode<DD, BB, kContig>(a, f32, s);                \
+    else if (a.c.bs_shift >= 4) launch_decode<DD, BB, kPages16>(a, f32, s); \
+    else launch_decode<DD, BB, kPagesSmall>(a, f32, s);                    \
   }
   SKV_QD(32, 4) SKV_QD(64, 4) SKV_QD(128, 4) SKV_QD(256, 4)
   SKV_QD(32, 8) SKV_QD(64, 8) SKV_QD(128, 8) SKV_QD(256, 8)

@@ -206,7 +206,7 @@ def _launch_append(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, k: torc
         raise ValueError("new_k and new_v must share a dtype")
     if cache.quantized:
         gpu_kv_quant.append(cache, layer, k, v)
-        layer.host_lens = _fills_after_append(layer.host_lens, _capacity(cache))[0]
+        layer.host_lens = np.minimum(layer.host_lens + 1, _capacity(cache))
         return
     L = _lib.lib()
     stream = _lib.stream_handle(dev)
@@ -414,12 +414,19 @@ def decode_attention(ctx: GPUContext, cache: KVCache, layer_idx: int, q: torch.T
     if q.numel() != cache.batch_size * e_q or out.numel() != cache.batch_size * e_q:
         raise ValueError(f"q_new/output must hold batch_size*n_heads*head_dim = "
                          f"{cache.batch_size * e_q} elements")
+    if layer.host_lens.size <= 64:  # (Python ints, as in _fills_after_append)
+        fills = layer.host_lens.tolist()
+        top, total = max(fills), sum(fills)
+    else:
+        top, total = int(layer.host_lens.max()), int(layer.host_lens.sum())
+    covering = max_len is not None
     if max_len is None:
-        max_len = int(layer.host_lens.max())
-    _check_max_len(max_len, layer.host_lens)
-    total = int(np.minimum(layer.host_lens, max_len).sum())
+        max_len = top
+    elif max_len < top:
+        _check_max_len(max_len, layer.host_lens)  # raises
+    # every fill is <= max_len here, so the total needs no clamp
     if cache.quantized:
-        gpu_kv_quant.attend(ctx, cache, layer, q, out, scale, max_len, total)
+        gpu_kv_quant.attend(ctx, cache, layer, q, out, scale, max_len, total, covering)
         return
     chunk, nchunks = _decode_plan_span(ctx, cache.batch_size, cache.n_heads, cache.n_kv_heads,
                                        max_len, total, cache.head_dim, cache.dtype)
@@ -482,12 +489,14 @@ def kv_cache_append_attend(ctx: GPUContext, cache: KVCache, layer_idx: int, new_
     batch_count(ctx)
     cap = cache.block_table.shape[1] * cache.block_size if cache.paged else cache.max_seq_len
     after, top, total = _fills_after_append(layer.host_lens, cap)
+    covering = max_len is not None
     if max_len is None:
         max_len = top
     elif max_len < top:
         _check_max_len(max_len, after)  # raises
     if cache.quantized:
-        gpu_kv_quant.attend(ctx, cache, layer, q, out, scale, max_len, total, new_k, new_v)
+        gpu_kv_quant.attend(ctx, cache, layer, q, out, scale, max_len, total, covering, new_k,
+                            new_v)
         layer.host_lens = after
         return after.copy()
     L = _lib.lib()
@@ -705,10 +714,12 @@ def kv_cache_read(ctx: GPUContext, cache: KVCache, layer_idx: int, k_out: torch.
         raise ValueError("k_out and v_out must share shape and dtype")
     if k_out.shape[1] == 0:
         raise ValueError("k_out must hold at least one row per sequence")
-    at = np.asarray(0 if start is None else start, dtype=np.int64)
-    if at.ndim and at.shape != (B,):
-        raise ValueError(f"start must be one integer or {B} of them, got shape {at.shape}")
-    if (at < 0).any() or (at > 2**31 - 1).any():
-        raise ValueError("start must lie in [0, 2^31)")
+    at = [0] if start is None else np.asarray(start, dtype=np.int64)
+    if start is not None:
+        if at.ndim and at.shape != (B,):
+            raise ValueError(f"start must be one integer or {B} of them, got shape {at.shape}")
+        at = at.tolist() if at.ndim else [int(at)]
+        if min(at) < 0 or max(at) >= 2**31:
+            raise ValueError("start must lie in [0, 2^31)")
     batch_count(ctx)
     gpu_kv_quant.read(cache, layer, k_out, v_out, at)

@@ -53,10 +53,13 @@ def create_layer(ctx: GPUContext, batch_size: int, rows: int, head_dim: int,
                         k_scale=buf(scales), v_scale=buf(scales))
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(dev: torch.device):
     """Launches go to the current device: make it the cache's."""
-    if torch.cuda.current_device() == (dev.index or 0):
-        return contextlib.nullcontext()
+    if torch._C._cuda_getDevice() == (dev.index or 0):
+        return _HERE
     return torch.cuda.device(dev)
 
 
@@ -84,47 +87,47 @@ def append(cache: KVCache, layer: KVCacheLayer, k: torch.Tensor, v: torch.Tensor
 
 
 def read(cache: KVCache, layer: KVCacheLayer, k_out: torch.Tensor, v_out: torch.Tensor,
-         start: np.ndarray) -> None:
+         start: list) -> None:
+    """start: first positions, one for every sequence or one for all."""
     dev = layer.lens.device
+    at = (ctypes.c_int * len(start))(*start)
     with _on(dev):
-        stream = _lib.stream_handle(dev)
-        at, first = None, int(start.flat[0])
-        if start.ndim and (start != first).any():
-            at = _lib.upload_i32(start, dev, stream)
         rc = _lib.lib().skv_q_read(k_out.data_ptr(), v_out.data_ptr(), *_storage(layer),
-                                   layer.lens.data_ptr(), at.data_ptr() if at is not None else None,
-                                   first, *_pages(cache), cache.batch_size, k_out.shape[1],
-                                   cache.n_kv_heads, cache.head_dim, cache.max_seq_len,
+                                   layer.lens.data_ptr(), at, len(start), *_pages(cache),
+                                   cache.batch_size, k_out.shape[1], cache.n_kv_heads,
+                                   cache.head_dim, cache.max_seq_len,
                                    _lib.QUANT_FORMATS[cache.dtype], _lib.dtype_code(k_out.dtype),
-                                   stream)
+                                   _lib.stream_handle(dev))
     _lib.check(rc, "skv_q_read")
 
 
 _PLAN_OUT = threading.local()
 
 
-def plan(batch_size: int, n_kv_heads: int, max_len: int, total_len: int,
-         hint: int = 0) -> tuple[int, int]:
-    """(chunk_tokens, n_chunks) of skv_q_decode_plan."""
+def plan(batch_size: int, n_kv_heads: int, max_len: int, total_len: int, covering: bool = False,
+         hint: int = 0) -> tuple[int, int, int]:
+    """(chunk_tokens, n_chunks, n_wg) of skv_q_decode_plan."""
     out = getattr(_PLAN_OUT, "refs", None)
     if out is None:  # per thread: the call releases the GIL while it fills them
-        c, n = ctypes.c_int(), ctypes.c_int()
-        out = _PLAN_OUT.refs = (c, n, ctypes.byref(c), ctypes.byref(n))
+        v = tuple(ctypes.c_int() for _ in range(3))
+        out = _PLAN_OUT.refs = v + tuple(ctypes.byref(x) for x in v)
     rc = _lib.lib().skv_q_decode_plan(batch_size, n_kv_heads, max(int(max_len), 1), int(total_len),
-                                      int(hint), out[2], out[3])
+                                      int(covering), int(hint), out[3], out[4], out[5])
     if rc:
         _lib.check(rc, "skv_q_decode_plan")
-    return out[0].value, out[1].value
+    return out[0].value, out[1].value, out[2].value
 
 
 def attend(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, q: torch.Tensor,
-           out: torch.Tensor, scale: Optional[float], max_len: int, total: int,
+           out: torch.Tensor, scale: Optional[float], max_len: int, total: int, covering: bool,
            new_k: Optional[torch.Tensor] = None, new_v: Optional[torch.Tensor] = None) -> None:
-    """decode_attention, after the append of new_k and new_v if given."""
+    """decode_attention, after the append of new_k and new_v if given. total: the
+    fills' sum; covering: the call serves any fills up to max_len (a captured
+    one is replayed as they grow), not only those that sum to it."""
     dev = layer.lens.device
     L = _lib.lib()
     B, Hq, Hkv, D = cache.batch_size, cache.n_heads, cache.n_kv_heads, cache.head_dim
-    chunk, n = plan(B, Hkv, max_len, total, ctx.config.decode_chunk_tokens)
+    chunk, n, n_wg = plan(B, Hkv, max_len, total, covering, ctx.config.decode_chunk_tokens)
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     nk = nv = None
     idt = 0
@@ -137,7 +140,7 @@ def attend(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, q: torch.Tensor
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
         rc = L.skv_q_decode_attn(out.data_ptr(), q.data_ptr(), *_storage(layer), nk, nv,
                                  layer.lens.data_ptr(), *_pages(cache), B, Hq, Hkv, D,
-                                 cache.max_seq_len, sc, chunk, n,
+                                 cache.max_seq_len, sc, chunk, n, n_wg,
                                  ws.data_ptr() if ws is not None else None, need,
                                  _lib.QUANT_FORMATS[cache.dtype], idt, _lib.dtype_code(q.dtype),
                                  _lib.dtype_code(out.dtype), _lib.stream_handle(dev))

@@ -134,10 +134,11 @@ def test_model_refuses_a_block_scaled_cache():
 
 # ---- C refusals ------------------------------------------------------------
 
+START = (ctypes.c_int * 2)()
 FAKE = 4096  # never dereferenced: each call below fails validation first
 BASE = dict(k=FAKE, ks=FAKE, v=FAKE, vs=FAKE, bt=None, mb=0, bs=0, B=2, Hq=8, H=4, D=64, T=128,
             fmt=_lib.MXFP4, idt=0, qdt=0, odt=0, C=3, new=FAKE, lens=FAKE, q=FAKE, out=FAKE,
-            chunk=128, n=2, ws=FAKE, nb=None, splits=1, scale=0.125)
+            chunk=128, n=2, wg=4, ws=FAKE, nb=None, splits=1, scale=0.125)
 
 
 def _call(which, **kw):
@@ -153,15 +154,15 @@ def _call(which, **kw):
         return L.skv_q_append_chunk(*st, a["new"], a["new"], a["lens"], None, *pg, a["B"], a["C"],
                                     a["H"], a["D"], a["T"], a["fmt"], a["idt"], None)
     if which == "read":
-        return L.skv_q_read(a["out"], a["out"], *st, a["lens"], None, 0, *pg, a["B"], a["C"],
-                            a["H"], a["D"], a["T"], a["fmt"], a["odt"], None)
+        return L.skv_q_read(a["out"], a["out"], *st, a["lens"], kw.get("start", START),
+                            a.get("n_start", 2), *pg, a["B"], a["C"], a["H"], a["D"], a["T"], a["fmt"], a["odt"], None)
     if which == "decode":
         if nb is None:
             nb = L.skv_q_decode_workspace_bytes(a["B"], a["Hq"], a["D"], a["n"])
         return L.skv_q_decode_attn(a["out"], a["q"], *st, a["new"], kw.get("new_v", a["new"]),
                                    a["lens"], *pg, a["B"], a["Hq"], a["H"], a["D"], a["T"],
-                                   a["scale"], a["chunk"], a["n"], a["ws"], nb, a["fmt"], a["idt"],
-                                   a["qdt"], a["odt"], None)
+                                   a["scale"], a["chunk"], a["n"], a["wg"], a["ws"], nb, a["fmt"],
+                                   a["idt"], a["qdt"], a["odt"], None)
     if nb is None:
         nb = L.skv_prefill_workspace_bytes(a["B"], a["C"], a["Hq"], a["D"], a["splits"])
     return L.skv_q_append_prefill_attn(a["out"], a["q"], *st, a["new"], a["new"], a["lens"], None,
@@ -190,6 +191,7 @@ def test_cache_arguments_refused(which, kw, rc):
     ("append", dict(new=None), INV), ("append", dict(new=FAKE + 4), INV),
     ("append", dict(idt=2), INV), ("chunk", dict(C=0), INV), ("chunk", dict(new=None), INV),
     ("chunk", dict(idt=3), INV), ("chunk", dict(new=FAKE + 8), INV), ("read", dict(C=0), INV),
+    ("read", dict(start=None), INV), ("read", dict(n_start=3), INV),
     ("read", dict(out=None), INV), ("read", dict(odt=2), INV), ("read", dict(out=FAKE + 4), INV),
     ("decode", dict(q=None), INV), ("decode", dict(out=None), INV),
     ("decode", dict(new_v=None), INV), ("decode", dict(qdt=2), INV), ("decode", dict(odt=5), INV),
@@ -197,6 +199,8 @@ def test_cache_arguments_refused(which, kw, rc):
     ("decode", dict(Hq=0), INV), ("decode", dict(Hq=68), UNS), ("decode", dict(chunk=96), INV),
     ("decode", dict(chunk=0), INV), ("decode", dict(n=0), INV), ("decode", dict(nb=16), WSP),
     ("decode", dict(ws=None), WSP), ("decode", dict(chunk=1 << 30, n=4), UNS),
+    ("decode", dict(wg=1), INV), ("decode", dict(wg=5), INV), ("decode", dict(B=300, wg=599), INV),
+    ("decode", dict(B=300, n=300, wg=90000), UNS),
     ("prefill", dict(C=0), INV), ("prefill", dict(q=None), INV), ("prefill", dict(Hq=12), UNS),
     ("prefill", dict(Hq=10), INV), ("prefill", dict(qdt=2), INV), ("prefill", dict(scale=0.0), INV),
     ("prefill", dict(splits=0), INV), ("prefill", dict(splits=33), INV),
@@ -206,22 +210,33 @@ def test_arguments_refused(which, kw, rc):
     assert _lib.lib().skv_last_error()
 
 
+@pytest.mark.parametrize("covering", [0, 1])
 @pytest.mark.parametrize("B,H,top,total,hint", [
-    (1, 1, 1, 0, 0), (4, 16, 32000, 0, 0), (64, 8, 8192, 100000, 0), (3, 5, 130, 131, 0),
+    (1, 1, 1, 0, 0), (257, 2, 5000, 70000, 0), (60000, 1, 4000, 0, 0), (256, 1, 300, 300, 0), (4, 16, 32000, 0, 0), (64, 8, 8192, 100000, 0), (3, 5, 130, 131, 0),
     (65535, 1, 1, 0, 0), (1, 1, 2**31 - 1, 0, 0), (2, 2, 1000, 0, 100), (2, 2, 1000, 0, 5000)])
-def test_decode_plan_covers_every_length(B, H, top, total, hint):
-    c, n = ctypes.c_int(), ctypes.c_int()
-    assert _lib.lib().skv_q_decode_plan(B, H, top, total, hint, ctypes.byref(c),
-                                        ctypes.byref(n)) == 0
+def test_decode_plan_covers_every_length(B, H, top, total, hint, covering):
+    c, n, wg = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+    assert _lib.lib().skv_q_decode_plan(B, H, top, total, covering, hint, ctypes.byref(c),
+                                        ctypes.byref(n), ctypes.byref(wg)) == 0
     assert c.value > 0 and c.value % 128 == 0 and n.value >= 1
     assert (n.value - 1) * c.value < top <= n.value * c.value
+    assert B <= wg.value <= 65535
+    if covering or B > 256:
+        assert wg.value == B * n.value
+    elif total:  # any lengths up to top that sum to total: the most chunks they can have
+        rng = np.random.default_rng(B)
+        for _ in range(20):
+            lens = rng.multinomial(total, rng.dirichlet(np.full(B, 0.3)))
+            if lens.max() <= top:
+                assert np.maximum(-(-lens // c.value), 1).sum() <= wg.value
 
 
 def test_decode_plan_refuses():
-    c, n = ctypes.c_int(), ctypes.c_int()
+    c, n, wg = (ctypes.c_int() for _ in range(3))
     L = _lib.lib()
-    for a in ((0, 1, 1), (1, 0, 1), (1, 1, 0)):
-        assert L.skv_q_decode_plan(*a, 0, 0, ctypes.byref(c), ctypes.byref(n)) == INV
-    assert L.skv_q_decode_plan(1, 1, 1, 0, 0, None, ctypes.byref(n)) == INV
-    assert L.skv_q_decode_workspace_bytes(2, 8, 64, 3) == 2 * 8 * 3 * 66 * 4
+    out = tuple(ctypes.byref(x) for x in (c, n, wg))
+    for a in ((0, 1, 1), (65536, 1, 1), (1, 0, 1), (1, 1, 0)):
+        assert L.skv_q_decode_plan(*a, 0, 0, 0, *out) == INV
+    assert L.skv_q_decode_plan(1, 1, 1, 0, 0, 0, None, out[1], out[2]) == INV
+    assert L.skv_q_decode_workspace_bytes(2, 8, 64, 3) == 2 * 8 * 3 * 68 * 4
     assert L.skv_q_decode_workspace_bytes(0, 8, 64, 3) == 0

@@ -378,13 +378,66 @@ def test_plan_that_does_not_cover_a_fill_gives_nan(gpu_ctx):
     for chunk in (128, 512):  # two chunks; one (no merge)
         gpu_ctx.config.decode_chunk_tokens = chunk
         out = torch.empty_like(q)
-        gq.attend(gpu_ctx, cache, layer, q, out, None, 150, 300, k, v)
+        gq.attend(gpu_ctx, cache, layer, q, out, None, 150, 300, True, k, v)
         m.append(_np(k)[:, None], _np(v)[:, None])
         layer.host_lens = m.lens.copy()
-        tokens, n = gq.plan(B, H, 150, 300, chunk)
+        tokens, n, _ = gq.plan(B, H, 150, 300, True, chunk)
         assert n == (2 if chunk == 128 else 1) and m.lens[1] <= tokens * n < m.lens[0]
         assert torch.isnan(out[0]).all()
         assert not torch.isnan(out[1]).any()
+    gpu_ctx.config.decode_chunk_tokens = 0
+    _check_stored(gpu, gpu_ctx, cache, m)
+
+
+@pytest.mark.parametrize("page", [0, 16])
+def test_grid_that_does_not_cover_the_batch_gives_nan(gpu_ctx, page):
+    """Fills that grew behind the host's back: the sequences whose chunks do not
+    fit in the planned workgroups are NaN, the others right, every token of a
+    fused append stored, every fill advanced."""
+    banner(f"quant cut grid page={page}")
+    rng = np.random.default_rng(10)
+    B, H, G, D = 6, 2, 4, 64
+    gpu, cache, m = _make(gpu_ctx, B, 600, H, G, D, "fp4", page)
+    _fill(gpu, gpu_ctx, cache, m, rng, [130, 300, 0, 500, 1, 257])
+    from simple_llm_amd.gpu import gpu_kv_quant as gq
+
+    layer = cache.layers[0]
+    q = _dev(rng.standard_normal((B, H * G, D)).astype(np.float32), F32)
+    gpu_ctx.config.decode_chunk_tokens = 128
+    for fused in (False, True):
+        new = [_dev(_rows(rng, B, H, D), F32) for _ in range(2)] if fused else []
+        out = torch.empty_like(q)
+        # planned for fills that sum to 200: 1 + 6 workgroups of 2 + 3 + 1 + 4 + 1 + 3
+        assert gq.plan(B, H, 512, 200, False, 128) == (128, 4, 7)
+        gq.attend(gpu_ctx, cache, layer, q, out, None, 512, 200, False, *new)
+        if fused:
+            m.append(_np(new[0])[:, None], _np(new[1])[:, None])
+            layer.host_lens = m.lens.copy()
+        assert torch.isnan(out[3:]).all() and not torch.isnan(out[:3]).any()
+        keep = Model(3, m.cap, H, D, "fp4")
+        keep.k, keep.v, keep.lens = m.k[:3], m.v[:3], m.lens[:3]
+        _check_attention(out[:3, None], q[:3, None], keep, G, D ** -0.5, True, False)
+    gpu_ctx.config.decode_chunk_tokens = 0
+    _check_stored(gpu, gpu_ctx, cache, m)
+
+
+@pytest.mark.parametrize("B", [65, 200, 300])
+def test_large_ragged_batches(gpu_ctx, B):
+    """Batches past one scan step, and past the scan."""
+    banner(f"quant ragged batch {B}")
+    rng = np.random.default_rng(B)
+    H, G, D = 1, 2, 32
+    lens = rng.integers(0, 400, B)
+    gpu, cache, m = _make(gpu_ctx, B, 402, H, G, D, "fp4")
+    _fill(gpu, gpu_ctx, cache, m, rng, lens, BF16)
+    q = _dev(rng.standard_normal((B, H * G, D)).astype(np.float32), F32)
+    for hint in (0, 128):
+        gpu_ctx.config.decode_chunk_tokens = hint
+        k, v = (_dev(_rows(rng, B, H, D), F32) for _ in range(2))
+        out = torch.empty_like(q)
+        gpu.kv_cache_append_attend(gpu_ctx, cache, 0, k, v, q, out)
+        m.append(_np(k)[:, None], _np(v)[:, None])
+        _check_attention(out[:, None], q[:, None], m, G, D ** -0.5, True, False)
     gpu_ctx.config.decode_chunk_tokens = 0
     _check_stored(gpu, gpu_ctx, cache, m)
 
