@@ -322,9 +322,11 @@ int skv_q_read(void* k_out, void* v_out, const void* k, const void* k_scale, con
  * and n_wg, the workgroups of a kv head. total_len: filled tokens over the
  * batch (<= 0: B * max_len). covering != 0: n_wg serves any lengths up to
  * max_len (B * n_chunks), else (B <= 256) those that sum to total_len.
- * chunk_hint > 0 forces the chunk size (rounded up). */
-int skv_q_decode_plan(int B, int H_kv, int max_len, long long total_len, int covering,
-                      int chunk_hint, int* chunk_tokens /* host */, int* n_chunks /* host */,
+ * chunk_hint > 0 forces the chunk size (rounded up). Any plan is valid for any
+ * call with these B, H_kv and max_len; the rest tunes it. */
+int skv_q_decode_plan(int B, int H_q, int H_kv, int D, int fmt, int q_dt, int out_dt,
+                      int max_len, long long total_len, int covering, int chunk_hint,
+                      int* chunk_tokens /* host */, int* n_chunks /* host */,
                       int* n_wg /* host */);
 
 /* Bytes of workspace skv_q_decode_attn needs for n_chunks > 1: fp32 partials

@@ -15,10 +15,10 @@
 //
 // A tile:
 //  * S = K q^T (v_mfma_f32_16x16x32_bf16). Lane (r, kb) of a 16-token half
-//    loads the codes of token r, elements [kb DP/4, (kb + 1) DP/4): the
+//    loads every fourth 16-byte piece of token r's codes, the kb-th first: the
 //    contraction may take the elements in any order as long as q does too, so
-//    the eight-element pieces go to the matrix core as they lie, and a lane's
-//    piece has one scale. Converted to bf16 with the scale they are exact.
+//    eight elements at a time go to the matrix core as they lie, and a piece
+//    has one scale. Converted to bf16 with the scale they are exact.
 //  * Online softmax in fp32, each lane holding 8 of the 32 scores of its
 //    column. The running max moves lazily: only when a score passes it by 8
 //    (log2 units), which is also the only time the four lanes of a column
@@ -80,23 +80,21 @@ __device__ __forceinline__ bool appends(const QDecodeArgs& a, int len) {
   return a.new_k != nullptr && len >= 0 && len < a.c.cap;
 }
 
-// W words from p (aligned to min(4 W, 16) bytes). Ordinary loads: a wavefront's
-// loads of one cache line are spread over several instructions or quarters of
-// one, which the non-temporal ones that the plain caches use fetched again
-// (64 ragged sequences of 8-bit rows: 82 -> 66 us).
+// W <= 4 words from p (aligned to 4 W bytes), read once: non-temporal (4 x 16 x
+// 128 of 32000 tokens, 4-bit, 59 -> 53 us). One instruction takes all that a
+// lane reads of its 64-byte stretch: as two of 16 bytes at a stride of 32 the
+// 8-bit rows were fetched twice (64 ragged sequences 66 -> 82 us).
 template <int W>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
-  if constexpr (W >= 4) {
-#pragma unroll
-    for (int i = 0; i < W / 4; ++i) {
-      const uint4 x = *reinterpret_cast<const uint4*>(p + 16 * i);
-      w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-    }
+  if constexpr (W == 4) {
+    const u32x4_t x = stream_load16(p);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
   } else if constexpr (W == 2) {
-    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    const u32x2_t x = stream_load8(p);
     w[0] = x.x; w[1] = x.y;
   } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
+    static_assert(W == 1, "1, 2 or 4 words");
+    w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
   }
 }
 
@@ -107,9 +105,9 @@ __device__ __forceinline__ i16x4 lds_read_tr16(const uint16_t* p) {
 }
 
 // The swizzle of a bf16 V row in LDS (element offset of 16-byte chunk ch of
-// token t). Two patterns must each hit distinct banks of the 256-byte sweep: a
-// store takes chunks 4 g + i (one i) of 128 bytes of lanes, a transposed read
-// two adjacent chunks of 8 consecutive rows. (With a key that spread four
+// token t). Two patterns must each hit distinct banks of the 256-byte sweep: eight
+// lanes' stores take every second (8-bit) or fourth chunk of their rows, a
+// transposed read two adjacent chunks of 8 consecutive rows. (With a key that spread four
 // adjacent chunks of four rows instead, LDS was busy 76 % of the time over
 // 4 x 16 x 128 of 32000 tokens, two thirds of it conflicts.)
 template <int DP>
@@ -285,27 +283,32 @@ __device__ __forceinline__ void left_over(const QDecodeArgs& a, int hk, const Pi
   }
 }
 
-// Wavefronts per SIMD the registers are kept for: as many as fit without
-// spilling. At head dim 128 four instead of three are worth 59 -> 52 us on
-// 4 x 16 x 128 over 32000 tokens.
-constexpr int min_waves(int DP, int BITS, int PG, int SL, bool F32) {
+// Wavefronts per SIMD the registers are kept for, and so workgroups per CU: as
+// many as fit without spilling. At head dim 128 four instead of three are worth
+// 59 -> 52 us on 4 x 16 x 128 of 32000 4-bit tokens; 8-bit ones need three
+// (100 -> 92 us; at four a few registers spill in the loop).
+constexpr int min_waves(int DP, int BITS, int SL, bool F32) {
   if (DP <= 64) return 4;
-  if (DP == 128 && !F32) return BITS == 8 && PG == kPagesSmall ? 3 : 4;
-  if (DP == 128) return SL == 4 ? (BITS == 4 ? 4 : 3) : 2;
-  return F32 && SL < 4 ? 1 : 2;
+  if (DP == 128) return F32 && SL < 4 ? 2 : BITS == 4 ? 4 : 3;
+  return F32 && (SL < 4 || BITS == 8) ? 1 : 2;
 }
+
+// Slots of 16 / slots columns for G heads.
+constexpr int slots_for(int G, bool F32) { return G > 8 ? 1 : F32 && G <= 4 ? 4 : 2; }
 
 // DP: head dim padded to a power of two (elements past D: q is zero, rows of
 // O^T are not stored). SL slots of HC = 16 / SL heads; F32: fp32 products.
 template <int DP, int BITS, int PG, int SL, bool F32>
-__global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, PG, SL, F32)) void k_q_decode(
+__global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, SL, F32)) void k_q_decode(
     QDecodeArgs a) {
   constexpr int NW = Fmt<BITS>::NW;
+  constexpr int E16 = 128 / BITS;                // elements in 16 bytes (one scale)
   constexpr int KE = DP / 4;                     // elements of a K row per lane
-  constexpr int KO = KE / 8;                     // ... in pieces of 8: MFMAs per half tile
-  constexpr int KS = KE > kGroup ? KE / kGroup : 1;  // scales per lane and half tile
-  constexpr int VL = DP / kGroup;                // lanes (groups) of a V row
-  constexpr int VR = VL == 1 ? kTile : 64 / VL;  // V rows a pass moves (head dim 32: half the lanes)
+  constexpr int KO = KE / 8;                     // ... by eight: MFMAs per half tile
+  constexpr int PE = KE < E16 ? KE : E16;        // elements of a lane's piece of a K row
+  constexpr int KP = KE / PE;                    // pieces
+  constexpr int VL = DP / E16;                   // lanes of a V row
+  constexpr int VR = VL == 1 ? kTile : 64 / VL;  // V rows a pass moves (one lane a row: half idle)
   constexpr int VP = kTile / VR;                 // passes
   constexpr int DB = DP / 16;
   constexpr int HC = 16 / SL;
@@ -354,48 +357,49 @@ __global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, PG, SL, F32)) void
   const int cl = lane & 15, kb = lane >> 4;  // MFMA row/column, k block
 
   const int cb = D * BITS / 8, sb = D / kGroup;  // code and scale bytes of a row
-  // this lane's place in a K row: code offset of each scale's run, scale index
-  int ko[KS], ks[KS];
+  // this lane's places in a K row: code offset and scale index of each piece
+  // (past the head dim: the first group's, which meet a zero query)
+  auto k_el = [&](int i) { return (4 * i + kb) * PE; };
+  int ko[KP], ks[KP];
 #pragma unroll
-  for (int i = 0; i < KS; ++i) {
-    const int e = kb * KE + i * kGroup;
-    ko[i] = e < D ? e * BITS / 8 : 0;
-    ks[i] = e < D ? e / kGroup : 0;
+  for (int i = 0; i < KP; ++i) {
+    ko[i] = k_el(i) < D ? k_el(i) * BITS / 8 : 0;
+    ks[i] = k_el(i) < D ? k_el(i) / kGroup : 0;
   }
   // ... and in a V row
   const int vg = VL == 1 ? 0 : lane % VL, vr = VL == 1 ? (lane & (kTile - 1)) : lane / VL;
-  const int vgl = vg < sb ? vg : 0;
+  const int vo = vg * E16 < D ? vg * 16 : 0, vs = vg * E16 < D ? vg * E16 / kGroup : 0;
 
-  constexpr int KWS = KO * NW / KS;  // words under one scale
-  uint32_t kw[2][KO * NW], kscale[2][KS], vw[VP][4 * NW], vscale[VP];
-  // Pages of the two halves of the tile that load_tile takes next (kPages16).
-  int blk[2] = {0, 0};
-  auto pages_of = [&](int t0) {
+  constexpr int PW = PE * BITS / 32;  // words of a K piece
+  uint32_t kw[2][KP * PW], kscale[2][KP], vw[VP][4], vscale[VP];
+  // Pages of this wavefront's next 32 tiles, lane 2 i + u holding half u of the
+  // i-th (kPages16): one load in 32 tiles instead of a scalar one in each, whose
+  // wait is for all LDS operations too.
+  int pages = 0, tile = 0;
+  // First row of each half of the tile at t0 and its last one that may be read
+  // (relative); a half wholly past the end rereads the first.
+  size_t r0[2] = {0, 0};
+  int lim[2] = {0, 0};
+  auto place = [&](int t0) {
     if constexpr (PG == kPages16) {
-      typedef const __attribute__((address_space(4))) int32_t* cptr;  // scalar loads
-      const cptr bt = (cptr)(a.c.bt + (size_t)b * a.c.max_blocks);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int T = t0 + 16 * u < end ? t0 + 16 * u : min(t0, end - 1);
-        blk[u] = bt[T >> a.c.bs_shift];
+      if (tile % 32 == 0) {
+        const int T = t0 + (lane >> 1) * (kWaves * kTile) + (lane & 1) * 16;
+        pages = a.c.bt[(size_t)b * a.c.max_blocks + (min(T, end - 1) >> a.c.bs_shift)];
       }
     }
-  };
-  auto load_tile = [&](int t0) {
-    // first row of each half and its last row that may be read; a half wholly
-    // past the end rereads the first
-    size_t r0[2];
-    int lim[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int T = t0 + 16 * u < end ? t0 + 16 * u : t0;
       lim[u] = min(15, end - 1 - T);
       if constexpr (PG == kPages16)
-        r0[u] = (((size_t)blk[u] * a.c.Hkv + hk) << a.c.bs_shift) +
-                (T & ((1 << a.c.bs_shift) - 1));
+        r0[u] = (((size_t)__builtin_amdgcn_readlane(pages, 2 * (tile & 31) + (T != t0 ? u : 0)) *
+                      a.c.Hkv + hk) << a.c.bs_shift) + (T & ((1 << a.c.bs_shift) - 1));
       else
         r0[u] = ((size_t)b * a.c.Hkv + hk) * a.c.T_cap + T;
     }
+    ++tile;
+  };
+  auto load_k = [&](int t0) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       size_t base = r0[u];
@@ -405,11 +409,13 @@ __global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, PG, SL, F32)) void
         r = 0;
       }
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        load_words<KWS>(a.c.k + base * cb + (r * (uint32_t)cb + ko[i]), &kw[u][i * KWS]);
+      for (int i = 0; i < KP; ++i) {
+        load_words<PW>(a.c.k + base * cb + (r * (uint32_t)cb + ko[i]), &kw[u][i * PW]);
         kscale[u][i] = (a.c.ks + base * sb)[r * (uint32_t)sb + ks[i]];
       }
     }
+  };
+  auto load_v = [&](int t0) {
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       size_t base;
@@ -428,26 +434,27 @@ __global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, PG, SL, F32)) void
         base = vr < 16 ? r0[0] : r0[1];
         r = min(vr & 15, vr < 16 ? lim[0] : lim[1]);
       }
-      load_words<4 * NW>(a.c.v + base * cb + (r * (uint32_t)cb + vgl * (kGroup * BITS / 8)), vw[p]);
-      vscale[p] = (a.c.vs + base * sb)[r * (uint32_t)sb + vgl];
+      load_words<4>(a.c.v + base * cb + (r * (uint32_t)cb + vo), vw[p]);
+      vscale[p] = (a.c.vs + base * sb)[r * (uint32_t)sb + vs];
     }
-    pages_of(t0 + kWaves * kTile);
   };
 
   // the first tile's codes, in flight while the queries are converted
   int t0 = start + wave * kTile;
   if (t0 < end) {
-    pages_of(t0);
-    load_tile(t0);
+    place(t0);
+    load_k(t0);
+    load_v(t0);
   }
 
-  // ---- queries, operand B: column cl is head cl % HC, elements kb KE + 8 i ----
+  // ---- queries, operand B: column cl is head cl % HC, in the
+  // order of a lane's pieces ----
   const int head = cl % HC, slot = cl / HC;
   const float sf[3] = {slot > 0 ? 1.f : 0.f, slot > 1 ? 1.f : 0.f, slot > 2 ? 1.f : 0.f};
   bf16x8 qf[QS][KO];
 #pragma unroll
   for (int i = 0; i < KO; ++i) {
-    const int e = kb * KE + 8 * i;
+    const int e = k_el(i / (PE / 8)) + i % (PE / 8) * 8;
     const bool used = head < G && e < D;
     float x[8];
     load8_f32(a.q, (head0 + (head < G ? head : 0)) * D + (e < D ? e : 0), a.q_dt, x);
@@ -478,7 +485,7 @@ __global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, PG, SL, F32)) void
       sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < KO; ++i) {
-        const bf16x8 kf = decode8_bf16<BITS>(&kw[u][i * NW], scale_f32(kscale[u][i * KS / KO]));
+        const bf16x8 kf = decode8_bf16<BITS>(&kw[u][i * NW], scale_f32(kscale[u][i * KP / KO]));
 #pragma unroll
         for (int t = 0; t < QS; ++t)
           sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][i], sc[u], 0, 0, 0);
@@ -487,16 +494,21 @@ __global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, PG, SL, F32)) void
 #pragma unroll
         for (int j = 0; j < 4; ++j) sc[u][j] = slot_sum<SL>(sc[u][j]);
     }
-    // ---- V to LDS as bf16 ----
+    // The next tile's codes are on their way as soon as this one's have left
+    // the registers: K's now, V's after they went to LDS as bf16.
+    const int tn = t0 + kWaves * kTile;
+    if (tn < end) {
+      place(tn);
+      load_k(tn);
+    }
 #pragma unroll
     for (int p = 0; p < VP; ++p)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < E16 / 8; ++i) {
         const bf16x8 x = decode8_bf16<BITS>(&vw[p][i * NW], scale_f32(vscale[p]));
-        *reinterpret_cast<bf16x8*>(svw + v_at<DP>(p * VR + vr, vg * 4 + i)) = x;
+        *reinterpret_cast<bf16x8*>(svw + v_at<DP>(p * VR + vr, vg * (E16 / 8) + i)) = x;
       }
-    // the next tile's codes, in flight over the rest of this one
-    if (t0 + kWaves * kTile < end) load_tile(t0 + kWaves * kTile);
+    if (tn < end) load_v(tn);
 
     // ---- softmax: lane (cl, kb) has tokens t0 + 16 u + 4 kb + j ----
     if (t0 + kTile > end) {  // uniform
@@ -602,12 +614,12 @@ __global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, PG, SL, F32)) void
 // Merge of the chunks' partials, grid (H_q, B): DP / 4 lanes of four elements
 // by 1024 / DP streams of chunks, then the streams through LDS. adv (fused
 // append): the fills, each advanced by its sequence's first workgroup; nothing
-// else here reads them (chunk 0 has the number of chunks). A chunk's (m, l) and
-// o are loaded together, before it is known whether the row has that chunk:
-// one round trip to memory instead of three.
+// else here reads them (chunk 0 has the number of chunks). The first four (m, l)
+// and o of a stream are loaded together, before it is known whether the row has
+// those chunks: one round trip to memory.
 template <int DP>
 __global__ __launch_bounds__(256) void k_q_merge(QDecodeArgs a, int32_t* adv) {
-  constexpr int LN = DP / 4, NS = 256 / LN;
+  constexpr int LN = DP / 4, NS = 256 / LN, U = 4;
   __shared__ __attribute__((aligned(16))) float so[NS][DP];
   __shared__ float sml[NS][2];
   const int h = blockIdx.x, b = blockIdx.y;
@@ -616,22 +628,35 @@ __global__ __launch_bounds__(256) void k_q_merge(QDecodeArgs a, int32_t* adv) {
   const size_t row = (size_t)b * a.Hq + h;
   const float* ml = a.ws_ml + row * a.n_chunks * 4;
   const float* po = a.ws_o + row * a.n_chunks * D + (li * 4 < D ? li * 4 : 0);
-  int n = a.n_chunks;
+  int n = __float_as_int(ml[2]);
   float M = -INFINITY, L = 0.f;
   f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = st; s < n; s += NS) {
-    const float2 x = *reinterpret_cast<const float2*>(ml + 4 * s);
-    const f32x4 v = *reinterpret_cast<const f32x4*>(po + (size_t)s * D);
-    if (s == st) {
-      n = __float_as_int(ml[2]);
-      if (s >= n) break;
+  for (int s0 = st; s0 < a.n_chunks; s0 += U * NS) {
+    float2 x[U];
+    f32x4 v[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int s = min(s0 + k * NS, a.n_chunks - 1);
+      x[k] = *reinterpret_cast<const float2*>(ml + 4 * s);
+      v[k] = *reinterpret_cast<const f32x4*>(po + (size_t)s * D);
     }
-    const float mn = fmaxf(M, x.x);
+    float mn = M;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (s0 + k * NS < n) mn = fmaxf(mn, x[k].x);
     const float ref = mn == -INFINITY ? 0.f : mn;
-    const float wa = fast_exp2(M - ref), wb = fast_exp2(x.x - ref);
-    L = fmaf(wb, x.y, wa * L);
-    O = O * wa + v * wb;
+    const float wa = fast_exp2(M - ref);
+    L *= wa;
+    O *= wa;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (s0 + k * NS < n) {
+        const float w = fast_exp2(x[k].x - ref);
+        L = fmaf(w, x[k].y, L);
+        O += w * v[k];
+      }
     M = mn;
+    if (s0 + U * NS >= n) break;
   }
   if (adv != nullptr && h == 0 && threadIdx.x == 0) {
     const int fill = adv[b];
@@ -671,10 +696,11 @@ template <int DP, int BITS, int PG>
 void launch_decode(const QDecodeArgs& a, bool f32, hipStream_t s) {
   const dim3 grid(a.c.Hkv, a.n_wg), block(kWaves * 64);
 #define SKV_QS(SL, F) hipLaunchKernelGGL((k_q_decode<DP, BITS, PG, SL, F>), grid, block, 0, s, a)
-  if (f32 && a.G <= 4) SKV_QS(4, true);
-  else if (f32 && a.G <= 8) SKV_QS(2, true);
+  const int sl = slots_for(a.G, f32);
+  if (f32 && sl == 4) SKV_QS(4, true);
+  else if (f32 && sl == 2) SKV_QS(2, true);
   else if (f32) SKV_QS(1, true);
-  else if (a.G <= 8) SKV_QS(2, false);
+  else if (sl == 2) SKV_QS(2, false);
   else SKV_QS(1, false);
 #undef SKV_QS
 }
@@ -684,15 +710,34 @@ void launch_decode(const QDecodeArgs& a, bool f32, hipStream_t s) {
 
 using namespace skv;
 
-extern "C" int skv_q_decode_plan(int B, int H_kv, int max_len, long long total_len, int covering,
-                                 int chunk_hint, int* chunk_tokens, int* n_chunks, int* n_wg) {
+// The chunk: one round of workgroups, all resident (slots below). Equal rows
+// take a whole number of chunks each; with two the merge costs more than the
+// halved rows gain (512 rows of 2288 tokens: 36 us in two, 33.5 in one).
+// Ragged ones leave half a chunk a row, which the round has to hold too (64
+// sequences x 8 heads, 146,000 tokens: 49 us without that, 44 with).
+extern "C" int skv_q_decode_plan(int B, int H_q, int H_kv, int D, int fmt, int q_dt, int out_dt,
+                                 int max_len, long long total_len, int covering, int chunk_hint,
+                                 int* chunk_tokens, int* n_chunks, int* n_wg) {
   const char* fn = "skv_q_decode_plan";
   SKV_REQUIRE(chunk_tokens && n_chunks && n_wg, SKV_E_INVALID, "%s: null output", fn);
-  SKV_REQUIRE(B > 0 && B <= 65535 && H_kv > 0 && max_len > 0, SKV_E_INVALID,
-              "%s: bad dims (B=%d H_kv=%d max_len=%d)", fn, B, H_kv, max_len);
+  SKV_REQUIRE(B > 0 && B <= 65535 && H_kv > 0 && H_q > 0 && H_q % H_kv == 0 && D > 0 &&
+                  max_len > 0,
+              SKV_E_INVALID, "%s: bad dims (B=%d H_q=%d H_kv=%d D=%d max_len=%d)", fn, B, H_q,
+              H_kv, D, max_len);
   if (total_len <= 0 || total_len > (long long)B * max_len) total_len = (long long)B * max_len;
+  const bool f32 = q_dt == SKV_F32 || out_dt == SKV_F32;
+  const long long slots =
+      (long long)kCUs * min_waves(padded(D), fmt == SKV_MXFP4 ? 4 : 8,
+                                  slots_for(H_q / H_kv, f32), f32);
+  const long long rows = (long long)B * H_kv;
   long long chunk = chunk_hint;
-  if (chunk <= 0) chunk = total_len * H_kv / (4 * kCUs);
+  if (chunk <= 0 && total_len == (long long)B * max_len) {
+    const long long n = slots / rows;
+    chunk = n <= 2 ? max_len : (max_len + n - 1) / n;
+  } else if (chunk <= 0) {
+    const long long whole = rows < slots ? slots - rows / 2 : slots / 2;
+    chunk = total_len * H_kv / whole;
+  }
   const long long most = ((long long)max_len + kStep - 1) / kStep * kStep;
   const long long n_most = 65535 / B;  // chunks a row that the grid holds
   const long long least = (max_len + n_most - 1) / n_most;

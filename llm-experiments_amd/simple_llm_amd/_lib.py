@@ -51,8 +51,8 @@ _SIGNATURES = {
                                 _I, _I, _P]),
     "skv_q_read": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I,
                         _I, _P]),
-    "skv_q_decode_plan": (_I, [_I, _I, _I, ctypes.c_longlong, _I, _I, ctypes.POINTER(_I),
-                               ctypes.POINTER(_I), ctypes.POINTER(_I)]),
+    "skv_q_decode_plan": (_I, [_I, _I, _I, _I, _I, _I, _I, _I, ctypes.c_longlong, _I, _I,
+                               ctypes.POINTER(_I), ctypes.POINTER(_I), ctypes.POINTER(_I)]),
     "skv_q_decode_workspace_bytes": (_Z, [_I, _I, _I, _I]),
     "skv_q_decode_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                _F, _I, _I, _I, _P, _Z, _I, _I, _I, _I, _P]),

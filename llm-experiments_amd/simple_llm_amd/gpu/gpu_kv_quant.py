@@ -104,15 +104,17 @@ def read(cache: KVCache, layer: KVCacheLayer, k_out: torch.Tensor, v_out: torch.
 _PLAN_OUT = threading.local()
 
 
-def plan(batch_size: int, n_kv_heads: int, max_len: int, total_len: int, covering: bool = False,
+def plan(cache: KVCache, q_dt: int, out_dt: int, max_len: int, total_len: int, covering: bool,
          hint: int = 0) -> tuple[int, int, int]:
     """(chunk_tokens, n_chunks, n_wg) of skv_q_decode_plan."""
     out = getattr(_PLAN_OUT, "refs", None)
     if out is None:  # per thread: the call releases the GIL while it fills them
         v = tuple(ctypes.c_int() for _ in range(3))
         out = _PLAN_OUT.refs = v + tuple(ctypes.byref(x) for x in v)
-    rc = _lib.lib().skv_q_decode_plan(batch_size, n_kv_heads, max(int(max_len), 1), int(total_len),
-                                      int(covering), int(hint), out[3], out[4], out[5])
+    rc = _lib.lib().skv_q_decode_plan(cache.batch_size, cache.n_heads, cache.n_kv_heads,
+                                      cache.head_dim, _lib.QUANT_FORMATS[cache.dtype], q_dt,
+                                      out_dt, max(max_len, 1), total_len, covering, hint, out[3],
+                                      out[4], out[5])
     if rc:
         _lib.check(rc, "skv_q_decode_plan")
     return out[0].value, out[1].value, out[2].value
@@ -127,7 +129,9 @@ def attend(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, q: torch.Tensor
     dev = layer.lens.device
     L = _lib.lib()
     B, Hq, Hkv, D = cache.batch_size, cache.n_heads, cache.n_kv_heads, cache.head_dim
-    chunk, n, n_wg = plan(B, Hkv, max_len, total, covering, ctx.config.decode_chunk_tokens)
+    qdt, odt = _lib.dtype_code(q.dtype), _lib.dtype_code(out.dtype)
+    chunk, n, n_wg = plan(cache, qdt, odt, int(max_len), total, covering,
+                          int(ctx.config.decode_chunk_tokens))
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     nk = nv = None
     idt = 0
@@ -142,8 +146,8 @@ def attend(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, q: torch.Tensor
                                  layer.lens.data_ptr(), *_pages(cache), B, Hq, Hkv, D,
                                  cache.max_seq_len, sc, chunk, n, n_wg,
                                  ws.data_ptr() if ws is not None else None, need,
-                                 _lib.QUANT_FORMATS[cache.dtype], idt, _lib.dtype_code(q.dtype),
-                                 _lib.dtype_code(out.dtype), _lib.stream_handle(dev))
+                                 _lib.QUANT_FORMATS[cache.dtype], idt, qdt, odt,
+                                 _lib.stream_handle(dev))
     _lib.check(rc, "skv_q_decode_attn")
 
 

@@ -216,8 +216,9 @@ def test_arguments_refused(which, kw, rc):
     (65535, 1, 1, 0, 0), (1, 1, 2**31 - 1, 0, 0), (2, 2, 1000, 0, 100), (2, 2, 1000, 0, 5000)])
 def test_decode_plan_covers_every_length(B, H, top, total, hint, covering):
     c, n, wg = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
-    assert _lib.lib().skv_q_decode_plan(B, H, top, total, covering, hint, ctypes.byref(c),
-                                        ctypes.byref(n), ctypes.byref(wg)) == 0
+    assert _lib.lib().skv_q_decode_plan(B, 2 * H, H, 128, _lib.MXFP4, 0, 0, top, total, covering,
+                                        hint, ctypes.byref(c), ctypes.byref(n),
+                                        ctypes.byref(wg)) == 0
     assert c.value > 0 and c.value % 128 == 0 and n.value >= 1
     assert (n.value - 1) * c.value < top <= n.value * c.value
     assert B <= wg.value <= 65535
@@ -235,8 +236,10 @@ def test_decode_plan_refuses():
     c, n, wg = (ctypes.c_int() for _ in range(3))
     L = _lib.lib()
     out = tuple(ctypes.byref(x) for x in (c, n, wg))
-    for a in ((0, 1, 1), (65536, 1, 1), (1, 0, 1), (1, 1, 0)):
-        assert L.skv_q_decode_plan(*a, 0, 0, 0, *out) == INV
-    assert L.skv_q_decode_plan(1, 1, 1, 0, 0, 0, None, out[1], out[2]) == INV
+    for a in ((0, 2, 1, 64), (65536, 2, 1, 64), (1, 2, 0, 64), (1, 0, 1, 64), (1, 3, 2, 64),
+              (1, 2, 1, 0)):
+        assert L.skv_q_decode_plan(*a, _lib.MXFP4, 0, 0, 10, 0, 0, 0, *out) == INV
+    assert L.skv_q_decode_plan(1, 2, 1, 64, _lib.MXFP4, 0, 0, 0, 0, 0, 0, *out) == INV
+    assert L.skv_q_decode_plan(1, 2, 1, 64, _lib.MXFP4, 0, 0, 9, 0, 0, 0, None, *out[1:]) == INV
     assert L.skv_q_decode_workspace_bytes(2, 8, 64, 3) == 2 * 8 * 3 * 68 * 4
     assert L.skv_q_decode_workspace_bytes(0, 8, 64, 3) == 0

@@ -381,7 +381,7 @@ def test_plan_that_does_not_cover_a_fill_gives_nan(gpu_ctx):
         gq.attend(gpu_ctx, cache, layer, q, out, None, 150, 300, True, k, v)
         m.append(_np(k)[:, None], _np(v)[:, None])
         layer.host_lens = m.lens.copy()
-        tokens, n, _ = gq.plan(B, H, 150, 300, True, chunk)
+        tokens, n, _ = gq.plan(cache, 0, 0, 150, 300, True, chunk)
         assert n == (2 if chunk == 128 else 1) and m.lens[1] <= tokens * n < m.lens[0]
         assert torch.isnan(out[0]).all()
         assert not torch.isnan(out[1]).any()
@@ -408,7 +408,7 @@ def test_grid_that_does_not_cover_the_batch_gives_nan(gpu_ctx, page):
         new = [_dev(_rows(rng, B, H, D), F32) for _ in range(2)] if fused else []
         out = torch.empty_like(q)
         # planned for fills that sum to 200: 1 + 6 workgroups of 2 + 3 + 1 + 4 + 1 + 3
-        assert gq.plan(B, H, 512, 200, False, 128) == (128, 4, 7)
+        assert gq.plan(cache, 0, 0, 512, 200, False, 128) == (128, 4, 7)
         gq.attend(gpu_ctx, cache, layer, q, out, None, 512, 200, False, *new)
         if fused:
             m.append(_np(new[0])[:, None], _np(new[1])[:, None])
