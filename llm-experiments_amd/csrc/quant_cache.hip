@@ -41,14 +41,22 @@ __global__ __launch_bounds__(256) void k_q_append_one(Cache c, const void* __res
   if (threadIdx.x == 0) lens[b] = pos + 1;
 }
 
-// Tokens of one head a workgroup moves: 256 / (D / 8), so its stores are one
-// run of the head's rows (1 KB of 4-bit codes at head dim 128) and its loads
-// whole rows of the token-major input.
+// Tokens of one head in a run, 256 / (D / 8): its code rows are one stretch of
+// the cache (1 KB of 4 bits at head dim 128), its other side that many rows of
+// the token-major tensor.
 __host__ __device__ __forceinline__ int tokens_per_wg(int D) { return 256 / (D / 8); }
 
+// Runs of tokens_per_wg tokens a workgroup takes: four where that still leaves
+// every CU eight workgroups, for loads in flight; one in smaller calls. (Runs
+// of four neighbouring heads, side by side in the token-major tensor, were no
+// faster: 4 x 8192 x 16 x 128 back to bf16 60 us against 57.)
+constexpr int kRuns = 4;
+
 // Chunk append, grid (token tiles, H_kv, B). Row i < n_new[b] goes to position
-// lens[b] + i; lens is read only.
-template <int BITS, bool PAGED>
+// lens[b] + i; lens is read only. The input is loaded before the fill is known
+// (its place depends on neither): one round trip to memory, not two (4 x 2048
+// x 16 x 128 bf16 into 4 bits: 18.8 us with the fill first and one run).
+template <int BITS, bool PAGED, int RUNS>
 __global__ __launch_bounds__(256) void k_q_append_chunk(Cache c, const void* __restrict__ kn,
                                                         const void* __restrict__ vn, int in_dt,
                                                         const int32_t* __restrict__ lens,
@@ -56,40 +64,70 @@ __global__ __launch_bounds__(256) void k_q_append_chunk(Cache c, const void* __r
   const int b = blockIdx.z, h = blockIdx.y;
   const int opr = c.D / 8, tpw = tokens_per_wg(c.D);
   const int r = threadIdx.x / opr, o = threadIdx.x - r * opr;
-  const int i = blockIdx.x * tpw + r;
+  if (r >= tpw) return;  // whole quads: opr % 4 == 0
+  const int i0 = blockIdx.x * (tpw * RUNS) + r;
+  float xk[RUNS][8], xv[RUNS][8];
+#pragma unroll
+  for (int u = 0; u < RUNS; ++u) {
+    const int i = min(i0 + u * tpw, C - 1);
+    const size_t src = (((size_t)b * C + i) * c.Hkv + h) * c.D + o * 8;
+    load8_f32(kn, src, in_dt, xk[u]);
+    load8_f32(vn, src, in_dt, xv[u]);
+  }
   const int n = n_new ? min(n_new[b], C) : C;
   const int p0 = lens[b];
-  if (r >= tpw || i >= n || p0 < 0 || i >= c.cap - p0) return;  // whole quads: opr % 4 == 0
-  const size_t src = (((size_t)b * C + i) * c.Hkv + h) * c.D + o * 8;
-  float xk[8], xv[8];
-  load8_f32(kn, src, in_dt, xk);
-  load8_f32(vn, src, in_dt, xv);
-  const size_t row = row_of<PAGED>(c, b, h, p0 + i);
-  uint32_t w[Fmt<BITS>::NW];
-  uint32_t byte = quantise8<BITS>(xk, w);
-  store8<BITS>(c.k, c.ks, row, c.D, o, w, byte);
-  byte = quantise8<BITS>(xv, w);
-  store8<BITS>(c.v, c.vs, row, c.D, o, w, byte);
-}
-
-// Eight elements out: 16 bytes of bf16 or 32 of fp32.
-template <int BITS>
-__device__ __forceinline__ void put8(void* out, size_t i, int out_dt, const uint32_t* w, float s,
-                                     bool here) {
-  if (out_dt == SKV_BF16) {
-    const bf16x8 x = decode8_bf16<BITS>(w, s);
-    const uint4 y = __builtin_bit_cast(uint4, x);
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + i) =
-        here ? y : make_uint4(0, 0, 0, 0);
-  } else {
-    float x[8];
-    decode8_f32<BITS>(w, s, x);
 #pragma unroll
-    for (int e = 0; e < 8; e += 4)
-      *reinterpret_cast<float4*>(static_cast<float*>(out) + i + e) =
-          here ? make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]) : make_float4(0, 0, 0, 0);
+  for (int u = 0; u < RUNS; ++u) {
+    const int i = i0 + u * tpw;
+    if (i >= n || p0 < 0 || i >= c.cap - p0) return;  // later runs are further on
+    const size_t row = row_of<PAGED>(c, b, h, p0 + i);
+    uint32_t w[Fmt<BITS>::NW];
+    uint32_t byte = quantise8<BITS>(xk[u], w);
+    store8<BITS>(c.k, c.ks, row, c.D, o, w, byte);
+    byte = quantise8<BITS>(xv[u], w);
+    store8<BITS>(c.v, c.vs, row, c.D, o, w, byte);
   }
 }
+
+// A lane's elements of a row on their way out: eight as 16 bytes of bf16, four
+// as 16 of fp32, so that a wavefront stores one stretch (two 16-byte stores a
+// lane, 32 bytes apart, took 84 us for 4 x 4096 x 16 x 128; 160 non-temporal).
+template <int BITS, int OUT>
+struct Piece {
+  static constexpr int N = OUT == SKV_BF16 ? 8 : 4;
+  static constexpr int BYTES = N * BITS / 8;  // 2, 4 or 8
+  uint32_t w[BYTES > 4 ? 2 : 1];
+  uint32_t scale;
+  __device__ __forceinline__ void load(const uint8_t* p, const uint8_t* s) {
+    if constexpr (BYTES == 8) {
+      const uint2 x = *reinterpret_cast<const uint2*>(p);
+      w[0] = x.x;
+      w[1] = x.y;
+    } else if constexpr (BYTES == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+    scale = *s;
+  }
+  __device__ __forceinline__ void zero() {
+    w[0] = scale = 0;
+    if constexpr (BYTES == 8) w[1] = 0;
+  }
+  __device__ __forceinline__ u32x4_t value() const {
+    const float s = scale_f32(scale);
+    if constexpr (OUT == SKV_BF16) {
+      return __builtin_bit_cast(u32x4_t, decode8_bf16<BITS>(w, s));
+    } else {
+      const f32x2 a = BITS == 4 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 0)
+                                : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[0], s, false);
+      const f32x2 b = BITS == 4 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 1)
+                                : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[0], s, true);
+      return u32x4_t{__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]),
+                     __float_as_uint(b[1])};
+    }
+  }
+};
 
 // First positions of a read, as a kernel argument: no copy to the device, which
 // would be a launch of its own (or hold the host until it landed).
@@ -100,35 +138,47 @@ struct Starts {
 
 // Rows back, grid (token tiles, H_kv, sequences b0 ..): row i is position
 // start.v[b - b0] + i, or zeros outside [0, fill).
-template <int BITS, bool PAGED>
+template <int BITS, bool PAGED, int RUNS, int OUT>
 __global__ __launch_bounds__(256) void k_q_read(Cache c, void* __restrict__ ko,
-                                                void* __restrict__ vo, int out_dt,
+                                                void* __restrict__ vo,
                                                 const int32_t* __restrict__ lens, Starts start,
                                                 int b0, int C) {
+  using P = Piece<BITS, OUT>;
   const int b = b0 + blockIdx.z, h = blockIdx.y;
-  const int opr = c.D / 8, tpw = tokens_per_wg(c.D);
-  const int r = threadIdx.x / opr, o = threadIdx.x - r * opr;
-  const int i = blockIdx.x * tpw + r;
-  if (r >= tpw || i >= C) return;
-  const long long pos = (long long)start.v[blockIdx.z] + i;
-  const bool here = pos >= 0 && pos < min(max(lens[b], 0), c.cap);
-  uint32_t wk[Fmt<BITS>::NW] = {}, wv[Fmt<BITS>::NW] = {};
-  uint32_t sk = 0, sv = 0;
-  if (here) {
-    const size_t row = row_of<PAGED>(c, b, h, (int)pos);
-    const size_t at = row * (size_t)(c.D * BITS / 8) + o * BITS;
-    const size_t sat = row * (size_t)(c.D / kGroup) + (o >> 2);
+  const int lpr = c.D / P::N, tpw = 256 / lpr;  // lanes a row, rows a run
+  const int r = threadIdx.x / lpr, o = threadIdx.x - r * lpr;
+  if (r >= tpw) return;
+  const int i0 = blockIdx.x * (tpw * RUNS) + r;
+  const int fill = min(max(lens[b], 0), c.cap);
+  P k[RUNS], v[RUNS];
 #pragma unroll
-    for (int j = 0; j < Fmt<BITS>::NW; ++j) {
-      wk[j] = reinterpret_cast<const uint32_t*>(c.k + at)[j];
-      wv[j] = reinterpret_cast<const uint32_t*>(c.v + at)[j];
+  for (int u = 0; u < RUNS; ++u) {
+    const long long pos = (long long)start.v[blockIdx.z] + i0 + u * tpw;
+    // Rows of a contiguous cache are loaded before the fill is known; a page
+    // past the fill may be no page.
+    k[u].zero();
+    v[u].zero();
+    if (pos >= 0 && pos < (PAGED ? fill : c.cap)) {
+      const size_t row = row_of<PAGED>(c, b, h, (int)pos);
+      const size_t at = row * (size_t)(c.D * BITS / 8) + o * P::BYTES;
+      const size_t sat = row * (size_t)(c.D / kGroup) + o * P::N / kGroup;
+      k[u].load(c.k + at, c.ks + sat);
+      v[u].load(c.v + at, c.vs + sat);
     }
-    sk = c.ks[sat];
-    sv = c.vs[sat];
   }
-  const size_t dst = (((size_t)b * C + i) * c.Hkv + h) * c.D + o * 8;
-  put8<BITS>(ko, dst, out_dt, wk, scale_f32(sk), here);
-  put8<BITS>(vo, dst, out_dt, wv, scale_f32(sv), here);
+#pragma unroll
+  for (int u = 0; u < RUNS; ++u) {
+    const int i = i0 + u * tpw;
+    if (i >= C) return;
+    const long long pos = (long long)start.v[blockIdx.z] + i;
+    const bool here = pos >= 0 && pos < fill;
+    const size_t dst = ((((size_t)b * C + i) * c.Hkv + h) * c.D + o * P::N) * (16 / P::N);
+    const u32x4_t z = u32x4_t{0, 0, 0, 0};
+    __builtin_nontemporal_store(here ? k[u].value() : z,
+                                reinterpret_cast<u32x4_t*>(static_cast<uint8_t*>(ko) + dst));
+    __builtin_nontemporal_store(here ? v[u].value() : z,
+                                reinterpret_cast<u32x4_t*>(static_cast<uint8_t*>(vo) + dst));
+  }
 }
 
 bool dt_ok(int dt) { return dt == SKV_F32 || dt == SKV_BF16; }
@@ -178,14 +228,20 @@ int quant_cache_args(quant::Cache* c, void* k, void* k_scale, void* v, void* v_s
 
 using namespace skv;
 
-// The kernel of (fmt, paged).
-#define SKV_Q_CASES(KERNEL, ...)                                                        \
-  do {                                                                                  \
-    if (fmt == SKV_MXFP4 && c.bt) hipLaunchKernelGGL((KERNEL<4, true>), __VA_ARGS__);   \
-    else if (fmt == SKV_MXFP4) hipLaunchKernelGGL((KERNEL<4, false>), __VA_ARGS__);     \
-    else if (c.bt) hipLaunchKernelGGL((KERNEL<8, true>), __VA_ARGS__);                  \
-    else hipLaunchKernelGGL((KERNEL<8, false>), __VA_ARGS__);                           \
+// The kernel of (fmt, paged), more template arguments after these.
+#define SKV_Q_CASES(LAUNCH)                                    \
+  do {                                                         \
+    if (fmt == SKV_MXFP4 && c.bt) LAUNCH(4, true);             \
+    else if (fmt == SKV_MXFP4) LAUNCH(4, false);               \
+    else if (c.bt) LAUNCH(8, true);                            \
+    else LAUNCH(8, false);                                     \
   } while (0)
+
+// Whether a call over C tokens of B * H_kv heads fills the card with kRuns runs
+// a workgroup (8 workgroups per CU).
+static bool long_call(int B, int H_kv, int C, int D) {
+  return (long)B * H_kv * (C / (tokens_per_wg(D) * kRuns)) >= 8 * 256;
+}
 
 extern "C" int skv_q_append(void* k, void* k_scale, void* v, void* v_scale, const void* k_new,
                             const void* v_new, int32_t* lens, const int32_t* block_table,
@@ -201,8 +257,11 @@ extern "C" int skv_q_append(void* k, void* k_scale, void* v, void* v_scale, cons
   SKV_REQUIRE(aligned16(k_new) && aligned16(v_new), SKV_E_INVALID,
               "%s: k_new and v_new must be 16-byte aligned", fn);
   SKV_REQUIRE((long)H_kv * D < (1L << 30), SKV_E_UNSUPPORTED, "%s: rows too wide", fn);
-  SKV_Q_CASES(k_q_append_one, dim3(B), dim3(256), 0, (hipStream_t)stream, c, k_new, v_new, in_dt,
-              lens);
+#define SKV_LAUNCH(BITS, PAGED)                                                              \
+  hipLaunchKernelGGL((k_q_append_one<BITS, PAGED>), dim3(B), dim3(256), 0, (hipStream_t)stream, \
+                     c, k_new, v_new, in_dt, lens)
+  SKV_Q_CASES(SKV_LAUNCH);
+#undef SKV_LAUNCH
   return check_launch(fn);
 }
 
@@ -220,9 +279,20 @@ extern "C" int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale
   SKV_REQUIRE(dt_ok(in_dt), SKV_E_INVALID, "%s: bad dtype", fn);
   SKV_REQUIRE(aligned16(k_new) && aligned16(v_new), SKV_E_INVALID,
               "%s: k_new and v_new must be 16-byte aligned", fn);
-  const int tpw = tokens_per_wg(D);
-  SKV_Q_CASES(k_q_append_chunk, dim3((unsigned)(((long)C + tpw - 1) / tpw), H_kv, B), dim3(256), 0,
-              (hipStream_t)stream, c, k_new, v_new, in_dt, lens, n_new, C);
+  const bool runs = long_call(B, H_kv, C, D);
+  const int tpw = tokens_per_wg(D) * (runs ? kRuns : 1);
+  const dim3 grid((unsigned)(((long)C + tpw - 1) / tpw), H_kv, B);
+#define SKV_LAUNCH(BITS, PAGED)                                                                \
+  do {                                                                                         \
+    if (runs)                                                                                  \
+      hipLaunchKernelGGL((k_q_append_chunk<BITS, PAGED, kRuns>), grid, dim3(256), 0,           \
+                         (hipStream_t)stream, c, k_new, v_new, in_dt, lens, n_new, C);         \
+    else                                                                                       \
+      hipLaunchKernelGGL((k_q_append_chunk<BITS, PAGED, 1>), grid, dim3(256), 0,               \
+                         (hipStream_t)stream, c, k_new, v_new, in_dt, lens, n_new, C);         \
+  } while (0)
+  SKV_Q_CASES(SKV_LAUNCH);
+#undef SKV_LAUNCH
   return check_launch(fn);
 }
 
@@ -242,13 +312,29 @@ extern "C" int skv_q_read(void* k_out, void* v_out, const void* k, const void* k
   SKV_REQUIRE(dt_ok(out_dt), SKV_E_INVALID, "%s: bad dtype", fn);
   SKV_REQUIRE(aligned16(k_out) && aligned16(v_out), SKV_E_INVALID,
               "%s: k_out and v_out must be 16-byte aligned", fn);
-  const int tpw = tokens_per_wg(D);
+  const bool runs = long_call(B, H_kv, C, D);
+  const int tpw = 256 / (D / (out_dt == SKV_BF16 ? 8 : 4)) * (runs ? kRuns : 1);
   for (int b0 = 0; b0 < B; b0 += kStarts) {
     const int nb = B - b0 < kStarts ? B - b0 : kStarts;
     Starts st;
     for (int i = 0; i < nb; ++i) st.v[i] = start[n_start == 1 ? 0 : b0 + i];
-    SKV_Q_CASES(k_q_read, dim3((unsigned)(((long)C + tpw - 1) / tpw), H_kv, nb), dim3(256), 0,
-                (hipStream_t)stream, c, k_out, v_out, out_dt, lens, st, b0, C);
+    const dim3 grid((unsigned)(((long)C + tpw - 1) / tpw), H_kv, nb);
+#define SKV_READ(BITS, PAGED, RUNS, OUT)                                                      \
+  hipLaunchKernelGGL((k_q_read<BITS, PAGED, RUNS, OUT>), grid, dim3(256), 0, (hipStream_t)stream, \
+                     c, k_out, v_out, lens, st, b0, C)
+#define SKV_LAUNCH(BITS, PAGED)                                       \
+  do {                                                                \
+    if (out_dt == SKV_BF16) {                                         \
+      if (runs) SKV_READ(BITS, PAGED, kRuns, SKV_BF16);               \
+      else SKV_READ(BITS, PAGED, 1, SKV_BF16);                        \
+    } else {                                                          \
+      if (runs) SKV_READ(BITS, PAGED, kRuns, SKV_F32);                \
+      else SKV_READ(BITS, PAGED, 1, SKV_F32);                         \
+    }                                                                 \
+  } while (0)
+    SKV_Q_CASES(SKV_LAUNCH);
+#undef SKV_LAUNCH
+#undef SKV_READ
   }
   return check_launch(fn);
 }
