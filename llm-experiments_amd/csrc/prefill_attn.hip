@@ -142,6 +142,19 @@ template <int D>
 __device__ __forceinline__ int swz(int row, int chunk) {  // element offset of a 16-B chunk
   return row * D + ((chunk ^ swz_key<D>(row)) * 8);
 }
+// The same for block-scaled tiles, which threads store, up to a group of four
+// chunks each: eight lanes' stores of every fourth (or second) chunk of one or
+// more rows must hit distinct banks too, so rows side by side also differ in
+// the low bits, and at D = 256 the two halves of a row.
+template <int D>
+__device__ __forceinline__ int swz_q(int row, int chunk) {
+  int key;
+  if constexpr (D >= 128) key = 4 * (row & 3) + (((row & 3) + (row >> 2)) & 3);
+  else if constexpr (D == 64) key = 4 * ((row >> 1) & 1) + ((((row >> 1) & 1) + (row >> 2)) & 3);
+  else key = (row >> 2) & 3;
+  if constexpr (D == 256) key ^= chunk >> 4;
+  return row * D + ((chunk ^ key) * 8);
+}
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
@@ -211,6 +224,8 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
     if constexpr (REG) return sm.v[s_];
     else return (s_ == 0 ? lds0 : lds1) + kBN * D;
   };
+
+  auto at = [](int row, int chunk) { return QF != 0 ? swz_q<D>(row, chunk) : swz<D>(row, chunk); };
 
   if (a.snap != nullptr && blockIdx.x == 0)
     for (int i = threadIdx.x; i < a.B; i += blockDim.x) a.snap[i] = a.start[i];
@@ -375,7 +390,7 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
         const quant::bf16x8 x = quant::decode8_bf16<QB>(&qw[u][i * (QB / 4)], sc_);
         uint4 y = __builtin_bit_cast(uint4, x);
         if (zero) y = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + swz<D>(unit_row(u), unit_el(u) / 8 + i)) = y;
+        *reinterpret_cast<uint4*>(dst + at(unit_row(u), unit_el(u) / 8 + i)) = y;
       }
     }
   };
@@ -494,7 +509,7 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb) {
         const bf16x8 ka =
-            *reinterpret_cast<const bf16x8*>(sk(stage) + swz<D>(tb * 32 + lc, kb * 2 + g));
+            *reinterpret_cast<const bf16x8*>(sk(stage) + at(tb * 32 + lc, kb * 2 + g));
 #pragma unroll
         for (int qb = 0; qb < kQB; ++qb)
           sc[tb][qb] =
@@ -573,8 +588,8 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
             const int d = db * 32 + dq;
             const int r0 = tb * 32 + kk * 16 + 4 * g + (L >> 2);
             const int r1 = r0 + 8;
-            const uint16_t* p0 = sv(stage) + swz<D>(r0, d >> 3) + (d & 7);
-            const uint16_t* p1 = sv(stage) + swz<D>(r1, d >> 3) + (d & 7);
+            const uint16_t* p0 = sv(stage) + at(r0, d >> 3) + (d & 7);
+            const uint16_t* p1 = sv(stage) + at(r1, d >> 3) + (d & 7);
             const i16x4 lo = lds_read_tr16(p0);
             const i16x4 hi = lds_read_tr16(p1);
             const bf16x8 va = __builtin_bit_cast(
@@ -963,7 +978,12 @@ int prefill_attn_impl(void* out, const void* q, const void* k_cache, const void*
   a.C = C; a.Hq = H_q; a.Hkv = H_kv; a.T_cap = T_cap;
   a.qscale = scale * LOG2E;
   a.q_dt = q_dt; a.out_dt = out_dt;
-  const int W = tile_waves(B, C, H_kv, G, D, n_splits, n_new != nullptr);
+  // (a block-scaled tile's codes cost the 128-row kernel a few spilled registers:
+  // 6 ragged x 8 kv heads x 4 x 128, <= 333 after <= 1900, 8-bit: 88.6 us, 82.5
+  // with 256 rows; 3 x 16 x 128, 640 after 8000, 4-bit: 186 and 273)
+  const int W = qc && n_new && DK <= 128
+                    ? kWaves
+                    : tile_waves(B, C, H_kv, G, D, n_splits, n_new != nullptr);
   a.n_qt = n_query_tiles(C, G, W);
   a.n_splits = n_splits;
   a.n_groups = B * H_kv * n_splits;

@@ -615,13 +615,18 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
     C = int(new_k.shape[1])
     if C <= 0:
         raise ValueError("the chunk must hold at least one token")
-    n_host = (np.full(B, C, np.int64) if n_new is None
-              else np.asarray(n_new, dtype=np.int64).reshape(B))
-    if (n_host < 0).any() or (n_host > C).any():
-        raise ValueError(f"n_new entries must lie in [0, {C}]")
     start = layer.host_lens.copy()
-    if int((start + n_host).max()) > T:
-        raise ValueError(f"Cache is full: chunk of {int(n_host.max())} tokens after "
+    if n_new is None:
+        n_host, n_min = C, C
+    else:
+        n_host = np.asarray(n_new, dtype=np.int64).reshape(B)
+        n_min = int(n_host.min())
+        if n_min < 0 or int(n_host.max()) > C:
+            raise ValueError(f"n_new entries must lie in [0, {C}]")
+    after = start + n_host
+    end = int(after.max())
+    if end > T:
+        raise ValueError(f"Cache is full: chunk of {int(np.max(n_host))} tokens after "
                          f"current_len={int(start.max())}, max_seq_len={T}")
     want_attn = q is not None
     if want_attn:
@@ -641,16 +646,14 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
     batch_count(ctx)
     if cache.quantized:
         gpu_kv_quant.prefill(ctx, cache, layer, new_k, new_v, q, out,
-                             n_host if n_new is not None else None,
-                             int((start + n_host).max()), scale, n_splits)
-        layer.host_lens = np.minimum(start + n_host, T)
-        return layer.host_lens.copy()
+                             None if n_min == C else n_host, end, scale, n_splits)
+        layer.host_lens = after
+        return after.copy()
     L = _lib.lib()
     stream = _lib.stream_handle(dev)
     cdt, idt = _lib.dtype_code(cache.dtype), _lib.dtype_code(new_k.dtype)
     # (counts that are all C are a chunk without counts: no copy to the device)
-    n_dev = (None if n_new is None or int(n_host.min()) == C else
-             _lib.upload_i32(n_host, dev, stream))
+    n_dev = None if n_min == C else _lib.upload_i32(n_host, dev, stream)
     n_ptr = n_dev.data_ptr() if n_dev is not None else None
     kc, vc = layer.k_cache.buffer, layer.v_cache.buffer
     if want_attn:
@@ -658,8 +661,8 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
         if n_splits > 0:
             ns.value = int(n_splits)
         else:
-            _lib.check(L.skv_prefill_plan(B, C, Hq, Hkv, int((start + n_host).max()),
-                                          ctypes.byref(ns)), "skv_prefill_plan")
+            _lib.check(L.skv_prefill_plan(B, C, Hq, Hkv, end, ctypes.byref(ns)),
+                       "skv_prefill_plan")
         need = L.skv_prefill_workspace_bytes(B, C, Hq, D, ns.value)
         ws = _prefill_workspace(ctx, need)
         sc = float(scale) if scale is not None else 1.0 / float(np.sqrt(D))
@@ -679,8 +682,8 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
         _lib.check(rc, "skv_append_chunk")
         rc = L.skv_advance(layer.lens.data_ptr(), n_ptr, C, B, T, stream)
         _lib.check(rc, "skv_advance")
-    layer.host_lens = np.minimum(start + n_host, T)
-    return layer.host_lens.copy()
+    layer.host_lens = after
+    return after.copy()
 
 
 # ============================================================================

@@ -166,7 +166,7 @@ def prefill(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, new_k: torch.T
     with _on(dev):
         stream = _lib.stream_handle(dev)
         n_dev = None
-        if counts is not None and int(counts.min()) < C:
+        if counts is not None:
             n_dev = _lib.upload_i32(counts, dev, stream)
         n_ptr = n_dev.data_ptr() if n_dev is not None else None
         if q is None:
