@@ -300,12 +300,14 @@ int skv_q_append(void* k, void* k_scale, void* v, void* v_scale, const void* k_n
                  int block_size, int B, int H_kv, int D, int T_cap, int fmt, int in_dt,
                  skv_stream_t stream);
 
-/* skv_append_chunk for a block-scaled cache: rows i < n_new[b] (NULL: C) of
- * k_new[b], [B, C, H_kv, D] of in_dt, to positions lens[b] + i; rows past the
- * capacity are not written, lens is not advanced. Paged caches too. */
+/* skv_append_chunk for a block-scaled cache: rows i < n[b] of k_new[b], [B, C,
+ * H_kv, D] of in_dt, to positions lens[b] + i; rows past the capacity are not
+ * written. n: n_new, or n_host (a host array, each entry in [0, C], read when
+ * the call returns), or C with both NULL. advance != 0: then the fills advanced
+ * as skv_advance does. Paged caches too. */
 int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale, const void* k_new,
-                       const void* v_new, const int32_t* lens, const int32_t* n_new,
-                       const int32_t* block_table, int max_blocks, int block_size, int B, int C,
+                       const void* v_new, int32_t* lens, const int32_t* n_new,
+                       const int32_t* n_host /* host */, int advance, const int32_t* block_table, int max_blocks, int block_size, int B, int C,
                        int H_kv, int D, int T_cap, int fmt, int in_dt, skv_stream_t stream);
 
 /* Rows back: k_out[b, i], v_out[b, i] ([B, C, H_kv, D] of out_dt, exact in
@@ -353,16 +355,18 @@ int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scale, void* v,
 /* skv_append_prefill_attn for a block-scaled cache (contiguous or paged):
  * skv_q_append_chunk, causal attention of the chunk's queries over prefix +
  * chunk, and the fills advanced, in one call. q, out [B, C, H_q, D] of q_dt /
- * out_dt; H_q / H_kv in {1, 2, 4, 8}; n_splits and ws as in skv_prefill_attn
- * (skv_prefill_plan, skv_prefill_workspace_bytes). Q and the probabilities
+ * out_dt; H_q / H_kv in {1, 2, 4, 8}; n_new and n_host as in
+ * skv_q_append_chunk; n_splits and ws as in skv_prefill_attn (skv_prefill_plan,
+ * skv_prefill_workspace_bytes), and with n_host B int32 more. Q and the probabilities
  * enter the matrix cores as bf16, K and V exactly, as over a bf16 cache that
  * holds the same values. */
 int skv_q_append_prefill_attn(void* out, const void* q, void* k, void* k_scale, void* v,
                               void* v_scale, const void* k_new, const void* v_new, int32_t* lens,
-                              const int32_t* n_new, const int32_t* block_table, int max_blocks,
-                              int block_size, int B, int C, int H_q, int H_kv, int D, int T_cap,
-                              float scale, int n_splits, void* ws, size_t ws_bytes, int fmt,
-                              int in_dt, int q_dt, int out_dt, skv_stream_t stream);
+                              const int32_t* n_new, const int32_t* n_host /* host */,
+                              const int32_t* block_table, int max_blocks, int block_size, int B,
+                              int C, int H_q, int H_kv, int D, int T_cap, float scale,
+                              int n_splits, void* ws, size_t ws_bytes, int fmt, int in_dt,
+                              int q_dt, int out_dt, skv_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Decode-step ops of the model around the cache (fp32). They replace the

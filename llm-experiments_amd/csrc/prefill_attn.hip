@@ -1069,22 +1069,37 @@ extern "C" int skv_append_prefill_attn(void* out, const void* q, void* k_cache, 
 extern "C" int skv_q_append_prefill_attn(void* out, const void* q, void* k, void* k_scale, void* v,
                                          void* v_scale, const void* k_new, const void* v_new,
                                          int32_t* lens, const int32_t* n_new,
-                                         const int32_t* block_table, int max_blocks,
-                                         int block_size, int B, int C, int H_q, int H_kv, int D,
-                                         int T_cap, float scale, int n_splits, void* ws,
-                                         size_t ws_bytes, int fmt, int in_dt, int q_dt, int out_dt,
-                                         skv_stream_t stream) {
+                                         const int32_t* n_host, const int32_t* block_table,
+                                         int max_blocks, int block_size, int B, int C, int H_q,
+                                         int H_kv, int D, int T_cap, float scale, int n_splits,
+                                         void* ws, size_t ws_bytes, int fmt, int in_dt, int q_dt,
+                                         int out_dt, skv_stream_t stream) {
   const char* fn = "skv_q_append_prefill_attn";
   quant::Cache c;
   int rc = quant_cache_args(&c, k, k_scale, v, v_scale, block_table, max_blocks, block_size, B,
                             H_kv, D, T_cap, fmt, fn);
   if (rc) return rc;
-  // every check of the attention first, so that a rejected call changes nothing
+  // every check first, so that a rejected call changes nothing
+  SKV_REQUIRE(k_new && v_new && dt_ok(in_dt) && (((uintptr_t)k_new | (uintptr_t)v_new) & 15) == 0,
+              SKV_E_INVALID, "%s: k_new and v_new: null, misaligned or of a bad dtype", fn);
+  SKV_REQUIRE(!n_new || !n_host, SKV_E_INVALID, "%s: counts on the device or the host", fn);
+  for (int b = 0; n_host && b < B; ++b)
+    SKV_REQUIRE(n_host[b] >= 0 && n_host[b] <= C, SKV_E_INVALID, "%s: n_host[%d]=%d outside [0, %d]",
+                fn, b, n_host[b], C);
+  int32_t* n_copy = nullptr;
+  if (n_host) {  // the append leaves the host's counts behind the attention's workspace
+    const size_t at = skv_prefill_workspace_bytes(B, C, H_q, D, n_splits);
+    SKV_REQUIRE(ws && ws_bytes >= at + (size_t)B * sizeof(int32_t), SKV_E_WORKSPACE,
+                "%s: workspace %zu bytes < %zu required", fn, ws_bytes,
+                at + (size_t)B * sizeof(int32_t));
+    n_copy = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + at);
+    n_new = n_copy;
+  }
   rc = prefill_attn_impl(out, q, k, v, lens, n_new, B, C, H_q, H_kv, D, c.cap, scale, n_splits, ws,
                          ws_bytes, fmt, q_dt, out_dt, stream, fn, lens, false, &c);
   if (rc) return rc;
-  rc = skv_q_append_chunk(k, k_scale, v, v_scale, k_new, v_new, lens, n_new, block_table,
-                          max_blocks, block_size, B, C, H_kv, D, T_cap, fmt, in_dt, stream);
+  rc = quant_append_chunk(c, fmt, k_new, v_new, lens, n_host ? nullptr : n_new, n_host, n_copy, B, C,
+                          in_dt, (hipStream_t)stream, fn);
   if (rc) return rc;
   rc = prefill_attn_impl(out, q, k, v, lens, n_new, B, C, H_q, H_kv, D, c.cap, scale, n_splits, ws,
                          ws_bytes, fmt, q_dt, out_dt, stream, fn, lens, true, &c);

@@ -179,9 +179,22 @@ __device__ __forceinline__ void store8(uint8_t* codes, uint8_t* scales, size_t r
   if ((o & 3) == 0) scales[row * (size_t)(D / kGroup) + (o >> 2)] = (uint8_t)byte;
 }
 
+// Small host integers, one a sequence, as a kernel argument: no copy to the
+// device, which would be a launch of its own (or hold the host until it landed).
+constexpr int kInts = 256;
+struct Ints {
+  int32_t v[kInts];
+};
+
 }  // namespace quant
 
 // ---- host ----
+
+// skv_q_append_chunk's kernel with the counts on the device (n_new), on the host
+// (n_host; copied to n_copy on the way unless that is NULL) or neither.
+int quant_append_chunk(const quant::Cache& c, int fmt, const void* k_new, const void* v_new,
+                       const int32_t* lens, const int32_t* n_new, const int32_t* n_host,
+                       int32_t* n_copy, int B, int C, int in_dt, hipStream_t s, const char* fn);
 
 // Whether fmt is a block-scaled format.
 inline bool is_quant(int fmt) { return fmt == SKV_MXFP4 || fmt == SKV_MXFP8; }

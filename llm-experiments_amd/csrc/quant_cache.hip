@@ -9,6 +9,8 @@
 // bf16, 32 of fp32, against 4 or 8 of codes and a quarter of a scale byte),
 // and the group's maximum is two DPP steps over the quad of lanes that holds
 // it. No LDS, no second pass over the input.
+#include <cstring>
+
 #include "quant.h"
 
 namespace skv {
@@ -52,16 +54,22 @@ __host__ __device__ __forceinline__ int tokens_per_wg(int D) { return 256 / (D /
 // faster: 4 x 8192 x 16 x 128 back to bf16 60 us against 57.)
 constexpr int kRuns = 4;
 
-// Chunk append, grid (token tiles, H_kv, B). Row i < n_new[b] goes to position
-// lens[b] + i; lens is read only. The input is loaded before the fill is known
+// Chunk append, grid (token tiles, H_kv, sequences b0 ..). Row i < n goes to
+// position lens[b] + i, n being n_new[b], or without n_new the host's count
+// (HOST; the first workgroup of a sequence stores it in n_copy[b] for the
+// kernels behind this one), or C; lens is read only. The input is loaded before the fill is known
 // (its place depends on neither): one round trip to memory, not two (4 x 2048
 // x 16 x 128 bf16 into 4 bits: 18.8 us with the fill first and one run).
-template <int BITS, bool PAGED, int RUNS>
+struct NoInts {};
+template <int BITS, bool PAGED, int RUNS, typename HOST>
 __global__ __launch_bounds__(256) void k_q_append_chunk(Cache c, const void* __restrict__ kn,
                                                         const void* __restrict__ vn, int in_dt,
                                                         const int32_t* __restrict__ lens,
-                                                        const int32_t* __restrict__ n_new, int C) {
-  const int b = blockIdx.z, h = blockIdx.y;
+                                                        const int32_t* __restrict__ n_new,
+                                                        HOST n_host, int32_t* __restrict__ n_copy,
+                                                        int b0, int C) {
+  constexpr bool kHost = sizeof(HOST) == sizeof(Ints);
+  const int b = b0 + blockIdx.z, h = blockIdx.y;
   const int opr = c.D / 8, tpw = tokens_per_wg(c.D);
   const int r = threadIdx.x / opr, o = threadIdx.x - r * opr;
   if (r >= tpw) return;  // whole quads: opr % 4 == 0
@@ -74,7 +82,13 @@ __global__ __launch_bounds__(256) void k_q_append_chunk(Cache c, const void* __r
     load8_f32(kn, src, in_dt, xk[u]);
     load8_f32(vn, src, in_dt, xv[u]);
   }
-  const int n = n_new ? min(n_new[b], C) : C;
+  int n = C;
+  if constexpr (kHost) {
+    n = n_host.v[blockIdx.z];
+    if (n_copy != nullptr && blockIdx.x == 0 && h == 0 && threadIdx.x == 0) n_copy[b] = n;
+  } else if (n_new) {
+    n = min(n_new[b], C);
+  }
   const int p0 = lens[b];
 #pragma unroll
   for (int u = 0; u < RUNS; ++u) {
@@ -129,19 +143,19 @@ struct Piece {
   }
 };
 
-// First positions of a read, as a kernel argument: no copy to the device, which
-// would be a launch of its own (or hold the host until it landed).
-constexpr int kStarts = 256;
-struct Starts {
-  int32_t v[kStarts];
-};
+// lens[b] advanced by the host's counts, as skv_advance.
+__global__ __launch_bounds__(kInts) void k_q_advance(int32_t* __restrict__ lens, Ints n, int b0,
+                                                     int nb, int cap) {
+  const int i = threadIdx.x;
+  if (i < nb) lens[b0 + i] = min(lens[b0 + i] + n.v[i], cap);
+}
 
 // Rows back, grid (token tiles, H_kv, sequences b0 ..): row i is position
 // start.v[b - b0] + i, or zeros outside [0, fill).
 template <int BITS, bool PAGED, int RUNS, int OUT>
 __global__ __launch_bounds__(256) void k_q_read(Cache c, void* __restrict__ ko,
                                                 void* __restrict__ vo,
-                                                const int32_t* __restrict__ lens, Starts start,
+                                                const int32_t* __restrict__ lens, Ints start,
                                                 int b0, int C) {
   using P = Piece<BITS, OUT>;
   const int b = b0 + blockIdx.z, h = blockIdx.y;
@@ -265,11 +279,43 @@ extern "C" int skv_q_append(void* k, void* k_scale, void* v, void* v_scale, cons
   return check_launch(fn);
 }
 
+int skv::quant_append_chunk(const quant::Cache& c, int fmt, const void* k_new, const void* v_new,
+                            const int32_t* lens, const int32_t* n_new, const int32_t* n_host,
+                            int32_t* n_copy, int B, int C, int in_dt, hipStream_t s,
+                            const char* fn) {
+  const bool runs = long_call(B, c.Hkv, C, c.D);
+  const int tpw = tokens_per_wg(c.D) * (runs ? kRuns : 1);
+  for (int b0 = 0; b0 < B; b0 += n_host ? kInts : B) {
+    const int nb = n_host && B - b0 > kInts ? kInts : B - b0;
+    const dim3 grid((unsigned)(((long)C + tpw - 1) / tpw), c.Hkv, nb);
+    Ints cnt;
+    if (n_host) memcpy(cnt.v, n_host + b0, (size_t)nb * sizeof(int32_t));
+#define SKV_CHUNK(BITS, PAGED, RUNS, COUNTS)                                                   \
+  hipLaunchKernelGGL((k_q_append_chunk<BITS, PAGED, RUNS, decltype(COUNTS)>), grid, dim3(256), 0, \
+                     s, c, k_new, v_new, in_dt, lens, n_new, COUNTS, n_copy, b0, C)
+#define SKV_LAUNCH(BITS, PAGED)                                  \
+  do {                                                           \
+    if (n_host) {                                                \
+      if (runs) SKV_CHUNK(BITS, PAGED, kRuns, cnt);              \
+      else SKV_CHUNK(BITS, PAGED, 1, cnt);                       \
+    } else {                                                     \
+      if (runs) SKV_CHUNK(BITS, PAGED, kRuns, NoInts{});         \
+      else SKV_CHUNK(BITS, PAGED, 1, NoInts{});                  \
+    }                                                            \
+  } while (0)
+    SKV_Q_CASES(SKV_LAUNCH);
+#undef SKV_LAUNCH
+#undef SKV_CHUNK
+  }
+  return check_launch(fn);
+}
+
 extern "C" int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale,
-                                  const void* k_new, const void* v_new, const int32_t* lens,
-                                  const int32_t* n_new, const int32_t* block_table,
-                                  int max_blocks, int block_size, int B, int C, int H_kv, int D,
-                                  int T_cap, int fmt, int in_dt, skv_stream_t stream) {
+                                  const void* k_new, const void* v_new, int32_t* lens,
+                                  const int32_t* n_new, const int32_t* n_host, int advance,
+                                  const int32_t* block_table, int max_blocks, int block_size,
+                                  int B, int C, int H_kv, int D, int T_cap, int fmt, int in_dt,
+                                  skv_stream_t stream) {
   const char* fn = "skv_q_append_chunk";
   quant::Cache c;
   int rc = quant_cache_args(&c, k, k_scale, v, v_scale, block_table, max_blocks, block_size, B,
@@ -279,20 +325,20 @@ extern "C" int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale
   SKV_REQUIRE(dt_ok(in_dt), SKV_E_INVALID, "%s: bad dtype", fn);
   SKV_REQUIRE(aligned16(k_new) && aligned16(v_new), SKV_E_INVALID,
               "%s: k_new and v_new must be 16-byte aligned", fn);
-  const bool runs = long_call(B, H_kv, C, D);
-  const int tpw = tokens_per_wg(D) * (runs ? kRuns : 1);
-  const dim3 grid((unsigned)(((long)C + tpw - 1) / tpw), H_kv, B);
-#define SKV_LAUNCH(BITS, PAGED)                                                                \
-  do {                                                                                         \
-    if (runs)                                                                                  \
-      hipLaunchKernelGGL((k_q_append_chunk<BITS, PAGED, kRuns>), grid, dim3(256), 0,           \
-                         (hipStream_t)stream, c, k_new, v_new, in_dt, lens, n_new, C);         \
-    else                                                                                       \
-      hipLaunchKernelGGL((k_q_append_chunk<BITS, PAGED, 1>), grid, dim3(256), 0,               \
-                         (hipStream_t)stream, c, k_new, v_new, in_dt, lens, n_new, C);         \
-  } while (0)
-  SKV_Q_CASES(SKV_LAUNCH);
-#undef SKV_LAUNCH
+  SKV_REQUIRE(!n_new || !n_host, SKV_E_INVALID, "%s: counts on the device or the host", fn);
+  for (int b = 0; n_host && b < B; ++b)
+    SKV_REQUIRE(n_host[b] >= 0 && n_host[b] <= C, SKV_E_INVALID, "%s: n_host[%d]=%d outside [0, %d]",
+                fn, b, n_host[b], C);
+  hipStream_t s = (hipStream_t)stream;
+  rc = quant_append_chunk(c, fmt, k_new, v_new, lens, n_new, n_host, nullptr, B, C, in_dt, s, fn);
+  if (rc || !advance) return rc;
+  if (!n_host) return skv_advance(lens, n_new, C, B, c.cap, stream);
+  for (int b0 = 0; b0 < B; b0 += kInts) {
+    const int nb = B - b0 < kInts ? B - b0 : kInts;
+    Ints cnt;
+    memcpy(cnt.v, n_host + b0, (size_t)nb * sizeof(int32_t));
+    hipLaunchKernelGGL(k_q_advance, dim3(1), dim3(kInts), 0, s, lens, cnt, b0, nb, c.cap);
+  }
   return check_launch(fn);
 }
 
@@ -314,9 +360,9 @@ extern "C" int skv_q_read(void* k_out, void* v_out, const void* k, const void* k
               "%s: k_out and v_out must be 16-byte aligned", fn);
   const bool runs = long_call(B, H_kv, C, D);
   const int tpw = 256 / (D / (out_dt == SKV_BF16 ? 8 : 4)) * (runs ? kRuns : 1);
-  for (int b0 = 0; b0 < B; b0 += kStarts) {
-    const int nb = B - b0 < kStarts ? B - b0 : kStarts;
-    Starts st;
+  for (int b0 = 0; b0 < B; b0 += kInts) {
+    const int nb = B - b0 < kInts ? B - b0 : kInts;
+    Ints st;
     for (int i = 0; i < nb; ++i) st.v[i] = start[n_start == 1 ? 0 : b0 + i];
     const dim3 grid((unsigned)(((long)C + tpw - 1) / tpw), H_kv, nb);
 #define SKV_READ(BITS, PAGED, RUNS, OUT)                                                      \

@@ -47,8 +47,8 @@ _SIGNATURES = {
     "skv_append_prefill_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
                                      _F, _I, _P, _Z, _I, _I, _I, _I, _P]),
     "skv_q_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
-    "skv_q_append_chunk": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
-                                _I, _I, _P]),
+    "skv_q_append_chunk": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I,
+                                _I, _I, _I, _I, _P]),
     "skv_q_read": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I,
                         _I, _P]),
     "skv_q_decode_plan": (_I, [_I, _I, _I, _I, _I, _I, _I, _I, ctypes.c_longlong, _I, _I,
@@ -56,7 +56,7 @@ _SIGNATURES = {
     "skv_q_decode_workspace_bytes": (_Z, [_I, _I, _I, _I]),
     "skv_q_decode_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                _F, _I, _I, _I, _P, _Z, _I, _I, _I, _I, _P]),
-    "skv_q_append_prefill_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I,
+    "skv_q_append_prefill_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I,
                                        _I, _I, _I, _I, _F, _I, _P, _Z, _I, _I, _I, _I, _P]),
     "skv_embed": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "skv_layernorm": (_I, [_P, _P, _P, _P, _I, _I, _F, _P]),
@@ -189,6 +189,11 @@ def upload_i32(values: np.ndarray, device: torch.device, stream: int) -> torch.T
     check(lib().skv_upload_i32(out.data_ptr(), host.ctypes.data, host.size, stream),
           "skv_upload_i32")
     return out
+
+
+def host_ptr(a: np.ndarray) -> int:
+    """Address of a host array's data, for calls that read it before they return."""
+    return a.__array_interface__["data"][0]
 
 
 def ptr(t: torch.Tensor) -> int:

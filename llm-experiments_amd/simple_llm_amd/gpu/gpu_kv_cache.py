@@ -717,12 +717,15 @@ def kv_cache_read(ctx: GPUContext, cache: KVCache, layer_idx: int, k_out: torch.
         raise ValueError("k_out and v_out must share shape and dtype")
     if k_out.shape[1] == 0:
         raise ValueError("k_out must hold at least one row per sequence")
-    at = [0] if start is None else np.asarray(start, dtype=np.int64)
-    if start is not None:
-        if at.ndim and at.shape != (B,):
+    if start is None or isinstance(start, int):
+        first = start or 0
+        ok, at = 0 <= first < 2**31, [first]
+    else:
+        at = np.ascontiguousarray(start, dtype=np.int64)  # 1-d at least
+        if at.shape not in ((1,), (B,)):
             raise ValueError(f"start must be one integer or {B} of them, got shape {at.shape}")
-        at = at.tolist() if at.ndim else [int(at)]
-        if min(at) < 0 or max(at) >= 2**31:
-            raise ValueError("start must lie in [0, 2^31)")
+        ok = int(at.view(np.uint64).max()) < 2**31  # (negative ones are past it too)
+    if not ok:
+        raise ValueError("start must lie in [0, 2^31)")
     batch_count(ctx)
-    gpu_kv_quant.read(cache, layer, k_out, v_out, at)
+    gpu_kv_quant.read(cache, layer, k_out, v_out, np.array(at, np.int32))

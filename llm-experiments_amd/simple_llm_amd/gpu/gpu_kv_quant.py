@@ -87,13 +87,13 @@ def append(cache: KVCache, layer: KVCacheLayer, k: torch.Tensor, v: torch.Tensor
 
 
 def read(cache: KVCache, layer: KVCacheLayer, k_out: torch.Tensor, v_out: torch.Tensor,
-         start: list) -> None:
-    """start: first positions, one for every sequence or one for all."""
+         start: np.ndarray) -> None:
+    """start: first positions (int32), one for every sequence or one for all."""
     dev = layer.lens.device
-    at = (ctypes.c_int * len(start))(*start)
     with _on(dev):
         rc = _lib.lib().skv_q_read(k_out.data_ptr(), v_out.data_ptr(), *_storage(layer),
-                                   layer.lens.data_ptr(), at, len(start), *_pages(cache),
+                                   layer.lens.data_ptr(), _lib.host_ptr(start), start.size,
+                                   *_pages(cache),
                                    cache.batch_size, k_out.shape[1], cache.n_kv_heads,
                                    cache.head_dim, cache.max_seq_len,
                                    _lib.QUANT_FORMATS[cache.dtype], _lib.dtype_code(k_out.dtype),
@@ -161,33 +161,29 @@ def prefill(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, new_k: torch.T
     B, Hq, Hkv, D = cache.batch_size, cache.n_heads, cache.n_kv_heads, cache.head_dim
     C = int(new_k.shape[1])
     fmt, idt = _lib.QUANT_FORMATS[cache.dtype], _lib.dtype_code(new_k.dtype)
-    table, max_blocks, page = _pages(cache)
-    cap = max_blocks * page if table is not None else cache.max_seq_len
+    n_host = None if counts is None else np.ascontiguousarray(counts, np.int32)
+    n_ptr = None if counts is None else _lib.host_ptr(n_host)
     with _on(dev):
         stream = _lib.stream_handle(dev)
-        n_dev = None
-        if counts is not None:
-            n_dev = _lib.upload_i32(counts, dev, stream)
-        n_ptr = n_dev.data_ptr() if n_dev is not None else None
         if q is None:
             rc = L.skv_q_append_chunk(*_storage(layer), new_k.data_ptr(), new_v.data_ptr(),
-                                      layer.lens.data_ptr(), n_ptr, table, max_blocks, page, B, C,
+                                      layer.lens.data_ptr(), None, n_ptr, 1, *_pages(cache), B, C,
                                       Hkv, D, cache.max_seq_len, fmt, idt, stream)
             _lib.check(rc, "skv_q_append_chunk")
-            rc = L.skv_advance(layer.lens.data_ptr(), n_ptr, C, B, cap, stream)
-            _lib.check(rc, "skv_advance")
             return
         ns = ctypes.c_int(int(n_splits))
         if n_splits <= 0:
             _lib.check(L.skv_prefill_plan(B, C, Hq, Hkv, max(max_end, 1), ctypes.byref(ns)),
                        "skv_prefill_plan")
         need = int(L.skv_prefill_workspace_bytes(B, C, Hq, D, ns.value))
+        if counts is not None:
+            need += 4 * B
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
         rc = L.skv_q_append_prefill_attn(out.data_ptr(), q.data_ptr(), *_storage(layer),
                                          new_k.data_ptr(), new_v.data_ptr(),
-                                         layer.lens.data_ptr(), n_ptr, table, max_blocks, page, B,
-                                         C, Hq, Hkv, D, cache.max_seq_len, sc, ns.value,
+                                         layer.lens.data_ptr(), None, n_ptr, *_pages(cache), B, C,
+                                         Hq, Hkv, D, cache.max_seq_len, sc, ns.value,
                                          ws.data_ptr() if ws is not None else None, need, fmt, idt,
                                          _lib.dtype_code(q.dtype), _lib.dtype_code(out.dtype),
                                          stream)

@@ -135,6 +135,7 @@ def test_model_refuses_a_block_scaled_cache():
 # ---- C refusals ------------------------------------------------------------
 
 START = (ctypes.c_int * 2)()
+TOO_MANY, NEGATIVE = (ctypes.c_int * 2)(1, 4), (ctypes.c_int * 2)(-1, 2)
 FAKE = 4096  # never dereferenced: each call below fails validation first
 BASE = dict(k=FAKE, ks=FAKE, v=FAKE, vs=FAKE, bt=None, mb=0, bs=0, B=2, Hq=8, H=4, D=64, T=128,
             fmt=_lib.MXFP4, idt=0, qdt=0, odt=0, C=3, new=FAKE, lens=FAKE, q=FAKE, out=FAKE,
@@ -151,8 +152,9 @@ def _call(which, **kw):
         return L.skv_q_append(*st, a["new"], a["new"], a["lens"], *pg, a["B"], a["H"], a["D"],
                               a["T"], a["fmt"], a["idt"], None)
     if which == "chunk":
-        return L.skv_q_append_chunk(*st, a["new"], a["new"], a["lens"], None, *pg, a["B"], a["C"],
-                                    a["H"], a["D"], a["T"], a["fmt"], a["idt"], None)
+        return L.skv_q_append_chunk(*st, a["new"], a["new"], a["lens"], kw.get("n_new"),
+                                    kw.get("n_host"), 1, *pg, a["B"], a["C"], a["H"], a["D"],
+                                    a["T"], a["fmt"], a["idt"], None)
     if which == "read":
         return L.skv_q_read(a["out"], a["out"], *st, a["lens"], kw.get("start", START),
                             a.get("n_start", 2), *pg, a["B"], a["C"], a["H"], a["D"], a["T"], a["fmt"], a["odt"], None)
@@ -165,10 +167,10 @@ def _call(which, **kw):
                                    a["idt"], a["qdt"], a["odt"], None)
     if nb is None:
         nb = L.skv_prefill_workspace_bytes(a["B"], a["C"], a["Hq"], a["D"], a["splits"])
-    return L.skv_q_append_prefill_attn(a["out"], a["q"], *st, a["new"], a["new"], a["lens"], None,
-                                       *pg, a["B"], a["C"], a["Hq"], a["H"], a["D"], a["T"],
-                                       a["scale"], a["splits"], a["ws"], nb, a["fmt"], a["idt"],
-                                       a["qdt"], a["odt"], None)
+    return L.skv_q_append_prefill_attn(a["out"], a["q"], *st, a["new"], a["new"], a["lens"],
+                                       kw.get("n_new"), kw.get("n_host"), *pg, a["B"], a["C"],
+                                       a["Hq"], a["H"], a["D"], a["T"], a["scale"], a["splits"],
+                                       a["ws"], nb, a["fmt"], a["idt"], a["qdt"], a["odt"], None)
 
 
 INV, UNS, WSP = _lib.SKV_E_INVALID, _lib.SKV_E_UNSUPPORTED, _lib.SKV_E_WORKSPACE
@@ -201,7 +203,11 @@ def test_cache_arguments_refused(which, kw, rc):
     ("decode", dict(ws=None), WSP), ("decode", dict(chunk=1 << 30, n=4), UNS),
     ("decode", dict(wg=1), INV), ("decode", dict(wg=5), INV), ("decode", dict(B=300, wg=599), INV),
     ("decode", dict(B=300, n=300, wg=90000), UNS),
-    ("prefill", dict(C=0), INV), ("prefill", dict(q=None), INV), ("prefill", dict(Hq=12), UNS),
+    ("chunk", dict(n_host=TOO_MANY), INV), ("chunk", dict(n_host=NEGATIVE), INV),
+    ("chunk", dict(n_host=START, n_new=FAKE), INV), ("prefill", dict(n_host=TOO_MANY), INV),
+    ("prefill", dict(n_host=START, n_new=FAKE), INV), ("prefill", dict(n_host=START, nb=4), WSP),
+    ("prefill", dict(new=None), INV), ("prefill", dict(new=FAKE + 8), INV),
+    ("prefill", dict(idt=2), INV), ("prefill", dict(C=0), INV), ("prefill", dict(q=None), INV), ("prefill", dict(Hq=12), UNS),
     ("prefill", dict(Hq=10), INV), ("prefill", dict(qdt=2), INV), ("prefill", dict(scale=0.0), INV),
     ("prefill", dict(splits=0), INV), ("prefill", dict(splits=33), INV),
     ("prefill", dict(splits=2, nb=16), WSP)])
@@ -243,3 +249,23 @@ def test_decode_plan_refuses():
     assert L.skv_q_decode_plan(1, 2, 1, 64, _lib.MXFP4, 0, 0, 9, 0, 0, 0, None, *out[1:]) == INV
     assert L.skv_q_decode_workspace_bytes(2, 8, 64, 3) == 2 * 8 * 3 * 68 * 4
     assert L.skv_q_decode_workspace_bytes(0, 8, 64, 3) == 0
+
+
+def test_read_refuses_bad_starts(monkeypatch):
+    """Before any device work; the tensor checks are stubbed out (no GPU here)."""
+    from simple_llm_amd.gpu import gpu_kv_cache as gk
+
+    ctx = _ctx()
+    cache = gpu.kv_cache_create(ctx, gpu.KVCacheConfig(2, 8, 1, 4, 64, dtype=FP8))
+    rows = torch.zeros(2, 3, 4, 64)
+    monkeypatch.setattr(gk, "_check_tensor", lambda *a: None)
+    seen = []
+    monkeypatch.setattr(gk.gpu_kv_quant, "read", lambda c, l, k, v, at: seen.append(at.tolist()))
+    for bad in (-1, 2**31, [0, -1], np.array([2**31, 0]), [1, 2, 3], np.zeros((2, 1))):
+        with pytest.raises(ValueError, match="start must"):
+            gpu.kv_cache_read(ctx, cache, 0, rows, rows, start=bad)
+    for good in (None, 5, np.int64(5), [1, 2], np.array([3, 4]), [7]):
+        gpu.kv_cache_read(ctx, cache, 0, rows, rows, start=good)
+    assert seen == [[0], [5], [5], [1, 2], [3, 4], [7]]
+    with pytest.raises(ValueError, match="at least one row"):
+        gpu.kv_cache_read(ctx, cache, 0, rows[:, :0], rows[:, :0])
