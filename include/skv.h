@@ -337,7 +337,8 @@ int skv_q_decode_plan(int B, int H_q, int H_kv, int D, int fmt, int q_dt, int ou
 size_t skv_q_decode_workspace_bytes(int B, int H_q, int D, int n_chunks);
 
 /* skv_decode_attn over a block-scaled cache: q, out [B, H_q, D] of q_dt /
- * out_dt, G = H_q / H_kv from 1 to 16. lens[b] == 0 gives zeros. Products are
+ * out_dt, G = H_q / H_kv from 1 to 16, any finite scale. lens[b] == 0 gives
+ * zeros. Products are
  * of fp32 accuracy where q or out is fp32; with both bf16, K, V and q are
  * exact and the probabilities carry 17 bits. A sequence longer than
  * chunk_tokens * n_chunks, or whose chunks do not fit in n_wg workgroups (in

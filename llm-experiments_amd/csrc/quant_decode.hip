@@ -28,6 +28,9 @@
 //    eight tokens of a lane would have eight), row-major with XOR-swizzled
 //    16-byte chunks, and comes back transposed (ds_read_b64_tr_b16). The
 //    probabilities are already in the operand's token order.
+//    (The scaled f8f6f4 product takes 4- and 8-bit codes unconverted, against q
+//    as two E4M3 parts: 1 to 2 % faster, but its sums carry fewer bits, and
+//    outputs moved by about 2^-15 where these move by 2^-19: not taken.)
 // Precision: K and V enter exactly. With fp32 in or out, q and p are three bf16
 // parts (all bits of q, 2^-24 of p); with bf16 in and out q is one part and p
 // two (2^-17). The parts use the matrix core's columns that few heads leave
@@ -42,6 +45,8 @@
 // the fill is touched, none of it meets a zero weight.
 // No atomics: results are bitwise reproducible, and a paged cache gives the
 // bits of the same rows in a contiguous one.
+#include <cmath>
+
 #include "quant.h"
 
 namespace skv {
@@ -153,10 +158,14 @@ __device__ __forceinline__ float slot_part(float x, const float (&f)[3]) {
 
 // x + the same head's values of the other slots, the same bits in each (SL
 // slots of 16 / SL columns; rotations within the 16-lane row).
+template <int CTRL>
+__device__ __forceinline__ float ror(float x) {  // every lane has a source: part of the add
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
+}
 template <int SL>
 __device__ __forceinline__ float slot_sum(float x) {
-  if constexpr (SL >= 2) x += dpp<0x128>(x);  // row_ror:8
-  if constexpr (SL >= 4) x += dpp<0x124>(x);  // row_ror:4
+  if constexpr (SL >= 2) x += ror<0x128>(x);  // row_ror:8
+  if constexpr (SL >= 4) x += ror<0x124>(x);  // row_ror:4
   return x;
 }
 
@@ -780,6 +789,7 @@ extern "C" int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scal
               SKV_E_INVALID, "%s: out, q, ws, new_k and new_v must be 16-byte aligned", fn);
   SKV_REQUIRE(H_q > 0 && H_q % H_kv == 0, SKV_E_INVALID, "%s: H_q=%d not a multiple of H_kv=%d",
               fn, H_q, H_kv);
+  SKV_REQUIRE(std::isfinite(scale), SKV_E_INVALID, "%s: scale must be finite", fn);
   SKV_REQUIRE(H_q / H_kv <= kMaxG, SKV_E_UNSUPPORTED,
               "%s: %d query heads per kv head (block-scaled caches take up to %d)", fn, H_q / H_kv,
               kMaxG);

@@ -327,6 +327,115 @@ def test_update_and_attention_of_the_reference(gpu_ctx):
         gpu.kv_cache_update(gpu_ctx, cache, 0, bk, bv)
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_scales_of_any_sign(gpu_ctx, scale):
+    banner(f"quant decode scale {scale}")
+    rng = np.random.default_rng(17)
+    B, H, G, D = 2, 2, 2, 64
+    gpu, cache, m = _make(gpu_ctx, B, 260, H, G, D, "fp8")
+    _fill(gpu, gpu_ctx, cache, m, rng, [257, 40])
+    q = _dev(rng.standard_normal((B, H * G, D)).astype(np.float32), F32)
+    out = torch.empty_like(q)
+    gpu.decode_attention(gpu_ctx, cache, 0, q, out, scale=scale)
+    got = _np(out)
+    for b in range(B):
+        n = int(m.lens[b])
+        for h in range(H * G):
+            want, mag, big = qo.attention(_np(q)[b, h][None], m.k[b, :n, h // G],
+                                          m.v[b, :n, h // G], scale, np.array([n - 1]))
+            big = abs(big[0])  # (the oracle's bound carries the scale's sign)
+            tol = 2 * (D + 8) * U * max(big, 0.0) + (n / 16 + 64) * U
+            assert (np.abs(got[b, h] - want[0]) <= tol * mag[0] + 1e-37).all()
+
+
+def test_empty_cache_gives_zeros(gpu_ctx):
+    banner("quant decode of nothing")
+    for page in (0, 16):
+        gpu, cache, m = _make(gpu_ctx, 3, 300, 2, 4, 128, "fp4", page)
+        for kw in ({}, {"max_len": 300}):
+            out = torch.full((3, 8, 128), 5.0, device="cuda:0")
+            gpu.decode_attention(gpu_ctx, cache, 0, torch.ones_like(out), out, **kw)
+            assert not out.any()
+        out = torch.full((3, 4, 8, 128), 5.0, device="cuda:0")
+        new = torch.ones((3, 4, 2, 128), device="cuda:0")
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, new, new, torch.ones_like(out), out, n_new=[0, 0, 0])
+        assert not out.any() and cache.current_len == 0
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+@pytest.mark.parametrize("page", [0, 8])
+def test_other_rows_stay_as_they_were(gpu_ctx, fmt, page):
+    """Appends write the bytes of their rows and no others; reading and attention none."""
+    banner(f"quant other rows {fmt} page={page}")
+    rng = np.random.default_rng(23)
+    B, T, H, G, D, C = 3, 40, 3, 2, 96, 9
+    gpu, cache, m = _make(gpu_ctx, B, T, H, G, D, fmt, page)
+    lay = cache.layers[0]
+    bufs = (lay.k_cache, lay.v_cache, lay.k_scale, lay.v_scale)
+    for t in bufs:
+        t.buffer.fill_(0xA5)
+    written = np.zeros((B, m.cap), bool)
+    lens = np.array([0, 7, T - 3])
+    lay.lens.copy_(torch.from_numpy(lens.astype(np.int32)))
+    lay.host_lens = lens.astype(np.int64)
+
+    def rows(n):
+        return [_dev(_rows(rng, B, n, H, D), F32) for _ in range(2)]
+
+    k, v = rows(C)
+    counts = [C, 4, 2]
+    q, out = (torch.zeros((B, C, H * G, D), dtype=BF16, device="cuda:0") for _ in range(2))
+    gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out, n_new=counts)
+    for b, n in enumerate(counts):
+        written[b, lens[b]:lens[b] + n] = True
+    lens = lens + counts
+    k, v = rows(1)
+    gpu.kv_cache_append(gpu_ctx, cache, 0, k, v)
+    q1, out1 = (torch.zeros((B, H * G, D), device="cuda:0") for _ in range(2))
+    k, v = rows(1)
+    gpu.kv_cache_append_attend(gpu_ctx, cache, 0, k, v, q1, out1)
+    for _ in range(2):
+        for b in range(B):
+            if lens[b] < m.cap:
+                written[b, lens[b]] = True
+                lens[b] += 1
+    gpu.decode_attention(gpu_ctx, cache, 0, q1, out1)
+    gpu.kv_cache_read(gpu_ctx, cache, 0, *(torch.empty((B, T, H, D), device="cuda:0") for _ in "kv"))
+    assert cache.layers[0].lens.cpu().tolist() == lens.tolist()
+    for t in bufs:
+        x = t.buffer.cpu().numpy().reshape(-1, H, page or m.cap, t.shape[1])
+        if page:
+            x = x[cache.block_table.cpu().numpy()].transpose(0, 2, 1, 3, 4)
+            x = x.reshape(B, H, m.cap, -1)
+        untouched = (x == 0xA5).all(-1)  # [B, H, T]
+        assert untouched[~np.repeat(written[:, None], H, 1)].all()
+        assert not untouched[np.repeat(written[:, None], H, 1)].any()
+
+
+def test_refused_calls_change_nothing(gpu_ctx):
+    banner("quant refused calls")
+    gpu, cache, m = _make(gpu_ctx, 2, 20, 1, 3, 64, "fp4")
+    _fill(gpu, gpu_ctx, cache, m, np.random.default_rng(1), [5, 9])
+    kv, q = torch.ones((2, 3, 1, 64), device="cuda:0"), torch.ones((2, 3, 3, 64), device="cuda:0")
+    row, q1 = torch.ones((2, 1, 64), device="cuda:0"), torch.ones((2, 3, 64), device="cuda:0")
+    half = row.half()
+    for call, match in (
+            (lambda: gpu.kv_cache_prefill(gpu_ctx, cache, 0, kv, kv, q, q.clone()), "query heads"),
+            (lambda: gpu.kv_cache_prefill(gpu_ctx, cache, 0, kv, kv, n_new=[1, 4]), "n_new"),
+            (lambda: gpu.kv_cache_prefill(gpu_ctx, cache, 0, kv.repeat(1, 5, 1, 1),
+                                          kv.repeat(1, 5, 1, 1)), "Cache is full"),
+            (lambda: gpu.kv_cache_append(gpu_ctx, cache, 0, half, half), "dtype"),
+            (lambda: gpu.kv_cache_append_attend(gpu_ctx, cache, 0, half, half, q1, q1.clone()), "dtype"),
+            (lambda: gpu.kv_cache_append_attend(gpu_ctx, cache, 0, row, row, q1, q1.clone(),
+                                                max_len=9), "max_len"),
+            (lambda: gpu.decode_attention(gpu_ctx, cache, 0, q1, q1.clone(), max_len=8), "max_len"),
+            (lambda: gpu.decode_attention(gpu_ctx, cache, 0, q1.half(), q1.clone()), "dtype"),
+            (lambda: gpu.kv_cache_read(gpu_ctx, cache, 0, kv, kv.clone(), start=[0, 1, 2]), "start")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    _check_stored(gpu, gpu_ctx, cache, m)
+
+
 def test_page_layout_does_not_change_the_bits(gpu_ctx):
     banner("quant paged against contiguous")
     rng = np.random.default_rng(4)
