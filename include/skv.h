@@ -289,7 +289,8 @@ int skv_append_prefill_attn(void* out, const void* q, void* k_cache, void* v_cac
  * [pages, H_kv, block_size, ...], block_size a power of two, and token t of
  * sequence b is row t % block_size of page block_table[b, t / block_size];
  * T_cap is not used. block_table NULL: contiguous. D: multiples of 32 up to
- * 256. The codes, inputs and outputs are 16-byte aligned.
+ * 256; sequences: up to 65535 of up to 2^30 tokens. The codes, inputs and
+ * outputs are 16-byte aligned.
  * ------------------------------------------------------------------------ */
 
 /* skv_append for a block-scaled cache: row k_new[b] (and v_new[b]), [B, H_kv,
@@ -307,8 +308,9 @@ int skv_q_append(void* k, void* k_scale, void* v, void* v_scale, const void* k_n
  * as skv_advance does. Paged caches too. */
 int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale, const void* k_new,
                        const void* v_new, int32_t* lens, const int32_t* n_new,
-                       const int32_t* n_host /* host */, int advance, const int32_t* block_table, int max_blocks, int block_size, int B, int C,
-                       int H_kv, int D, int T_cap, int fmt, int in_dt, skv_stream_t stream);
+                       const int32_t* n_host /* host */, int advance, const int32_t* block_table,
+                       int max_blocks, int block_size, int B, int C, int H_kv, int D, int T_cap,
+                       int fmt, int in_dt, skv_stream_t stream);
 
 /* Rows back: k_out[b, i], v_out[b, i] ([B, C, H_kv, D] of out_dt, exact in
  * either type) = position start[b] + i, or zeros outside [0, lens[b]). start
@@ -316,8 +318,8 @@ int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale, const voi
  * read when the call returns. */
 int skv_q_read(void* k_out, void* v_out, const void* k, const void* k_scale, const void* v,
                const void* v_scale, const int32_t* lens, const int32_t* start /* host */,
-               int n_start, const int32_t* block_table, int max_blocks, int block_size, int B, int C, int H_kv,
-               int D, int T_cap, int fmt, int out_dt, skv_stream_t stream);
+               int n_start, const int32_t* block_table, int max_blocks, int block_size, int B,
+               int C, int H_kv, int D, int T_cap, int fmt, int out_dt, skv_stream_t stream);
 
 /* Split sizing of skv_q_decode_attn (host-only): chunk_tokens (a multiple of
  * 128) of one kv head per workgroup, n_chunks = ceil(max_len / chunk_tokens)
@@ -338,11 +340,10 @@ size_t skv_q_decode_workspace_bytes(int B, int H_q, int D, int n_chunks);
 
 /* skv_decode_attn over a block-scaled cache: q, out [B, H_q, D] of q_dt /
  * out_dt, G = H_q / H_kv from 1 to 16, any finite scale. lens[b] == 0 gives
- * zeros. Products are
- * of fp32 accuracy where q or out is fp32; with both bf16, K, V and q are
- * exact and the probabilities carry 17 bits. A sequence longer than
- * chunk_tokens * n_chunks, or whose chunks do not fit in n_wg workgroups (in
- * batch order), gets NaN outputs.
+ * zeros. Products are of fp32 accuracy where q or out is fp32; with both bf16,
+ * K, V and q are exact and the probabilities carry 17 bits. A sequence longer
+ * than chunk_tokens * n_chunks, or whose chunks do not fit in n_wg workgroups
+ * (in batch order), gets NaN outputs.
  * new_k, new_v ([B, H_kv, D] of in_dt; both or neither): exactly skv_q_append
  * before the attention, which then covers the new token, with lens advanced
  * after it; the plan covers the lengths after the append. */
@@ -358,9 +359,9 @@ int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scale, void* v,
  * chunk, and the fills advanced, in one call. q, out [B, C, H_q, D] of q_dt /
  * out_dt; H_q / H_kv in {1, 2, 4, 8}; n_new and n_host as in
  * skv_q_append_chunk; n_splits and ws as in skv_prefill_attn (skv_prefill_plan,
- * skv_prefill_workspace_bytes), and with n_host B int32 more. Q and the probabilities
- * enter the matrix cores as bf16, K and V exactly, as over a bf16 cache that
- * holds the same values. */
+ * skv_prefill_workspace_bytes), and with n_host B int32 more. Q and the
+ * probabilities enter the matrix cores as bf16, K and V exactly, as over a bf16
+ * cache that holds the same values. */
 int skv_q_append_prefill_attn(void* out, const void* q, void* k, void* k_scale, void* v,
                               void* v_scale, const void* k_new, const void* v_new, int32_t* lens,
                               const int32_t* n_new, const int32_t* n_host /* host */,

@@ -34,6 +34,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kGroup = 32;  // elements that share a scale
 constexpr int kMaxD = 256;  // largest head dim
+constexpr int kMaxCap = 1 << 30;  // most tokens of a sequence, so that sums with a tile stay ints
 
 // A quantised cache of one layer. Rows are head-major: row (b, h, t) of a
 // contiguous cache is (b * Hkv + h) * T_cap + t, of a paged one

@@ -57,9 +57,10 @@ constexpr int kRuns = 4;
 // Chunk append, grid (token tiles, H_kv, sequences b0 ..). Row i < n goes to
 // position lens[b] + i, n being n_new[b], or without n_new the host's count
 // (HOST; the first workgroup of a sequence stores it in n_copy[b] for the
-// kernels behind this one), or C; lens is read only. The input is loaded before the fill is known
-// (its place depends on neither): one round trip to memory, not two (4 x 2048
-// x 16 x 128 bf16 into 4 bits: 18.8 us with the fill first and one run).
+// kernels behind this one), or C; lens is read only. The input is loaded before
+// the fill is known (its place depends on neither): one round trip to memory,
+// not two (4 x 2048 x 16 x 128 bf16 into 4 bits: 18.8 us with the fill first
+// and one run).
 struct NoInts {};
 template <int BITS, bool PAGED, int RUNS, typename HOST>
 __global__ __launch_bounds__(256) void k_q_append_chunk(Cache c, const void* __restrict__ kn,
@@ -235,6 +236,8 @@ int quant_cache_args(quant::Cache* c, void* k, void* k_scale, void* v, void* v_s
     SKV_REQUIRE(T_cap > 0, SKV_E_INVALID, "%s: T_cap must be > 0", fn);
     c->cap = T_cap;
   }
+  SKV_REQUIRE(c->cap <= quant::kMaxCap, SKV_E_UNSUPPORTED,
+              "%s: a sequence of %d tokens (block-scaled caches take up to 2^30)", fn, c->cap);
   return SKV_OK;
 }
 

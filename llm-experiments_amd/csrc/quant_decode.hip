@@ -754,6 +754,7 @@ extern "C" int skv_q_decode_plan(int B, int H_q, int H_kv, int D, int fmt, int q
   chunk = (chunk + kStep - 1) / kStep * kStep;
   if (chunk < kStep) chunk = kStep;
   if (chunk > most) chunk = most;
+  if (chunk > quant::kMaxCap) chunk = quant::kMaxCap;
   const long long n = (max_len + chunk - 1) / chunk;
   // sum of ceil(len / chunk) <= total / chunk + B
   const long long some = total_len / chunk + B;
@@ -796,7 +797,7 @@ extern "C" int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scal
   SKV_REQUIRE(chunk_tokens > 0 && chunk_tokens % kStep == 0 && n_chunks >= 1, SKV_E_INVALID,
               "%s: chunk_tokens=%d must be a positive multiple of %d, n_chunks=%d positive", fn,
               chunk_tokens, kStep, n_chunks);
-  SKV_REQUIRE((long long)chunk_tokens * n_chunks < (1LL << 31) &&
+  SKV_REQUIRE(chunk_tokens <= quant::kMaxCap && (long long)chunk_tokens * n_chunks < (1LL << 31) &&
                   (long long)B * H_q * n_chunks < (1LL << 31),
               SKV_E_UNSUPPORTED, "%s: plan too large", fn);
   // every chunk of every sequence, unless a batch small enough to be scanned
@@ -833,9 +834,9 @@ extern "C" int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scal
   hipStream_t s = (hipStream_t)stream;
 #define SKV_QD(DD, BB)                                                                          \
   if (DP == DD && bits == BB) {                                                                 \
-    if (!a.c.bt) launch_decode<DD, BB, kContig>(a, f32, s);                \
-    else if (a.c.bs_shift >= 4) launch_decode<DD, BB, kPages16>(a, f32, s); \
-    else launch_decode<DD, BB, kPagesSmall>(a, f32, s);                    \
+    if (!a.c.bt) launch_decode<DD, BB, kContig>(a, f32, s);                                     \
+    else if (a.c.bs_shift >= 4) launch_decode<DD, BB, kPages16>(a, f32, s);                     \
+    else launch_decode<DD, BB, kPagesSmall>(a, f32, s);                                         \
   }
   SKV_QD(32, 4) SKV_QD(64, 4) SKV_QD(128, 4) SKV_QD(256, 4)
   SKV_QD(32, 8) SKV_QD(64, 8) SKV_QD(128, 8) SKV_QD(256, 8)

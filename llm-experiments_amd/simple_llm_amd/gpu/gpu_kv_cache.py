@@ -83,7 +83,9 @@ def kv_cache_create(ctx: GPUContext, config: KVCacheConfig) -> KVCache:
         raise ValueError("dtype must be torch.float32, torch.bfloat16, torch.float4_e2m1fn_x2 or "
                          f"torch.float8_e4m3fn, got {config.dtype}")
     if quant:
-        gpu_kv_quant.check_sizes(config.batch_size, config.n_heads, n_kv, config.head_dim)
+        bs = config.block_size
+        gpu_kv_quant.check_sizes(config.batch_size, config.n_heads, n_kv, config.head_dim,
+                                 -(-config.max_seq_len // bs) * bs if bs > 0 else config.max_seq_len)
 
     e_kv = n_kv * config.head_dim
     B = config.batch_size
@@ -204,7 +206,7 @@ def _launch_append(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, k: torc
         _check_tensor(t, n, dev)
     if k.dtype != v.dtype:
         raise ValueError("new_k and new_v must share a dtype")
-    if cache.quantized:
+    if layer.k_scale is not None:  # block-scaled
         gpu_kv_quant.append(cache, layer, k, v)
         layer.host_lens = np.minimum(layer.host_lens + 1, _capacity(cache))
         return
@@ -403,7 +405,9 @@ def decode_attention(ctx: GPUContext, cache: KVCache, layer_idx: int, q: torch.T
     q, out: contiguous device tensors of [batch_size, n_heads, head_dim]
     elements (float32 or bfloat16). max_len: an upper bound of the fills
     (default: the host mirror's maximum), used to size the split-K grid; the
-    chunk size follows the batch's total fill (host mirror).
+    chunk size follows the batch's total fill (host mirror). A call captured
+    into a graph that is replayed as the fills grow takes the bound of its
+    replays: a sequence that outgrows it comes back as NaN.
     """
     _check_layer(cache, layer_idx)
     layer = cache.layers[layer_idx]
@@ -425,7 +429,7 @@ def decode_attention(ctx: GPUContext, cache: KVCache, layer_idx: int, q: torch.T
     elif max_len < top:
         _check_max_len(max_len, layer.host_lens)  # raises
     # every fill is <= max_len here, so the total needs no clamp
-    if cache.quantized:
+    if layer.k_scale is not None:  # block-scaled
         gpu_kv_quant.attend(ctx, cache, layer, q, out, scale, max_len, total, covering)
         return
     chunk, nchunks = _decode_plan_span(ctx, cache.batch_size, cache.n_heads, cache.n_kv_heads,
@@ -494,7 +498,7 @@ def kv_cache_append_attend(ctx: GPUContext, cache: KVCache, layer_idx: int, new_
         max_len = top
     elif max_len < top:
         _check_max_len(max_len, after)  # raises
-    if cache.quantized:
+    if layer.k_scale is not None:  # block-scaled
         gpu_kv_quant.attend(ctx, cache, layer, q, out, scale, max_len, total, covering, new_k,
                             new_v)
         layer.host_lens = after
@@ -625,7 +629,9 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
             raise ValueError(f"n_new entries must lie in [0, {C}]")
     after = start + n_host
     end = int(after.max())
-    if end > T:
+    # (appends may fill a paged sequence's last page, past max_seq_len; it takes
+    # no chunk then, and is no obstacle to those of others)
+    if end > T and (n_min > 0 or int(after[n_host > 0].max(initial=0)) > T):
         raise ValueError(f"Cache is full: chunk of {int(np.max(n_host))} tokens after "
                          f"current_len={int(start.max())}, max_seq_len={T}")
     want_attn = q is not None

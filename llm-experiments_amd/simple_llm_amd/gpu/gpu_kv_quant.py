@@ -23,11 +23,14 @@ from .gpu_types import GPUBuffer2D, GPUContext, KVCache, KVCacheLayer
 GROUP = 32  # elements that share a scale
 MAX_HEAD_DIM = 256
 MAX_GROUPS = 16  # query heads per kv head
+MAX_TOKENS = 1 << 30  # of a sequence
 
 _BITS = {torch.float4_e2m1fn_x2: 4, torch.float8_e4m3fn: 8}
 
 
-def check_sizes(batch_size: int, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
+def check_sizes(batch_size: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                tokens: int) -> None:
+    """tokens: what a sequence can hold."""
     if head_dim % GROUP or head_dim > MAX_HEAD_DIM:
         raise ValueError(f"head_dim must be a multiple of {GROUP} up to {MAX_HEAD_DIM} in a "
                          f"block-scaled cache, got {head_dim}")
@@ -37,6 +40,9 @@ def check_sizes(batch_size: int, n_heads: int, n_kv_heads: int, head_dim: int) -
     if batch_size > 65535 or n_kv_heads > 65535:
         raise ValueError("a block-scaled cache takes up to 65535 sequences and kv heads, got "
                          f"{batch_size} and {n_kv_heads}")
+    if tokens > MAX_TOKENS:
+        raise ValueError("a block-scaled cache takes sequences of up to 2^30 tokens, got "
+                         f"{tokens}")
 
 
 def create_layer(ctx: GPUContext, batch_size: int, rows: int, head_dim: int,
@@ -93,9 +99,8 @@ def read(cache: KVCache, layer: KVCacheLayer, k_out: torch.Tensor, v_out: torch.
     with _on(dev):
         rc = _lib.lib().skv_q_read(k_out.data_ptr(), v_out.data_ptr(), *_storage(layer),
                                    layer.lens.data_ptr(), _lib.host_ptr(start), start.size,
-                                   *_pages(cache),
-                                   cache.batch_size, k_out.shape[1], cache.n_kv_heads,
-                                   cache.head_dim, cache.max_seq_len,
+                                   *_pages(cache), cache.batch_size, k_out.shape[1],
+                                   cache.n_kv_heads, cache.head_dim, cache.max_seq_len,
                                    _lib.QUANT_FORMATS[cache.dtype], _lib.dtype_code(k_out.dtype),
                                    _lib.stream_handle(dev))
     _lib.check(rc, "skv_q_read")
@@ -124,20 +129,23 @@ def attend(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, q: torch.Tensor
            out: torch.Tensor, scale: Optional[float], max_len: int, total: int, covering: bool,
            new_k: Optional[torch.Tensor] = None, new_v: Optional[torch.Tensor] = None) -> None:
     """decode_attention, after the append of new_k and new_v if given. total: the
-    fills' sum; covering: the call serves any fills up to max_len (a captured
-    one is replayed as they grow), not only those that sum to it."""
+    fills' sum; covering: the call serves any fills up to max_len, not only those
+    that sum to it. A captured call does: it may be replayed with others."""
     dev = layer.lens.device
+    max_len = min(int(max_len), cache.block_table.shape[1] * cache.block_size if cache.paged
+                  else cache.max_seq_len)  # more is workspace that no fill reaches
     L = _lib.lib()
     B, Hq, Hkv, D = cache.batch_size, cache.n_heads, cache.n_kv_heads, cache.head_dim
     qdt, odt = _lib.dtype_code(q.dtype), _lib.dtype_code(out.dtype)
-    chunk, n, n_wg = plan(cache, qdt, odt, int(max_len), total, covering,
-                          int(ctx.config.decode_chunk_tokens))
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     nk = nv = None
     idt = 0
     if new_k is not None:
         nk, nv, idt = new_k.data_ptr(), new_v.data_ptr(), _lib.dtype_code(new_k.dtype)
     with _on(dev):
+        chunk, n, n_wg = plan(cache, qdt, odt, max_len, total,
+                              covering or torch.cuda.is_current_stream_capturing(),
+                              int(ctx.config.decode_chunk_tokens))
         ws, need = None, 0
         if n > 1:
             need = int(L.skv_q_decode_workspace_bytes(B, Hq, D, n))

@@ -132,7 +132,8 @@ class KVCache:
     Fields of the reference: layers, batch_size, max_seq_len, current_len,
     n_heads, head_dim. Extensions (defaults reproduce the reference):
     n_kv_heads (grouped-query attention), dtype (float32, bfloat16 or
-    block-scaled storage, see KVCacheConfig), block_size / n_blocks / block_table (paged layout).
+    block-scaled storage, see KVCacheConfig), block_size / n_blocks /
+    block_table (paged layout).
 
     current_len is the number of filled positions. Each layer tracks its own
     fill, so updating layers 0..L-1 once per token writes every layer at the

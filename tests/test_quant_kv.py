@@ -81,6 +81,7 @@ def test_groups_that_are_not_finite_read_as_nan():
     (dict(head_dim=48), "multiple of 32"), (dict(head_dim=288), "up to 256"),
     (dict(n_heads=34, n_kv_heads=2), "up to 16 query heads"),
     (dict(dtype=torch.float16), "dtype must be"), (dict(dtype=torch.float8_e5m2), "dtype must be"),
+    (dict(max_seq_len=2**30 + 1), "2\\^30"), (dict(max_seq_len=2**30 + 1, block_size=16), "2\\^30"),
     (dict(block_size=12), "power of two"), (dict(batch_size=70000, max_seq_len=1), "65535")])
 def test_create_refuses(kw, match):
     args = dict(batch_size=2, max_seq_len=8, n_layers=1, n_heads=4, head_dim=64, dtype=FP4)
@@ -157,7 +158,8 @@ def _call(which, **kw):
                                     a["T"], a["fmt"], a["idt"], None)
     if which == "read":
         return L.skv_q_read(a["out"], a["out"], *st, a["lens"], kw.get("start", START),
-                            a.get("n_start", 2), *pg, a["B"], a["C"], a["H"], a["D"], a["T"], a["fmt"], a["odt"], None)
+                            a.get("n_start", 2), *pg, a["B"], a["C"], a["H"], a["D"], a["T"],
+                            a["fmt"], a["odt"], None)
     if which == "decode":
         if nb is None:
             nb = L.skv_q_decode_workspace_bytes(a["B"], a["Hq"], a["D"], a["n"])
@@ -183,7 +185,8 @@ INV, UNS, WSP = _lib.SKV_E_INVALID, _lib.SKV_E_UNSUPPORTED, _lib.SKV_E_WORKSPACE
     (dict(D=0), INV), (dict(D=48), UNS), (dict(D=288), UNS), (dict(B=0), INV), (dict(H=0), INV),
     (dict(B=65536), UNS), (dict(T=0), INV), (dict(k=FAKE + 8), INV),
     (dict(bt=FAKE, mb=4, bs=12), INV), (dict(bt=FAKE, mb=0, bs=16), INV),
-    (dict(bt=FAKE, mb=1 << 28, bs=16), INV)])
+    (dict(bt=FAKE, mb=1 << 28, bs=16), INV), (dict(bt=FAKE, mb=(1 << 26) + 1, bs=16), UNS),
+    (dict(T=(1 << 30) + 1), UNS)])
 def test_cache_arguments_refused(which, kw, rc):
     assert _call(which, **kw) == rc
     assert _lib.lib().skv_last_error()
@@ -202,13 +205,14 @@ def test_cache_arguments_refused(which, kw, rc):
     ("decode", dict(chunk=0), INV), ("decode", dict(n=0), INV), ("decode", dict(nb=16), WSP),
     ("decode", dict(ws=None), WSP), ("decode", dict(chunk=1 << 30, n=4), UNS),
     ("decode", dict(scale=float("inf")), INV), ("decode", dict(scale=float("nan")), INV),
-    ("decode", dict(wg=1), INV), ("decode", dict(wg=5), INV), ("decode", dict(B=300, wg=599), INV),
+    ("decode", dict(chunk=(1 << 30) + 128, n=1, wg=2), UNS), ("decode", dict(wg=1), INV), ("decode", dict(wg=5), INV), ("decode", dict(B=300, wg=599), INV),
     ("decode", dict(B=300, n=300, wg=90000), UNS),
     ("chunk", dict(n_host=TOO_MANY), INV), ("chunk", dict(n_host=NEGATIVE), INV),
     ("chunk", dict(n_host=START, n_new=FAKE), INV), ("prefill", dict(n_host=TOO_MANY), INV),
     ("prefill", dict(n_host=START, n_new=FAKE), INV), ("prefill", dict(n_host=START, nb=4), WSP),
     ("prefill", dict(new=None), INV), ("prefill", dict(new=FAKE + 8), INV),
-    ("prefill", dict(idt=2), INV), ("prefill", dict(C=0), INV), ("prefill", dict(q=None), INV), ("prefill", dict(Hq=12), UNS),
+    ("prefill", dict(idt=2), INV), ("prefill", dict(C=0), INV), ("prefill", dict(q=None), INV),
+    ("prefill", dict(Hq=12), UNS),
     ("prefill", dict(Hq=10), INV), ("prefill", dict(qdt=2), INV), ("prefill", dict(scale=0.0), INV),
     ("prefill", dict(splits=0), INV), ("prefill", dict(splits=33), INV),
     ("prefill", dict(splits=2, nb=16), WSP)])
@@ -219,8 +223,9 @@ def test_arguments_refused(which, kw, rc):
 
 @pytest.mark.parametrize("covering", [0, 1])
 @pytest.mark.parametrize("B,H,top,total,hint", [
-    (1, 1, 1, 0, 0), (257, 2, 5000, 70000, 0), (60000, 1, 4000, 0, 0), (256, 1, 300, 300, 0), (4, 16, 32000, 0, 0), (64, 8, 8192, 100000, 0), (3, 5, 130, 131, 0),
-    (65535, 1, 1, 0, 0), (1, 1, 2**31 - 1, 0, 0), (2, 2, 1000, 0, 100), (2, 2, 1000, 0, 5000)])
+    (1, 1, 1, 0, 0), (257, 2, 5000, 70000, 0), (60000, 1, 4000, 0, 0), (256, 1, 300, 300, 0),
+    (4, 16, 32000, 0, 0), (64, 8, 8192, 100000, 0), (3, 5, 130, 131, 0), (65535, 1, 1, 0, 0),
+    (1, 1, 2**31 - 1, 0, 0), (1, 900, 2**31 - 1, 0, 0), (2, 2, 1000, 0, 100), (2, 2, 1000, 0, 5000)])
 def test_decode_plan_covers_every_length(B, H, top, total, hint, covering):
     c, n, wg = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
     assert _lib.lib().skv_q_decode_plan(B, 2 * H, H, 128, _lib.MXFP4, 0, 0, top, total, covering,

@@ -704,6 +704,61 @@ def test_captured_steps(gpu_ctx):
         assert torch.equal(a.buffer, b.buffer)
 
 
+def test_captured_call_without_a_bound(gpu_ctx):
+    """Replayed with fills that sum to more than at the capture, none past its longest."""
+    banner("quant captured without a bound")
+    rng = np.random.default_rng(37)
+    B, H, G, D = 3, 2, 2, 64
+    gpu, cache, m = _make(gpu_ctx, B, 2200, H, G, D, "fp8")
+    _fill(gpu, gpu_ctx, cache, m, rng, [2100, 5, 0])
+    q = _dev(rng.standard_normal((B, H * G, D)).astype(np.float32), F32)
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    gpu.decode_attention(gpu_ctx, cache, 0, q, out)  # eager before the capture
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.decode_attention(gpu_ctx, cache, 0, q, out)
+    for counts in ([0, 1000, 1], [0, 1095, 2099]):
+        _fill(gpu, gpu_ctx, cache, m, rng, counts)
+        gpu.decode_attention(gpu_ctx, cache, 0, q, want)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all()
+        assert torch.allclose(out, want, rtol=0, atol=2e-5 * float(want.abs().max()))
+
+
+def test_bound_past_the_capacity(gpu_ctx):
+    """A max_len of any size plans for what the cache can hold."""
+    banner("quant bound past the capacity")
+    rng = np.random.default_rng(38)
+    for page in (0, 16):
+        gpu, cache, m = _make(gpu_ctx, 2, 300, 2, 2, 64, "fp4", page)
+        _fill(gpu, gpu_ctx, cache, m, rng, [300, 17])
+        q = _dev(rng.standard_normal((2, 4, 64)).astype(np.float32), F32)
+        a, b = torch.empty_like(q), torch.empty_like(q)
+        gpu.decode_attention(gpu_ctx, cache, 0, q, a, max_len=m.cap)
+        gpu.decode_attention(gpu_ctx, cache, 0, q, b, max_len=10**12)
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+def test_chunk_beside_a_sequence_past_max_seq_len(gpu_ctx):
+    """Appends fill a paged sequence's last page; others go on taking chunks."""
+    banner("quant chunk beside a full sequence")
+    rng = np.random.default_rng(39)
+    gpu, cache, m = _make(gpu_ctx, 2, 20, 2, 1, 32, "fp8", 16)
+    _fill(gpu, gpu_ctx, cache, m, rng, [20, 3])
+    for _ in range(2):
+        k, v = (_dev(_rows(rng, 2, 1, 2, 32), F32) for _ in range(2))
+        gpu.kv_cache_append(gpu_ctx, cache, 0, k, v)
+        m.append(_np(k), _np(v))
+    _fill(gpu, gpu_ctx, cache, m, rng, [0, 15])
+    with pytest.raises(ValueError, match="Cache is full"):
+        _fill(gpu, gpu_ctx, cache, m, rng, [1, 0])
+    with pytest.raises(ValueError, match="Cache is full"):
+        _fill(gpu, gpu_ctx, cache, m, rng, [0, 1])
+    _check_stored(gpu, gpu_ctx, cache, m)
+
+
 def test_two_streams_at_once(gpu_ctx):
     """Calls of one context on two streams share no workspace."""
     banner("quant two streams")
