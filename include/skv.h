@@ -359,7 +359,7 @@ int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scale, void* v,
  * chunk, and the fills advanced, in one call. q, out [B, C, H_q, D] of q_dt /
  * out_dt; H_q / H_kv in {1, 2, 4, 8}; n_new and n_host as in
  * skv_q_append_chunk; n_splits and ws as in skv_prefill_attn (skv_prefill_plan,
- * skv_prefill_workspace_bytes), and with n_host B int32 more. Q and the
+ * skv_prefill_workspace_bytes) with 2 B int32 more. Q and the
  * probabilities enter the matrix cores as bf16, K and V exactly, as over a bf16
  * cache that holds the same values. */
 int skv_q_append_prefill_attn(void* out, const void* q, void* k, void* k_scale, void* v,

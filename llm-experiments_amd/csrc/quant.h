@@ -192,10 +192,12 @@ struct Ints {
 // ---- host ----
 
 // skv_q_append_chunk's kernel with the counts on the device (n_new), on the host
-// (n_host; copied to n_copy on the way unless that is NULL) or neither.
+// (n_host; copied to n_copy on the way unless that is NULL) or neither; the
+// fills, which it does not advance, copied to start unless that is NULL.
 int quant_append_chunk(const quant::Cache& c, int fmt, const void* k_new, const void* v_new,
                        const int32_t* lens, const int32_t* n_new, const int32_t* n_host,
-                       int32_t* n_copy, int B, int C, int in_dt, hipStream_t s, const char* fn);
+                       int32_t* n_copy, int32_t* start, int B, int C, int in_dt, hipStream_t s,
+                       const char* fn);
 
 // Whether fmt is a block-scaled format.
 inline bool is_quant(int fmt) { return fmt == SKV_MXFP4 || fmt == SKV_MXFP8; }

@@ -56,8 +56,9 @@ constexpr int kRuns = 4;
 
 // Chunk append, grid (token tiles, H_kv, sequences b0 ..). Row i < n goes to
 // position lens[b] + i, n being n_new[b], or without n_new the host's count
-// (HOST; the first workgroup of a sequence stores it in n_copy[b] for the
-// kernels behind this one), or C; lens is read only. The input is loaded before
+// (HOST), or C; lens is read only. The first workgroup of a sequence stores the
+// host's count in n_copy[b] and the fill in start[b] (unless NULL) for the
+// kernels behind this one. The input is loaded before
 // the fill is known (its place depends on neither): one round trip to memory,
 // not two (4 x 2048 x 16 x 128 bf16 into 4 bits: 18.8 us with the fill first
 // and one run).
@@ -68,7 +69,8 @@ __global__ __launch_bounds__(256) void k_q_append_chunk(Cache c, const void* __r
                                                         const int32_t* __restrict__ lens,
                                                         const int32_t* __restrict__ n_new,
                                                         HOST n_host, int32_t* __restrict__ n_copy,
-                                                        int b0, int C) {
+                                                        int32_t* __restrict__ start, int b0,
+                                                        int C) {
   constexpr bool kHost = sizeof(HOST) == sizeof(Ints);
   const int b = b0 + blockIdx.z, h = blockIdx.y;
   const int opr = c.D / 8, tpw = tokens_per_wg(c.D);
@@ -83,14 +85,16 @@ __global__ __launch_bounds__(256) void k_q_append_chunk(Cache c, const void* __r
     load8_f32(kn, src, in_dt, xk[u]);
     load8_f32(vn, src, in_dt, xv[u]);
   }
+  const bool first = blockIdx.x == 0 && h == 0 && threadIdx.x == 0;
   int n = C;
   if constexpr (kHost) {
     n = n_host.v[blockIdx.z];
-    if (n_copy != nullptr && blockIdx.x == 0 && h == 0 && threadIdx.x == 0) n_copy[b] = n;
+    if (n_copy != nullptr && first) n_copy[b] = n;
   } else if (n_new) {
     n = min(n_new[b], C);
   }
   const int p0 = lens[b];
+  if (start != nullptr && first) start[b] = p0;
 #pragma unroll
   for (int u = 0; u < RUNS; ++u) {
     const int i = i0 + u * tpw;
@@ -284,8 +288,8 @@ extern "C" int skv_q_append(void* k, void* k_scale, void* v, void* v_scale, cons
 
 int skv::quant_append_chunk(const quant::Cache& c, int fmt, const void* k_new, const void* v_new,
                             const int32_t* lens, const int32_t* n_new, const int32_t* n_host,
-                            int32_t* n_copy, int B, int C, int in_dt, hipStream_t s,
-                            const char* fn) {
+                            int32_t* n_copy, int32_t* start, int B, int C, int in_dt,
+                            hipStream_t s, const char* fn) {
   const bool runs = long_call(B, c.Hkv, C, c.D);
   const int tpw = tokens_per_wg(c.D) * (runs ? kRuns : 1);
   for (int b0 = 0; b0 < B; b0 += n_host ? kInts : B) {
@@ -295,7 +299,7 @@ int skv::quant_append_chunk(const quant::Cache& c, int fmt, const void* k_new, c
     if (n_host) memcpy(cnt.v, n_host + b0, (size_t)nb * sizeof(int32_t));
 #define SKV_CHUNK(BITS, PAGED, RUNS, COUNTS)                                                   \
   hipLaunchKernelGGL((k_q_append_chunk<BITS, PAGED, RUNS, decltype(COUNTS)>), grid, dim3(256), 0, \
-                     s, c, k_new, v_new, in_dt, lens, n_new, COUNTS, n_copy, b0, C)
+                     s, c, k_new, v_new, in_dt, lens, n_new, COUNTS, n_copy, start, b0, C)
 #define SKV_LAUNCH(BITS, PAGED)                                  \
   do {                                                           \
     if (n_host) {                                                \
@@ -333,7 +337,8 @@ extern "C" int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale
     SKV_REQUIRE(n_host[b] >= 0 && n_host[b] <= C, SKV_E_INVALID, "%s: n_host[%d]=%d outside [0, %d]",
                 fn, b, n_host[b], C);
   hipStream_t s = (hipStream_t)stream;
-  rc = quant_append_chunk(c, fmt, k_new, v_new, lens, n_new, n_host, nullptr, B, C, in_dt, s, fn);
+  rc = quant_append_chunk(c, fmt, k_new, v_new, lens, n_new, n_host, nullptr, nullptr, B, C, in_dt, s,
+                          fn);
   if (rc || !advance) return rc;
   if (!n_host) return skv_advance(lens, n_new, C, B, c.cap, stream);
   for (int b0 = 0; b0 < B; b0 += kInts) {

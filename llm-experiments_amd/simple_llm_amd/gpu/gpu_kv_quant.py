@@ -183,16 +183,13 @@ def prefill(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, new_k: torch.T
         if n_splits <= 0:
             _lib.check(L.skv_prefill_plan(B, C, Hq, Hkv, max(max_end, 1), ctypes.byref(ns)),
                        "skv_prefill_plan")
-        need = int(L.skv_prefill_workspace_bytes(B, C, Hq, D, ns.value))
-        if counts is not None:
-            need += 4 * B
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        need = int(L.skv_prefill_workspace_bytes(B, C, Hq, D, ns.value)) + 8 * B
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
         rc = L.skv_q_append_prefill_attn(out.data_ptr(), q.data_ptr(), *_storage(layer),
                                          new_k.data_ptr(), new_v.data_ptr(),
                                          layer.lens.data_ptr(), None, n_ptr, *_pages(cache), B, C,
                                          Hq, Hkv, D, cache.max_seq_len, sc, ns.value,
-                                         ws.data_ptr() if ws is not None else None, need, fmt, idt,
-                                         _lib.dtype_code(q.dtype), _lib.dtype_code(out.dtype),
-                                         stream)
+                                         ws.data_ptr(), need, fmt, idt, _lib.dtype_code(q.dtype),
+                                         _lib.dtype_code(out.dtype), stream)
         _lib.check(rc, "skv_q_append_prefill_attn")
