@@ -239,8 +239,31 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
   // ---- which (sequence, kv head, split, query tile) this workgroup is ----
   const int w = blockIdx.x;
   const int xcd = w % kXCD, rest = w / kXCD;
-  const int qt = rest % a.n_qt;
-  const int gi = (rest / a.n_qt) * kXCD + xcd;
+  int qt = rest % a.n_qt;
+  int gi = (rest / a.n_qt) * kXCD + xcd;
+  if constexpr (QF != 0) {
+    // Ragged chunks: the tiles that have rows first (lane j counts those of the
+    // XCD's j-th group), then the others, which at most store zeros. In the
+    // order of the grid two with rows could share a CU while others stood
+    // empty (16 ragged x 8 kv heads x 4 x 128, <= 400 after <= 1000: 105 us, 94
+    // so; 12 x 4 x 8 x 128, <= 100 after <= 2000, 2 splits: 69 and 55).
+    if (a.n_new != nullptr && a.n_groups <= 64 * kXCD) {
+      const int gl = (int)(threadIdx.x & 63) * kXCD + xcd;
+      int t = 0;
+      if (gl < a.n_groups) {
+        const int bl = gl / a.n_splits / a.Hkv;
+        t = (max(0, min(a.n_new[bl], a.C)) * G + BM - 1) / BM;
+      }
+      const int upto = quant::wave_scan(t), all = __builtin_amdgcn_readlane(upto, 63);
+      const int none = gl < a.n_groups ? a.n_qt - t : 0, upto_none = quant::wave_scan(none);
+      const bool has = rest < all;
+      const int at = __popcll(__ballot(has ? upto <= rest : upto_none <= rest - all));
+      if (at >= 64) return;  // past the XCD's last group
+      gi = at * kXCD + xcd;
+      qt = has ? rest - __builtin_amdgcn_readlane(upto - t, at)
+               : __builtin_amdgcn_readlane(t - (upto_none - none), at) + rest - all;
+    }
+  }
   if (gi >= a.n_groups) return;
   const int split = gi % a.n_splits;
   const int bh = gi / a.n_splits;
@@ -1071,6 +1094,54 @@ extern "C" int skv_append_prefill_attn(void* out, const void* q, void* k_cache, 
   // the split bf16 path's merge pass has advanced the fills; the others advance here
   if (cache_dt == SKV_BF16 && n_splits > 1) return SKV_OK;
   return skv_advance(lens, n_new, C, B, T_cap, stream);
+}
+
+// The time of a ragged chunk over n splits, us, fitted to 100 measured calls (12
+// shapes of 2 to 32 sequences, head dims 64 to 256, n = 1 to 32; off by 7 %; the
+// choice took at most 7 % longer than the best n measured there, in 9 other
+// shapes at most 9 %, but 13 % with 40 queries of 64 sequences): the longest
+// workgroup alone (L tiles of 64 tokens) or all of them in turn (S tiles and W
+// workgroups per CU), each workgroup costing 4 tiles more, and the partials
+// written and merged.
+// skv_prefill_plan counts the tiles of the longest chunk for every sequence and
+// takes all prefixes for the longest: 6 ragged x 8 kv heads x 4 x 128, <= 333
+// after <= 12000: 331 us in its one split, 162 in the four chosen here; <= 333
+// after <= 1900: 64.2 and 63.9 in one and two.
+extern "C" int skv_q_prefill_plan(int B, int C, int H_q, int H_kv, int D, const int32_t* lens,
+                                  const int32_t* n_host, int* n_splits) {
+  const char* fn = "skv_q_prefill_plan";
+  SKV_REQUIRE(lens && n_host && n_splits, SKV_E_INVALID, "%s: null pointer argument", fn);
+  SKV_REQUIRE(B > 0 && C > 0 && H_kv > 0 && H_q > 0 && H_q % H_kv == 0 && D > 0 &&
+                  D <= quant::kMaxD,
+              SKV_E_INVALID, "%s: bad dims (B=%d C=%d H_q=%d H_kv=%d D=%d)", fn, B, C, H_q, H_kv,
+              D);
+  const int DK = kernel_dim(D), G = H_q / H_kv, rows = (DK > 128 ? 4 : kWaves) * kQB * 32;
+  long long end = 0, wg = 0, work = 0, tokens = 0;
+  for (int b = 0; b < B; ++b) {
+    SKV_REQUIRE(lens[b] >= 0 && n_host[b] >= 0 && n_host[b] <= C, SKV_E_INVALID,
+                "%s: sequence %d: %d tokens after %d", fn, b, n_host[b], lens[b]);
+    if (n_host[b] == 0) continue;
+    const long long e = (long long)lens[b] + n_host[b];
+    const long long tiles = ((long long)n_host[b] * G + rows - 1) / rows;
+    end = e > end ? e : end;
+    wg += tiles;
+    work += tiles * ((e + kBN - 1) / kBN);
+    tokens += n_host[b];
+  }
+  *n_splits = 1;
+  const double S = (double)work * H_kv / kCUs, W = (double)wg * H_kv / kCUs;
+  const double MB = (double)tokens * H_q * (DK + 2) * 8 / 1e6;  // written and read, a split
+  const double tile = DK <= 64 ? 1.0 : DK == 128 ? 1.6 : 3.4;
+  double best = 0.;
+  for (int n = 1; n <= 32 && (n == 1 || n <= (end + 4 * kBN - 1) / (4 * kBN)); ++n) {
+    const double L = (double)((end + n * kBN - 1) / (n * kBN)) + 4.;
+    const double all = S + 4. * W * n + 0.35 * L;
+    const double t = tile * (L > all ? L : all) + (n > 1 ? 2.6 + 0.19 * MB * n : 0.);
+    if (n > 1 && t >= best) continue;
+    best = t;
+    *n_splits = n;
+  }
+  return SKV_OK;
 }
 
 extern "C" int skv_q_append_prefill_attn(void* out, const void* q, void* k, void* k_scale, void* v,

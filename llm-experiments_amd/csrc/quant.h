@@ -180,6 +180,19 @@ __device__ __forceinline__ void store8(uint8_t* codes, uint8_t* scales, size_t r
   if ((o & 3) == 0) scales[row * (size_t)(D / kGroup) + (o >> 2)] = (uint8_t)byte;
 }
 
+// Inclusive prefix sum over the wavefront (DPP row shifts and broadcasts).
+__device__ __forceinline__ int wave_scan(int x) {
+#define SKV_SCAN(CTRL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, true)
+  SKV_SCAN(0x111, 0xF);
+  SKV_SCAN(0x112, 0xF);
+  SKV_SCAN(0x114, 0xF);
+  SKV_SCAN(0x118, 0xF);
+  SKV_SCAN(0x142, 0xA);  // lane 15 of each row to the next row (rows 1, 3)
+  SKV_SCAN(0x143, 0xC);  // lane 31 to rows 2, 3
+#undef SKV_SCAN
+  return x;
+}
+
 // Small host integers, one a sequence, as a kernel argument: no copy to the
 // device, which would be a launch of its own (or hold the host until it landed).
 constexpr int kInts = 256;

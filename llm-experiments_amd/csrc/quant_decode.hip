@@ -223,19 +223,6 @@ __device__ __forceinline__ int n_pieces(const QDecodeArgs& a, int len) {
 // 146,000 tokens in 8 chunks of the longest, 45 us against 33 for equal ones.)
 constexpr int kMaxScan = 256;
 
-// Inclusive prefix sum over the wavefront (DPP row shifts and broadcasts).
-__device__ __forceinline__ int wave_scan(int x) {
-#define SKV_SCAN(CTRL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, true)
-  SKV_SCAN(0x111, 0xF);
-  SKV_SCAN(0x112, 0xF);
-  SKV_SCAN(0x114, 0xF);
-  SKV_SCAN(0x118, 0xF);
-  SKV_SCAN(0x142, 0xA);  // lane 15 of each row to the next row (rows 1, 3)
-  SKV_SCAN(0x143, 0xC);  // lane 31 to rows 2, 3
-#undef SKV_SCAN
-  return x;
-}
-
 // Uniform over the wavefront. b = a.B: no sequence.
 __device__ __forceinline__ Piece find_piece(const QDecodeArgs& a, int w, int lane) {
   Piece p;

@@ -56,6 +56,7 @@ _SIGNATURES = {
     "skv_q_decode_workspace_bytes": (_Z, [_I, _I, _I, _I]),
     "skv_q_decode_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                _F, _I, _I, _I, _P, _Z, _I, _I, _I, _I, _P]),
+    "skv_q_prefill_plan": (_I, [_I, _I, _I, _I, _I, _P, _P, ctypes.POINTER(_I)]),
     "skv_q_append_prefill_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I,
                                        _I, _I, _I, _I, _F, _I, _P, _Z, _I, _I, _I, _I, _P]),
     "skv_embed": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),

@@ -180,9 +180,13 @@ def prefill(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, new_k: torch.T
             _lib.check(rc, "skv_q_append_chunk")
             return
         ns = ctypes.c_int(int(n_splits))
-        if n_splits <= 0:
+        if n_splits <= 0 and counts is None:
             _lib.check(L.skv_prefill_plan(B, C, Hq, Hkv, max(max_end, 1), ctypes.byref(ns)),
                        "skv_prefill_plan")
+        elif n_splits <= 0:
+            fills = np.ascontiguousarray(layer.host_lens, np.int32)
+            _lib.check(L.skv_q_prefill_plan(B, C, Hq, Hkv, D, _lib.host_ptr(fills), n_ptr,
+                                            ctypes.byref(ns)), "skv_q_prefill_plan")
         need = int(L.skv_prefill_workspace_bytes(B, C, Hq, D, ns.value)) + 8 * B
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)

@@ -257,6 +257,43 @@ def test_decode_plan_refuses():
     assert L.skv_q_decode_workspace_bytes(0, 8, 64, 3) == 0
 
 
+def _prefill_plan(B, C, Hq, H, D, lens, n):
+    a, b = (np.asarray(x, np.int32) for x in (lens, n))
+    ns = ctypes.c_int(-1)
+    rc = _lib.lib().skv_q_prefill_plan(B, C, Hq, H, D, _lib.host_ptr(a), _lib.host_ptr(b),
+                                       ctypes.byref(ns))
+    return rc, ns.value
+
+
+def test_prefill_plan():
+    rng = np.random.default_rng(3)
+    for _ in range(300):
+        B, H, G, C = (int(rng.integers(1, m)) for m in (40, 17, 9, 700))
+        lens, n = rng.integers(0, 1 << int(rng.integers(1, 28)), B), rng.integers(0, C + 1, B)
+        rc, ns = _prefill_plan(B, C, H * G, H, int(rng.choice([32, 64, 96, 128, 256])), lens, n)
+        assert rc == 0 and 1 <= ns <= 32
+        assert ns == 1 or (ns - 1) * 256 < (lens + n)[n > 0].max()
+    # a few rows after long prefixes are split, many after short ones are not,
+    # and sequences without a chunk do not count
+    assert _prefill_plan(2, 64, 16, 2, 128, [20000, 9000], [64, 5])[1] > 8
+    assert _prefill_plan(16, 400, 32, 8, 128, [500] * 16, [399] * 16)[1] == 1
+    assert _prefill_plan(2, 8, 8, 8, 64, [2**30, 10], [0, 8])[1] == 1
+    assert _prefill_plan(2, 8, 8, 8, 64, [2**30, 10], [0, 0])[1] == 1
+
+
+def test_prefill_plan_refuses():
+    ok = (2, 8, 8, 4, 64)
+    for i, bad in ((0, 0), (1, 0), (2, 0), (2, 6), (3, 0), (4, 0), (4, 288)):
+        assert _prefill_plan(*ok[:i], bad, *ok[i + 1:], [1, 1], [1, 1])[0] == INV
+    for lens, n in (([-1, 0], [1, 1]), ([1, 1], [1, 9]), ([1, 1], [-1, 1])):
+        assert _prefill_plan(*ok, lens, n)[0] == INV
+    f = _lib.lib().skv_q_prefill_plan
+    ns = ctypes.c_int()
+    assert f(*ok, None, FAKE, ctypes.byref(ns)) == INV
+    assert f(*ok, FAKE, None, ctypes.byref(ns)) == INV
+    assert f(*ok, FAKE, FAKE, None) == INV
+
+
 def test_read_refuses_bad_starts(monkeypatch):
     """Before any device work; the tensor checks are stubbed out (no GPU here)."""
     from simple_llm_amd.gpu import gpu_kv_cache as gk

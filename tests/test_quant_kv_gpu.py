@@ -578,6 +578,28 @@ def test_prefill(gpu_ctx, fmt, B, Hkv, G, D, lens, C, counts, page, io):
         _check_stored(gpu, gpu_ctx, cache, m)
 
 
+@pytest.mark.parametrize("B,Hkv,splits", [(70, 2, 0), (70, 8, 1), (33, 8, 2), (33, 8, 1), (64, 1, 8),
+                                          (13, 5, 3)])
+def test_prefill_of_ragged_batches(gpu_ctx, B, Hkv, splits):
+    """More (sequence, head, split) groups than the 512 that are ordered by their rows, and
+    as many; sequences without rows among them."""
+    banner(f"quant ragged prefill B={B} Hkv={Hkv} splits={splits}")
+    rng = np.random.default_rng(B * Hkv + splits)
+    G, D, C = 2, 32, 300  # three tiles of 256 rows a group
+    gpu, cache, m = _make(gpu_ctx, B, C + 150, Hkv, G, D, "fp8")
+    _fill(gpu, gpu_ctx, cache, m, rng, rng.integers(0, 150, B))
+    counts = rng.integers(0, 20, B)
+    counts[::5] = 0
+    counts[[3, B - 2]] = C, 129
+    k, v = (_dev(_rows(rng, B, C, Hkv, D), BF16) for _ in range(2))
+    q = _dev(rng.standard_normal((B, C, Hkv * G, D)).astype(np.float32), BF16)
+    out = torch.full_like(q, 9.0)
+    gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out, n_new=counts, n_splits=splits)
+    m.append(_np(k), _np(v), counts)
+    _check_attention(out, q, m, G, D ** -0.5, False, True, counts, True, False)
+    _check_stored(gpu, gpu_ctx, cache, m)
+
+
 def test_prefill_equals_a_bf16_cache_of_the_same_values(gpu_ctx):
     """K and V enter as a bf16 cache holding the stored values would give them."""
     banner("quant prefill against bf16 cache")
