@@ -32,8 +32,8 @@
 //    as two E4M3 parts: 1 to 2 % faster, but its sums carry fewer bits, and
 //    outputs moved by about 2^-15 where these move by 2^-19: not taken.)
 // Precision: K and V enter exactly. With fp32 in or out, q and p are three bf16
-// parts (all bits of q, 2^-24 of p); with bf16 in and out q is one part and p
-// two (2^-17). The parts use the matrix core's columns that few heads leave
+// parts (all bits of q, 2^-24 of p; what lies below 2^-133 is lost); with bf16
+// in and out q is one part and p two (2^-17). The parts use the matrix core's columns that few heads leave
 // idle: column c is head c % HC, slot c / HC, HC = 16, 8 or (three parts
 // only) 4 being the smallest that holds G, and slot s takes part s (as the
 // plain grouped-query kernel's duplicated columns do); parts beyond the slots
@@ -448,15 +448,34 @@ __global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, SL, F32)) void k_q
   const int head = cl % HC, slot = cl / HC;
   const float sf[3] = {slot > 0 ? 1.f : 0.f, slot > 1 ? 1.f : 0.f, slot > 2 ? 1.f : 0.f};
   bf16x8 qf[QS][KO];
+  float xq[KO][8];
+#pragma unroll
+  for (int i = 0; i < KO; ++i) {
+    const int e = k_el(i / (PE / 8)) + i % (PE / 8) * 8;
+    load8_f32(a.q, (head0 + (head < G ? head : 0)) * D + (e < D ? e : 0), a.q_dt, xq[i]);
+  }
+  // Parts below bf16's smallest number (2^-133) are lost: a query whose elements
+  // all are below 2^-64 enters 2^40 times as large.
+  float qsign = a.qsign, qscale = a.qscale;
+  if constexpr (F32) {
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < KO; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(xq[i][j]));
+    big = xor32_max(fmaxf(big, __shfl_xor(big, 16)));
+    if (big < 0x1p-64f) {
+      qsign *= 0x1p40f;
+      qscale *= 0x1p-40f;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < KO; ++i) {
     const int e = k_el(i / (PE / 8)) + i % (PE / 8) * 8;
     const bool used = head < G && e < D;
-    float x[8];
-    load8_f32(a.q, (head0 + (head < G ? head : 0)) * D + (e < D ? e : 0), a.q_dt, x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float r = used ? x[j] * a.qsign : 0.f;
+      float r = used ? xq[i][j] * qsign : 0.f;
 #pragma unroll
       for (int t = 0; t < QS; ++t) {
         // bf16: every slot takes q itself and has the whole score
@@ -517,7 +536,7 @@ __global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, SL, F32)) void k_q
     float mt = sc[0][0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) mt = fmaxf(mt, sc[j >> 2][j & 3]);
-    mt *= a.qscale;
+    mt *= qscale;
     if (__ballot(mt > m_run + kLazy) != 0ull) {  // uniform
       mt = fmaxf(mt, __shfl_xor(mt, 16));
       mt = xor32_max(mt);
@@ -532,7 +551,7 @@ __global__ __launch_bounds__(kWaves * 64, min_waves(DP, BITS, SL, F32)) void k_q
     bf16x8 pf[PS];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float r = fast_exp2(fmaf(sc[j >> 2][j & 3], a.qscale, -m_use));
+      float r = fast_exp2(fmaf(sc[j >> 2][j & 3], qscale, -m_use));
       l_run += r;
 #pragma unroll
       for (int t = 0; t < PS; ++t) {

@@ -348,6 +348,26 @@ def test_scales_of_any_sign(gpu_ctx, scale):
             assert (np.abs(got[b, h] - want[0]) <= tol * mag[0] + 1e-37).all()
 
 
+@pytest.mark.parametrize("io", [F32, BF16])
+@pytest.mark.parametrize("G", [1, 6, 12])
+def test_tiny_queries_of_large_keys(gpu_ctx, G, io):
+    """Scores of ordinary size from queries whose last bits bf16 cannot hold unscaled."""
+    banner(f"quant tiny queries G={G} {io}")
+    rng = np.random.default_rng(19)
+    B, H, D, n = 2, 2, 96, 140
+    gpu, cache, m = _make(gpu_ctx, B, n, H, G, D, "fp8")
+    k = _rows(rng, B, n, H, D).astype(np.float64) * 2.0 ** 118
+    k, v = _dev(k.astype(np.float32), F32), _dev(_rows(rng, B, n, H, D), F32)
+    gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v)
+    m.append(_np(k), _np(v))
+    x = rng.standard_normal((B, H * G, D)) * 2.0 ** -122
+    q = _dev(x.astype(np.float32), io)
+    out = torch.empty_like(q)
+    scale = 16 * D ** -0.5
+    gpu.decode_attention(gpu_ctx, cache, 0, q, out, scale=scale)
+    _check_attention(out[:, None], q[:, None], m, G, scale, io == F32, io == BF16)
+
+
 def test_empty_cache_gives_zeros(gpu_ctx):
     banner("quant decode of nothing")
     for page in (0, 16):
