@@ -769,6 +769,54 @@ def test_captured_call_without_a_bound(gpu_ctx):
         assert torch.allclose(out, want, rtol=0, atol=2e-5 * float(want.abs().max()))
 
 
+@pytest.mark.parametrize("fmt,page,splits", [("fp4", 0, 1), ("fp8", 16, 2), ("fp4", 8, 0)])
+def test_captured_chunk(gpu_ctx, fmt, page, splits):
+    """A ragged chunk with attention, one without and a read in a captured graph: replays
+    go on from the fills they find, with the counts and starts of the capture."""
+    banner(f"quant captured chunk {fmt} page={page} splits={splits}")
+    rng = np.random.default_rng(43)
+    B, H, G, D, C, T = 3, 2, 4, 64, 30, 400
+    gpu, cache, m = _make(gpu_ctx, B, T, H, G, D, fmt, page)
+    _, twin, _ = _make(gpu_ctx, B, T, H, G, D, fmt, page)
+    counts, more = [C, 0, 7], [1, 12, 0]
+    k, v = (torch.zeros(B, C, H, D, device="cuda:0") for _ in range(2))
+    q = torch.zeros(B, C, H * G, D, dtype=BF16, device="cuda:0")
+    outs = [torch.empty_like(q), *(torch.empty(B, 50, H, D, device="cuda:0") for _ in "kv")]
+    want = [torch.empty_like(x) for x in outs]
+
+    def calls(c, o):
+        gpu.kv_cache_prefill(gpu_ctx, c, 0, k, v, q, o[0], n_new=counts, n_splits=splits)
+        gpu.kv_cache_prefill(gpu_ctx, c, 0, k, v, n_new=more)
+        gpu.kv_cache_read(gpu_ctx, c, 0, o[1], o[2], start=[10, 0, 3])
+
+    lay = cache.layers[0]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):  # before the capture, undone
+        calls(cache, outs)
+    side.synchronize()
+    lay.lens.zero_()
+    lay.host_lens[:] = 0
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(cache, outs)
+    lay.host_lens[:] = 0
+    for _ in range(4):
+        k.copy_(_dev(_rows(rng, B, C, H, D), F32))
+        v.copy_(_dev(_rows(rng, B, C, H, D), F32))
+        q.copy_(_dev(rng.standard_normal((B, C, H * G, D)).astype(np.float32), BF16))
+        calls(twin, want)
+        graph.replay()
+        torch.cuda.synchronize()
+        lay.host_lens += np.array(counts) + more
+        assert lay.lens.cpu().tolist() == twin.layers[0].lens.cpu().tolist() == lay.host_lens.tolist()
+        for a, b in zip(outs[1:], want[1:]):
+            assert torch.equal(a, b)
+        # (the splits of the eager call follow its fills: each side rounds p by 2^-8)
+        assert torch.allclose(outs[0].float(), want[0].float(), rtol=2.0 ** -7,
+                              atol=2.0 ** -6 * float(v.abs().max()))
+
+
 def test_bound_past_the_capacity(gpu_ctx):
     """A max_len of any size plans for what the cache can hold."""
     banner("quant bound past the capacity")
