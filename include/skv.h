@@ -354,9 +354,9 @@ int skv_q_decode_attn(void* out, const void* q, void* k, void* k_scale, void* v,
                       int n_wg, void* ws, size_t ws_bytes, int fmt, int in_dt, int q_dt, int out_dt,
                       skv_stream_t stream);
 
-/* n_splits of a ragged chunk over a block-scaled cache (host-only): n_host[b]
- * tokens (of at most C) after lens[b], both host arrays of B. Tunes the call;
- * any n_splits is valid for any lengths. */
+/* n_splits of a chunk over a block-scaled cache (host-only): n_host[b] tokens
+ * (NULL: C each) after lens[b], both host arrays of B. Tunes the call; any
+ * n_splits is valid for any lengths. */
 int skv_q_prefill_plan(int B, int C, int H_q, int H_kv, int D, const int32_t* lens /* host */,
                        const int32_t* n_host /* host */, int* n_splits /* host */);
 
@@ -364,8 +364,8 @@ int skv_q_prefill_plan(int B, int C, int H_q, int H_kv, int D, const int32_t* le
  * skv_q_append_chunk, causal attention of the chunk's queries over prefix +
  * chunk, and the fills advanced, in one call. q, out [B, C, H_q, D] of q_dt /
  * out_dt; H_q / H_kv in {1, 2, 4, 8}; n_new and n_host as in
- * skv_q_append_chunk; n_splits and ws as in skv_prefill_attn (skv_prefill_plan
- * or skv_q_prefill_plan, skv_prefill_workspace_bytes) with 2 B int32 more. Q and the
+ * skv_q_append_chunk; n_splits (skv_q_prefill_plan) and ws as in
+ * skv_prefill_attn (skv_prefill_workspace_bytes) with 2 B int32 more. Q and the
  * probabilities enter the matrix cores as bf16, K and V exactly, as over a bf16
  * cache that holds the same values. */
 int skv_q_append_prefill_attn(void* out, const void* q, void* k, void* k_scale, void* v,

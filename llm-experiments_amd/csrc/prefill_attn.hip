@@ -55,6 +55,7 @@
 //    group of V goes into LDS as zeros and its tile is marked: a masked
 //    probability of 0 would make it NaN for queries that do not attend the
 //    token; those that do get their NaN from the scales afterwards.
+#include <cmath>
 #include <type_traits>
 
 #include "quant.h"
@@ -1096,13 +1097,13 @@ extern "C" int skv_append_prefill_attn(void* out, const void* q, void* k_cache, 
   return skv_advance(lens, n_new, C, B, T_cap, stream);
 }
 
-// The time of a ragged chunk over n splits, us, fitted to 100 measured calls (12
-// shapes of 2 to 32 sequences, head dims 64 to 256, n = 1 to 32; off by 7 %; the
-// choice took at most 7 % longer than the best n measured there, in 9 other
-// shapes at most 9 %, but 13 % with 40 queries of 64 sequences): the longest
-// workgroup alone (L tiles of 64 tokens) or all of them in turn (S tiles and W
-// workgroups per CU), each workgroup costing 4 tiles more, and the partials
-// written and merged.
+// The time of a chunk over n splits, us, fitted to 350 measured calls (52 shapes of
+// 1 to 32 sequences, all head dims, ragged and equal, n = 1 to 32; off by 9 %, and the
+// choice on average 2 % and at most 18 % behind the best n measured). A workgroup
+// is the tiles of 64 tokens it goes through and 3 more. Up to one per CU, the
+// longest (L) sets the time; past that the work per CU (S tiles, W n workgroups) does, and
+// a part of the longest, or, the more equal they are, of a last round that is
+// not full. Then the partials, written and merged.
 // skv_prefill_plan counts the tiles of the longest chunk for every sequence and
 // takes all prefixes for the longest: 6 ragged x 8 kv heads x 4 x 128, <= 333
 // after <= 12000: 331 us in its one split, 162 in the four chosen here; <= 333
@@ -1110,7 +1111,7 @@ extern "C" int skv_append_prefill_attn(void* out, const void* q, void* k_cache, 
 extern "C" int skv_q_prefill_plan(int B, int C, int H_q, int H_kv, int D, const int32_t* lens,
                                   const int32_t* n_host, int* n_splits) {
   const char* fn = "skv_q_prefill_plan";
-  SKV_REQUIRE(lens && n_host && n_splits, SKV_E_INVALID, "%s: null pointer argument", fn);
+  SKV_REQUIRE(lens && n_splits, SKV_E_INVALID, "%s: null pointer argument", fn);
   SKV_REQUIRE(B > 0 && C > 0 && H_kv > 0 && H_q > 0 && H_q % H_kv == 0 && D > 0 &&
                   D <= quant::kMaxD,
               SKV_E_INVALID, "%s: bad dims (B=%d C=%d H_q=%d H_kv=%d D=%d)", fn, B, C, H_q, H_kv,
@@ -1118,25 +1119,32 @@ extern "C" int skv_q_prefill_plan(int B, int C, int H_q, int H_kv, int D, const 
   const int DK = kernel_dim(D), G = H_q / H_kv, rows = (DK > 128 ? 4 : kWaves) * kQB * 32;
   long long end = 0, wg = 0, work = 0, tokens = 0;
   for (int b = 0; b < B; ++b) {
-    SKV_REQUIRE(lens[b] >= 0 && n_host[b] >= 0 && n_host[b] <= C, SKV_E_INVALID,
-                "%s: sequence %d: %d tokens after %d", fn, b, n_host[b], lens[b]);
-    if (n_host[b] == 0) continue;
-    const long long e = (long long)lens[b] + n_host[b];
-    const long long tiles = ((long long)n_host[b] * G + rows - 1) / rows;
+    const int n = n_host ? n_host[b] : C;
+    SKV_REQUIRE(lens[b] >= 0 && n >= 0 && n <= C, SKV_E_INVALID,
+                "%s: sequence %d: %d tokens after %d", fn, b, n, lens[b]);
+    if (n == 0) continue;
+    const long long e = (long long)lens[b] + n;
+    const long long tiles = ((long long)n * G + rows - 1) / rows;
     end = e > end ? e : end;
     wg += tiles;
     work += tiles * ((e + kBN - 1) / kBN);
-    tokens += n_host[b];
+    tokens += n;
   }
   *n_splits = 1;
   const double S = (double)work * H_kv / kCUs, W = (double)wg * H_kv / kCUs;
   const double MB = (double)tokens * H_q * (DK + 2) * 8 / 1e6;  // written and read, a split
-  const double tile = DK <= 64 ? 1.0 : DK == 128 ? 1.6 : 3.4;
+  const double tile = DK == 32 ? 0.8 : DK == 64 ? 1.14 : DK == 128 ? 1.62 : 4.0;
   double best = 0.;
   for (int n = 1; n <= 32 && (n == 1 || n <= (end + 4 * kBN - 1) / (4 * kBN)); ++n) {
-    const double L = (double)((end + n * kBN - 1) / (n * kBN)) + 4.;
-    const double all = S + 4. * W * n + 0.35 * L;
-    const double t = tile * (L > all ? L : all) + (n > 1 ? 2.6 + 0.19 * MB * n : 0.);
+    const double L = (double)((end + n * kBN - 1) / (n * kBN)) + 3.1;
+    double span = L;
+    if (W * n > 1.) {
+      const double all = S + 3.1 * W * n, mean = all / (W * n), even = mean < L ? mean / L : 1.;
+      const double t = all + 1.6 * (1. - even) * even * L +
+                       even * even * even * even * (std::ceil(W * n) - W * n) * mean;
+      span = t > L ? t : L;
+    }
+    const double t = tile * span + (n > 1 ? 2.0 + 0.193 * MB * n : 0.);
     if (n > 1 && t >= best) continue;
     best = t;
     *n_splits = n;

@@ -652,7 +652,7 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
     batch_count(ctx)
     if cache.quantized:
         gpu_kv_quant.prefill(ctx, cache, layer, new_k, new_v, q, out,
-                             None if n_min == C else n_host, end, scale, n_splits)
+                             None if n_min == C else n_host, scale, n_splits)
         layer.host_lens = after
         return after.copy()
     L = _lib.lib()

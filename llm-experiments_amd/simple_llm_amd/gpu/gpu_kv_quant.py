@@ -161,8 +161,7 @@ def attend(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, q: torch.Tensor
 
 def prefill(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, new_k: torch.Tensor,
             new_v: torch.Tensor, q: Optional[torch.Tensor], out: Optional[torch.Tensor],
-            counts: Optional[np.ndarray], max_end: int, scale: Optional[float],
-            n_splits: int) -> None:
+            counts: Optional[np.ndarray], scale: Optional[float], n_splits: int) -> None:
     """kv_cache_prefill; counts: tokens per sequence, or None for whole chunks."""
     dev = layer.lens.device
     L = _lib.lib()
@@ -180,10 +179,7 @@ def prefill(ctx: GPUContext, cache: KVCache, layer: KVCacheLayer, new_k: torch.T
             _lib.check(rc, "skv_q_append_chunk")
             return
         ns = ctypes.c_int(int(n_splits))
-        if n_splits <= 0 and counts is None:
-            _lib.check(L.skv_prefill_plan(B, C, Hq, Hkv, max(max_end, 1), ctypes.byref(ns)),
-                       "skv_prefill_plan")
-        elif n_splits <= 0:
+        if n_splits <= 0:
             fills = np.ascontiguousarray(layer.host_lens, np.int32)
             _lib.check(L.skv_q_prefill_plan(B, C, Hq, Hkv, D, _lib.host_ptr(fills), n_ptr,
                                             ctypes.byref(ns)), "skv_q_prefill_plan")

@@ -258,10 +258,10 @@ def test_decode_plan_refuses():
 
 
 def _prefill_plan(B, C, Hq, H, D, lens, n):
-    a, b = (np.asarray(x, np.int32) for x in (lens, n))
+    a, b = (np.asarray(0 if x is None else x, np.int32) for x in (lens, n))
     ns = ctypes.c_int(-1)
-    rc = _lib.lib().skv_q_prefill_plan(B, C, Hq, H, D, _lib.host_ptr(a), _lib.host_ptr(b),
-                                       ctypes.byref(ns))
+    rc = _lib.lib().skv_q_prefill_plan(B, C, Hq, H, D, _lib.host_ptr(a),
+                                       None if n is None else _lib.host_ptr(b), ctypes.byref(ns))
     return rc, ns.value
 
 
@@ -278,6 +278,8 @@ def test_prefill_plan():
     assert _prefill_plan(2, 64, 16, 2, 128, [20000, 9000], [64, 5])[1] > 8
     assert _prefill_plan(16, 400, 32, 8, 128, [500] * 16, [399] * 16)[1] == 1
     assert _prefill_plan(2, 8, 8, 8, 64, [2**30, 10], [0, 8])[1] == 1
+    assert (_prefill_plan(4, 512, 16, 16, 128, [32256] * 4, None)
+            == _prefill_plan(4, 512, 16, 16, 128, [32256] * 4, [512] * 4) == (0, 2))
     assert _prefill_plan(2, 8, 8, 8, 64, [2**30, 10], [0, 0])[1] == 1
 
 
@@ -290,7 +292,6 @@ def test_prefill_plan_refuses():
     f = _lib.lib().skv_q_prefill_plan
     ns = ctypes.c_int()
     assert f(*ok, None, FAKE, ctypes.byref(ns)) == INV
-    assert f(*ok, FAKE, None, ctypes.byref(ns)) == INV
     assert f(*ok, FAKE, FAKE, None) == INV
 
 
