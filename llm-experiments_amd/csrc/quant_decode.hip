@@ -15,7 +15,7 @@
 //
 // Bound by HBM: 4 x 16 x 128 of 32000 4-bit tokens (279 MB of codes and scales)
 // take 49 us in the first launch (5.7 TB/s; its loads alone as long) and 4.6 in
-// the merge, 52 us a call; 64 ragged paged sequences of 8 x 4 x 128 (144,900
+// the merge, 52 to 53 us a call; 64 ragged paged sequences of 8 x 4 x 128 (144,900
 // tokens) 37 us (159 MB, 4-bit) and 68 us (308 MB, 8-bit). Calls of different
 // size fit 7.6 TB/s and 12 us of start and end.
 //
@@ -735,7 +735,13 @@ using namespace skv;
 // take a whole number of chunks each; with two the merge costs more than the
 // halved rows gain (512 rows of 2288 tokens: 36 us in two, 33.5 in one).
 // Ragged ones leave half a chunk a row, which the round has to hold too (64
-// sequences x 8 heads, 146,000 tokens: 49 us without that, 44 with).
+// sequences x 8 heads, 146,000 tokens: 49 us without that, 44 with). A chunk of
+// 1024 tokens or more is no multiple of 512: workgroups that start whole multiples
+// of 32 KB apart meet in the same memory channels (4 x 16 x 128 of 32000 4-bit
+// tokens in a cache of 131072 positions, chunks of 2048 and 2176: 59.2 and 52.1
+// us, in one of 32001 both 53.8; 1 x 8 x 4 x 128 of 131000, 1024 and 1152: 37.7
+// and 35.4; 64 ragged x 8 x 4 x 128, 1536 and 1664: 39.8 and 38.8. Multiples of
+// 256 gain nothing by a step more).
 extern "C" int skv_q_decode_plan(int B, int H_q, int H_kv, int D, int fmt, int q_dt, int out_dt,
                                  int max_len, long long total_len, int covering, int chunk_hint,
                                  int* chunk_tokens, int* n_chunks, int* n_wg) {
@@ -764,6 +770,7 @@ extern "C" int skv_q_decode_plan(int B, int H_q, int H_kv, int D, int fmt, int q
   const long long least = (max_len + n_most - 1) / n_most;
   if (chunk < least) chunk = least;
   chunk = (chunk + kStep - 1) / kStep * kStep;
+  if (chunk_hint <= 0 && chunk >= 1024 && chunk % 512 == 0) chunk += kStep;
   if (chunk < kStep) chunk = kStep;
   if (chunk > most) chunk = most;
   if (chunk > quant::kMaxCap) chunk = quant::kMaxCap;
