@@ -1139,9 +1139,11 @@ extern "C" int skv_q_prefill_plan(int B, int C, int H_q, int H_kv, int D, const 
     const double L = (double)((end + n * kBN - 1) / (n * kBN)) + 3.1;
     double span = L;
     if (W * n > 1.) {
+      // (two of 128 rows a CU, which whole chunks may run as, fill a round in halves)
+      const int parts = !n_host && DK <= 128 && tile_waves(B, C, H_kv, G, D, n, false) == 4 ? 2 : 1;
       const double all = S + 3.1 * W * n, mean = all / (W * n), even = mean < L ? mean / L : 1.;
-      const double t = all + 1.6 * (1. - even) * even * L +
-                       even * even * even * even * (std::ceil(W * n) - W * n) * mean;
+      const double rest = std::ceil(parts * W * n) / parts - W * n;
+      const double t = all + 1.6 * (1. - even) * even * L + even * even * even * even * rest * mean;
       span = t > L ? t : L;
     }
     const double t = tile * span + (n > 1 ? 2.0 + 0.193 * MB * n : 0.);
