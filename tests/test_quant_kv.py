@@ -205,7 +205,8 @@ def test_cache_arguments_refused(which, kw, rc):
     ("decode", dict(chunk=0), INV), ("decode", dict(n=0), INV), ("decode", dict(nb=16), WSP),
     ("decode", dict(ws=None), WSP), ("decode", dict(chunk=1 << 30, n=4), UNS),
     ("decode", dict(scale=float("inf")), INV), ("decode", dict(scale=float("nan")), INV),
-    ("decode", dict(chunk=(1 << 30) + 128, n=1, wg=2), UNS), ("decode", dict(wg=1), INV), ("decode", dict(wg=5), INV), ("decode", dict(B=300, wg=599), INV),
+    ("decode", dict(chunk=(1 << 30) + 128, n=1, wg=2), UNS), ("decode", dict(wg=1), INV),
+    ("decode", dict(wg=5), INV), ("decode", dict(B=300, wg=599), INV),
     ("decode", dict(B=300, n=300, wg=90000), UNS),
     ("chunk", dict(n_host=TOO_MANY), INV), ("chunk", dict(n_host=NEGATIVE), INV),
     ("chunk", dict(n_host=START, n_new=FAKE), INV), ("prefill", dict(n_host=TOO_MANY), INV),

@@ -599,7 +599,7 @@ def test_prefill(gpu_ctx, fmt, B, Hkv, G, D, lens, C, counts, page, io):
 
 
 @pytest.mark.parametrize("B,Hkv,splits", [(70, 2, 0), (70, 8, 1), (33, 8, 2), (33, 8, 1), (64, 1, 8),
-                                          (13, 5, 3)])
+                                          (13, 5, 3), (300, 1, 0), (300, 1, 2)])
 def test_prefill_of_ragged_batches(gpu_ctx, B, Hkv, splits):
     """More (sequence, head, split) groups than the 512 that are ordered by their rows, and
     as many; sequences without rows among them."""
