@@ -772,9 +772,11 @@ constexpr int kMergeBatch = 4;  // splits whose partials the merge loads in one 
 // thread per 4 consecutive d of a row, 16-byte partial loads, 32-bit index
 // arithmetic. (One thread per element with 64-bit divisions took 31 us on
 // C4's 55 MB, 1.7 TB/s, measured on MI355X.) Rows i >= n_new[b] are zeros.
-// Splits that saw no token of a row (m = -inf, l = 0) drop out. The partials
-// have the kernel's (padded) row stride D; GEN: outputs have the real head
-// dim a.D, stored element by element.
+// Splits that saw no token of a row (m = -inf, l = 0) drop out; one whose
+// scores all are NaN (the running maximum passes over NaN: m = -inf, l = NaN)
+// makes the row NaN, as it would be in one split. The partials have the
+// kernel's (padded) row stride D; GEN: outputs have the real head dim a.D,
+// stored element by element.
 template <int D, bool GEN>
 __global__ __launch_bounds__(256) void k_prefill_merge(PrefillArgs a) {
   constexpr int V = D / 4;  // threads per row
@@ -795,8 +797,8 @@ __global__ __launch_bounds__(256) void k_prefill_merge(PrefillArgs a) {
   float o[4] = {0.f, 0.f, 0.f, 0.f};
   // One split's weighted partial into (L, o), in split order.
   auto add = [&](float2 ml, float4 x, float M, float& L) {
-    if (ml.x == -INFINITY) return;
-    const float wgt = fast_exp2(ml.x - M);
+    if (ml.x == -INFINITY && ml.y == 0.f) return;
+    const float wgt = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);  // (0 * NaN is NaN)
     L = fmaf(wgt, ml.y, L);
     o[0] = fmaf(wgt, x.x, o[0]);
     o[1] = fmaf(wgt, x.y, o[1]);

@@ -354,3 +354,33 @@ def test_workgroup_sizes_give_the_same_bits(D, G, C):
     want = torch.softmax(sc, -1) @ vv
     for o in outs[1::2]:
         assert rel_err(o[3, :, 0].double().cpu().numpy(), want.numpy()) < BF16_TOL
+
+
+@pytest.mark.parametrize("D", [64, 80])
+@pytest.mark.parametrize("n_splits", [1, 2, 3, 5])
+def test_prefill_keeps_nan_keys_of_any_split(gpu_ctx, D, n_splits):
+    """Queries whose every token in one split has a NaN key are NaN, as with one split:
+    the first position of a later split, a whole split, every split. The rows that
+    attend none of them keep the bits of a call without NaN."""
+    banner(f"prefill NaN split D={D} n_splits={n_splits}")
+    gpu = _gpu()
+    rng = np.random.default_rng(16)
+    B, H, G, P, C = 2, 3, 2, 70, 150  # 220 positions; splits of 128 (2, 3) or 64 tokens
+    k, v = (rng.standard_normal((B, P + C, H, D)).astype(np.float32) for _ in range(2))
+    q = to_dev(rng.standard_normal((B, C, H * G, D)).astype(np.float32), torch.bfloat16)
+    bad, want = k.copy(), np.zeros((B, C, H, D), bool)
+    bad[0, 128, 0, 3] = bad[0, 192, 1, 3] = np.nan
+    bad[0, 128:, 2, 40] = bad[1, :, 1, 7] = np.nan
+    want[0, 128 - P:, [0, 2]] = want[0, 192 - P:, 1] = want[1, :, 1] = True
+    outs = []
+    for keys in (k, bad):
+        cache = gpu.kv_cache_create(gpu_ctx, gpu.KVCacheConfig(B, P + C, 1, H * G, D, n_kv_heads=H,
+                                                               dtype=torch.bfloat16))
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, to_dev(keys[:, :P]), to_dev(v[:, :P]))
+        out = torch.empty_like(q)
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, to_dev(keys[:, P:]), to_dev(v[:, P:]), q, out,
+                             n_splits=n_splits)
+        outs.append(out)
+    want = torch.from_numpy(np.repeat(want, G, 2)).to("cuda")
+    assert torch.equal(torch.isnan(outs[1]), want)
+    assert torch.equal(outs[1][~want], outs[0][~want])

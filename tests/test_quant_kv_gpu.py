@@ -896,3 +896,39 @@ def test_offsets_past_32_bits(gpu_ctx):
     m.append(_np(k), _np(v))
     _check_attention(out, q, m, G, D ** -0.5, False, True, None, True)
     _check_stored(gpu, gpu_ctx, cache, m)
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5])
+def test_prefill_keeps_nan_keys_of_any_split(gpu_ctx, fmt, page, splits):
+    """Queries whose every token in one split has a NaN key are NaN, as with one
+    split: the first position of a later split, a whole split, every split. The
+    rows that attend none of them keep the bits of a call without NaN."""
+    banner(f"quant prefill NaN split {fmt} page={page} splits={splits}")
+    rng = np.random.default_rng(15)
+    B, H, G, D, P, C = 2, 3, 2, 64, 70, 150  # 220 positions; splits of 128 (2, 3) or 64 tokens
+    prefix = [_rows(rng, B, P, H, D) for _ in range(2)]
+    k, v = _rows(rng, B, C, H, D), _rows(rng, B, C, H, D)
+    q = _dev(rng.standard_normal((B, C, H * G, D)).astype(np.float32), BF16)
+    want = np.zeros((B, C, H, D), bool)
+    bad_prefix, bad = prefix[0].copy(), k.copy()
+    for at, h in ((128, 0), (192, 1)):  # the first position of a split
+        bad[0, at - P, h, 3] = np.nan
+        want[0, at - P:, h] = True
+    bad[0, 128 - P:, 2, 40] = np.nan  # every position past 127
+    want[0, 128 - P:, 2] = True
+    bad_prefix[1, :, 1, 7] = np.nan  # every key of a head
+    bad[1, :, 1, 7] = np.nan
+    want[1, :, 1] = True
+    outs = []
+    for first, keys in ((prefix[0], k), (bad_prefix, bad)):
+        gpu, cache, _ = _make(gpu_ctx, B, P + C, H, G, D, fmt, page)
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, _dev(first, F32), _dev(prefix[1], F32))
+        out = torch.empty_like(q)
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, _dev(keys, F32), _dev(v, F32), q, out,
+                             n_splits=splits)
+        outs.append(out)
+    want = torch.from_numpy(np.repeat(want, G, 2)).to("cuda:0")
+    assert torch.equal(torch.isnan(outs[1]), want)
+    assert torch.equal(outs[1][~want], outs[0][~want])
