@@ -365,9 +365,10 @@ int skv_q_prefill_plan(int B, int C, int H_q, int H_kv, int D, const int32_t* le
  * chunk, and the fills advanced, in one call. q, out [B, C, H_q, D] of q_dt /
  * out_dt; H_q / H_kv in {1, 2, 4, 8}; n_new and n_host as in
  * skv_q_append_chunk; n_splits (skv_q_prefill_plan) and ws as in
- * skv_prefill_attn (skv_prefill_workspace_bytes) with 2 B int32 more. Q and the
- * probabilities enter the matrix cores as bf16, K and V exactly, as over a bf16
- * cache that holds the same values. */
+ * skv_prefill_attn (skv_prefill_workspace_bytes) with 2 B int32 more. K and V
+ * enter the products exactly. Products are of fp32 accuracy where q or out is
+ * fp32 (three matrix-core products of one); with both bf16 the probabilities
+ * are rounded to bf16, as over a bf16 cache that holds the same values. */
 int skv_q_append_prefill_attn(void* out, const void* q, void* k, void* k_scale, void* v,
                               void* v_scale, const void* k_new, const void* v_new, int32_t* lens,
                               const int32_t* n_new, const int32_t* n_host /* host */,

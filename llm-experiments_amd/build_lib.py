@@ -17,9 +17,9 @@ LIB = os.path.join(HERE, "libskv.so")
 SOURCES = ["skv_api.hip", "append.hip", "decode_attn.hip", "decode_attn_generic.hip",
            "decode_attn_generic_paged.hip", "decode_gqa_mfma.hip",
            "decode_direct.hip", "prefill_attn.hip", "prefill_attn.hip:mxfp4",
-           "prefill_attn.hip:mxfp8", "quant_cache.hip", "quant_decode.hip", "model_ops.hip",
-           "gemm.hip", "sample.hip", "flash_split.hip", "flash_fp32.hip",
-           "flash_fp32.hip:wide_bwd", "bpe_tokenizer.cpp"]
+           "prefill_attn.hip:mxfp8", "prefill_attn.hip:mxfp4_f32", "prefill_attn.hip:mxfp8_f32",
+           "quant_cache.hip", "quant_decode.hip", "model_ops.hip", "gemm.hip", "sample.hip",
+           "flash_split.hip", "flash_fp32.hip", "flash_fp32.hip:wide_bwd", "bpe_tokenizer.cpp"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -48,9 +48,11 @@ SOURCE_FLAGS = {"flash_fp32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                 # the flash backward past a head dim of 128: the same source as its own
                 # translation unit, accumulators free to live in AGPRs
                 "flash_fp32.hip:wide_bwd": ["-DSKV_FLASH_WIDE_BWD=1"],
-                # the prefill over block-scaled caches
+                # the prefill over block-scaled caches, and with fp32 products
                 "prefill_attn.hip:mxfp4": ["-DSKV_PREFILL_QF=4"],
-                "prefill_attn.hip:mxfp8": ["-DSKV_PREFILL_QF=8"]}
+                "prefill_attn.hip:mxfp8": ["-DSKV_PREFILL_QF=8"],
+                "prefill_attn.hip:mxfp4_f32": ["-DSKV_PREFILL_QF=4", "-DSKV_PREFILL_F32=1"],
+                "prefill_attn.hip:mxfp8_f32": ["-DSKV_PREFILL_QF=8", "-DSKV_PREFILL_F32=1"]}
 
 _NOISE = "is not a recognized feature for this target"  # hipcc's host pass on -packed-fp32-ops
 

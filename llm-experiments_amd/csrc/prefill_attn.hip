@@ -55,15 +55,28 @@
 //    group of V goes into LDS as zeros and its tile is marked: a masked
 //    probability of 0 would make it NaN for queries that do not attend the
 //    token; those that do get their NaN from the scales afterwards.
+//  * Precision: bf16 queries, K and V enter exactly, sums and statistics are
+//    fp32, and the probabilities are rounded to bf16 (2^-8 of each; their sum
+//    l takes them unrounded): one product, where a second part of p would cost
+//    half as many MFMAs again. Over a bf16 cache fp32 queries are rounded to
+//    bf16 too. Over a block-scaled cache fp32 in or out gets products of fp32
+//    accuracy, as in decode and as over an fp32 cache (F32): K and V are exact
+//    in bf16, so q and p as three bf16 parts each (all 24 bits; what lies below
+//    2^-133 is lost) make three products of one. q's parts are 3 x D / 16
+//    operands, so a wavefront has its SIMD to itself past D = 64 and a
+//    workgroup 128 rows; at 256 about 190 registers spill. MI355X, us, bf16
+//    in and out | fp32: 4-bit, 4 x 16 x 128, 512 after 32256 506 | 1434 (1.14
+//    PFLOP/s of the three products, bound as the one); 4 x 8 x 2 x 256, 512
+//    after 1000 124 | 467; 8-bit, 4 x 12 x 64, 512 after 2000 47.6 | 76.5.
 #include <cmath>
 #include <type_traits>
 
 #include "quant.h"
 #include "skv_common.h"
 
-// This file is three translation units: the plain caches' kernels and the C
+// This file is five translation units: the plain caches' kernels and the C
 // entry points, and with SKV_PREFILL_QF = 4 or 8 the kernels of that
-// block-scaled format.
+// block-scaled format, with SKV_PREFILL_F32 those of fp32 accuracy.
 
 namespace skv {
 namespace prefill {
@@ -96,9 +109,11 @@ struct PrefillArgs {
 };
 
 // The kernel of a block-scaled cache at the padded head dim DK with W
-// wavefronts a workgroup; 0, or SKV_E_UNSUPPORTED without one.
+// wavefronts a workgroup (f32: 4); 0, or SKV_E_UNSUPPORTED without one.
 int launch_q4(const PrefillArgs& a, int DK, int G, int W, unsigned blocks, hipStream_t s);
 int launch_q8(const PrefillArgs& a, int DK, int G, int W, unsigned blocks, hipStream_t s);
+int launch_q4_f32(const PrefillArgs& a, int DK, int G, int W, unsigned blocks, hipStream_t s);
+int launch_q8_f32(const PrefillArgs& a, int DK, int G, int W, unsigned blocks, hipStream_t s);
 
 }  // namespace prefill
 
@@ -201,8 +216,12 @@ __device__ __forceinline__ void store4(void* out, size_t i, int dt, const float 
 // W: wavefronts per workgroup (4 at D = 256, where a wavefront holds twice
 // the queries and accumulators, ~310 registers: one per SIMD).
 // QF: 4 or 8 for a block-scaled cache of that many bits (PAGED: in pages), else 0.
-template <int D, int G, int LV, int W, int QF = 0, bool PAGED = false>
-__global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(PrefillArgs a) {
+// F32 (block-scaled): products of fp32 accuracy.
+template <int D, int G, int LV, int W, int QF = 0, bool PAGED = false, bool F32 = false>
+__global__ __launch_bounds__(W * 64, D > (F32 ? 64 : 128) ? 1 : 2) void k_prefill_mfma(
+    PrefillArgs a) {
+  static_assert(!F32 || QF != 0, "K and V exact in bf16");
+  constexpr int NP = F32 ? 3 : 1;  // bf16 parts of q and p
   constexpr int KB = D / 16;  // k-blocks of the QK^T product
   constexpr int DB = D / 32;  // 32-row d blocks of O^T
   constexpr int BM = W * kQB * 32;  // query rows of the workgroup
@@ -289,9 +308,10 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
   const int s1 = row0 < R ? min(min(s0 + span, kv_end), P + last_row / G + 1) : s0;
   const int first_q = row0 / G;  // smallest query index of the tile
 
-  // ---- queries of this wavefront's two row blocks, as MFMA operand B ----
-  bf16x8 qf[kQB][KB];
+  // ---- queries of this wavefront's row blocks, as MFMA operand B ----
+  bf16x8 qf[NP][kQB][KB];
   int qrow[kQB];
+  float qscale[kQB];  // scores to log2 units
 #pragma unroll
   for (int qb = 0; qb < kQB; ++qb) {
     const int r = row0 + (wave * kQB + qb) * 32 + lc;
@@ -300,6 +320,25 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
     const int i = r / G, h = hk * G + r % G;
     const size_t qoff = (((size_t)b * a.C + i) * a.Hq + h) * RS;
     const size_t qsafe = ok ? qoff : 0;  // rows past the chunk read row 0 and are zeroed
+    qscale[qb] = a.qscale;
+    float qsize = 1.f;
+    if constexpr (F32) {
+      // A query whose elements all are below 2^-64 enters 2^40 times as large,
+      // for its parts not to end below bf16's smallest number.
+      float big = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int e = kb * 16 + g * 8;
+        float v[8];
+        load8_f32(a.q, qsafe + (e < RS ? e : 0), a.q_dt, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(v[j]));
+      }
+      if (xor32_max(big) < 0x1p-64f) {  // lanes l and l ^ 32 hold the same query
+        qsize = 0x1p40f;
+        qscale[qb] *= 0x1p-40f;
+      }
+    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       float v[8];
@@ -319,7 +358,15 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
         load8_f32(a.q, qsafe + kb * 16 + g * 8, a.q_dt, v);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) qf[qb][kb][j] = (__bf16)(ok ? v[j] : 0.f);
+      for (int j = 0; j < 8; ++j) {
+        float r = ok ? v[j] : 0.f;
+        if constexpr (F32) r *= qsize;
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+          qf[t][qb][kb][j] = (__bf16)r;
+          r -= (float)qf[t][qb][kb][j];  // exact
+        }
+      }
     }
   }
 
@@ -541,9 +588,11 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
         const bf16x8 ka =
             *reinterpret_cast<const bf16x8*>(sk(stage) + at(tb * 32 + lc, kb * 2 + g));
 #pragma unroll
-        for (int qb = 0; qb < kQB; ++qb)
-          sc[tb][qb] =
-              __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qf[qb][kb], sc[tb][qb], 0, 0, 0);
+        for (int t = 0; t < NP; ++t)
+#pragma unroll
+          for (int qb = 0; qb < kQB; ++qb)
+            sc[tb][qb] =
+                __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qf[t][qb][kb], sc[tb][qb], 0, 0, 0);
       }
     // Accumulator slot r of half tb holds token t0 + tb*32 + (r/4)*8 + 4g + r%4.
     if (need_mask) {
@@ -574,7 +623,7 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
       // <= 2^8 (exact in fp32, in range for bf16) and O, l are rescaled
       // on a few tiles instead of every one. O and l always refer to the
       // same m.
-      const float tm = tmax * a.qscale;
+      const float tm = tmax * qscale[qb];
       const bool upd = tm > m[qb] + 8.f;  // also true on the first finite tile
       if (__ballot(upd) != 0ull) {        // wave-uniform branch
         const float alpha = upd ? fast_exp2(m[qb] - tm) : 1.f;  // m = -inf: 0
@@ -591,9 +640,10 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float p = fast_exp2(fmaf(sc[tb][qb][kk * 8 + j], a.qscale, -m_use));
+            const float p = fast_exp2(fmaf(sc[tb][qb][kk * 8 + j], qscale[qb], -m_use));
             ls += p;
-            pf[qb][tb * 2 + kk][j] = (__bf16)p;
+            if constexpr (F32) sc[tb][qb][kk * 8 + j] = p;  // split where it is used
+            else pf[qb][tb * 2 + kk][j] = (__bf16)p;
           }
       l[qb] += ls;
     }
@@ -612,7 +662,24 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+        for (int kk = 0; kk < 2; ++kk) {
+          bf16x8 pp[kQB][NP];
+#pragma unroll
+          for (int qb = 0; qb < kQB; ++qb) {
+            if constexpr (F32) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                float r = sc[tb][qb][kk * 8 + j];
+#pragma unroll
+                for (int t = 0; t < NP; ++t) {
+                  pp[qb][t][j] = (__bf16)r;
+                  r -= (float)pp[qb][t][j];  // exact
+                }
+              }
+            } else {
+              pp[qb][0] = pf[qb][tb * 2 + kk];
+            }
+          }
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
             const int d = db * 32 + dq;
@@ -625,10 +692,13 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
             const bf16x8 va = __builtin_bit_cast(
                 bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-            for (int qb = 0; qb < kQB; ++qb)
-              o[qb][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[qb][tb * 2 + kk],
-                                                                   o[qb][db], 0, 0, 0);
+            for (int t = 0; t < NP; ++t)
+#pragma unroll
+              for (int qb = 0; qb < kQB; ++qb)
+                o[qb][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pp[qb][t], o[qb][db], 0,
+                                                                     0, 0);
           }
+        }
     }
 
     if constexpr (QF != 0) {
@@ -730,37 +800,47 @@ __global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void k_prefill_mfma(Prefil
 }  // namespace
 
 // (LV = 8: rows of a runtime stride; a head dim is a multiple of 32 here)
-template <int QF>
+template <int QF, bool F32>
 static int launch_q(const PrefillArgs& a, int DK, int G, int W, unsigned blocks, hipStream_t s) {
 #define SKV_PQ(DD, GG, WW)                                                                    \
   if (DK == DD && G == GG && W == WW) {                                                       \
     if (a.c.bt)                                                                               \
-      hipLaunchKernelGGL((k_prefill_mfma<DD, GG, 8, WW, QF, true>), dim3(blocks),             \
+      hipLaunchKernelGGL((k_prefill_mfma<DD, GG, 8, WW, QF, true, F32>), dim3(blocks),        \
                          dim3(WW * 64), 0, s, a);                                             \
     else                                                                                      \
-      hipLaunchKernelGGL((k_prefill_mfma<DD, GG, 8, WW, QF, false>), dim3(blocks),            \
+      hipLaunchKernelGGL((k_prefill_mfma<DD, GG, 8, WW, QF, false, F32>), dim3(blocks),       \
                          dim3(WW * 64), 0, s, a);                                             \
     return 0;                                                                                 \
   }
 #define SKV_PQG(DD, WW) SKV_PQ(DD, 1, WW) SKV_PQ(DD, 2, WW) SKV_PQ(DD, 4, WW) SKV_PQ(DD, 8, WW)
-  SKV_PQG(32, 4) SKV_PQG(32, 8) SKV_PQG(64, 4) SKV_PQG(64, 8)
-  SKV_PQG(128, 4) SKV_PQG(128, 8) SKV_PQG(256, 4)
+  SKV_PQG(32, 4) SKV_PQG(64, 4) SKV_PQG(128, 4) SKV_PQG(256, 4)
+  if constexpr (!F32) {
+    SKV_PQG(32, 8) SKV_PQG(64, 8) SKV_PQG(128, 8)
+  }
 #undef SKV_PQG
 #undef SKV_PQ
   return SKV_E_UNSUPPORTED;
 }
 
+#ifdef SKV_PREFILL_F32
+#define SKV_PQ_NAME(BITS) launch_q##BITS##_f32
+constexpr bool kF32 = true;
+#else
+#define SKV_PQ_NAME(BITS) launch_q##BITS
+constexpr bool kF32 = false;
+#endif
 #if SKV_PREFILL_QF == 4
-int prefill::launch_q4(const PrefillArgs& a, int DK, int G, int W, unsigned blocks,
-                       hipStream_t s) {
-  return launch_q<4>(a, DK, G, W, blocks, s);
+int prefill::SKV_PQ_NAME(4)(const PrefillArgs& a, int DK, int G, int W, unsigned blocks,
+                            hipStream_t s) {
+  return launch_q<4, kF32>(a, DK, G, W, blocks, s);
 }
 #else
-int prefill::launch_q8(const PrefillArgs& a, int DK, int G, int W, unsigned blocks,
-                       hipStream_t s) {
-  return launch_q<8>(a, DK, G, W, blocks, s);
+int prefill::SKV_PQ_NAME(8)(const PrefillArgs& a, int DK, int G, int W, unsigned blocks,
+                            hipStream_t s) {
+  return launch_q<8, kF32>(a, DK, G, W, blocks, s);
 }
 #endif
+#undef SKV_PQ_NAME
 
 }  // namespace skv
 
@@ -1014,9 +1094,10 @@ int prefill_attn_impl(void* out, const void* q, const void* k_cache, const void*
   // (a block-scaled tile's codes cost the 128-row kernel a few spilled registers:
   // 6 ragged x 8 kv heads x 4 x 128, <= 333 after <= 1900, 8-bit: 88.6 us, 82.5
   // with 256 rows; 3 x 16 x 128, 640 after 8000, 4-bit: 186 and 273)
-  const int W = qc && n_new && DK <= 128
-                    ? kWaves
-                    : tile_waves(B, C, H_kv, G, D, n_splits, n_new != nullptr);
+  const bool f32 = qc && (q_dt == SKV_F32 || out_dt == SKV_F32);
+  const int W = f32                        ? 4
+                : qc && n_new && DK <= 128 ? kWaves
+                                           : tile_waves(B, C, H_kv, G, D, n_splits, n_new != nullptr);
   a.n_qt = n_query_tiles(C, G, W);
   a.n_splits = n_splits;
   a.n_groups = B * H_kv * n_splits;
@@ -1031,8 +1112,10 @@ int prefill_attn_impl(void* out, const void* q, const void* k_cache, const void*
   const int LV = load_form(D);
   if (qc) {
     a.c = *qc;
-    const int rc = cache_dt == SKV_MXFP4 ? prefill::launch_q4(a, DK, G, W, (unsigned)blocks, s)
-                                         : prefill::launch_q8(a, DK, G, W, (unsigned)blocks, s);
+    const auto launch_q = cache_dt == SKV_MXFP4
+                              ? (f32 ? prefill::launch_q4_f32 : prefill::launch_q4)
+                              : (f32 ? prefill::launch_q8_f32 : prefill::launch_q8);
+    const int rc = launch_q(a, DK, G, W, (unsigned)blocks, s);
     if (rc) return set_error(rc, "%s: no kernel for head_dim %d, G=%d", fn, D, G);
   } else {
 #define SKV_PF(DD, GG, LL, WW)                                                                \

@@ -594,9 +594,11 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
     flash_attention, gpu/gpu_kernels.py:695-701, shifted by the cached
     prefix). The layer's fills advance by n_new. Returns the new fills.
 
-    A bfloat16 or block-scaled cache runs the bf16 MFMA prefill; a float32
-    cache runs every product with fp32 accuracy (float32 q and out). The
-    queries attend the chunk's rows as the cache stores them.
+    A bfloat16 cache runs the bf16 MFMA prefill (float32 q is rounded to
+    bfloat16), and so does a block-scaled one with bfloat16 q and out; with
+    float32 q or out its products have fp32 accuracy, at up to three times the
+    work. A float32 cache runs every product with fp32 accuracy (float32 q and
+    out). The queries attend the chunk's rows as the cache stores them.
 
     Raises ValueError (before any GPU work) on a bad layer, shapes, a chunk
     that would overflow a sequence ("Cache is full"), a paged cache that is

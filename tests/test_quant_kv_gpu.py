@@ -932,3 +932,91 @@ def test_prefill_keeps_nan_keys_of_any_split(gpu_ctx, fmt, page, splits):
     want = torch.from_numpy(np.repeat(want, G, 2)).to("cuda:0")
     assert torch.equal(torch.isnan(outs[1]), want)
     assert torch.equal(outs[1][~want], outs[0][~want])
+
+
+def _check_prefill_fp32(got, q, m, G, scale, rows, out_bf16):
+    """Prefill with fp32 q or out, got, q [B, C, Hq, D]. The bounds at the top of the
+    file, with what this kernel does otherwise: a score is 3 D / 16 products of 16
+    elements (the second and third parts of q are 2^-8 and 2^-16 of it): (D + 3 D / 16
+    + 8) u A, within 2 (D + 8) u A. A lane sums its column's tokens alone: of each 16,
+    three products and one more rounding inside them, so n / 4 steps, 64 for the
+    rescalings, the sum of p, the merge and the division. Three parts hold all of p."""
+    got, q = _np(got), _np(q)
+    B, C, Hq, D = q.shape
+    for b in range(B):
+        n, r = int(m.lens[b]), int(rows[b])
+        assert not got[b, r:].any(), f"rows past the count of sequence {b} are not zeros"
+        last = n - r + np.arange(r)
+        for h in range(Hq):
+            want, mag, big = qo.attention(q[b, :r, h], m.k[b, :n, h // G], m.v[b, :n, h // G],
+                                          scale, last)
+            tol = (2 * (D + 8) * U * big + (n / 4 + 64) * U)[:, None] * mag
+            bound = tol + (2.0 ** -8 * (np.abs(want) + tol) if out_bf16 else 0.0) + 1e-37
+            err = np.abs(got[b, :r, h] - want)
+            assert not np.isnan(got[b, :r, h]).any()
+            assert (err <= bound).all(), (
+                f"sequence {b} head {h}: off by {(err / bound).max():.2f} of the bound")
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+@pytest.mark.parametrize("B,Hkv,G,D,lens,C,counts,page", [
+    (1, 1, 1, 32, [0], 1, None, 0), (2, 2, 8, 32, [3, 200], 47, [47, 9], 16),
+    (2, 2, 1, 64, [0, 70], 33, [33, 5], 0), (1, 3, 4, 64, [300], 257, None, 8),
+    (2, 1, 2, 96, [129, 3], 40, None, 8), (3, 2, 4, 128, [0, 64, 200], 50, [50, 0, 17], 16),
+    (2, 1, 1, 128, [1000, 40], 130, [7, 130], 0), (1, 1, 8, 128, [63], 65, None, 1),
+    (1, 2, 1, 160, [65], 31, None, 1), (2, 1, 2, 256, [100, 0], 66, None, 0),
+    (1, 1, 8, 256, [5], 20, [11], 4), (1, 2, 4, 224, [500], 70, None, 0)])
+def test_prefill_of_fp32_keeps_fp32(gpu_ctx, fmt, B, Hkv, G, D, lens, C, counts, page):
+    """fp32 q or output: products of fp32 accuracy, as in decode over the same cache."""
+    banner(f"quant prefill fp32 {fmt} B={B} Hkv={Hkv} G={G} D={D} lens={lens} C={C} {counts} {page}")
+    rng = np.random.default_rng(C + D)
+    rows = np.full(B, C) if counts is None else np.asarray(counts)
+    for splits, qt, ot in ((0, F32, F32), (1, F32, F32), (3, F32, F32), (1, BF16, F32),
+                           (2, F32, BF16)):
+        gpu, cache, m = _make(gpu_ctx, B, max(lens) + C + 1, Hkv, G, D, fmt, page)
+        _fill(gpu, gpu_ctx, cache, m, rng, lens)
+        k, v = (_dev(_rows(rng, B, C, Hkv, D), F32) for _ in range(2))
+        q = _dev(rng.standard_normal((B, C, Hkv * G, D)).astype(np.float32), qt)
+        out = torch.full(q.shape, 9.0, dtype=ot, device="cuda:0")
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out, n_new=counts, n_splits=splits)
+        m.append(_np(k), _np(v), counts)
+        _check_prefill_fp32(out, q, m, G, D ** -0.5, rows, ot == BF16)
+        _check_stored(gpu, gpu_ctx, cache, m)
+
+
+@pytest.mark.parametrize("G,D", [(1, 64), (2, 96), (4, 256)])
+def test_prefill_of_tiny_queries(gpu_ctx, G, D):
+    """Scores of ordinary size from queries whose last bits bf16 cannot hold unscaled."""
+    banner(f"quant prefill tiny queries G={G} D={D}")
+    rng = np.random.default_rng(29)
+    B, H, C = 1, 2, 130
+    gpu, cache, m = _make(gpu_ctx, B, C, H, G, D, "fp8")
+    k = _dev(_rows(rng, B, C, H, D).astype(np.float64) * 2.0 ** 118, F32)
+    v = _dev(_rows(rng, B, C, H, D), F32)
+    q = _dev((rng.standard_normal((B, C, H * G, D)) * 2.0 ** -122).astype(np.float32), F32)
+    out = torch.empty_like(q)
+    scale = 16 * D ** -0.5
+    gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out, scale=scale)
+    m.append(_np(k), _np(v))
+    _check_prefill_fp32(out, q, m, G, scale, [C], False)
+
+
+def test_prefill_of_fp32_nan_groups(gpu_ctx):
+    """NaN groups of K and V reach the queries that attend their tokens, no others."""
+    banner("quant prefill fp32 NaN")
+    rng = np.random.default_rng(14)
+    B, H, D, C = 1, 2, 64, 150
+    for splits in (1, 2):
+        gpu, cache, m = _make(gpu_ctx, B, 300, H, 1, D, "fp8")
+        _fill(gpu, gpu_ctx, cache, m, rng, [70])
+        k, v = _rows(rng, B, C, H, D), _rows(rng, B, C, H, D)
+        k[0, 60, 0, 3] = np.nan
+        v[0, 100, 1, 40] = np.nan
+        q = _dev(rng.standard_normal((B, C, H, D)).astype(np.float32), F32)
+        out = torch.empty_like(q)
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, _dev(k, F32), _dev(v, F32), q, out,
+                             n_splits=splits)
+        want = np.zeros((B, C, H, D), bool)
+        want[0, 60:, 0] = True
+        want[0, 100:, 1, 32:] = True
+        np.testing.assert_array_equal(torch.isnan(out).cpu().numpy(), want)
