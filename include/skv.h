@@ -363,7 +363,7 @@ int skv_q_prefill_plan(int B, int C, int H_q, int H_kv, int D, const int32_t* le
 /* skv_append_prefill_attn for a block-scaled cache (contiguous or paged):
  * skv_q_append_chunk, causal attention of the chunk's queries over prefix +
  * chunk, and the fills advanced, in one call. q, out [B, C, H_q, D] of q_dt /
- * out_dt; H_q / H_kv in {1, 2, 4, 8}; n_new and n_host as in
+ * out_dt; H_q / H_kv in {1, 2, 4, 8}; scale > 0 and finite; n_new and n_host as in
  * skv_q_append_chunk; n_splits (skv_q_prefill_plan) and ws as in
  * skv_prefill_attn (skv_prefill_workspace_bytes) with 2 B int32 more. K and V
  * enter the products exactly. Products are of fp32 accuracy where q or out is

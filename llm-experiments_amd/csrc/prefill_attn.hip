@@ -1037,7 +1037,8 @@ int prefill_attn_impl(void* out, const void* q, const void* k_cache, const void*
               H_kv);
   SKV_REQUIRE((qc ? is_quant(cache_dt) : dt_ok(cache_dt)) && dt_ok(q_dt) && dt_ok(out_dt),
               SKV_E_INVALID, "%s: bad dtype", fn);
-  SKV_REQUIRE(scale > 0.f, SKV_E_INVALID, "%s: scale must be > 0", fn);
+  SKV_REQUIRE(scale > 0.f && (!qc || std::isfinite(scale)), SKV_E_INVALID,
+              "%s: scale must be > 0%s", fn, qc ? " and finite" : "");
   if (cache_dt == SKV_F32) {  // fp32 cache: the fp32 MFMA path, no split
     SKV_REQUIRE(q_dt == SKV_F32 && out_dt == SKV_F32, SKV_E_UNSUPPORTED,
                 "%s: an fp32 cache takes fp32 q and out", fn);

@@ -601,8 +601,9 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
     out). The queries attend the chunk's rows as the cache stores them.
 
     Raises ValueError (before any GPU work) on a bad layer, shapes, a chunk
-    that would overflow a sequence ("Cache is full"), a paged cache that is
-    not block-scaled, or a float32 cache with non-float32 q/output.
+    that would overflow a sequence ("Cache is full"), a scale that is not > 0
+    (with a block-scaled cache: and finite), a paged cache that is not
+    block-scaled, or a float32 cache with non-float32 q/output.
     """
     _check_layer(cache, layer_idx)
     if cache.paged and not cache.quantized:

@@ -314,3 +314,9 @@ def test_read_refuses_bad_starts(monkeypatch):
     assert seen == [[0], [5], [5], [1, 2], [3, 4], [7]]
     with pytest.raises(ValueError, match="at least one row"):
         gpu.kv_cache_read(ctx, cache, 0, rows[:, :0], rows[:, :0])
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -0.125])
+def test_prefill_refuses_a_scale_that_is_not_positive_and_finite(scale):
+    assert _call("prefill", scale=scale) == INV
+    assert b"scale" in _lib.lib().skv_last_error()
