@@ -303,9 +303,9 @@ int skv_q_append(void* k, void* k_scale, void* v, void* v_scale, const void* k_n
 
 /* skv_append_chunk for a block-scaled cache: rows i < n[b] of k_new[b], [B, C,
  * H_kv, D] of in_dt, to positions lens[b] + i; rows past the capacity are not
- * written. n: n_new, or n_host (a host array, each entry in [0, C], read when
- * the call returns), or C with both NULL. advance != 0: then the fills advanced
- * as skv_advance does. Paged caches too. */
+ * written. n: n_new (device memory, each entry in [0, C]), or n_host (a host
+ * array, each entry in [0, C], read when the call returns), or C with both NULL.
+ * advance != 0: then the fills advanced as skv_advance does. Paged caches too. */
 int skv_q_append_chunk(void* k, void* k_scale, void* v, void* v_scale, const void* k_new,
                        const void* v_new, int32_t* lens, const int32_t* n_new,
                        const int32_t* n_host /* host */, int advance, const int32_t* block_table,

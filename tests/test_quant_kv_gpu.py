@@ -1020,3 +1020,52 @@ def test_prefill_of_fp32_nan_groups(gpu_ctx):
         want[0, 60:, 0] = True
         want[0, 100:, 1, 32:] = True
         np.testing.assert_array_equal(torch.isnan(out).cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("fmt,page,splits,io", [("fp4", 0, 1, BF16), ("fp8", 16, 2, BF16),
+                                                ("fp8", 0, 3, F32), ("fp4", 8, 1, F32)])
+def test_c_counts_on_the_device(gpu_ctx, fmt, page, splits, io):
+    """The C entry points with the counts in device memory, and an append that does
+    not advance: the bytes, fills and outputs of counts on the host."""
+    banner(f"quant device counts {fmt} page={page} splits={splits} {io}")
+    from simple_llm_amd import _lib
+    from simple_llm_amd.gpu import gpu_kv_quant as gq
+
+    rng = np.random.default_rng(47)
+    B, H, G, D, C, T = 4, 2, 4, 96, 37, 300
+    gpu, cache, m = _make(gpu_ctx, B, T, H, G, D, fmt, page)
+    _, twin, _ = _make(gpu_ctx, B, T, H, G, D, fmt, page)
+    lay, L = cache.layers[0], _lib.lib()
+    code = _lib.dtype_code(io)
+    q = _dev(rng.standard_normal((B, C, H * G, D)).astype(np.float32), io)
+    ws = torch.empty(L.skv_prefill_workspace_bytes(B, C, H * G, D, splits) + 8 * B,
+                     dtype=torch.uint8, device="cuda:0")
+    for counts in ([C, 0, 5, 36], [0, 1, C, 2], None):
+        n = None if counts is None else torch.tensor(counts, dtype=torch.int32, device="cuda:0")
+        n_ptr = None if n is None else n.data_ptr()
+        k, v = (_dev(_rows(rng, B, C, H, D), io) for _ in range(2))
+        sizes = (*gq._pages(cache), B, C, H, D, T, _lib.QUANT_FORMATS[cache.dtype], code,
+                 _lib.stream_handle(lay.lens.device))
+        chunk = (*gq._storage(lay), k.data_ptr(), v.data_ptr(), lay.lens.data_ptr(), n_ptr, None)
+        fills = lay.lens.clone()
+        assert L.skv_q_append_chunk(*chunk, 0, *sizes) == 0  # the rows alone
+        assert torch.equal(lay.lens, fills)
+        assert L.skv_q_append_chunk(*chunk, 1, *sizes) == 0  # the same rows again, and the fills
+        gpu.kv_cache_prefill(gpu_ctx, twin, 0, k, v, n_new=counts)
+        m.append(_np(k), _np(v), counts)
+        assert torch.equal(lay.lens, twin.layers[0].lens)
+        k, v = (_dev(_rows(rng, B, C, H, D), io) for _ in range(2))
+        out, want = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
+        rc = L.skv_q_append_prefill_attn(
+            out.data_ptr(), q.data_ptr(), *gq._storage(lay), k.data_ptr(), v.data_ptr(),
+            lay.lens.data_ptr(), n_ptr, None, *gq._pages(cache), B, C, H * G, H, D, T, D ** -0.5,
+            splits, ws.data_ptr(), ws.numel(), _lib.QUANT_FORMATS[cache.dtype], code, code, code,
+            _lib.stream_handle(lay.lens.device))
+        assert rc == 0
+        gpu.kv_cache_prefill(gpu_ctx, twin, 0, k, v, q, want, n_new=counts, n_splits=splits)
+        m.append(_np(k), _np(v), counts)
+        assert torch.equal(out, want)
+        for x in ("k_cache", "k_scale", "v_cache", "v_scale"):
+            assert torch.equal(getattr(lay, x).buffer, getattr(twin.layers[0], x).buffer)
+    lay.host_lens = m.lens.copy()
+    _check_stored(gpu, gpu_ctx, cache, m)
