@@ -1069,3 +1069,49 @@ def test_c_counts_on_the_device(gpu_ctx, fmt, page, splits, io):
             assert torch.equal(getattr(lay, x).buffer, getattr(twin.layers[0], x).buffer)
     lay.host_lens = m.lens.copy()
     _check_stored(gpu, gpu_ctx, cache, m)
+
+
+@pytest.mark.parametrize("fmt,page,splits,io", [("fp4", 0, 1, BF16), ("fp8", 16, 2, BF16),
+                                                ("fp4", 8, 0, BF16), ("fp8", 0, 0, F32),
+                                                ("fp4", 16, 3, F32)])
+def test_captured_chunk_outputs(gpu_ctx, fmt, page, splits, io):
+    """A captured ragged chunk, replayed: the eager call's bits where both take the same
+    splits, else within the bounds of float64 over the stored values."""
+    banner(f"quant captured chunk outputs {fmt} page={page} splits={splits} {io}")
+    rng = np.random.default_rng(53)
+    B, H, G, D, C, T = 3, 2, 4, 64, 30, 400
+    gpu, cache, m = _make(gpu_ctx, B, T, H, G, D, fmt, page)
+    _, twin, _ = _make(gpu_ctx, B, T, H, G, D, fmt, page)
+    counts = np.array([C, 0, 7])
+    k, v = (torch.zeros(B, C, H, D, device="cuda:0") for _ in range(2))
+    q = torch.zeros(B, C, H * G, D, dtype=io, device="cuda:0")
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    lay = cache.layers[0]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):  # before the capture, undone
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out, n_new=counts, n_splits=splits)
+    side.synchronize()
+    lay.lens.zero_()
+    lay.host_lens[:] = 0
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out, n_new=counts, n_splits=splits)
+    lay.host_lens[:] = 0
+    for _ in range(4):
+        k.copy_(_dev(_rows(rng, B, C, H, D), F32))
+        v.copy_(_dev(_rows(rng, B, C, H, D), F32))
+        q.copy_(_dev(rng.standard_normal((B, C, H * G, D)).astype(np.float32), io))
+        out.fill_(9.0)
+        gpu.kv_cache_prefill(gpu_ctx, twin, 0, k, v, q, want, n_new=counts, n_splits=splits)
+        graph.replay()
+        torch.cuda.synchronize()
+        lay.host_lens += counts
+        m.append(_np(k), _np(v), counts)
+        if splits:
+            assert torch.equal(out, want)
+        if io == F32:
+            _check_prefill_fp32(out, q, m, G, D ** -0.5, counts, False)
+        else:
+            _check_attention(out, q, m, G, D ** -0.5, False, True, counts, True)
+    _check_stored(gpu, gpu_ctx, cache, m)
