@@ -134,25 +134,6 @@ __device__ __forceinline__ bf16x8 decode8_bf16(const uint32_t* w, float s) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Eight codes to fp32 (exact).
-template <int BITS>
-__device__ __forceinline__ void decode8_f32(const uint32_t* w, float s, float (&x)[8]) {
-  f32x2 a, b, c, d;
-  if constexpr (BITS == 4) {
-    a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 0);
-    b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 2);
-    d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 3);
-  } else {
-    a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[0], s, false);
-    b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[0], s, true);
-    c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], s, false);
-    d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], s, true);
-  }
-  x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
-  x[4] = c[0]; x[5] = c[1]; x[6] = d[0]; x[7] = d[1];
-}
-
 // Eight elements of a runtime-dtype row quantised by this lane, four
 // neighbouring lanes (an aligned quad, all active) holding a group: the codes
 // in w, the group's scale byte returned. NaN orders above infinity as bits, so
