@@ -281,7 +281,10 @@ int skv_append_prefill_attn(void* out, const void* q, void* k_cache, void* v_cac
  * nearest even, saturating. A group that holds a NaN or an infinity is stored
  * as scale byte 255 and zero codes and reads back as NaN. The stored bytes do
  * not depend on the entry point or the input's type, and every value a cache
- * can hold is exact in bf16.
+ * can hold is exact in bf16. Attention divides by the softmax's sum last and
+ * moves its reference maximum in steps, so before the division a sum of n
+ * values of V is up to 2^8 n of the largest: V past 2^120 / n can overflow to an
+ * infinity or NaN.
  *
  * Layout: codes [B, H_kv, T_cap, D * bits / 8], scales [B, H_kv, T_cap,
  * D / 32] (head-major, unlike the plain caches: a head's rows lie end to end).
@@ -324,10 +327,12 @@ int skv_q_read(void* k_out, void* v_out, const void* k, const void* k_scale, con
 /* Split sizing of skv_q_decode_attn (host-only): chunk_tokens (a multiple of
  * 128) of one kv head per workgroup, n_chunks = ceil(max_len / chunk_tokens)
  * and n_wg, the workgroups of a kv head. total_len: filled tokens over the
- * batch (<= 0: B * max_len). covering != 0: n_wg serves any lengths up to
- * max_len (B * n_chunks), else (B <= 256) those that sum to total_len.
- * chunk_hint > 0 forces the chunk size (rounded up). Any plan is valid for any
- * call with these B, H_kv and max_len; the rest tunes it. */
+ * batch (<= 0: B * max_len). covering != 0, or B > 256: n_wg serves any lengths
+ * up to max_len (B * n_chunks). Else it serves those that sum to total_len or
+ * less: other lengths are served as far as sum(max(1, ceil(len / chunk_tokens)))
+ * <= n_wg holds, and the sequences past that come out as NaN. chunk_hint > 0
+ * forces the chunk size (rounded up). H_q, D, fmt, q_dt and out_dt tune the plan
+ * only. */
 int skv_q_decode_plan(int B, int H_q, int H_kv, int D, int fmt, int q_dt, int out_dt,
                       int max_len, long long total_len, int covering, int chunk_hint,
                       int* chunk_tokens /* host */, int* n_chunks /* host */,

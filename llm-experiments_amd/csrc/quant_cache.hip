@@ -9,9 +9,9 @@
 // bf16, 32 of fp32, against 4 or 8 of codes and a quarter of a scale byte),
 // and the group's maximum is two DPP steps over the quad of lanes that holds
 // it. No LDS, no second pass over the input. 4 x 16 x 128, 2048 tokens of bf16
-// into 4 bits: 21 us (85 MB, 4.0 TB/s; a copy reads and writes at 5.0), back to
-// bf16 15; 8192 tokens back 53 us a call (340 MB, 6.4 TB/s); one token of 64
-// sequences 3.0.
+// into 4 bits: 22 us (85 MB, 3.9 TB/s; a copy reads and writes at 5.0), back to
+// bf16 16; 8192 tokens back 54 to 60 us a call (340 MB, 5.7 to 6.3 TB/s), from 8
+// bits 67 (6.1), to fp32 100 (6.1) and 101 (6.7); one token of 64 sequences 3.1.
 #include <cstring>
 
 #include "quant.h"

@@ -15,9 +15,15 @@
 //
 // Bound by HBM: 4 x 16 x 128 of 32000 4-bit tokens (279 MB of codes and scales)
 // take 49 us in the first launch (5.7 TB/s; its loads alone as long) and 4.6 in
-// the merge, 52 to 53 us a call; 64 ragged paged sequences of 8 x 4 x 128 (144,900
-// tokens) 37 us (159 MB, 4-bit) and 68 us (308 MB, 8-bit). Calls of different
-// size fit 7.6 TB/s and 12 us of start and end.
+// the merge, 50 to 53 us a call; 64 ragged paged sequences of 8 x 4 x 128 (144,900
+// tokens) 38 us (159 MB, 4-bit) and 68 us (308 MB, 8-bit). Calls of different
+// size fit 7.6 TB/s and 12 us of start and end. With 32000 tokens of 4 sequences,
+// us a call, bf16 | fp32 in and out (4 x Hkv x G x D; 0.28 GB of 4-bit, 0.54 of
+// 8-bit rows each):
+//   4-bit  16 x 1 x 128 50 | 53,  x 4 51 | 54,  x 5 52 | 63,  x 16 58 | 70
+//   8-bit  16 x 1 x 128 89 | 89,  x 16 94 | 97
+//   4-bit   8 x 1 x 256 53 | 55,  x 8 57 | 78
+//   8-bit   8 x 1 x 256 94 | 98,  x 8 97 | 105,  x 16 102 | 118
 //
 // A tile:
 //  * S = K q^T (v_mfma_f32_16x16x32_bf16). Lane (r, kb) of a 16-token half
@@ -226,7 +232,9 @@ __device__ __forceinline__ int n_pieces(const QDecodeArgs& a, int len) {
 // tokens: each finds its place by a prefix sum over the sequences' chunk
 // counts. (With one for every chunk of the longest row, those of shorter rows
 // wait for a workgroup's LDS only to leave: 64 ragged sequences of 8 kv heads,
-// 146,000 tokens in 8 chunks of the longest, 45 us against 33 for equal ones.)
+// 146,000 tokens in 8 chunks of the longest, 45 us against 33 for equal ones.
+// In larger batches the chunks of the longest row are few: ragged, 8 kv heads x
+// 4 x 128, 256 sequences with the scan 3.8 TB/s, 257 without it 4.4.)
 constexpr int kMaxScan = 256;
 
 // Uniform over the wavefront. b = a.B: no sequence.
@@ -732,8 +740,14 @@ void launch_decode(const QDecodeArgs& a, bool f32, hipStream_t s) {
 using namespace skv;
 
 // The chunk: one round of workgroups, all resident (slots below). Equal rows
-// take a whole number of chunks each; with two the merge costs more than the
-// halved rows gain (512 rows of 2288 tokens: 36 us in two, 33.5 in one).
+// take a whole number of chunks each, and one where the round holds two or
+// fewer. That is the better choice past 512 rows only, us in one | two chunks
+// (8 kv heads x 128, 4-bit, in bf16):
+//   400 rows of 2288 tokens 31 | 29, of 8000 94 | 80, of 32000 354 | 278
+//   512                     32 | 31,         99 | 95,          373 | 330
+//   640                     37 | 45,        114 | 136,         435 | 484
+// Rows that differ, by a token already, take the second rule, whose chunk comes
+// out a little shorter than such rows: 640 of 32000, one of 31999, 650 us.
 // Ragged ones leave half a chunk a row, which the round has to hold too (64
 // sequences x 8 heads, 146,000 tokens: 49 us without that, 44 with). A chunk of
 // 1024 tokens or more is no multiple of 512: workgroups that start whole multiples

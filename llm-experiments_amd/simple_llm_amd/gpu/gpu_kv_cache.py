@@ -17,7 +17,9 @@ Differences from the reference, all supersets of its behaviour:
     attention_workgroup_size = 256, gpu_kv_cache.py:250-257);
   * bf16 and block-scaled 4- and 8-bit storage, grouped-query heads and a
     paged layout are options of KVCacheConfig; the defaults reproduce the
-    reference's fp32 MHA cache. Every function here takes every storage.
+    reference's fp32 MHA cache. Every function here takes every storage, but
+    kv_cache_read, which is for block-scaled caches, and kv_cache_prefill,
+    which takes paged caches only if they are block-scaled.
 
 Extensions beyond the reference's four functions:
   kv_cache_append           append with per-sequence positions (no
@@ -598,12 +600,14 @@ def kv_cache_prefill(ctx: GPUContext, cache: KVCache, layer_idx: int, new_k: tor
     bfloat16), and so does a block-scaled one with bfloat16 q and out; with
     float32 q or out its products have fp32 accuracy, at up to three times the
     work. A float32 cache runs every product with fp32 accuracy (float32 q and
-    out). The queries attend the chunk's rows as the cache stores them.
+    out). The queries attend the chunk's rows as the cache stores them. With q,
+    bfloat16 and block-scaled caches take 1, 2, 4 or 8 query heads per kv head.
 
     Raises ValueError (before any GPU work) on a bad layer, shapes, a chunk
     that would overflow a sequence ("Cache is full"), a scale that is not > 0
-    (with a block-scaled cache: and finite), a paged cache that is not
-    block-scaled, or a float32 cache with non-float32 q/output.
+    (with a block-scaled cache: and finite), query heads per kv head without a
+    kernel, a paged cache that is not block-scaled, or a float32 cache with
+    non-float32 q/output.
     """
     _check_layer(cache, layer_idx)
     if cache.paged and not cache.quantized:

@@ -206,6 +206,7 @@ class KVCacheConfig:
                   torch.float4_e2m1fn_x2, 4.25 bits an element, or
                   torch.float8_e4m3fn, 8.25. Those take head dims that are
                   multiples of 32 up to 256 and up to 16 query heads per kv head
+                  (kv_cache_prefill with queries: 1, 2, 4 or 8)
       block_size  > 0 selects the paged layout with pages of this many tokens
                   (a power of two); max_seq_len is then the per-sequence limit
       n_blocks    pages in the pool (0: batch_size * ceil(max_seq_len/block_size))
