@@ -1115,3 +1115,25 @@ def test_captured_chunk_outputs(gpu_ctx, fmt, page, splits, io):
         else:
             _check_attention(out, q, m, G, D ** -0.5, False, True, counts, True)
     _check_stored(gpu, gpu_ctx, cache, m)
+
+
+@pytest.mark.parametrize("B,Hkv,D,splits", [(70, 2, 32, 0), (33, 8, 32, 2), (33, 8, 64, 1),
+                                            (13, 5, 128, 3), (300, 1, 32, 2)])
+def test_prefill_of_fp32_ragged_batches(gpu_ctx, B, Hkv, D, splits):
+    """Tiles of 128 rows, several a group: groups that are ordered by their rows and, past
+    512 of them, not; sequences without rows among them."""
+    banner(f"quant ragged prefill fp32 B={B} Hkv={Hkv} D={D} splits={splits}")
+    rng = np.random.default_rng(B * Hkv + splits)
+    G, C = 2, 300
+    gpu, cache, m = _make(gpu_ctx, B, C + 150, Hkv, G, D, "fp4")
+    _fill(gpu, gpu_ctx, cache, m, rng, rng.integers(0, 150, B))
+    counts = rng.integers(0, 20, B)
+    counts[::5] = 0
+    counts[[3, B - 2]] = C, 129
+    k, v = (_dev(_rows(rng, B, C, Hkv, D), F32) for _ in range(2))
+    q = _dev(rng.standard_normal((B, C, Hkv * G, D)).astype(np.float32), F32)
+    out = torch.full_like(q, 9.0)
+    gpu.kv_cache_prefill(gpu_ctx, cache, 0, k, v, q, out, n_new=counts, n_splits=splits)
+    m.append(_np(k), _np(v), counts)
+    _check_prefill_fp32(out, q, m, G, D ** -0.5, counts, False)
+    _check_stored(gpu, gpu_ctx, cache, m)
