@@ -234,7 +234,8 @@ __device__ __forceinline__ int n_pieces(const QDecodeArgs& a, int len) {
 // wait for a workgroup's LDS only to leave: 64 ragged sequences of 8 kv heads,
 // 146,000 tokens in 8 chunks of the longest, 45 us against 33 for equal ones.
 // In larger batches the chunks of the longest row are few: ragged, 8 kv heads x
-// 4 x 128, 256 sequences with the scan 3.8 TB/s, 257 without it 4.4.)
+// 4 x 128, 192 and 256 sequences with the scan 3.4 and 3.8 TB/s, 257, 288 and 320
+// without it 4.4, 3.7 and 4.4.)
 constexpr int kMaxScan = 256;
 
 // Uniform over the wavefront. b = a.B: no sequence.
