@@ -706,6 +706,116 @@ int skv_flash_bwd(float* dq, float* dk, float* dv, const float* q, const float* 
                   int H, int D, float scale, void* ws, size_t ws_bytes, skv_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Around the attention of a training step: LayerNorm, embedding, loss and
+ * optimizer. Activations, logits and their gradients are fp32 or bf16 (dt);
+ * weights, their gradients and row statistics are fp32. Sums run in a fixed
+ * order without atomics: results are bitwise reproducible. Buffers are
+ * contiguous and 16-byte aligned unless noted; workspaces need no contents, and
+ * calls that share one must be stream ordered.
+ * ------------------------------------------------------------------------ */
+
+/* y = (x - mean) rstd gamma + beta of every row, rstd = 1 / sqrt(var + eps),
+ * population variance: the reference's layernorm (simple-llm/src/gpu/
+ * gpu_pass_forward.py:140-176, kernel gpu_kernels.py:137-249) with the rows'
+ * statistics kept for the backward. x, y: [M, d] of dt, y may be x; gamma, beta:
+ * [d]; mean, rstd: [M] or NULL. d <= 16384. */
+int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* x, const float* gamma,
+                      const float* beta, int M, int d, float eps, int dt, skv_stream_t stream);
+
+/* Workspace of skv_layernorm_bwd: partial sums of the weight gradients. */
+size_t skv_layernorm_bwd_workspace_bytes(int M, int d);
+
+/* Gradients of skv_layernorm_fwd (the reference's layernorm_backward and its
+ * reductions, gpu_pass_backward.py:304-336, gpu_kernels.py:1451-1815):
+ *   xh = (x - mean) rstd, g = dy gamma,
+ *   dx = rstd (g - mean(g) - xh mean(g xh)) [+ residual],
+ *   dgamma = sum over rows of dy xh, dbeta = sum over rows of dy,
+ * the latter two added to what is there with accumulate != 0. dx, dy, x,
+ * residual (or NULL): [M, d] of dt; dx may be dy, x or residual. */
+int skv_layernorm_bwd(void* dx, float* dgamma, float* dbeta, const void* dy, const void* x,
+                      const float* gamma, const float* mean, const float* rstd,
+                      const void* residual, int M, int d, int accumulate, void* ws,
+                      size_t ws_bytes, int dt, skv_stream_t stream);
+
+/* out[i] = scale table[ids[i]] + pos_table[i mod n_pos] (the reference's
+ * embedding, gpu_pass_forward.py:84-137, gpu_kernels.py:384-449, with a scale).
+ * out: [T, d] of out_dt; table: [V, d] of table_dt; pos_table: [n_pos, d] fp32 or
+ * NULL. An id outside [0, V) is padding: its row of the table counts as zeros. */
+int skv_embedding_fwd(void* out, const int32_t* ids, const void* table, const float* pos_table,
+                      int T, int V, int d, int n_pos, float scale, int table_dt, int out_dt,
+                      skv_stream_t stream);
+
+/* Workspace of skv_embedding_bwd: the tokens in order of their ids, and the parts
+ * of rows with many tokens. */
+size_t skv_embedding_bwd_workspace_bytes(int T, int V, int d);
+
+/* grad[v] = scale * sum of dout[i] over ids[i] = v, in token order, for every row
+ * of grad [V, d] fp32; with accumulate != 0 added to the rows that have tokens, and
+ * the others are left alone (the reference's embedding_backward and its reduction,
+ * gpu_pass_backward.py:183-240, gpu_kernels.py:2946-3068). dout: [T, d] of dt. An
+ * id outside [0, V) adds nothing. T, V <= 2^30. */
+int skv_embedding_bwd(float* grad, const void* dout, const int32_t* ids, int T, int V, int d,
+                      float scale, int accumulate, void* ws, size_t ws_bytes, int dt,
+                      skv_stream_t stream);
+
+/* Workspace of skv_cross_entropy. */
+size_t skv_cross_entropy_workspace_bytes(int M);
+
+/* The mean cross-entropy of the rows that count, and its gradient (the reference's
+ * cross_entropy_loss, gpu_pass_forward.py:331-416, gpu_kernels.py:995-1198):
+ *   row_loss[m] = logsumexp(x[m]) - x[m][targets[m]], loss[0] = their mean,
+ *   dx[m] = (softmax(x[m]) - onehot(targets[m])) grad_scale / rows that count.
+ * A row counts if its target lies in [0, V); the others have a loss and a gradient
+ * of 0 and their logits are not read; if none counts the loss is 0. x, dx: [M, V]
+ * of dt, dx may be x, or NULL; row_loss: [M] or NULL. Logits of -inf have
+ * probability 0; a row with a NaN or +inf, or of -inf only, has NaN results. */
+int skv_cross_entropy(float* loss, float* row_loss, void* dx, const void* x,
+                      const int32_t* targets, int M, int V, float grad_scale, void* ws,
+                      size_t ws_bytes, int dt, skv_stream_t stream);
+
+/* A tensor of skv_adamw: n elements of p (fp32, updated), g (of grad_dt) and copy
+ * (bf16 copies of the new weights, or NULL), whose moments begin at element `at` of
+ * the state, a multiple of 128. decay != 0: weight decay applies. */
+typedef struct skv_adamw_tensor {
+  float* p;
+  const void* g;
+  void* copy;
+  long long n, at, decay;
+} skv_adamw_tensor;
+
+/*
+ * One AdamW step of many tensors in one launch (the reference's adamw, one tensor a
+ * launch, gpu_pass_optimizer.py:28-393, gpu_kernels.py:2457-2539), t = count[0] + 1:
+ *   g' = grad_scale g, m = beta1 m + (1 - beta1) g', v = beta2 v + (1 - beta2) g'^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps).
+ * tensors: device memory. chunks: [n_chunks] pairs of int32 in device memory, (tensor,
+ * c) for its elements [2048 c, 2048 c + 2048), each chunk of each tensor once. count:
+ * two int32, t (advanced by the call, on the device, so that a captured step counts on)
+ * and 0. lr_dev, grad_scale_dev: where not NULL, fp32 in device memory in place of
+ * lr and grad_scale.
+ * bits = 32: m, v fp32, by element of the state (the places between tensors are not
+ * touched). bits = 8: a byte an element and m_scale, v_scale a byte k + 127 for 128
+ * elements, k the exponent of their largest magnitude in [-90, 126]: m as sign and
+ * E4M3 of m 2^(7 - k), v without a sign, with 5 exponent and 3 mantissa bits, of v 2^-k
+ * (exponent 30 for [1, 2)); rounded to one of the two neighbours, the upper with a
+ * probability of its distance from the lower, by a hash of (seed, t, place in the state);
+ * a v above 0 takes no 0. The step itself uses the moments before they are
+ * rounded. 128 moments with a NaN or an infinity are stored as scale 255 and codes 0 and
+ * read back as NaN. p, g and copy of any alignment (16 bytes: vectors).
+ */
+int skv_adamw(const skv_adamw_tensor* tensors, const int32_t* chunks, int n_chunks, void* m,
+              void* v, uint8_t* m_scale, uint8_t* v_scale, int32_t* count, int bits, int grad_dt,
+              double lr, const float* lr_dev, double beta1, double beta2, double eps,
+              double weight_decay, double grad_scale, const float* grad_scale_dev, uint32_t seed,
+              skv_stream_t stream);
+
+/* The 8-bit moments of a state of n elements (a multiple of 128) as values, exact in
+ * either out_dt. */
+int skv_adamw_read(void* m_out, void* v_out, const uint8_t* m, const uint8_t* v,
+                   const uint8_t* m_scale, const uint8_t* v_scale, long long n, int out_dt,
+                   skv_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Byte-level BPE tokenizer (host code, no device work), replacing the
  * reference's C tokenizer (simple-llm/src/common/bpe_tokenizer.c) that
  * common/bpe_tokenizer.py runs as a subprocess.

@@ -19,7 +19,8 @@ SOURCES = ["skv_api.hip", "append.hip", "decode_attn.hip", "decode_attn_generic.
            "decode_direct.hip", "prefill_attn.hip", "prefill_attn.hip:mxfp4",
            "prefill_attn.hip:mxfp8", "prefill_attn.hip:mxfp4_f32", "prefill_attn.hip:mxfp8_f32",
            "quant_cache.hip", "quant_decode.hip", "model_ops.hip", "gemm.hip", "sample.hip",
-           "flash_split.hip", "flash_fp32.hip", "flash_fp32.hip:wide_bwd", "bpe_tokenizer.cpp"]
+           "flash_split.hip", "flash_fp32.hip", "flash_fp32.hip:wide_bwd", "train_norm.hip",
+           "train_embed.hip", "train_loss.hip", "train_adamw.hip", "bpe_tokenizer.cpp"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -26,6 +26,7 @@ SKV_E_INVALID, SKV_E_UNSUPPORTED, SKV_E_WORKSPACE, SKV_E_HIP = -22, -95, -28, -5
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 _Z = ctypes.c_size_t
 
 # name -> (restype, argtypes); every function declared in include/skv.h
@@ -100,6 +101,17 @@ _SIGNATURES = {
                                           _I, _F, _I, _I, _P, _Z, _I, _I, _I, _I, _P]),
     "skv_decode_attn_paged": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I,
                                    _I, _P, _Z, _I, _I, _I, _P]),
+    "skv_layernorm_fwd": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _F, _I, _P]),
+    "skv_layernorm_bwd_workspace_bytes": (_Z, [_I, _I]),
+    "skv_layernorm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _Z, _I, _P]),
+    "skv_embedding_fwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P]),
+    "skv_embedding_bwd_workspace_bytes": (_Z, [_I, _I, _I]),
+    "skv_embedding_bwd": (_I, [_P, _P, _P, _I, _I, _I, _F, _I, _P, _Z, _I, _P]),
+    "skv_cross_entropy_workspace_bytes": (_Z, [_I]),
+    "skv_cross_entropy": (_I, [_P, _P, _P, _P, _P, _I, _I, _F, _P, _Z, _I, _P]),
+    "skv_adamw": (_I, [_P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _D, _P, _D, _D, _D, _D, _D, _P,
+                       ctypes.c_uint32, _P]),
+    "skv_adamw_read": (_I, [_P, _P, _P, _P, _P, _P, ctypes.c_longlong, _I, _P]),
     "skv_decode_attn_noalloc": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I,
                                      _I, _P]),
 }

@@ -27,8 +27,9 @@ from .gpu_kv_cache import (
     kv_cache_set_block_table,
     kv_cache_update,
 )
-from .gpu_pass_backward import flash_attention_backward
-from .gpu_pass_forward import flash_attention
+from .gpu_pass_backward import embedding_backward, flash_attention_backward, layernorm_backward
+from .gpu_pass_forward import cross_entropy_loss, embedding, flash_attention, layernorm
+from .gpu_pass_optimizer import AdamWState, adamw_create, adamw_read, adamw_update
 from .gpu_ops import batch_begin, batch_commit, validate_buffer_shape_1d, validate_buffer_shape_2d
 from .gpu_types import (
     BatchState,
@@ -84,7 +85,16 @@ __all__ = [
     "kv_cache_set_block_table",
     "decode_attention",
     "decode_plan",
-    # Training-side attention
+    # Training: forward, backward, optimizer
+    "embedding",
+    "layernorm",
     "flash_attention",
+    "cross_entropy_loss",
+    "layernorm_backward",
     "flash_attention_backward",
+    "embedding_backward",
+    "AdamWState",
+    "adamw_create",
+    "adamw_update",
+    "adamw_read",
 ]

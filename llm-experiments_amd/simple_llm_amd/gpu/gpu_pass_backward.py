@@ -1,6 +1,11 @@
-"""Training-side attention: causal FlashAttention backward on gfx950.
+"""Backward passes of a training step on gfx950: LayerNorm, the embedding and causal
+FlashAttention.
 
-Drop-in for flash_attention_backward of simple-llm/src/gpu/gpu_pass_backward.py:445-580:
+layernorm_backward and embedding_backward have the work of their namesakes in
+simple-llm/src/gpu/gpu_pass_backward.py (:304-336, :183-240) with this package's own
+arguments, and take fp32 and bf16 activations, GPUBuffers or contiguous device tensors.
+
+flash_attention_backward: drop-in for its namesake of simple-llm/src/gpu/gpu_pass_backward.py:445-580:
 same arguments, checks and error messages. The reference runs one stage-1
 pass per Q block, each writing partial dK/dV into grad_K_workspace and
 grad_V_workspace, then a reduce pass (gpu/gpu_kernels.py:2038-2455). Here
@@ -12,10 +17,14 @@ are kept in the first bytes of grad_K_workspace.
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import numpy as np
 import torch
 
 from .. import _lib
+from .gpu_pass_common import (F32, FLOATS, I32, Operand, apart, on, operand, ptr, rows_of, stream,
+                              workspace)
 from .gpu_ops import batch_count, validate_buffer_shape_1d, validate_buffer_shape_2d
 from .gpu_types import GPUBuffer1D, GPUBuffer2D, GPUContext
 
@@ -98,4 +107,71 @@ def flash_attention_backward(
     _lib.check(rc, "skv_flash_bwd")
 
 
-__all__ = ["flash_attention_backward"]
+def layernorm_backward(ctx: GPUContext, grad_output: Operand, input: Operand, gamma: Operand,
+                       mean: Operand, rstd: Operand, grad_input: Operand, grad_gamma: Operand,
+                       grad_beta: Operand, residual: Optional[Operand] = None,
+                       accumulate: bool = False) -> None:
+    """Gradients of layernorm.
+
+    grad_output, input, grad_input: [rows, d], all float32 or all bfloat16; gamma,
+    grad_gamma, grad_beta: float32 [d]; mean, rstd: float32 [rows], the forward's.
+    residual: a gradient like grad_input that is added to it (the one that goes past the
+    layer), or None. grad_input may be grad_output, input or residual.
+    accumulate: grad_gamma and grad_beta are added to (grad_input is not).
+    """
+    x = rows_of(ctx, input, "input", FLOATS)
+    rows, d = x.shape
+    like = (x.dtype,)
+    dy = operand(ctx, grad_output, "grad_output", (rows, d), like)
+    dx = operand(ctx, grad_input, "grad_input", (rows, d), like)
+    res = None if residual is None else operand(ctx, residual, "residual", (rows, d), like)
+    g = operand(ctx, gamma, "gamma", (d,), F32)
+    mu = operand(ctx, mean, "mean", (rows,), F32, 4)
+    rs = operand(ctx, rstd, "rstd", (rows,), F32, 4)
+    dg = operand(ctx, grad_gamma, "grad_gamma", (d,), F32, 4)
+    db = operand(ctx, grad_beta, "grad_beta", (d,), F32, 4)
+    ins = [(dy, "grad_output"), (x, "input"), (res, "residual")]
+    apart([(dx, "grad_input"), (dg, "grad_gamma"), (db, "grad_beta")],
+          [(g, "gamma"), (mu, "mean"), (rs, "rstd")]
+          + [i for i in ins if i[0] is None or i[0].data_ptr() != dx.data_ptr()])
+    apart([(dg, "grad_gamma"), (db, "grad_beta")], ins)
+    lib = _lib.lib()
+    batch_count(ctx)
+    with on(x.device):
+        ws = workspace(lib.skv_layernorm_bwd_workspace_bytes(rows, d), x.device)
+        rc = lib.skv_layernorm_bwd(dx.data_ptr(), dg.data_ptr(), db.data_ptr(), dy.data_ptr(),
+                                   x.data_ptr(), g.data_ptr(), mu.data_ptr(), rs.data_ptr(),
+                                   ptr(res), rows, d, int(bool(accumulate)), ws.data_ptr(),
+                                   ws.numel(), _lib.dtype_code(x.dtype), stream(x.device))
+    _lib.check(rc, "skv_layernorm_bwd")
+
+
+def embedding_backward(ctx: GPUContext, grad_output: Operand, tokens: Operand,
+                       grad_table: Operand, scale: float = 1.0,
+                       accumulate: bool = False) -> None:
+    """grad_table[v] = scale * the sum of grad_output[i] over tokens[i] == v, in token order.
+
+    grad_output: [n, d], float32 or bfloat16; tokens: int32 [n]; grad_table: float32
+    [vocab, d]. accumulate: the sums are added to grad_table (rows without tokens are not
+    touched), as where the tied logits have left their part. Tokens outside [0, vocab) are
+    padding and add nothing.
+    """
+    dy = rows_of(ctx, grad_output, "grad_output", FLOATS)
+    n, d = dy.shape
+    ids = operand(ctx, tokens, "tokens", (n,), I32, 4)
+    grad = rows_of(ctx, grad_table, "grad_table", F32)
+    if grad.shape[1] != d:
+        raise ValueError(f"grad_table shape mismatch: got {tuple(grad.shape)}, expected (*, {d})")
+    vocab = grad.shape[0]
+    apart([(grad, "grad_table")], [(dy, "grad_output"), (ids, "tokens")])
+    lib = _lib.lib()
+    batch_count(ctx)
+    with on(grad.device):
+        ws = workspace(lib.skv_embedding_bwd_workspace_bytes(n, vocab, d), grad.device)
+        rc = lib.skv_embedding_bwd(grad.data_ptr(), dy.data_ptr(), ids.data_ptr(), n, vocab, d,
+                                   float(scale), int(bool(accumulate)), ws.data_ptr(), ws.numel(),
+                                   _lib.dtype_code(dy.dtype), stream(grad.device))
+    _lib.check(rc, "skv_embedding_bwd")
+
+
+__all__ = ["embedding_backward", "flash_attention_backward", "layernorm_backward"]

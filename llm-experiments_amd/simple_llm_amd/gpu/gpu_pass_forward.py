@@ -1,5 +1,12 @@
-"""Training-side attention forward: causal FlashAttention with its row
-statistics, fp32, on gfx950.
+"""Forward passes of a training step on gfx950: the embedding, LayerNorm, causal
+FlashAttention and the cross-entropy loss.
+
+embedding, layernorm and cross_entropy_loss have the work of their namesakes in
+simple-llm/src/gpu/gpu_pass_forward.py (:84-137, :140-176, :331-416); their arguments
+are this package's own: they take fp32 and bf16 activations, and GPUBuffers or
+contiguous device tensors.
+
+flash_attention: causal FlashAttention with its row statistics, fp32.
 
 Drop-in for flash_attention of simple-llm/src/gpu/gpu_pass_forward.py:497-588:
 same arguments, checks and error messages. The reference's WGSL kernel
@@ -11,10 +18,14 @@ maxima of the scaled scores), which flash_attention_backward consumes.
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import numpy as np
 import torch
 
 from .. import _lib
+from .gpu_pass_common import (F32, FLOATS, I32, Operand, apart, on, operand, ptr, rows_of, stream,
+                              workspace)
 from .gpu_ops import batch_count, validate_buffer_shape_1d, validate_buffer_shape_2d
 from .gpu_types import GPUBuffer1D, GPUBuffer2D, GPUContext
 
@@ -73,4 +84,95 @@ def flash_attention(
     _lib.check(rc, "skv_flash_fwd")
 
 
-__all__ = ["flash_attention"]
+def embedding(ctx: GPUContext, tokens: Operand, table: Operand, output: Operand,
+              scale: float = 1.0, pos_table: Optional[Operand] = None) -> None:
+    """output[i] = scale * table[tokens[i]] + pos_table[i % len(pos_table)].
+
+    tokens: int32 [n], a batch's sequences end to end; table: [vocab, d], output: [n, d],
+    each float32 or bfloat16; pos_table: float32 [context, d] or None (positions of sequences
+    of exactly `context` tokens). A token outside [0, vocab) is padding: its table row counts
+    as zeros.
+    """
+    w = rows_of(ctx, table, "table", FLOATS)
+    ids = operand(ctx, tokens, "tokens", None, I32, 4)
+    if ids.dim() != 1 or ids.numel() == 0:
+        raise ValueError(f"tokens must be 1-D and hold elements, got shape {tuple(ids.shape)}")
+    n, (vocab, d) = ids.shape[0], w.shape
+    out = operand(ctx, output, "output", (n, d), FLOATS)
+    pos = None
+    if pos_table is not None:
+        pos = rows_of(ctx, pos_table, "pos_table", F32)
+        if pos.shape[1] != d:
+            raise ValueError(f"pos_table shape mismatch: got {tuple(pos.shape)}, expected (*, {d})")
+    apart([(out, "output")], [(w, "table"), (ids, "tokens"), (pos, "pos_table")])
+    lib = _lib.lib()
+    batch_count(ctx)
+    with on(out.device):
+        rc = lib.skv_embedding_fwd(out.data_ptr(), ids.data_ptr(), w.data_ptr(), ptr(pos), n, vocab,
+                                   d, 0 if pos is None else pos.shape[0], float(scale),
+                                   _lib.dtype_code(w.dtype), _lib.dtype_code(out.dtype),
+                                   stream(out.device))
+    _lib.check(rc, "skv_embedding_fwd")
+
+
+def layernorm(ctx: GPUContext, input: Operand, gamma: Operand, beta: Operand, output: Operand,
+              mean: Optional[Operand] = None, rstd: Optional[Operand] = None,
+              eps: float = 1e-5) -> None:
+    """output = (input - mean) * rstd * gamma + beta of every row.
+
+    input, output: [rows, d], both float32 or both bfloat16, d up to 16384; output may be
+    input. gamma, beta: float32 [d]. mean, rstd: float32 [rows], the rows' statistics for
+    layernorm_backward (rstd = 1 / sqrt(var + eps)), or None.
+    """
+    x = rows_of(ctx, input, "input", FLOATS)
+    rows, d = x.shape
+    y = operand(ctx, output, "output", (rows, d), (x.dtype,))
+    g = operand(ctx, gamma, "gamma", (d,), F32)
+    b = operand(ctx, beta, "beta", (d,), F32)
+    mu = None if mean is None else operand(ctx, mean, "mean", (rows,), F32, 4)
+    rs = None if rstd is None else operand(ctx, rstd, "rstd", (rows,), F32, 4)
+    if not eps >= 0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    apart([(y, "output"), (mu, "mean"), (rs, "rstd")],
+          [(g, "gamma"), (b, "beta")] + ([(x, "input")] if y.data_ptr() != x.data_ptr() else []))
+    apart([(mu, "mean"), (rs, "rstd")], [(x, "input")])
+    lib = _lib.lib()
+    batch_count(ctx)
+    with on(x.device):
+        rc = lib.skv_layernorm_fwd(y.data_ptr(), ptr(mu), ptr(rs), x.data_ptr(), g.data_ptr(),
+                                   b.data_ptr(), rows, d, float(eps), _lib.dtype_code(x.dtype),
+                                   stream(x.device))
+    _lib.check(rc, "skv_layernorm_fwd")
+
+
+def cross_entropy_loss(ctx: GPUContext, logits: Operand, targets: Operand, loss: Operand,
+                       grad_logits: Optional[Operand] = None,
+                       row_losses: Optional[Operand] = None, grad_scale: float = 1.0) -> None:
+    """loss[0] = the mean of logsumexp(logits[i]) - logits[i, targets[i]] over the rows with a
+    target in [0, vocab); the other rows are ignored. 0 if there are none.
+
+    logits: [rows, vocab], float32 or bfloat16; targets: int32 [rows]; loss: float32 [1].
+    grad_logits: the loss's gradient times grad_scale, like logits and possibly the same
+    buffer, or None. row_losses: float32 [rows], 0 where ignored, or None.
+    """
+    x = rows_of(ctx, logits, "logits", FLOATS)
+    rows, vocab = x.shape
+    t = operand(ctx, targets, "targets", (rows,), I32, 4)
+    out = operand(ctx, loss, "loss", (1,), F32, 4)
+    dx = None if grad_logits is None else operand(ctx, grad_logits, "grad_logits", (rows, vocab),
+                                                  (x.dtype,))
+    row = None if row_losses is None else operand(ctx, row_losses, "row_losses", (rows,), F32, 4)
+    same = dx is not None and dx.data_ptr() == x.data_ptr()
+    apart([(out, "loss"), (row, "row_losses"), (dx, "grad_logits")],
+          [(t, "targets")] + ([] if same else [(x, "logits")]))
+    lib = _lib.lib()
+    batch_count(ctx)
+    with on(x.device):
+        ws = workspace(lib.skv_cross_entropy_workspace_bytes(rows), x.device)
+        rc = lib.skv_cross_entropy(out.data_ptr(), ptr(row), ptr(dx), x.data_ptr(), t.data_ptr(),
+                                   rows, vocab, float(grad_scale), ws.data_ptr(), ws.numel(),
+                                   _lib.dtype_code(x.dtype), stream(x.device))
+    _lib.check(rc, "skv_cross_entropy")
+
+
+__all__ = ["cross_entropy_loss", "embedding", "flash_attention", "layernorm"]
