@@ -399,6 +399,12 @@ extern "C" int skv_adamw_read(void* m_out, void* v_out, const uint8_t* m, const 
   SKV_REQUIRE(out_dt == SKV_F32 || out_dt == SKV_BF16, SKV_E_INVALID, "skv_adamw_read: bad dtype");
   SKV_REQUIRE(aligned16(m_out) && aligned16(v_out) && aligned16(m) && aligned16(v), SKV_E_INVALID,
               "skv_adamw_read: pointers must be 16-byte aligned");
+  const size_t out = (size_t)n * (out_dt == SKV_BF16 ? 2 : 4);
+  if (int rc = apart("skv_adamw_read", {{m_out, out, "m"}, {v_out, out, "v"}},
+                     {{m, (size_t)n, "the state's m"}, {v, (size_t)n, "the state's v"},
+                      {m_scale, (size_t)n / kBlock, "the state's m_scale"},
+                      {v_scale, (size_t)n / kBlock, "the state's v_scale"}}))
+    return rc;
   const unsigned grid = (unsigned)((n / 8 + 255) / 256);
   hipStream_t s = (hipStream_t)stream;
   if (out_dt == SKV_BF16)

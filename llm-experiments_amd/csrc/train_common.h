@@ -36,6 +36,7 @@ struct Vec<float, N> {
     for (int i = 0; i < N; ++i) v[i] = 0.f;
   }
   __device__ __forceinline__ float get(int i) const { return v[i]; }
+  __device__ __forceinline__ void keep() {}
   static __device__ __forceinline__ void store(float* p, const float (&x)[N]) {
     if constexpr (N == 1) {
       *p = x[0];
@@ -48,8 +49,10 @@ struct Vec<float, N> {
   }
 };
 
+// Two values rounded to nearest even, in one instruction.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  return (uint32_t)f32_to_bf16(lo) | ((uint32_t)f32_to_bf16(hi) << 16);
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, bf16x2_t));
 }
 
 template <int N>
@@ -73,6 +76,12 @@ struct Vec<uint16_t, N> {  // N even
   __device__ __forceinline__ float get(int i) const {
     return (i & 1) ? bf16w_hi(w[i >> 1]) : bf16w_lo(w[i >> 1]);
   }
+  // What get() returned before is not kept in registers for later calls: the packed
+  // words are half as many.
+  __device__ __forceinline__ void keep() {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) asm volatile("" : "+v"(w[i]));
+  }
   static __device__ __forceinline__ void store(uint16_t* p, const float (&x)[N]) {
     if constexpr (NW == 1) {
       *reinterpret_cast<uint32_t*>(p) = pack_bf16(x[0], x[1]);
@@ -91,6 +100,7 @@ struct Vec<uint16_t, 1> {
   __device__ __forceinline__ void load(const uint16_t* p) { h = *p; }
   __device__ __forceinline__ void zero() { h = 0; }
   __device__ __forceinline__ float get(int) const { return bf16_to_f32(h); }
+  __device__ __forceinline__ void keep() {}
   static __device__ __forceinline__ void store(uint16_t* p, const float (&x)[1]) {
     *p = f32_to_bf16(x[0]);
   }
@@ -111,6 +121,33 @@ __device__ __forceinline__ float wave_sum(float x) { return xor32_sum(xor16_sum(
 __device__ __forceinline__ float wave_max(float x) { return xor32_max(xor16_max(row16_max(x))); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// An operand's memory (p NULL: there is none). may_be: the number of an output that
+// may be the same buffer, or -1.
+struct Span {
+  const void* p;
+  size_t bytes;
+  const char* name;
+  int may_be = -1;
+};
+
+// An error if an output overlaps another output or an input that it may not be.
+template <int NO, int NI>
+int apart(const char* fn, const Span (&out)[NO], const Span (&in)[NI]) {
+  const auto over = [](const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return x && y && x < y + b.bytes && y < x + a.bytes;
+  };
+  for (int i = 0; i < NO; ++i) {
+    for (int j = i + 1; j < NO; ++j)
+      SKV_REQUIRE(!over(out[i], out[j]), SKV_E_INVALID, "%s: %s overlaps %s", fn, out[i].name,
+                  out[j].name);
+    for (int j = 0; j < NI; ++j)
+      SKV_REQUIRE(!over(out[i], in[j]) || (in[j].may_be == i && in[j].p == out[i].p), SKV_E_INVALID,
+                  "%s: %s overlaps %s", fn, out[i].name, in[j].name);
+  }
+  return SKV_OK;
+}
 
 }  // namespace train
 }  // namespace skv

@@ -316,6 +316,12 @@ extern "C" int skv_embedding_fwd(void* out, const int32_t* ids, const void* tabl
               SKV_E_INVALID, "skv_embedding_fwd: bad dtype");
   SKV_REQUIRE(aligned16(out) && aligned16(table) && aligned16(pos_table), SKV_E_INVALID,
               "skv_embedding_fwd: pointers must be 16-byte aligned");
+  if (int rc = apart("skv_embedding_fwd",
+                     {{out, (size_t)T * d * (out_dt == SKV_BF16 ? 2 : 4), "output"}},
+                     {{table, (size_t)V * d * (table_dt == SKV_BF16 ? 2 : 4), "table"},
+                      {ids, (size_t)T * 4, "tokens"},
+                      {pos_table, (size_t)n_pos * d * 4, "pos_table"}}))
+    return rc;
   const dim3 grid((T + 3) / 4);
   const auto run = [&](auto* o, auto* t) {
     using TO = std::remove_pointer_t<decltype(o)>;
@@ -358,6 +364,11 @@ extern "C" int skv_embedding_bwd(float* grad, const void* dout, const int32_t* i
   SKV_REQUIRE(ws_bytes >= skv_embedding_bwd_workspace_bytes(T, V, d), SKV_E_WORKSPACE,
               "skv_embedding_bwd: workspace of %zu bytes, %zu needed", ws_bytes,
               skv_embedding_bwd_workspace_bytes(T, V, d));
+  if (int rc = apart("skv_embedding_bwd",
+                     {{grad, (size_t)V * d * 4, "grad_table"}, {ws, ws_bytes, "the workspace"}},
+                     {{dout, (size_t)T * d * (dt == SKV_BF16 ? 2 : 4), "grad_output"},
+                      {ids, (size_t)T * 4, "tokens"}}))
+    return rc;
   hipStream_t st = (hipStream_t)stream;
   Sorted s;
   s.pos = (int32_t*)ws;

@@ -29,34 +29,23 @@ struct LossArgs {
   void* dx;
   const int32_t* targets;
   float* row;  // [M]
-  const float* inv;  // grad_scale / rows that count
+  const float* inv;  // grad_scale / rows that count, or NULL: every wavefront counts them
+  float grad_scale;
   int M, V;
 };
 
-// Over the workgroup's NW wavefronts; sh [NW].
-template <int NW>
-__device__ __forceinline__ float group_max(float x, float* sh) {
-  x = wave_max(x);
-  if constexpr (NW > 1) {
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = sh[0];
+// Where the wavefronts count the rows themselves: one launch less (255 x 257 fp32: two
+// launches of 2 us instead of three), and at most 4 MB more from L2.
+constexpr int kCountRows = 1024;
+
+__device__ __forceinline__ float row_scale(const LossArgs& a) {
+  if (a.inv) return *a.inv;
+  int n = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x & 63; i < a.M; i += 64) n += (unsigned)a.targets[i] < (unsigned)a.V;
 #pragma unroll
-    for (int i = 1; i < NW; ++i) x = fmaxf(x, sh[i]);
-  }
-  return x;
-}
-template <int NW>
-__device__ __forceinline__ float group_sum(float x, float* sh) {
-  x = wave_sum(x);
-  if constexpr (NW > 1) {
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) x += sh[i];
-  }
-  return x;
+  for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o);
+  return a.grad_scale / (float)max(n, 1);
 }
 
 // 2^(x log2(e) - top2), the difference rounded once
@@ -68,6 +57,33 @@ __device__ __forceinline__ float exp_from(float x, float top2) {
 // is top log2(e) rounded, and what the rounding left is taken out again.
 __device__ __forceinline__ float loss_of(float top, float top2, float sum, float picked) {
   return (top - picked) + (logf(sum) - fmaf(top, LOG2E, -top2) * LN2);
+}
+
+// A maximum and the sum of 2^(x log2(e) - ref2) of what a wavefront has seen. ref2
+// is top log2(e) rounded, or 0 where top is -inf (nothing seen, or only NaN).
+struct Stats {
+  float top, sum;
+};
+__device__ __forceinline__ float ref2_of(float top) {
+#pragma clang fp contract(off)  // rounded on its own, wherever it is used
+  const float r = top * LOG2E;
+  return top == -INFINITY ? 0.f : r;
+}
+
+// The statistics of the workgroup's NW wavefronts: one barrier, and then a lane has
+// those of wavefront lane % NW (so a row of 16 lanes has each 16 / NW times).
+template <int NW>
+__device__ __forceinline__ Stats group_stats(Stats s, float2* sh) {
+  if constexpr (NW > 1) {
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = make_float2(s.top, s.sum);
+    __syncthreads();
+    const float2 o = sh[threadIdx.x % NW];
+    s.top = row16_max(o.x);
+    // a NaN sum stays one under a factor of 0
+    const float f = o.x == -INFINITY ? 0.f : fast_exp2(ref2_of(o.x) - ref2_of(s.top));
+    s.sum = row16_sum(o.y * f) * (NW / 16.f);
+  }
+  return s;
 }
 
 template <typename T>
@@ -83,6 +99,14 @@ struct Row {
     n_vec = (V - head) / kVec<T>;
     tail_at = head + n_vec * kVec<T>;
   }
+  // vector j of a row that begins at p (its own or the gradient's): the offset in bytes
+  // fits 32 bits, so that a lane keeps one register for its address
+  __device__ __forceinline__ const T* vec(const T* p, unsigned j) const {
+    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p + head) + j * 16u);
+  }
+  __device__ __forceinline__ T* vec(T* p, unsigned j) const {
+    return reinterpret_cast<T*>(reinterpret_cast<char*>(p + head) + j * 16u);
+  }
   // the single element of thread t, or -1
   __device__ __forceinline__ int edge(int t, int V) const {
     if (t < head) return t;
@@ -96,13 +120,18 @@ __device__ __forceinline__ float as_f32(uint16_t x) { return bf16_to_f32(x); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(uint16_t* p, float v) { *p = f32_to_bf16(v); }
 
-// A row on NW wavefronts, NV vectors a lane; with NW = 1 a workgroup has four.
+// The vectors of a lane that every lane has: all but the last three of NV.
+constexpr int sure(int NV) { return NV > 3 ? NV - 3 : 0; }
+
+// A row on NW wavefronts, NV vectors a lane, sure(NV) of them without a test for the
+// row's end; with NW = 1 a workgroup has four.
 template <typename T, int NW, int NV, bool GRAD>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs a) {
-  __shared__ float sh[2][NW];
+  __shared__ float2 sh[NW];
   constexpr int N = kVec<T>;
   const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int m = NW == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const int m = NW == 1 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
+                        : blockIdx.x;
   if (m >= a.M) return;
   const Row<T> row((const T*)a.x, m, a.V);
   T* dx = (T*)a.dx + (size_t)m * a.V;
@@ -113,8 +142,8 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
       const float z[N] = {};
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int j = i * NW * 64 + t;
-        if (j < row.n_vec) Vec<T, N>::store(dx + row.head + j * N, z);
+        const unsigned j = i * NW * 64 + t;
+        if (i < sure(NV) || j < (unsigned)row.n_vec) Vec<T, N>::store(row.vec(dx, j), z);
       }
       if (at >= 0) put(dx + at, 0.f);
     }
@@ -123,42 +152,50 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
   Vec<T, N> v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int j = i * NW * 64 + t;
-    if (j < row.n_vec) v[i].load(row.x + row.head + j * N);
+    const unsigned j = i * NW * 64 + t;
+    if (i < sure(NV) || j < (unsigned)row.n_vec) v[i].load(row.vec(row.x, j));
   }
   const float edge = at >= 0 ? as_f32(row.x[at]) : 0.f;
   const float picked = as_f32(row.x[target]);
-  const float inv = GRAD ? *a.inv : 0.f;
+  const float inv = GRAD ? row_scale(a) : 0.f;
   float top = at >= 0 ? edge : -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (i * NW * 64 + t < row.n_vec) {
+    if (i < sure(NV) || i * NW * 64 + t < row.n_vec) {
 #pragma unroll
       for (int e = 0; e < N; ++e) top = fmaxf(top, v[i].get(e));
     }
-  top = group_max<NW>(top, sh[0]);
-  const float top2 = top * LOG2E;
-  float sum = at >= 0 ? exp_from(edge, top2) : 0.f;
+  top = wave_max(top);
+  const float ref2 = ref2_of(top);
+  float sum = at >= 0 ? exp_from(edge, ref2) : 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * NW * 64 + t < row.n_vec) {
+  for (int i = 0; i < NV; ++i) {
+    v[i].keep();
+    if (i < sure(NV) || i * NW * 64 + t < row.n_vec) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += exp_from(v[i].get(e), top2);
+      for (int e = 0; e < N; ++e) sum += exp_from(v[i].get(e), ref2);
     }
-  sum = group_sum<NW>(sum, sh[1]);
-  if (t == 0) a.row[m] = loss_of(top, top2, sum, picked);
+  }
+  const Stats s = group_stats<NW>({top, wave_sum(sum)}, sh);
+  const float top2 = s.top == -INFINITY ? -INFINITY : ref2_of(s.top);  // NaN where all is -inf
+  if (t == 0) a.row[m] = loss_of(s.top, top2, s.sum, picked);
   if constexpr (GRAD) {
-    const float k = inv / sum;
+    const float k = inv / s.sum;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = i * NW * 64 + t;
-      if (j < row.n_vec) {
-        const int first = row.head + j * N;
+      unsigned j = i * NW * 64 + t;
+      asm volatile("" : "+v"(j));  // formed here, not kept since the loads
+      v[i].keep();
+      if (i < sure(NV) || j < (unsigned)row.n_vec) {
+        const unsigned first = row.head + j * N;
         float o[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-          o[e] = exp_from(v[i].get(e), top2) * k - (first + e == target ? inv : 0.f);
-        Vec<T, N>::store(dx + first, o);
+        for (int e = 0; e < N; ++e) o[e] = exp_from(v[i].get(e), top2) * k;
+        if ((unsigned)target - first < (unsigned)N) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[e] -= first + e == (unsigned)target ? inv : 0.f;
+        }
+        Vec<T, N>::store(row.vec(dx, j), o);
       }
     }
     if (at >= 0) put(dx + at, exp_from(edge, top2) * k - (at == target ? inv : 0.f));
@@ -168,53 +205,57 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
 // Any length: the row is read for its statistics and again for its gradient.
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(1024) void k_loss_long(LossArgs a) {
-  __shared__ float sh[2][16];
+  __shared__ float2 sh[16];
   constexpr int N = kVec<T>;
   const int t = threadIdx.x, m = blockIdx.x;
   const Row<T> row((const T*)a.x, m, a.V);
   T* dx = (T*)a.dx + (size_t)m * a.V;
   const int target = a.targets[m], at = row.edge(t, a.V);
   const bool counts = (unsigned)target < (unsigned)a.V;
-  const float inv = GRAD && counts ? *a.inv : 0.f;
+  const float inv = GRAD && counts ? row_scale(a) : 0.f;
   const float edge = at >= 0 ? as_f32(row.x[at]) : 0.f;
   float top2 = 0.f, k = 0.f;
   if (counts) {
     const float picked = as_f32(row.x[target]);
-    float top = at >= 0 ? edge : -INFINITY;
+    // a lane's sum is taken on to a larger maximum where its vectors have one
+    float top = at >= 0 ? edge : -INFINITY, ref2 = ref2_of(top);
+    float sum = at >= 0 ? exp_from(edge, ref2) : 0.f;
 #pragma unroll 4
-    for (int j = t; j < row.n_vec; j += 1024) {
+    for (unsigned j = t; j < (unsigned)row.n_vec; j += 1024) {
       Vec<T, N> v;
-      v.load(row.x + row.head + j * N);
+      v.load(row.vec(row.x, j));
+      float most = top;
 #pragma unroll
-      for (int e = 0; e < N; ++e) top = fmaxf(top, v.get(e));
-    }
-    top = group_max<16>(top, sh[0]);
-    top2 = top * LOG2E;
-    float sum = at >= 0 ? exp_from(edge, top2) : 0.f;
-#pragma unroll 4
-    for (int j = t; j < row.n_vec; j += 1024) {
-      Vec<T, N> v;
-      v.load(row.x + row.head + j * N);
+      for (int e = 0; e < N; ++e) most = fmaxf(most, v.get(e));
+      if (most > top) {
+        const float to2 = ref2_of(most);
+        sum *= top == -INFINITY ? 1.f : fast_exp2(ref2 - to2);
+        top = most;
+        ref2 = to2;
+      }
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += exp_from(v.get(e), top2);
+      for (int e = 0; e < N; ++e) sum += exp_from(v.get(e), ref2);
     }
-    sum = group_sum<16>(sum, sh[1]);
-    if (t == 0) a.row[m] = loss_of(top, top2, sum, picked);
-    k = inv / sum;
+    const float wtop = wave_max(top), wref2 = ref2_of(wtop);
+    sum *= top == -INFINITY ? 1.f : fast_exp2(ref2 - wref2);
+    const Stats s = group_stats<16>({wtop, wave_sum(sum)}, sh);
+    top2 = s.top == -INFINITY ? -INFINITY : ref2_of(s.top);
+    if (t == 0) a.row[m] = loss_of(s.top, top2, s.sum, picked);
+    k = inv / s.sum;
   } else if (t == 0) {
     a.row[m] = 0.f;
   }
   if constexpr (GRAD) {
 #pragma unroll 4
-    for (int j = t; j < row.n_vec; j += 1024) {
-      const int first = row.head + j * N;
+    for (unsigned j = t; j < (unsigned)row.n_vec; j += 1024) {
+      const unsigned first = row.head + j * N;
       Vec<T, N> v;
       float o[N];
-      v.load(row.x + first);
+      v.load(row.vec(row.x, j));
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        o[e] = counts ? exp_from(v.get(e), top2) * k - (first + e == target ? inv : 0.f) : 0.f;
-      Vec<T, N>::store(dx + first, o);
+        o[e] = counts ? exp_from(v.get(e), top2) * k - (first + e == (unsigned)target ? inv : 0.f) : 0.f;
+      Vec<T, N>::store(row.vec(dx, j), o);
     }
     if (at >= 0)
       put(dx + at, counts ? exp_from(edge, top2) * k - (at == target ? inv : 0.f) : 0.f);
@@ -273,9 +314,9 @@ __global__ __launch_bounds__(1024) void k_loss_mean(float* __restrict__ loss,
   }
 }
 
-// By the row's aligned vectors: one wavefront up to 4 vectors a lane (no
-// barrier), 4 wavefronts up to 8, 8 wavefronts up to 16; fp32 rows past that, and
-// up to 65536 logits, on 16.
+// By the row's vectors: one wavefront up to 4 vectors a lane (no barrier), then 4 and 8
+// wavefronts up to 8 and 16 up to 16, so that a CU's registers hold many rows in different
+// phases (50304 bf16 logits x 8192: 16 wavefronts of 7 vectors, 290 us, 8 of 13, 295).
 template <typename T, bool GRAD>
 void launch_rows(const LossArgs& a, hipStream_t s) {
   const int n = (a.V + kVec<T> - 1) / kVec<T>;
@@ -284,14 +325,24 @@ void launch_rows(const LossArgs& a, hipStream_t s) {
     k_loss_rows<T, nw, NV.value, GRAD>
         <<<nw == 1 ? (a.M + 3) / 4 : a.M, nw == 1 ? 256 : nw * 64, 0, s>>>(a);
   };
+  const auto with = [&](auto NW) {  // even numbers of vectors
+    const int nv = (n + NW.value * 64 - 1) / (NW.value * 64);
+    if (nv <= 6) rows(NW, std::integral_constant<int, 6>{});
+    else if (nv <= 8) rows(NW, std::integral_constant<int, 8>{});
+    else if (nv <= 10) rows(NW, std::integral_constant<int, 10>{});
+    else if (nv <= 12) rows(NW, std::integral_constant<int, 12>{});
+    else if (nv <= 14) rows(NW, std::integral_constant<int, 14>{});
+    else rows(NW, std::integral_constant<int, 16>{});
+  };
   using std::integral_constant;
   if (n <= 64) rows(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  else if (n <= 128) rows(integral_constant<int, 1>{}, integral_constant<int, 2>{});
   else if (n <= 256) rows(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  else if (n <= 512) rows(integral_constant<int, 4>{}, integral_constant<int, 2>{});
   else if (n <= 1024) rows(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-  else if (n <= 2048) rows(integral_constant<int, 4>{}, integral_constant<int, 8>{});
-  else if (n <= 4096) rows(integral_constant<int, 8>{}, integral_constant<int, 8>{});
-  else if (n <= 8192) rows(integral_constant<int, 8>{}, integral_constant<int, 16>{});
-  else if (n <= 16384) rows(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+  else if (n <= 2048) with(integral_constant<int, 4>{});
+  else if (n <= 4096) with(integral_constant<int, 8>{});
+  else if (n <= 16384) with(integral_constant<int, 16>{});
   else k_loss_long<T, GRAD><<<a.M, 1024, 0, s>>>(a);
 }
 
@@ -310,15 +361,23 @@ extern "C" int skv_cross_entropy(float* loss, float* row_loss, void* dx, const v
   SKV_REQUIRE(loss && x && targets && ws, SKV_E_INVALID, "skv_cross_entropy: null pointer argument");
   SKV_REQUIRE(M > 0 && V > 0, SKV_E_INVALID, "skv_cross_entropy: dims must be > 0");
   SKV_REQUIRE(dt == SKV_F32 || dt == SKV_BF16, SKV_E_INVALID, "skv_cross_entropy: bad dtype");
+  SKV_REQUIRE(V <= 1 << 28, SKV_E_UNSUPPORTED, "skv_cross_entropy: V=%d > 2^28", V);
   SKV_REQUIRE(aligned16(dx) && aligned16(x) && aligned16(ws), SKV_E_INVALID,
               "skv_cross_entropy: pointers must be 16-byte aligned");
   SKV_REQUIRE(ws_bytes >= skv_cross_entropy_workspace_bytes(M), SKV_E_WORKSPACE,
               "skv_cross_entropy: workspace of %zu bytes, %zu needed", ws_bytes,
               skv_cross_entropy_workspace_bytes(M));
+  const size_t n = (size_t)M * V * (dt == SKV_BF16 ? 2 : 4), row = (size_t)M * 4;
+  if (int rc = apart("skv_cross_entropy",
+                     {{dx, n, "grad_logits"}, {loss, 4, "loss"}, {row_loss, row, "row_losses"},
+                      {ws, ws_bytes, "the workspace"}},
+                     {{x, n, "logits", 0}, {targets, row, "targets"}}))
+    return rc;
   hipStream_t s = (hipStream_t)stream;
   float* inv = (float*)ws;
-  LossArgs a = {x, dx, targets, row_loss ? row_loss : inv + 4, inv, M, V};
-  if (dx) k_loss_count<<<1, 1024, 0, s>>>(inv, targets, M, V, grad_scale);
+  LossArgs a = {x, dx, targets, row_loss ? row_loss : inv + 4, M > kCountRows ? inv : nullptr,
+                grad_scale, M, V};
+  if (dx && a.inv) k_loss_count<<<1, 1024, 0, s>>>(inv, targets, M, V, grad_scale);
   if (dt == SKV_BF16) {
     if (dx) launch_rows<uint16_t, true>(a, s);
     else launch_rows<uint16_t, false>(a, s);

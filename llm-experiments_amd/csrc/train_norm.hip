@@ -319,6 +319,12 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
   if (int rc = check("skv_layernorm_fwd", M, d, dt)) return rc;
   SKV_REQUIRE(aligned16(y) && aligned16(x) && aligned16(gamma) && aligned16(beta), SKV_E_INVALID,
               "skv_layernorm_fwd: pointers must be 16-byte aligned");
+  const size_t act = (size_t)M * d * (dt == SKV_BF16 ? 2 : 4), row = (size_t)M * 4;
+  if (int rc = apart("skv_layernorm_fwd",
+                     {{y, act, "output"}, {mean, row, "mean"}, {rstd, row, "rstd"}},
+                     {{x, act, "input", 0}, {gamma, (size_t)d * 4, "gamma"},
+                      {beta, (size_t)d * 4, "beta"}}))
+    return rc;
   const int rows = waves_of(d) == 1 ? 4 : 1;
   const dim3 grid((M + rows - 1) / rows);
   auto run = [&](auto* yt, auto FULL) {
@@ -353,6 +359,15 @@ extern "C" int skv_layernorm_bwd(void* dx, float* dgamma, float* dbeta, const vo
   SKV_REQUIRE(ws_bytes >= skv_layernorm_bwd_workspace_bytes(M, d), SKV_E_WORKSPACE,
               "skv_layernorm_bwd: workspace of %zu bytes, %zu needed", ws_bytes,
               skv_layernorm_bwd_workspace_bytes(M, d));
+  const size_t act = (size_t)M * d * (dt == SKV_BF16 ? 2 : 4), row = (size_t)M * 4,
+               col = (size_t)d * 4;
+  if (int rc = apart("skv_layernorm_bwd",
+                     {{dx, act, "grad_input"}, {dgamma, col, "grad_gamma"},
+                      {dbeta, col, "grad_beta"}, {ws, ws_bytes, "the workspace"}},
+                     {{dy, act, "grad_output", 0}, {x, act, "input", 0},
+                      {residual, act, "residual", 0}, {gamma, col, "gamma"}, {mean, row, "mean"},
+                      {rstd, row, "rstd"}}))
+    return rc;
   const int P = bwd_groups(M, d), dp = padded(d);
   float* part = (float*)ws;
   auto run = [&](auto* xt, auto FULL) {

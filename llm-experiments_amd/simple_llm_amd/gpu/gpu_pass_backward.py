@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .gpu_pass_common import (F32, FLOATS, I32, Operand, apart, on, operand, ptr, rows_of, stream,
+from .gpu_pass_common import (F32, FLOATS, I32, Operand, on, operand, ptr, rows_of, stream,
                               workspace)
 from .gpu_ops import batch_count, validate_buffer_shape_1d, validate_buffer_shape_2d
 from .gpu_types import GPUBuffer1D, GPUBuffer2D, GPUContext
@@ -130,15 +130,10 @@ def layernorm_backward(ctx: GPUContext, grad_output: Operand, input: Operand, ga
     rs = operand(ctx, rstd, "rstd", (rows,), F32, 4)
     dg = operand(ctx, grad_gamma, "grad_gamma", (d,), F32, 4)
     db = operand(ctx, grad_beta, "grad_beta", (d,), F32, 4)
-    ins = [(dy, "grad_output"), (x, "input"), (res, "residual")]
-    apart([(dx, "grad_input"), (dg, "grad_gamma"), (db, "grad_beta")],
-          [(g, "gamma"), (mu, "mean"), (rs, "rstd")]
-          + [i for i in ins if i[0] is None or i[0].data_ptr() != dx.data_ptr()])
-    apart([(dg, "grad_gamma"), (db, "grad_beta")], ins)
     lib = _lib.lib()
     batch_count(ctx)
     with on(x.device):
-        ws = workspace(lib.skv_layernorm_bwd_workspace_bytes(rows, d), x.device)
+        ws = workspace("skv_layernorm_bwd_workspace_bytes", x.device, rows, d)
         rc = lib.skv_layernorm_bwd(dx.data_ptr(), dg.data_ptr(), db.data_ptr(), dy.data_ptr(),
                                    x.data_ptr(), g.data_ptr(), mu.data_ptr(), rs.data_ptr(),
                                    ptr(res), rows, d, int(bool(accumulate)), ws.data_ptr(),
@@ -163,11 +158,10 @@ def embedding_backward(ctx: GPUContext, grad_output: Operand, tokens: Operand,
     if grad.shape[1] != d:
         raise ValueError(f"grad_table shape mismatch: got {tuple(grad.shape)}, expected (*, {d})")
     vocab = grad.shape[0]
-    apart([(grad, "grad_table")], [(dy, "grad_output"), (ids, "tokens")])
     lib = _lib.lib()
     batch_count(ctx)
     with on(grad.device):
-        ws = workspace(lib.skv_embedding_bwd_workspace_bytes(n, vocab, d), grad.device)
+        ws = workspace("skv_embedding_bwd_workspace_bytes", grad.device, n, vocab, d)
         rc = lib.skv_embedding_bwd(grad.data_ptr(), dy.data_ptr(), ids.data_ptr(), n, vocab, d,
                                    float(scale), int(bool(accumulate)), ws.data_ptr(), ws.numel(),
                                    _lib.dtype_code(dy.dtype), stream(grad.device))

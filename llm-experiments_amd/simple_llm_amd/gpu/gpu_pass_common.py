@@ -30,53 +30,56 @@ def on(dev: torch.device):
     return torch.cuda.device(dev)
 
 
-def operand(ctx: GPUContext, buf: Operand, name: str, shape: Optional[Sequence[int]],
+def operand(ctx: GPUContext, buf: Operand, name: str, shape: Optional[tuple],
             dtypes: Sequence[torch.dtype], align: int = 16) -> torch.Tensor:
     """The operand's tensor: of `shape` (None: any), one of `dtypes`, contiguous and
     aligned, on the context's device."""
     t = buf if isinstance(buf, torch.Tensor) else getattr(buf, "buffer", None)
+    dev = ctx.device
+    # Fast path first: every check again below, to say what is wrong.
+    if (isinstance(t, torch.Tensor) and (shape is None or t.shape == shape) and t.dtype in dtypes
+            and t.is_cuda and t.get_device() == (dev.index or 0) and t.is_contiguous()
+            and not t.data_ptr() % align):
+        return t
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a GPUBuffer or a tensor, got {type(buf).__name__}")
-    if shape is not None and t.shape != torch.Size(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} shape mismatch: got {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    dev = ctx.device
     if not t.is_cuda or t.get_device() != (dev.index or 0):
         raise ValueError(f"{name} must live on {dev}, got {t.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if t.data_ptr() % align:
-        raise ValueError(f"{name} must be {align}-byte aligned")
-    return t
+    raise ValueError(f"{name} must be {align}-byte aligned")
 
 
 def rows_of(ctx: GPUContext, buf: Operand, name: str, dtypes: Sequence[torch.dtype],
             align: int = 16) -> torch.Tensor:
     """A 2-D operand of any shape that holds elements."""
     t = operand(ctx, buf, name, None, dtypes, align)
-    if t.dim() != 2 or t.numel() == 0:
-        raise ValueError(f"{name} must be 2-D and hold elements, got shape {tuple(t.shape)}")
-    if max(t.shape) >= 1 << 31:
-        raise ValueError(f"{name} is too large: {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 2 or not shape[0] or not shape[1]:
+        raise ValueError(f"{name} must be 2-D and hold elements, got shape {tuple(shape)}")
+    if shape[0] >= 1 << 31 or shape[1] >= 1 << 31:
+        raise ValueError(f"{name} is too large: {tuple(shape)}")
     return t
 
 
-def apart(outputs: Sequence[tuple], inputs: Sequence[tuple]) -> None:
-    """ValueError if an output (tensor, name) overlaps another output or an input."""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name)
-             for t, name in (*outputs, *inputs) if t is not None]
-    n_out = sum(t is not None for t, _ in outputs)
-    for i in range(n_out):
-        for j in range(i + 1, len(spans)):
-            if spans[i][0] < spans[j][1] and spans[j][0] < spans[i][1]:
-                raise ValueError(f"{spans[i][2]} overlaps {spans[j][2]}")
+_WS_BYTES: dict = {}
 
 
-def workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
-    """Workspace of one call, from torch's caching allocator in stream order: calls on
-    different streams, and captured calls, do not share one."""
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=dev)
+def workspace(query: str, dev: torch.device, *sizes: int) -> torch.Tensor:
+    """Workspace of one call, of the bytes that the C function `query` asks for, from torch's
+    caching allocator in stream order: calls on different streams, and captured calls, do not
+    share one."""
+    key = (query, *sizes)
+    need = _WS_BYTES.get(key)
+    if need is None:
+        if len(_WS_BYTES) > 4096:
+            _WS_BYTES.clear()
+        need = _WS_BYTES[key] = max(int(getattr(_lib.lib(), query)(*sizes)), 16)
+    return torch.empty(need, dtype=torch.uint8, device=dev)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -24,7 +24,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .gpu_pass_common import (F32, FLOATS, I32, Operand, apart, on, operand, ptr, rows_of, stream,
+from .gpu_pass_common import (F32, FLOATS, I32, Operand, on, operand, ptr, rows_of, stream,
                               workspace)
 from .gpu_ops import batch_count, validate_buffer_shape_1d, validate_buffer_shape_2d
 from .gpu_types import GPUBuffer1D, GPUBuffer2D, GPUContext
@@ -95,7 +95,7 @@ def embedding(ctx: GPUContext, tokens: Operand, table: Operand, output: Operand,
     """
     w = rows_of(ctx, table, "table", FLOATS)
     ids = operand(ctx, tokens, "tokens", None, I32, 4)
-    if ids.dim() != 1 or ids.numel() == 0:
+    if ids.dim() != 1 or not 0 < ids.shape[0] < 1 << 31:
         raise ValueError(f"tokens must be 1-D and hold elements, got shape {tuple(ids.shape)}")
     n, (vocab, d) = ids.shape[0], w.shape
     out = operand(ctx, output, "output", (n, d), FLOATS)
@@ -104,7 +104,6 @@ def embedding(ctx: GPUContext, tokens: Operand, table: Operand, output: Operand,
         pos = rows_of(ctx, pos_table, "pos_table", F32)
         if pos.shape[1] != d:
             raise ValueError(f"pos_table shape mismatch: got {tuple(pos.shape)}, expected (*, {d})")
-    apart([(out, "output")], [(w, "table"), (ids, "tokens"), (pos, "pos_table")])
     lib = _lib.lib()
     batch_count(ctx)
     with on(out.device):
@@ -133,9 +132,6 @@ def layernorm(ctx: GPUContext, input: Operand, gamma: Operand, beta: Operand, ou
     rs = None if rstd is None else operand(ctx, rstd, "rstd", (rows,), F32, 4)
     if not eps >= 0:
         raise ValueError(f"eps must be >= 0, got {eps}")
-    apart([(y, "output"), (mu, "mean"), (rs, "rstd")],
-          [(g, "gamma"), (b, "beta")] + ([(x, "input")] if y.data_ptr() != x.data_ptr() else []))
-    apart([(mu, "mean"), (rs, "rstd")], [(x, "input")])
     lib = _lib.lib()
     batch_count(ctx)
     with on(x.device):
@@ -162,13 +158,10 @@ def cross_entropy_loss(ctx: GPUContext, logits: Operand, targets: Operand, loss:
     dx = None if grad_logits is None else operand(ctx, grad_logits, "grad_logits", (rows, vocab),
                                                   (x.dtype,))
     row = None if row_losses is None else operand(ctx, row_losses, "row_losses", (rows,), F32, 4)
-    same = dx is not None and dx.data_ptr() == x.data_ptr()
-    apart([(out, "loss"), (row, "row_losses"), (dx, "grad_logits")],
-          [(t, "targets")] + ([] if same else [(x, "logits")]))
     lib = _lib.lib()
     batch_count(ctx)
     with on(x.device):
-        ws = workspace(lib.skv_cross_entropy_workspace_bytes(rows), x.device)
+        ws = workspace("skv_cross_entropy_workspace_bytes", x.device, rows)
         rc = lib.skv_cross_entropy(out.data_ptr(), ptr(row), ptr(dx), x.data_ptr(), t.data_ptr(),
                                    rows, vocab, float(grad_scale), ws.data_ptr(), ws.numel(),
                                    _lib.dtype_code(x.dtype), stream(x.device))

@@ -14,7 +14,7 @@ import torch
 
 from .. import _lib
 from .gpu_ops import batch_count
-from .gpu_pass_common import F32, FLOATS, Operand, apart, on, operand, ptr, stream
+from .gpu_pass_common import F32, FLOATS, Operand, on, operand, ptr, stream
 from .gpu_types import GPUContext
 
 _CHUNK = 2048  # elements of a tensor that a workgroup takes at a time
@@ -203,7 +203,6 @@ def adamw_read(ctx: GPUContext, state: AdamWState, m: Operand, v: Operand) -> No
     n = state.m.numel()
     mo = operand(ctx, m, "m", (n,), FLOATS)
     vo = operand(ctx, v, "v", (n,), (mo.dtype,))
-    apart([(mo, "m"), (vo, "v")], [(state.m, "the state"), (state.v, "the state")])
     dev = state.m.device
     lib = _lib.lib()
     batch_count(ctx)
