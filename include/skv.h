@@ -789,7 +789,7 @@ typedef struct skv_adamw_tensor {
  *   g' = grad_scale g, m = beta1 m + (1 - beta1) g', v = beta2 v + (1 - beta2) g'^2,
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps).
  * tensors: device memory. chunks: [n_chunks] pairs of int32 in device memory, (tensor,
- * c) for its elements [2048 c, 2048 c + 2048), each chunk of each tensor once. count:
+ * c) for its elements [4096 c, 4096 c + 4096), each chunk of each tensor once. count:
  * two int32, t (advanced by the call, on the device, so that a captured step counts on)
  * and 0. lr_dev, grad_scale_dev: where not NULL, fp32 in device memory in place of
  * lr and grad_scale.

@@ -4,8 +4,12 @@
 //   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v' / (1 - b2^t)) + eps)
 //
 // Bound by HBM: 28 bytes an element with fp32 gradients and moments. The tensors
-// are cut into chunks of 2048 elements, a table on the device names each chunk's
-// tensor, and a fixed number of workgroups walk over the chunks.
+// are cut into chunks of 4096 elements, a table on the device names each chunk's
+// tensor, and one workgroup of 512 lanes a CU walks over the chunks, the next
+// chunk's place read ahead. More workgroups are slower, in HBM (203 million elements,
+// bf16 gradients and copies: 1101 us = 5.15 TB/s with 256 x 512 lanes, 1129 with 512 x
+// 512, 1170 with 1024 x 256; a copy runs at 4.71 TB/s read and write) and for their
+// arrivals below (3.2 million elements: 16.5, 18.8 and 22.7 us).
 //
 // The step count t is in device memory, so that a captured step counts on when
 // it is replayed: every workgroup reads t before it does anything, and the last
@@ -34,7 +38,8 @@ namespace {
 
 using namespace train;
 
-constexpr int kChunk = 2048;  // elements of a workgroup and turn: 256 lanes of 8
+constexpr int kThreads = 512;
+constexpr int kChunk = kThreads * 8;  // elements of a workgroup and turn
 constexpr int kBlock = 128;   // elements that share a scale: 16 lanes of 8
 
 struct Tensor {  // skv_adamw_tensor
@@ -47,8 +52,6 @@ struct Tensor {  // skv_adamw_tensor
 };
 
 struct Step {
-  const Tensor* tensors;
-  const int2* chunks;  // (tensor, its chunk)
   int n_chunks;
   void* m;
   void* v;
@@ -200,12 +203,112 @@ __device__ __forceinline__ void store_bf16(uint16_t* p, const float (&x)[E], boo
   }
 }
 
-// BITS of a moment; TG: how gradients are stored. A lane has E consecutive
-// elements at a time: 4 of them where the moments are fp32, so that every load of a
-// wavefront is 1 KB in a row, and 8 where they are bytes.
+// One chunk of a tensor. BITS of a moment; TG: how gradients are stored. A lane has E
+// consecutive elements at a time: 4 of them where the moments are fp32, so that every
+// load of a wavefront is 1 KB in a row, and 8 where they are bytes. FULL: the chunk
+// lies inside the tensor and its vectors are aligned. All loads come before any store:
+// the compiler cannot tell the tensors apart.
+template <typename TG, int BITS, bool FULL>
+__device__ __forceinline__ void step_chunk(const Step& a, const Tensor& x, int chunk, const Coef& c,
+                                           uint32_t key) {
+  constexpr int E = BITS == 32 ? 4 : 8, kParts = 8 / E;
+  const float keep = x.decay ? c.keep : 1.f;
+  // a tensor's place in the state is filled up to whole blocks
+  const int64_t blocks_end = (x.n + kBlock - 1) / kBlock * kBlock;
+  float p[kParts][E], g[kParts][E], m[kParts][E], v[kParts][E];
+  const auto first = [&](int part) {
+    return (int64_t)chunk * kChunk + part * kThreads * E + threadIdx.x * E;
+  };
+  const auto left_of = [&](int part) {
+    return FULL ? E : (int)min((int64_t)E, max((int64_t)0, x.n - first(part)));
+  };
+#pragma unroll
+  for (int part = 0; part < kParts; ++part) {
+    const int64_t i0 = first(part);
+    const size_t at = (size_t)(x.at + i0);  // in the state
+    const int left = left_of(part);
+    const bool here = FULL || i0 < blocks_end;
+    load_f32<E>(p[part], x.p + i0, FULL, left);
+    load_f32<E>(g[part], (const TG*)x.g + i0, FULL, left);
+    if constexpr (BITS == 32) {
+      load_f32<E>(m[part], (const float*)a.m + at, here, 0);
+      load_f32<E>(v[part], (const float*)a.v + at, here, 0);
+    } else {
+      uint2 wm = make_uint2(0, 0), wv = make_uint2(0, 0);
+      uint32_t bm = 0, bv = 0;
+      if (here) {
+        wm = *reinterpret_cast<const uint2*>((const uint8_t*)a.m + at);
+        wv = *reinterpret_cast<const uint2*>((const uint8_t*)a.v + at);
+        bm = a.m_scale[at / kBlock];
+        bv = a.v_scale[at / kBlock];
+      }
+      const float dm = dec_m(bm), dv = dec_v(bv);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        m[part][e] = value_m(((e < 4 ? wm.x : wm.y) >> (8 * (e & 3))) & 255u, dm);
+        v[part][e] = value_v(((e < 4 ? wv.x : wv.y) >> (8 * (e & 3))) & 255u, dv);
+      }
+    }
+  }
+#pragma unroll
+  for (int part = 0; part < kParts; ++part) {
+    const int64_t i0 = first(part);
+    const size_t at = (size_t)(x.at + i0);
+    const int left = left_of(part);
+    const bool here = FULL || i0 < blocks_end;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      moments(m[part][e], v[part][e], g[part][e] * c.gs, c);
+      p[part][e] = stepped(p[part][e], m[part][e], v[part][e], c, keep);
+    }
+    store_f32<E>(x.p + i0, p[part], FULL, left);
+    if (x.copy) store_bf16<E>(x.copy + i0, p[part], FULL, left);
+    if constexpr (BITS == 32) {
+      store_f32<E>((float*)a.m + at, m[part], FULL, left);
+      store_f32<E>((float*)a.v + at, v[part], FULL, left);
+    } else {
+      uint32_t am = 0, av = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (e >= left) m[part][e] = v[part][e] = 0.f;  // a block read back as NaN has them too
+        am = max(am, __float_as_uint(m[part][e]) & 0x7fffffffu);
+        av = max(av, __float_as_uint(v[part][e]));
+      }
+      am = row16_umax(am);
+      av = row16_umax(av);
+      const uint32_t bm = block_byte(am), bv = block_byte(av);
+      const float em = pow2(127 + 7 - (int)min(bm, 253u)), ev = pow2(127 - (int)min(bv, 253u));
+      uint32_t u = (uint32_t)at * kMul1 + key;
+      uint32_t wm[2] = {0, 0}, wv[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t h = hash_mix(u);
+        u += kMul1;
+        wm[e / 4] |= code_m(m[part][e], em, h & 0xffffu) << (8 * (e & 3));
+        wv[e / 4] |= code_v(v[part][e], ev, h >> 16) << (8 * (e & 3));
+      }
+      if (here) {
+        *reinterpret_cast<uint2*>((uint8_t*)a.m + at) =
+            bm == 255u ? make_uint2(0, 0) : make_uint2(wm[0], wm[1]);
+        *reinterpret_cast<uint2*>((uint8_t*)a.v + at) =
+            bv == 255u ? make_uint2(0, 0) : make_uint2(wv[0], wv[1]);
+        if ((threadIdx.x & 15) == 0) {
+          a.m_scale[at / kBlock] = (uint8_t)bm;
+          a.v_scale[at / kBlock] = (uint8_t)bv;
+        }
+      }
+    }
+  }
+}
+
+// tensors, chunks: (tensor, its chunk). The next chunk's tensor is known before this
+// chunk's data are waited for.
 template <typename TG, int BITS>
-__global__ __launch_bounds__(256) void k_adamw(Step a) {
-  constexpr int E = BITS == 32 ? 4 : 8;
+__global__ __launch_bounds__(kThreads) void k_adamw(Step a, const Tensor* __restrict__ tensors,
+                                                    const int2* __restrict__ chunks) {
+  int ch = blockIdx.x;
+  int2 which = chunks[ch];
+  Tensor x = tensors[which.x];
   const int t = a.count[0] + 1;
   Coef c;
   c.b1 = a.b1;
@@ -221,85 +324,20 @@ __global__ __launch_bounds__(256) void k_adamw(Step a) {
     c.gs = a.grad_scale_dev ? *a.grad_scale_dev : a.grad_scale;
   }
   const uint32_t key = hash_key(a.seed, (uint32_t)t);
-  for (int ch = blockIdx.x; ch < a.n_chunks; ch += gridDim.x) {
-    const int2 which = a.chunks[ch];
-    const Tensor x = a.tensors[which.x];
+  for (;;) {
+    const int after = ch + gridDim.x;
+    const int2 next = chunks[min(after, a.n_chunks - 1)];
+    const Tensor next_x = tensors[next.x];
     const bool aligned = ((reinterpret_cast<uintptr_t>(x.p) | reinterpret_cast<uintptr_t>(x.g) |
                            reinterpret_cast<uintptr_t>(x.copy)) & 15) == 0;
-    const float keep = x.decay ? c.keep : 1.f;
-#pragma unroll
-    for (int part = 0; part < 8 / E; ++part) {
-      const int64_t i0 = (int64_t)which.y * kChunk + part * 256 * E + threadIdx.x * E;
-      const size_t at = (size_t)(x.at + i0);  // in the state
-      const int left = (int)min((int64_t)E, max((int64_t)0, x.n - i0));
-      const bool vec = aligned && left == E;
-      float p[E], g[E], m[E], v[E];
-      load_f32<E>(p, x.p + i0, vec, left);
-      load_f32<E>(g, (const TG*)x.g + i0, vec, left);
-      // a tensor's place in the state is filled up to whole blocks
-      const bool here = i0 < (x.n + kBlock - 1) / kBlock * kBlock;
-      if constexpr (BITS == 32) {
-        load_f32<E>(m, (const float*)a.m + at, here, 0);
-        load_f32<E>(v, (const float*)a.v + at, here, 0);
-      } else {
-        uint2 wm = make_uint2(0, 0), wv = make_uint2(0, 0);
-        uint32_t bm = 0, bv = 0;
-        if (here) {
-          wm = *reinterpret_cast<const uint2*>((const uint8_t*)a.m + at);
-          wv = *reinterpret_cast<const uint2*>((const uint8_t*)a.v + at);
-          bm = a.m_scale[at / kBlock];
-          bv = a.v_scale[at / kBlock];
-        }
-        const float dm = dec_m(bm), dv = dec_v(bv);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          m[e] = value_m(((e < 4 ? wm.x : wm.y) >> (8 * (e & 3))) & 255u, dm);
-          v[e] = value_v(((e < 4 ? wv.x : wv.y) >> (8 * (e & 3))) & 255u, dv);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        moments(m[e], v[e], g[e] * c.gs, c);
-        p[e] = stepped(p[e], m[e], v[e], c, keep);
-      }
-      store_f32<E>(x.p + i0, p, vec, left);
-      if (x.copy) store_bf16<E>(x.copy + i0, p, vec, left);
-      if constexpr (BITS == 32) {
-        store_f32<E>((float*)a.m + at, m, here && left == E, here ? left : 0);
-        store_f32<E>((float*)a.v + at, v, here && left == E, here ? left : 0);
-      } else {
-        uint32_t am = 0, av = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          if (e >= left) m[e] = v[e] = 0.f;  // a block that read back as NaN has them too
-          am = max(am, __float_as_uint(m[e]) & 0x7fffffffu);
-          av = max(av, __float_as_uint(v[e]));
-        }
-        am = row16_umax(am);
-        av = row16_umax(av);
-        const uint32_t bm = block_byte(am), bv = block_byte(av);
-        const float em = pow2(127 + 7 - (int)min(bm, 253u)), ev = pow2(127 - (int)min(bv, 253u));
-        uint32_t u = (uint32_t)at * kMul1 + key;
-        uint32_t wm[2] = {0, 0}, wv[2] = {0, 0};
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t h = hash_mix(u);
-          u += kMul1;
-          wm[e / 4] |= code_m(m[e], em, h & 0xffffu) << (8 * (e & 3));
-          wv[e / 4] |= code_v(v[e], ev, h >> 16) << (8 * (e & 3));
-        }
-        if (here) {
-          *reinterpret_cast<uint2*>((uint8_t*)a.m + at) =
-              bm == 255u ? make_uint2(0, 0) : make_uint2(wm[0], wm[1]);
-          *reinterpret_cast<uint2*>((uint8_t*)a.v + at) =
-              bv == 255u ? make_uint2(0, 0) : make_uint2(wv[0], wv[1]);
-          if ((threadIdx.x & 15) == 0) {
-            a.m_scale[at / kBlock] = (uint8_t)bm;
-            a.v_scale[at / kBlock] = (uint8_t)bv;
-          }
-        }
-      }
-    }
+    if (aligned && (int64_t)(which.y + 1) * kChunk <= x.n)
+      step_chunk<TG, BITS, true>(a, x, which.y, c, key);
+    else
+      step_chunk<TG, BITS, false>(a, x, which.y, c, key);
+    if (after >= a.n_chunks) break;
+    ch = after;
+    which = next;
+    x = next_x;
   }
   __syncthreads();  // every lane has read the count
   if (threadIdx.x == 0 && atomicAdd(a.count + 1, 1) == (int)gridDim.x - 1) {
@@ -355,8 +393,6 @@ extern "C" int skv_adamw(const skv_adamw_tensor* tensors, const int32_t* chunks,
   SKV_REQUIRE(aligned16(m) && aligned16(v), SKV_E_INVALID,
               "skv_adamw: the state must be 16-byte aligned");
   Step a;
-  a.tensors = (const Tensor*)tensors;
-  a.chunks = (const int2*)chunks;
   a.n_chunks = n_chunks;
   a.m = m;
   a.v = v;
@@ -376,14 +412,16 @@ extern "C" int skv_adamw(const skv_adamw_tensor* tensors, const int32_t* chunks,
   a.lr_dev = lr_dev;
   a.grad_scale_dev = grad_scale_dev;
   a.seed = seed;
-  const dim3 grid(n_chunks < 2048 ? n_chunks : 2048);
+  const Tensor* x = (const Tensor*)tensors;
+  const int2* ch = (const int2*)chunks;
+  const dim3 grid(n_chunks < 256 ? n_chunks : 256);
   hipStream_t s = (hipStream_t)stream;
   if (bits == 32) {
-    if (grad_dt == SKV_BF16) k_adamw<uint16_t, 32><<<grid, 256, 0, s>>>(a);
-    else k_adamw<float, 32><<<grid, 256, 0, s>>>(a);
+    if (grad_dt == SKV_BF16) k_adamw<uint16_t, 32><<<grid, kThreads, 0, s>>>(a, x, ch);
+    else k_adamw<float, 32><<<grid, kThreads, 0, s>>>(a, x, ch);
   } else {
-    if (grad_dt == SKV_BF16) k_adamw<uint16_t, 8><<<grid, 256, 0, s>>>(a);
-    else k_adamw<float, 8><<<grid, 256, 0, s>>>(a);
+    if (grad_dt == SKV_BF16) k_adamw<uint16_t, 8><<<grid, kThreads, 0, s>>>(a, x, ch);
+    else k_adamw<float, 8><<<grid, kThreads, 0, s>>>(a, x, ch);
   }
   return check_launch("skv_adamw");
 }

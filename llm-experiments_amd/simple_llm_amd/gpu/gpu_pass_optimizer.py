@@ -17,7 +17,7 @@ from .gpu_ops import batch_count
 from .gpu_pass_common import F32, FLOATS, Operand, on, operand, ptr, stream
 from .gpu_types import GPUContext
 
-_CHUNK = 2048  # elements of a tensor that a workgroup takes at a time
+_CHUNK = 4096  # elements of a tensor that a workgroup takes at a time
 _BLOCK = 128  # moments that share a scale; a tensor's begin a block
 _ZERO_SCALE = 127 - 90  # the scale byte of a block of zeros
 

@@ -376,7 +376,7 @@ def test_cross_entropy_hard_rows(gpu_ctx, vocab):
 
 # ---- AdamW -----------------------------------------------------------------
 
-SIZES = [(3,), (128,), (127, 5), (1,), (2048,), (2049,), (64, 100), (4097,), (129,)]
+SIZES = [(3,), (128,), (127, 5), (1,), (2048,), (64, 100), (4096,), (4097,), (129,), (2, 8191)]
 HYPER = dict(lr=2e-3, beta1=0.9, beta2=0.98, eps=1e-8, weight_decay=0.1)
 
 
