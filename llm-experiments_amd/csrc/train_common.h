@@ -31,6 +31,16 @@ struct Vec<float, N> {
       for (int i = 0; i < N; ++i) v[i] = r[i];
     }
   }
+  // what is read once (nt bit): it does not push other lines out of the caches
+  __device__ __forceinline__ void stream(const float* p) {
+    if constexpr (N == 1) {
+      v[0] = __builtin_nontemporal_load(p);
+    } else {
+      const raw_t r = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(p));
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = r[i];
+    }
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.f;
@@ -45,6 +55,16 @@ struct Vec<float, N> {
 #pragma unroll
       for (int i = 0; i < N; ++i) r[i] = x[i];
       *reinterpret_cast<raw_t*>(p) = r;
+    }
+  }
+  static __device__ __forceinline__ void store_stream(float* p, const float (&x)[N]) {
+    if constexpr (N == 1) {
+      __builtin_nontemporal_store(x[0], p);
+    } else {
+      raw_t r;
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = x[i];
+      __builtin_nontemporal_store(r, reinterpret_cast<raw_t*>(p));
     }
   }
 };
@@ -65,6 +85,15 @@ struct Vec<uint16_t, N> {  // N even
       w[0] = *reinterpret_cast<const uint32_t*>(p);
     } else {
       const raw_t r = *reinterpret_cast<const raw_t*>(p);
+#pragma unroll
+      for (int i = 0; i < NW; ++i) w[i] = r[i];
+    }
+  }
+  __device__ __forceinline__ void stream(const uint16_t* p) {
+    if constexpr (NW == 1) {
+      w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      const raw_t r = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(p));
 #pragma unroll
       for (int i = 0; i < NW; ++i) w[i] = r[i];
     }
@@ -92,17 +121,31 @@ struct Vec<uint16_t, N> {  // N even
       *reinterpret_cast<raw_t*>(p) = r;
     }
   }
+  static __device__ __forceinline__ void store_stream(uint16_t* p, const float (&x)[N]) {
+    if constexpr (NW == 1) {
+      __builtin_nontemporal_store(pack_bf16(x[0], x[1]), reinterpret_cast<uint32_t*>(p));
+    } else {
+      raw_t r;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) r[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+      __builtin_nontemporal_store(r, reinterpret_cast<raw_t*>(p));
+    }
+  }
 };
 
 template <>
 struct Vec<uint16_t, 1> {
   uint16_t h;
   __device__ __forceinline__ void load(const uint16_t* p) { h = *p; }
+  __device__ __forceinline__ void stream(const uint16_t* p) { h = __builtin_nontemporal_load(p); }
   __device__ __forceinline__ void zero() { h = 0; }
   __device__ __forceinline__ float get(int) const { return bf16_to_f32(h); }
   __device__ __forceinline__ void keep() {}
   static __device__ __forceinline__ void store(uint16_t* p, const float (&x)[1]) {
     *p = f32_to_bf16(x[0]);
+  }
+  static __device__ __forceinline__ void store_stream(uint16_t* p, const float (&x)[1]) {
+    __builtin_nontemporal_store(f32_to_bf16(x[0]), p);
   }
 };
 

@@ -11,15 +11,18 @@
 //
 //   sort  a workgroup has a bucket of consecutive ids. It counts their tokens
 //         and the tokens of all smaller ids (where its part of the order begins)
-//         in one scan over the ids, and places the tokens in a second; the ids
-//         come from L2 after the first workgroup's read. It also writes the zero
-//         rows of ids without tokens, which are most of a large table and most of
-//         what this operator writes, while the scans wait on loads.
+//         in a scan over all ids, and places the tokens. Beside these workgroups
+//         others set the table to zero, which is most of what this operator
+//         writes and would otherwise wait for the order.
 //   sum   a wavefront has 64 columns' vectors and a range of kRange sorted tokens,
 //         whatever their ids: the work is even however unevenly the ids occur. A
 //         row whose tokens all lie in the range is written; one that crosses a
 //         range's border leaves its part.
 //   join  adds the parts of each such row, in order.
+//
+// 16384 zipf tokens, table 50304 x 768 fp32 (154 MB written, 50 read): sort 24 us (7
+// without the zeros), sum 22 (17 where HBM is not still writing zeros), join 5; 47 us in
+// all. One bucket per CU and not two: 52.5 against 57 us. Zeros with the nt bit: 51 -> 47.
 #include "train_common.h"
 
 namespace skv {
@@ -29,8 +32,10 @@ using namespace train;
 
 constexpr int kBucket = 256;  // ids of a bucket, at most
 constexpr int kWaves = 16;    // wavefronts of a sorting workgroup
-constexpr int kRange = 32;    // sorted tokens of a summing wavefront
+constexpr int kBatches = 16;  // batches of 64 tokens a sorting wavefront reads at a time
+constexpr int kRange = 16;    // sorted tokens of a summing wavefront
 constexpr int kJoinWaves = 8;
+constexpr int kZeroGroups = 128;  // workgroups that zero the table
 
 // ---------------------------------------------------------------------------
 // lookup
@@ -61,7 +66,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(TO* __restrict__ out,
     float r[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) r[e] = t.get(e) * scale + p.get(e);
-    Vec<TO, VEC>::store(o + j, r);
+    Vec<TO, VEC>::store_stream(o + j, r);
   }
 }
 
@@ -73,6 +78,8 @@ struct Sorted {
   int32_t* pos;    // [T] tokens in order of their ids
   int32_t* id;     // [T] their ids
   int32_t* begin;  // [V + 1] where an id's tokens begin
+  int2* goes_on;   // [ranges] of a row that begins in a range and goes on: its id and the
+                   // number of ranges it lies in; or (-1, 0)
 };
 
 __device__ __forceinline__ int wave_isum(int x) {
@@ -82,33 +89,72 @@ __device__ __forceinline__ int wave_isum(int x) {
 }
 
 // width: ids of a bucket. Each wavefront has a run of consecutive tokens in both
-// scans; an id's tokens are placed by wavefront, then by token.
-__global__ __launch_bounds__(kWaves * 64) void k_embed_sort(Sorted s,
-                                                            const int32_t* __restrict__ ids,
-                                                            float* __restrict__ grad, int T, int V,
-                                                            int d, int width, int fill_zero) {
+// scans; an id's tokens are placed by wavefront, then by token. Tokens are read 16 x 64
+// at a time and the bucket's own go to a list in LDS, in order: it is short but for a
+// bucket of frequent ids (of 16384 zipf tokens a bucket of 99 ids has 32 on average and
+// 1000 at most, 60 a wavefront), and what finds an id's rank among 64 tokens costs 0.3 us.
+__global__ __launch_bounds__(kWaves * 64, 8) void k_embed_sort(Sorted s,
+                                                               const int32_t* __restrict__ ids,
+                                                               int T, int V, int width, int buckets,
+                                                               float* __restrict__ grad,
+                                                               size_t n_zero) {
+  if ((int)blockIdx.x >= buckets) {
+    const size_t step = (size_t)(gridDim.x - buckets) * kWaves * 64 * 4;
+    const size_t i0 = (size_t)(blockIdx.x - buckets) * kWaves * 64 + threadIdx.x;
+    for (size_t i = i0 * 4; i + 4 <= n_zero; i += step)
+      __builtin_nontemporal_store(f32x4_t{0.f, 0.f, 0.f, 0.f}, reinterpret_cast<f32x4_t*>(grad + i));
+    if (i0 < n_zero % 4) grad[n_zero - 1 - i0] = 0.f;
+    return;
+  }
+  constexpr int kRead = kBatches * 64;
   __shared__ int cnt[kWaves][kBucket];
   __shared__ int tot[kBucket];   // tokens of an id
   __shared__ int base[kBucket];  // where they begin in the bucket
   __shared__ int less[kWaves];
+  __shared__ uint16_t list_t[kWaves][kRead];  // the bucket's tokens of those read last
+  __shared__ uint8_t list_l[kWaves][kRead];   // and their ids' places in the bucket
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int lo = blockIdx.x * width, n_ids = min(width, V - lo);
-  for (int j = threadIdx.x; j < kWaves * kBucket; j += kWaves * 64) cnt[j / kBucket][j % kBucket] = 0;
-  __syncthreads();
   const int per = ((T + kWaves * 64 - 1) / (kWaves * 64)) * 64;
   const int t0 = min(w * per, T), t1 = min(t0 + per, T);
   int below = 0;
-#pragma unroll 8
-  for (int t = t0 + lane; t < t1; t += 64) {
-    const int id = ids[t], l = id - lo;
-    below += id >= 0 && l < 0;
-    if ((unsigned)l < (unsigned)n_ids) atomicAdd(&cnt[w][l], 1);
+  // tokens t .. t + kRead of the wavefront to its list; their number
+  const auto read = [&](int t) {
+    int id[kBatches], n = 0;
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i) {
+      const int k = t + i * 64 + lane;
+      id[i] = k < t1 ? ids[k] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i) {
+      const int l = id[i] - lo;
+      const bool in = id[i] >= 0 && (unsigned)l < (unsigned)n_ids;
+      below += id[i] >= 0 && l < 0;
+      const uint64_t mask = __ballot(in);
+      if (in) {
+        const int at = n + __popcll(mask & ((1ull << lane) - 1));
+        list_t[w][at] = (uint16_t)(i * 64 + lane);
+        list_l[w][at] = (uint8_t)l;
+      }
+      n += __popcll(mask);
+    }
+    __builtin_amdgcn_wave_barrier();
+    return n;
+  };
+  for (int j = lane; j < kBucket; j += 64) cnt[w][j] = 0;  // the wavefront's own
+  __builtin_amdgcn_wave_barrier();
+  int n = 0;
+  for (int t = t0; t < t1; t += kRead) {
+    n = read(t);
+    for (int i = lane; i < n; i += 64) atomicAdd(&cnt[w][list_l[w][i]], 1);
   }
   below = wave_isum(below);
   if (lane == 0) less[w] = below;
   __syncthreads();
   if (threadIdx.x < kBucket) {
     int sum = 0;
+#pragma unroll
     for (int i = 0; i < kWaves; ++i) {
       const int c = cnt[i][threadIdx.x];
       cnt[i][threadIdx.x] = sum;  // tokens of this id in earlier wavefronts' runs
@@ -117,10 +163,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_embed_sort(Sorted s,
     tot[threadIdx.x] = sum;
   }
   __syncthreads();
-  int first = 0;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) first += less[i];
   if (w == 0) {  // exclusive sums over the bucket's ids, four a lane
+    const int first = wave_isum(lane < kWaves ? less[lane] : 0);
     int c[4], sum = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -134,65 +178,63 @@ __global__ __launch_bounds__(kWaves * 64) void k_embed_sort(Sorted s,
       if (lane >= o) incl += up;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) base[lane * 4 + i] = first + incl - sum + c[i];
-    if (blockIdx.x == gridDim.x - 1 && lane == 63) s.begin[V] = first + incl;
+    for (int i = 0; i < 4; ++i) {
+      const int b = first + incl - sum + c[i];
+      base[lane * 4 + i] = b;
+      if (lane * 4 + i < n_ids) s.begin[lo + lane * 4 + i] = b;
+    }
+    if ((int)blockIdx.x == buckets - 1 && lane == 63) s.begin[V] = first + incl;
   }
   __syncthreads();
-  for (int j = threadIdx.x; j < n_ids; j += kWaves * 64) s.begin[lo + j] = base[j];
-  for (int j = threadIdx.x; j < kWaves * kBucket; j += kWaves * 64)
-    cnt[j / kBucket][j % kBucket] += base[j % kBucket];
-  __syncthreads();
-  for (int t = t0; t < t1; t += 64) {
-    const int id = t + lane < t1 ? ids[t + lane] : -1, l = id - lo;
-    const bool in = id >= 0 && (unsigned)l < (unsigned)n_ids;
-    uint64_t same = __ballot(in);
-    if (!same) continue;
+  for (int t = t0; t < t1; t += kRead) {
+    if (per > kRead) n = read(t);  // else the list of the first scan is still there
+    for (int i = 0; i < n; i += 64) {
+      const bool in = i + lane < n;
+      const int l = in ? list_l[w][i + lane] : 0;
+      uint64_t same = __ballot(in);
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {  // lanes whose id is this lane's
-      const uint64_t has = __ballot(in && ((l >> b) & 1));
-      same &= (l >> b) & 1 ? has : ~has;
-    }
-    if (in) {
-      const int at = cnt[w][l] + __popcll(same & ((1ull << lane) - 1));
-      s.pos[at] = t + lane;
-      s.id[at] = id;
-    }
-    __builtin_amdgcn_wave_barrier();
-    if (in && (same >> lane) == 1) cnt[w][l] += __popcll(same);  // the last of them
-    __builtin_amdgcn_wave_barrier();
-  }
-  if (fill_zero) {
-    for (int j = w; j < n_ids; j += kWaves) {
-      if (tot[j]) continue;
-      float* g = grad + (size_t)(lo + j) * d;
-      if (d % 4 == 0) {
-        for (int c = lane * 4; c < d; c += 256)
-          *reinterpret_cast<f32x4_t*>(g + c) = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      } else {
-        for (int c = lane; c < d; c += 64) g[c] = 0.f;
+      for (int b = 0; b < 8; ++b) {  // lanes whose id is this lane's
+        const uint64_t has = __ballot(in && ((l >> b) & 1));
+        same &= (l >> b) & 1 ? has : ~has;
       }
+      if (in) {
+        const int to = base[l] + cnt[w][l] + __popcll(same & ((1ull << lane) - 1));
+        s.pos[to] = t + list_t[w][i + lane];
+        s.id[to] = lo + l;
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (in && (same >> lane) == 1) cnt[w][l] += __popcll(same);  // the last of them
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
 
 // part: [ranges][2][dp]: of a row that began in an earlier range, and of one that
 // goes on in the next.
-template <typename T, int VEC, bool ACC>
+template <typename TY, int VEC, bool ACC>
 __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
                                                    float* __restrict__ part,
-                                                   const T* __restrict__ dy, Sorted s, int V, int d,
-                                                   int dp, float scale, int tiles) {
-  const int lane = threadIdx.x & 63;
-  const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int r = unit / tiles, c = (unit - r * tiles) * 64 * VEC + lane * VEC;
-  const int n = s.begin[V], k0 = r * kRange, cnt = min(kRange, n - k0);
-  if (cnt <= 0) return;
+                                                   const TY* __restrict__ dy, Sorted s, int T, int V,
+                                                   int d, int dp, float scale, int tiles,
+                                                   int ranges) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int unit = blockIdx.x * 4 + w;
+  const int r = unit / tiles, tile = unit - r * tiles, c = tile * 64 * VEC + lane * VEC;
+  if (r >= ranges) return;
+  const int k0 = r * kRange;
   const bool here = c < d;
-  // lane i: token i of the range, lane kRange the first of the next one
+  // lane i: token i of the range, lane kRange the first of the next one; read before the
+  // number of sorted tokens is known (what lies behind them is not used)
   int my_pos = 0, my_id = -1;
-  if (lane < cnt) my_pos = s.pos[k0 + lane];
-  if (lane <= cnt && k0 + lane < n) my_id = s.id[k0 + lane];
+  if (lane < kRange && k0 + lane < T) my_pos = s.pos[k0 + lane];
+  if (lane <= kRange && k0 + lane < T) my_id = s.id[k0 + lane];
   const int before = k0 > 0 ? s.id[k0 - 1] : -1;
+  const int n = s.begin[V], cnt = min(kRange, n - k0);
+  if (cnt <= 0) {
+    if (lane == 0 && tile == 0) s.goes_on[r] = make_int2(-1, 0);
+    return;
+  }
+  if (k0 + lane >= n) my_id = -1;
   // where an id's tokens end, the last token of the range included
   const int next_id = __shfl_down(my_id, 1);  // by all lanes, before any branch
   const uint64_t ends = __ballot(lane < cnt && (lane == cnt - 1 || my_id != next_id));
@@ -200,12 +242,20 @@ __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
   const bool opened = before == __builtin_amdgcn_readlane(my_id, 0);
   const bool goes_on = __builtin_amdgcn_readlane(my_id, cnt) ==
                        __builtin_amdgcn_readlane(my_id, cnt - 1);
+  if (tile == 0) {
+    int2 on = make_int2(-1, 0);
+    if (goes_on && !(opened && first_end == cnt - 1)) {
+      on.x = __builtin_amdgcn_readlane(my_id, cnt - 1);
+      on.y = (s.begin[on.x + 1] - 1) / kRange - r + 1;
+    }
+    if (lane == 0) s.goes_on[r] = on;
+  }
   float acc[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
   constexpr int U = 8;
   for (int k = 0; k < cnt; k += U) {
-    Vec<T, VEC> v[U];
+    Vec<TY, VEC> v[U];
     Vec<float, VEC> was[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -246,59 +296,93 @@ __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
   }
 }
 
-// One workgroup a range and column tile; those whose last row goes on in the
-// next range, and began in this one, add up its parts: each wavefront a run of
-// consecutive ranges, then the wavefronts' sums in order.
-template <int VEC>
+// grad's row `id`, columns from c on, is (what was there +) scale * sum
+template <int VEC, bool ACC>
+__device__ __forceinline__ void put_row(float* __restrict__ grad, int id, int c, int d, float scale,
+                                        const Vec<float, VEC>& was, const float (&sum)[VEC]) {
+  float o[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) o[e] = ACC ? was.get(e) + sum[e] * scale : sum[e] * scale;
+  Vec<float, VEC>::store(grad + (size_t)id * d + c, o);
+}
+
+// A workgroup has kJoinWaves ranges and a column tile: a wavefront the row that begins
+// in its range and goes on, where that is a row of few ranges (most are: about every
+// other range ends inside a row); then, together, those of many, each wavefront a run
+// of consecutive ranges and the wavefronts' sums in order.
+template <int VEC, bool ACC>
 __global__ __launch_bounds__(kJoinWaves * 64) void k_embed_join(float* __restrict__ grad,
                                                                 const float* __restrict__ part,
-                                                                Sorted s, int V, int d, int dp,
-                                                                float scale, int accumulate) {
+                                                                const int2* __restrict__ goes_on,
+                                                                int ranges, int d, int dp,
+                                                                float scale) {
   __shared__ float sh[kJoinWaves][64 * VEC];
-  const int r = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int k1 = (r + 1) * kRange;
-  if (k1 >= s.begin[V]) return;
-  const int id = s.id[k1 - 1];
-  if (s.id[k1] != id) return;
-  const int b = s.begin[id], e1 = s.begin[id + 1];
-  if (b < k1 - kRange) return;  // an earlier range's
-  const int last = (e1 - 1) / kRange, n = last - r + 1;  // ranges of this row
-  const int per = (n + kJoinWaves - 1) / kJoinWaves;
+  constexpr int kFew = 8;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r0 = blockIdx.x * kJoinWaves;
   const int c = blockIdx.y * 64 * VEC + lane * VEC;
+  int2 mine = make_int2(-1, 0);
+  if (lane < kJoinWaves && r0 + lane < ranges) mine = goes_on[r0 + lane];
+  uint64_t rows = __ballot(mine.y > kFew);  // the same in every wavefront
+  Vec<float, VEC> was;
+  was.zero();
   float acc[VEC];
+  {
+    const int id = __builtin_amdgcn_readlane(mine.x, w), n = __builtin_amdgcn_readlane(mine.y, w);
+    if (id >= 0 && n <= kFew && c < d) {
+      const float* p = part + (size_t)(r0 + w) * 2 * dp + c;
+      Vec<float, VEC> v[kFew];
+      if (ACC) was.load(grad + (size_t)id * d + c);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-  if (c < d) {
-#pragma unroll 8
-    for (int i = w * per; i < min((w + 1) * per, n); ++i) {
-      Vec<float, VEC> v;
-      v.load(part + ((size_t)(r + i) * 2 + (i == 0)) * dp + c);
+      for (int j = 0; j < kFew; ++j) {
+        v[j].zero();
+        if (j < n) v[j].load(p + ((size_t)j * 2 + (j == 0)) * dp);
+      }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] += v.get(e);
+      for (int e = 0; e < VEC; ++e) {
+        acc[e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < kFew; ++j) acc[e] += v[j].get(e);
+      }
+      put_row<VEC, ACC>(grad, id, c, d, scale, was, acc);
     }
   }
-  Vec<float, VEC>::store(&sh[w][lane * VEC], acc);
-  __syncthreads();
-  if (w == 0 && c < d) {
-    float* g = grad + (size_t)id * d + c;
-    Vec<float, VEC> was;
-    was.zero();
-    if (accumulate) was.load(g);
-    float o[VEC];
+  while (rows) {
+    const int i = __builtin_ctzll(rows), r = r0 + i;
+    rows &= rows - 1;
+    const int id = __builtin_amdgcn_readlane(mine.x, i), n = __builtin_amdgcn_readlane(mine.y, i);
+    const int per = (n + kJoinWaves - 1) / kJoinWaves;
+    if (ACC && w == 0 && c < d) was.load(grad + (size_t)id * d + c);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float t = 0.f;
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+    if (c < d) {
+#pragma unroll 8
+      for (int j = w * per; j < min((w + 1) * per, n); ++j) {
+        Vec<float, VEC> v;
+        v.load(part + ((size_t)(r + j) * 2 + (j == 0)) * dp + c);
 #pragma unroll
-      for (int i = 0; i < kJoinWaves; ++i) t += sh[i][lane * VEC + e];
-      o[e] = was.get(e) + t * scale;
+        for (int e = 0; e < VEC; ++e) acc[e] += v.get(e);
+      }
     }
-    Vec<float, VEC>::store(g, o);
+    __syncthreads();  // the sums of the row before have been read
+    Vec<float, VEC>::store(&sh[w][lane * VEC], acc);
+    __syncthreads();
+    if (w == 0 && c < d) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        acc[e] = 0.f;
+#pragma unroll
+        for (int q = 0; q < kJoinWaves; ++q) acc[e] += sh[q][lane * VEC + e];
+      }
+      put_row<VEC, ACC>(grad, id, c, d, scale, was, acc);
+    }
   }
 }
 
 int ranges_of(int T) { return (T + kRange - 1) / kRange; }
 int padded(int d) { return (d + 3) / 4 * 4; }
-size_t ints_of(int T, int V) { return ((size_t)2 * T + V + 1 + 3) / 4 * 4; }
+size_t ints_of(int T, int V) {
+  return ((size_t)2 * ranges_of(T) + 2 * (size_t)T + V + 1 + 3) / 4 * 4;
+}
 
 }  // namespace
 }  // namespace skv
@@ -371,32 +455,36 @@ extern "C" int skv_embedding_bwd(float* grad, const void* dout, const int32_t* i
     return rc;
   hipStream_t st = (hipStream_t)stream;
   Sorted s;
-  s.pos = (int32_t*)ws;
+  const int ranges = ranges_of(T), dp = padded(d);
+  s.goes_on = (int2*)ws;
+  s.pos = (int32_t*)(s.goes_on + ranges);
   s.id = s.pos + T;
   s.begin = s.id + T;
   float* part = (float*)((int32_t*)ws + ints_of(T, V));
-  const int dp = padded(d);
-  // about two buckets to a CU, so that the zero rows are written by all of them
-  int width = (V + 511) / 512;
+  // about two buckets to a CU
+  int width = (V + 255) / 256;
   width = width < 16 ? 16 : width > kBucket ? kBucket : width;
-  k_embed_sort<<<(V + width - 1) / width, kWaves * 64, 0, st>>>(s, ids, grad, T, V, d, width,
-                                                                !accumulate);
+  const int buckets = (V + width - 1) / width;
+  const size_t n_zero = accumulate ? 0 : (size_t)V * d;
+  const int sort_grid = buckets + (n_zero ? kZeroGroups : 0);
+  k_embed_sort<<<sort_grid, kWaves * 64, 0, st>>>(s, ids, T, V, width, buckets, grad, n_zero);
   if (int rc = check_launch("skv_embedding_bwd")) return rc;
-  const int ranges = ranges_of(T);
   const auto run = [&](auto* y, auto VEC) {
     using TY = std::remove_const_t<std::remove_pointer_t<decltype(y)>>;
     const int tiles = (d + 64 * VEC.value - 1) / (64 * VEC.value);
-    const size_t units = (size_t)ranges * tiles;
-    const unsigned grid = (unsigned)((units + 3) / 4);
-    if (accumulate)
-      k_embed_sum<TY, VEC.value, true><<<grid, 256, 0, st>>>(grad, part, y, s, V, d, dp, scale,
-                                                             tiles);
-    else
-      k_embed_sum<TY, VEC.value, false><<<grid, 256, 0, st>>>(grad, part, y, s, V, d, dp, scale,
-                                                              tiles);
-    if (ranges > 1)
-      k_embed_join<VEC.value><<<dim3(ranges - 1, tiles), kJoinWaves * 64, 0, st>>>(
-          grad, part, s, V, d, dp, scale, accumulate);
+    const unsigned grid = (unsigned)(((size_t)ranges * tiles + 3) / 4);
+    const dim3 join((ranges + kJoinWaves - 1) / kJoinWaves, tiles);
+    if (accumulate) {
+      k_embed_sum<TY, VEC.value, true><<<grid, 256, 0, st>>>(grad, part, y, s, T, V, d, dp, scale,
+                                                             tiles, ranges);
+      k_embed_join<VEC.value, true><<<join, kJoinWaves * 64, 0, st>>>(grad, part, s.goes_on, ranges,
+                                                                      d, dp, scale);
+    } else {
+      k_embed_sum<TY, VEC.value, false><<<grid, 256, 0, st>>>(grad, part, y, s, T, V, d, dp, scale,
+                                                              tiles, ranges);
+      k_embed_join<VEC.value, false><<<join, kJoinWaves * 64, 0, st>>>(grad, part, s.goes_on, ranges,
+                                                                       d, dp, scale);
+    }
   };
   const auto with = [&](auto* y) {
     if (d % 4 == 0) run(y, std::integral_constant<int, 4>{});
