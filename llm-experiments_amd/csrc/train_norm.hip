@@ -222,35 +222,33 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_bwd(
 }
 
 // dgamma and dbeta: the columns' sums over the P workgroups' parts, in a fixed
-// order. A workgroup has 64 columns: 16 lanes of 4 by 64 groups of rows.
+// order. A workgroup has 64 columns: 16 lanes of 4 by 64 groups of rows, four to a
+// wavefront; up to 512 parts each group's loads are in flight at once.
 __global__ __launch_bounds__(1024) void k_ln_wgrad(float* __restrict__ dgamma,
                                                    float* __restrict__ dbeta,
                                                    const float* __restrict__ part, int P, int d,
                                                    int dp, int accumulate) {
-  __shared__ f32x4_t sh[64][16];
+  __shared__ float sh[16][64];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
   const int j = blockIdx.x * 64 + c * 4;  // of 2 dp columns
   f32x4_t s = {0.f, 0.f, 0.f, 0.f};
   if (j < 2 * dp) {
 #pragma unroll 8
-    for (int p = r; p < P; p += 64) {
-      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(part + (size_t)p * 2 * dp + j);
-      s += v;
-    }
+    for (int p = r; p < P; p += 64)
+      s += *reinterpret_cast<const f32x4_t*>(part + (size_t)p * 2 * dp + j);
   }
-  sh[r][c] = s;
-  __syncthreads();
-  for (int o = 32; o >= 1; o >>= 1) {
-    if (r < o) sh[r][c] += sh[r + o][c];
-    __syncthreads();
-  }
-  if (r == 0 && j < 2 * dp) {
-    s = sh[0][c];
-    float* out = j < dp ? dgamma + j : dbeta + (j - dp);
-    const int col = j < dp ? j : j - dp;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (col + e < d) out[e] = accumulate ? out[e] + s[e] : s[e];
+  for (int e = 0; e < 4; ++e) s[e] = xor32_sum(xor16_sum(s[e]));
+  if ((threadIdx.x & 63) < 16) *reinterpret_cast<f32x4_t*>(&sh[threadIdx.x >> 6][c * 4]) = s;
+  __syncthreads();
+  const int at = blockIdx.x * 64 + threadIdx.x;
+  if (threadIdx.x < 64 && at < 2 * dp) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) t += sh[w][threadIdx.x];
+    const int col = at < dp ? at : at - dp;
+    float* out = (at < dp ? dgamma : dbeta) + col;
+    if (col < d) *out = accumulate ? *out + t : t;
   }
 }
 

@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .gpu_pass_common import (F32, FLOATS, I32, Operand, on, operand, ptr, rows_of, stream,
+from .gpu_pass_common import (F32, FLOATS, I32, Operand, launch, operand, required, rows_of,
                               workspace)
 from .gpu_ops import batch_count, validate_buffer_shape_1d, validate_buffer_shape_2d
 from .gpu_types import GPUBuffer1D, GPUBuffer2D, GPUContext
@@ -119,26 +119,19 @@ def layernorm_backward(ctx: GPUContext, grad_output: Operand, input: Operand, ga
     layer), or None. grad_input may be grad_output, input or residual.
     accumulate: grad_gamma and grad_beta are added to (grad_input is not).
     """
-    x = rows_of(ctx, input, "input", FLOATS)
-    rows, d = x.shape
-    like = (x.dtype,)
-    dy = operand(ctx, grad_output, "grad_output", (rows, d), like)
-    dx = operand(ctx, grad_input, "grad_input", (rows, d), like)
-    res = None if residual is None else operand(ctx, residual, "residual", (rows, d), like)
-    g = operand(ctx, gamma, "gamma", (d,), F32)
-    mu = operand(ctx, mean, "mean", (rows,), F32, 4)
-    rs = operand(ctx, rstd, "rstd", (rows,), F32, 4)
-    dg = operand(ctx, grad_gamma, "grad_gamma", (d,), F32, 4)
-    db = operand(ctx, grad_beta, "grad_beta", (d,), F32, 4)
-    lib = _lib.lib()
-    batch_count(ctx)
-    with on(x.device):
-        ws = workspace("skv_layernorm_bwd_workspace_bytes", x.device, rows, d)
-        rc = lib.skv_layernorm_bwd(dx.data_ptr(), dg.data_ptr(), db.data_ptr(), dy.data_ptr(),
-                                   x.data_ptr(), g.data_ptr(), mu.data_ptr(), rs.data_ptr(),
-                                   ptr(res), rows, d, int(bool(accumulate)), ws.data_ptr(),
-                                   ws.numel(), _lib.dtype_code(x.dtype), stream(x.device))
-    _lib.check(rc, "skv_layernorm_bwd")
+    x, rows, d, dtype = rows_of(ctx, input, "input", FLOATS)
+    like, shape = (dtype,), (rows, d)
+    dy = required(ctx, grad_output, "grad_output", shape, like)
+    dx = required(ctx, grad_input, "grad_input", shape, like)
+    res = operand(ctx, residual, "residual", shape, like)
+    g = required(ctx, gamma, "gamma", (d,), F32)
+    mu = required(ctx, mean, "mean", (rows,), F32, 4)
+    rs = required(ctx, rstd, "rstd", (rows,), F32, 4)
+    dg = required(ctx, grad_gamma, "grad_gamma", (d,), F32, 4)
+    db = required(ctx, grad_beta, "grad_beta", (d,), F32, 4)
+    ws = workspace(ctx, "skv_layernorm_bwd_workspace_bytes", rows, d)
+    launch(ctx, "skv_layernorm_bwd", dx, dg, db, dy, x, g, mu, rs, res, rows, d,
+           int(bool(accumulate)), ws.data_ptr(), ws.numel(), _lib.dtype_code(dtype))
 
 
 def embedding_backward(ctx: GPUContext, grad_output: Operand, tokens: Operand,
@@ -151,21 +144,12 @@ def embedding_backward(ctx: GPUContext, grad_output: Operand, tokens: Operand,
     touched), as where the tied logits have left their part. Tokens outside [0, vocab) are
     padding and add nothing.
     """
-    dy = rows_of(ctx, grad_output, "grad_output", FLOATS)
-    n, d = dy.shape
-    ids = operand(ctx, tokens, "tokens", (n,), I32, 4)
-    grad = rows_of(ctx, grad_table, "grad_table", F32)
-    if grad.shape[1] != d:
-        raise ValueError(f"grad_table shape mismatch: got {tuple(grad.shape)}, expected (*, {d})")
-    vocab = grad.shape[0]
-    lib = _lib.lib()
-    batch_count(ctx)
-    with on(grad.device):
-        ws = workspace("skv_embedding_bwd_workspace_bytes", grad.device, n, vocab, d)
-        rc = lib.skv_embedding_bwd(grad.data_ptr(), dy.data_ptr(), ids.data_ptr(), n, vocab, d,
-                                   float(scale), int(bool(accumulate)), ws.data_ptr(), ws.numel(),
-                                   _lib.dtype_code(dy.dtype), stream(grad.device))
-    _lib.check(rc, "skv_embedding_bwd")
+    dy, n, d, dtype = rows_of(ctx, grad_output, "grad_output", FLOATS)
+    ids = required(ctx, tokens, "tokens", (n,), I32, 4)
+    grad, vocab, _, _ = rows_of(ctx, grad_table, "grad_table", F32, d)
+    ws = workspace(ctx, "skv_embedding_bwd_workspace_bytes", n, vocab, d)
+    launch(ctx, "skv_embedding_bwd", grad, dy, ids, n, vocab, d, float(scale),
+           int(bool(accumulate)), ws.data_ptr(), ws.numel(), _lib.dtype_code(dtype))
 
 
 __all__ = ["embedding_backward", "flash_attention_backward", "layernorm_backward"]

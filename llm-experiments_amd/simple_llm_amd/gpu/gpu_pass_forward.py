@@ -24,8 +24,8 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .gpu_pass_common import (F32, FLOATS, I32, Operand, on, operand, ptr, rows_of, stream,
-                              workspace)
+from .gpu_pass_common import (F32, FLOATS, I32, Operand, launch, operand, required, rows_of,
+                              tensor_of, workspace)
 from .gpu_ops import batch_count, validate_buffer_shape_1d, validate_buffer_shape_2d
 from .gpu_types import GPUBuffer1D, GPUBuffer2D, GPUContext
 
@@ -93,25 +93,18 @@ def embedding(ctx: GPUContext, tokens: Operand, table: Operand, output: Operand,
     of exactly `context` tokens). A token outside [0, vocab) is padding: its table row counts
     as zeros.
     """
-    w = rows_of(ctx, table, "table", FLOATS)
-    ids = operand(ctx, tokens, "tokens", None, I32, 4)
-    if ids.dim() != 1 or not 0 < ids.shape[0] < 1 << 31:
-        raise ValueError(f"tokens must be 1-D and hold elements, got shape {tuple(ids.shape)}")
-    n, (vocab, d) = ids.shape[0], w.shape
-    out = operand(ctx, output, "output", (n, d), FLOATS)
-    pos = None
+    w, vocab, d, w_dtype = rows_of(ctx, table, "table", FLOATS)
+    ids = required(ctx, tokens, "tokens", None, I32, 4)
+    shape = tensor_of(tokens).shape
+    if len(shape) != 1 or not 0 < shape[0] < 1 << 31:
+        raise ValueError(f"tokens must be 1-D and hold elements, got shape {tuple(shape)}")
+    n = shape[0]
+    out = required(ctx, output, "output", (n, d), FLOATS)
+    pos, n_pos = None, 0
     if pos_table is not None:
-        pos = rows_of(ctx, pos_table, "pos_table", F32)
-        if pos.shape[1] != d:
-            raise ValueError(f"pos_table shape mismatch: got {tuple(pos.shape)}, expected (*, {d})")
-    lib = _lib.lib()
-    batch_count(ctx)
-    with on(out.device):
-        rc = lib.skv_embedding_fwd(out.data_ptr(), ids.data_ptr(), w.data_ptr(), ptr(pos), n, vocab,
-                                   d, 0 if pos is None else pos.shape[0], float(scale),
-                                   _lib.dtype_code(w.dtype), _lib.dtype_code(out.dtype),
-                                   stream(out.device))
-    _lib.check(rc, "skv_embedding_fwd")
+        pos, n_pos, _, _ = rows_of(ctx, pos_table, "pos_table", F32, d)
+    launch(ctx, "skv_embedding_fwd", out, ids, w, pos, n, vocab, d, n_pos, float(scale),
+           _lib.dtype_code(w_dtype), _lib.dtype_code(tensor_of(output).dtype))
 
 
 def layernorm(ctx: GPUContext, input: Operand, gamma: Operand, beta: Operand, output: Operand,
@@ -123,22 +116,16 @@ def layernorm(ctx: GPUContext, input: Operand, gamma: Operand, beta: Operand, ou
     input. gamma, beta: float32 [d]. mean, rstd: float32 [rows], the rows' statistics for
     layernorm_backward (rstd = 1 / sqrt(var + eps)), or None.
     """
-    x = rows_of(ctx, input, "input", FLOATS)
-    rows, d = x.shape
-    y = operand(ctx, output, "output", (rows, d), (x.dtype,))
-    g = operand(ctx, gamma, "gamma", (d,), F32)
-    b = operand(ctx, beta, "beta", (d,), F32)
-    mu = None if mean is None else operand(ctx, mean, "mean", (rows,), F32, 4)
-    rs = None if rstd is None else operand(ctx, rstd, "rstd", (rows,), F32, 4)
+    x, rows, d, dtype = rows_of(ctx, input, "input", FLOATS)
+    y = required(ctx, output, "output", (rows, d), (dtype,))
+    g = required(ctx, gamma, "gamma", (d,), F32)
+    b = required(ctx, beta, "beta", (d,), F32)
+    mu = operand(ctx, mean, "mean", (rows,), F32, 4)
+    rs = operand(ctx, rstd, "rstd", (rows,), F32, 4)
     if not eps >= 0:
         raise ValueError(f"eps must be >= 0, got {eps}")
-    lib = _lib.lib()
-    batch_count(ctx)
-    with on(x.device):
-        rc = lib.skv_layernorm_fwd(y.data_ptr(), ptr(mu), ptr(rs), x.data_ptr(), g.data_ptr(),
-                                   b.data_ptr(), rows, d, float(eps), _lib.dtype_code(x.dtype),
-                                   stream(x.device))
-    _lib.check(rc, "skv_layernorm_fwd")
+    launch(ctx, "skv_layernorm_fwd", y, mu, rs, x, g, b, rows, d, float(eps),
+           _lib.dtype_code(dtype))
 
 
 def cross_entropy_loss(ctx: GPUContext, logits: Operand, targets: Operand, loss: Operand,
@@ -151,21 +138,14 @@ def cross_entropy_loss(ctx: GPUContext, logits: Operand, targets: Operand, loss:
     grad_logits: the loss's gradient times grad_scale, like logits and possibly the same
     buffer, or None. row_losses: float32 [rows], 0 where ignored, or None.
     """
-    x = rows_of(ctx, logits, "logits", FLOATS)
-    rows, vocab = x.shape
-    t = operand(ctx, targets, "targets", (rows,), I32, 4)
-    out = operand(ctx, loss, "loss", (1,), F32, 4)
-    dx = None if grad_logits is None else operand(ctx, grad_logits, "grad_logits", (rows, vocab),
-                                                  (x.dtype,))
-    row = None if row_losses is None else operand(ctx, row_losses, "row_losses", (rows,), F32, 4)
-    lib = _lib.lib()
-    batch_count(ctx)
-    with on(x.device):
-        ws = workspace("skv_cross_entropy_workspace_bytes", x.device, rows)
-        rc = lib.skv_cross_entropy(out.data_ptr(), ptr(row), ptr(dx), x.data_ptr(), t.data_ptr(),
-                                   rows, vocab, float(grad_scale), ws.data_ptr(), ws.numel(),
-                                   _lib.dtype_code(x.dtype), stream(x.device))
-    _lib.check(rc, "skv_cross_entropy")
+    x, rows, vocab, dtype = rows_of(ctx, logits, "logits", FLOATS)
+    t = required(ctx, targets, "targets", (rows,), I32, 4)
+    out = required(ctx, loss, "loss", (1,), F32, 4)
+    dx = operand(ctx, grad_logits, "grad_logits", (rows, vocab), (dtype,))
+    row = operand(ctx, row_losses, "row_losses", (rows,), F32, 4)
+    ws = workspace(ctx, "skv_cross_entropy_workspace_bytes", rows)
+    launch(ctx, "skv_cross_entropy", out, row, dx, x, t, rows, vocab, float(grad_scale),
+           ws.data_ptr(), ws.numel(), _lib.dtype_code(dtype))
 
 
 __all__ = ["cross_entropy_loss", "embedding", "flash_attention", "layernorm"]

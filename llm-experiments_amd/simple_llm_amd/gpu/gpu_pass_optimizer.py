@@ -13,8 +13,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .gpu_ops import batch_count
-from .gpu_pass_common import F32, FLOATS, Operand, on, operand, ptr, stream
+from .gpu_pass_common import F32, FLOATS, Operand, launch, required, tensor_of
 from .gpu_types import GPUContext
 
 _CHUNK = 4096  # elements of a tensor that a workgroup takes at a time
@@ -58,6 +57,11 @@ class AdamWState:
         self._held = [*params, *grads, *(copies or [])]
         self._at = [t.data_ptr() for t in self._held]
 
+    def _scales(self) -> tuple:
+        if self.bits == 32:
+            return None, None
+        return self.m_scale.data_ptr(), self.v_scale.data_ptr()
+
     def __repr__(self) -> str:
         return (f"AdamWState(tensors={len(self.params)}, elements={self.m.numel()}, "
                 f"bits={self.bits})")
@@ -89,14 +93,16 @@ def adamw_create(ctx: GPUContext, params: Sequence[Operand], grads: Sequence[Ope
         raise ValueError("grads must have an entry for each of the params")
     ps, gs, cs = [], [], []
     for i in range(n):
-        p = operand(ctx, params[i], f"params[{i}]", None, F32, 4)
+        required(ctx, params[i], f"params[{i}]", None, F32, 4)
+        p = tensor_of(params[i])
         if p.numel() == 0:
             raise ValueError(f"params[{i}] holds no elements")
         ps.append(p)
-        gs.append(operand(ctx, grads[i], f"grads[{i}]", p.shape,
-                          FLOATS if i == 0 else (gs[0].dtype,), 2))
+        required(ctx, grads[i], f"grads[{i}]", p.shape, FLOATS if i == 0 else (gs[0].dtype,), 2)
+        gs.append(tensor_of(grads[i]))
         if copies is not None:
-            cs.append(operand(ctx, copies[i], f"copies[{i}]", p.shape, (torch.bfloat16,), 2))
+            required(ctx, copies[i], f"copies[{i}]", p.shape, (torch.bfloat16,), 2)
+            cs.append(tensor_of(copies[i]))
     _disjoint([(p, f"params[{i}]", True) for i, p in enumerate(ps)]
               + [(c, f"copies[{i}]", True) for i, c in enumerate(cs)]
               + [(g, f"grads[{i}]", False) for i, g in enumerate(gs)])
@@ -150,12 +156,12 @@ def _disjoint(tensors: Sequence[tuple]) -> None:
 
 
 def _number(ctx: GPUContext, x: Union[float, Operand], name: str) -> tuple:
-    """(value, None) of a number, (0, its tensor) of one in device memory."""
+    """(value, None) of a number, (0, its address) of one in device memory."""
     if isinstance(x, (int, float)):
         if not math.isfinite(x):
             raise ValueError(f"{name} must be finite, got {x}")
         return float(x), None
-    return 0.0, operand(ctx, x, name, (1,), F32, 4)
+    return 0.0, required(ctx, x, name, (1,), F32, 4)
 
 
 def adamw_update(ctx: GPUContext, state: AdamWState, lr: Union[float, Operand],
@@ -177,22 +183,20 @@ def adamw_update(ctx: GPUContext, state: AdamWState, lr: Union[float, Operand],
                          f"{weight_decay}")
     lr, lr_dev = _number(ctx, lr, "lr")
     grad_scale, scale_dev = _number(ctx, grad_scale, "grad_scale")
-    dev = state.m.device
-    if dev.index != (ctx.device.index or 0):
-        raise ValueError(f"the state lives on {dev}, the context on {ctx.device}")
+    _check_state(ctx, state)
+    launch(ctx, "skv_adamw", state._tensors.data_ptr(), state._chunks.data_ptr(),
+           state._chunks.shape[0], state.m.data_ptr(), state.v.data_ptr(), *state._scales(),
+           state._count.data_ptr(), state.bits, _lib.dtype_code(state.grads[0].dtype), lr, lr_dev,
+           float(beta1), float(beta2), float(eps), float(weight_decay), grad_scale, scale_dev,
+           state.seed)
+
+
+def _check_state(ctx: GPUContext, state: AdamWState) -> None:
+    if state.m.get_device() != (ctx.device.index or 0):
+        raise ValueError(f"the state lives on {state.m.device}, the context on {ctx.device}")
     if [t.data_ptr() for t in state._held] != state._at:
         raise ValueError("a parameter, gradient or copy is no longer where it was when the state "
                          "was made: write into their buffers, or make a new state")
-    lib = _lib.lib()
-    batch_count(ctx)
-    with on(dev):
-        rc = lib.skv_adamw(state._tensors.data_ptr(), state._chunks.data_ptr(),
-                           state._chunks.shape[0], state.m.data_ptr(), state.v.data_ptr(),
-                           ptr(state.m_scale), ptr(state.v_scale), state._count.data_ptr(),
-                           state.bits, _lib.dtype_code(state.grads[0].dtype), lr, ptr(lr_dev),
-                           float(beta1), float(beta2), float(eps), float(weight_decay), grad_scale,
-                           ptr(scale_dev), state.seed, stream(dev))
-    _lib.check(rc, "skv_adamw")
 
 
 def adamw_read(ctx: GPUContext, state: AdamWState, m: Operand, v: Operand) -> None:
@@ -201,16 +205,12 @@ def adamw_read(ctx: GPUContext, state: AdamWState, m: Operand, v: Operand) -> No
     if state.bits != 8:
         raise ValueError("adamw_read reads 8-bit moments; a 32-bit state holds them in m and v")
     n = state.m.numel()
-    mo = operand(ctx, m, "m", (n,), FLOATS)
-    vo = operand(ctx, v, "v", (n,), (mo.dtype,))
-    dev = state.m.device
-    lib = _lib.lib()
-    batch_count(ctx)
-    with on(dev):
-        rc = lib.skv_adamw_read(mo.data_ptr(), vo.data_ptr(), state.m.data_ptr(),
-                                state.v.data_ptr(), state.m_scale.data_ptr(),
-                                state.v_scale.data_ptr(), n, _lib.dtype_code(mo.dtype), stream(dev))
-    _lib.check(rc, "skv_adamw_read")
+    mo = required(ctx, m, "m", (n,), FLOATS)
+    dtype = tensor_of(m).dtype
+    vo = required(ctx, v, "v", (n,), (dtype,))
+    _check_state(ctx, state)
+    launch(ctx, "skv_adamw_read", mo, vo, state.m.data_ptr(), state.v.data_ptr(),
+           *state._scales(), n, _lib.dtype_code(dtype))
 
 
 __all__ = ["AdamWState", "adamw_create", "adamw_read", "adamw_update"]
