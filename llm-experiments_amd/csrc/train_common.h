@@ -13,139 +13,141 @@ namespace train {
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
-// N consecutive elements of a row as they are stored; the pointer is a multiple
-// of N elements' bytes.
-template <typename T, int N>
-struct Vec;
-
-template <int N>
-struct Vec<float, N> {
-  typedef float raw_t __attribute__((ext_vector_type(N == 1 ? 2 : N), aligned(N < 4 ? 8 : 16)));
-  float v[N];
-  __device__ __forceinline__ void load(const float* p) {
-    if constexpr (N == 1) {
-      v[0] = *p;
-    } else {
-      const raw_t r = *reinterpret_cast<const raw_t*>(p);
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = r[i];
-    }
-  }
-  // what is read once (nt bit): it does not push other lines out of the caches
-  __device__ __forceinline__ void stream(const float* p) {
-    if constexpr (N == 1) {
-      v[0] = __builtin_nontemporal_load(p);
-    } else {
-      const raw_t r = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(p));
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = r[i];
-    }
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.f;
-  }
-  __device__ __forceinline__ float get(int i) const { return v[i]; }
-  __device__ __forceinline__ void keep() {}
-  static __device__ __forceinline__ void store(float* p, const float (&x)[N]) {
-    if constexpr (N == 1) {
-      *p = x[0];
-    } else {
-      raw_t r;
-#pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = x[i];
-      *reinterpret_cast<raw_t*>(p) = r;
-    }
-  }
-  static __device__ __forceinline__ void store_stream(float* p, const float (&x)[N]) {
-    if constexpr (N == 1) {
-      __builtin_nontemporal_store(x[0], p);
-    } else {
-      raw_t r;
-#pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = x[i];
-      __builtin_nontemporal_store(r, reinterpret_cast<raw_t*>(p));
-    }
-  }
-};
-
 // Two values rounded to nearest even, in one instruction.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, bf16x2_t));
 }
 
-template <int N>
-struct Vec<uint16_t, N> {  // N even
-  static constexpr int NW = N / 2;
-  typedef uint32_t raw_t __attribute__((ext_vector_type(NW == 1 ? 2 : NW), aligned(NW < 4 ? 8 : 16)));
+// N consecutive elements of a row as they are stored (T float, or uint16_t for bf16),
+// N elements a power of two of words. load, stream and store take aligned vectors.
+// load_row and stream_row read elements j .. j + N of a row of d, zeros past its end, j a
+// multiple of N below d. Rows that are no multiple of N elements (kOdd): gfx950 reads and
+// writes vectors at any address, so they are read like any other; a vector that would
+// leave its row is the row's last N elements instead, and settle(), called before the
+// values are used, shifts it to its place: no load waits for another. Rows below N
+// elements (kTiny) are read one by one. stream and store_stream carry the nt bit: what is
+// read or written once does not push other lines out of the caches.
+enum RowKind { kEven, kOdd, kTiny };
+inline RowKind row_kind(int d, int N) { return d % N == 0 ? kEven : d > N ? kOdd : kTiny; }
+
+template <typename T, int N>
+struct Vec {
+  static constexpr bool kF32 = sizeof(T) == 4;
+  static constexpr int NW = N * (int)sizeof(T) / 4;  // words
+  typedef uint32_t raw_t __attribute__((ext_vector_type(NW), aligned(NW < 4 ? NW * 4 : 16)));
+  typedef uint32_t any_t __attribute__((ext_vector_type(NW), aligned(sizeof(T))));
   uint32_t w[NW];
-  __device__ __forceinline__ void load(const uint16_t* p) {
-    if constexpr (NW == 1) {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    } else {
-      const raw_t r = *reinterpret_cast<const raw_t*>(p);
-#pragma unroll
-      for (int i = 0; i < NW; ++i) w[i] = r[i];
-    }
-  }
-  __device__ __forceinline__ void stream(const uint16_t* p) {
-    if constexpr (NW == 1) {
-      w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
-    } else {
-      const raw_t r = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(p));
-#pragma unroll
-      for (int i = 0; i < NW; ++i) w[i] = r[i];
-    }
-  }
+
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < NW; ++i) w[i] = 0u;
   }
+  template <typename R>
+  __device__ __forceinline__ void set(const R& r) {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) w[i] = r[i];
+  }
+  __device__ __forceinline__ void load(const T* p) { set(*reinterpret_cast<const raw_t*>(p)); }
+  __device__ __forceinline__ void stream(const T* p) {
+    set(__builtin_nontemporal_load(reinterpret_cast<const raw_t*>(p)));
+  }
+  template <int KIND>
+  __device__ __forceinline__ void load_row(const T* row, int j, int d) {
+    if constexpr (KIND == kEven) load(row + j);
+    else if constexpr (KIND == kOdd) set(*reinterpret_cast<const any_t*>(row + min(j, d - N)));
+    else load_part(row + j, d - j);
+  }
+  template <int KIND>
+  __device__ __forceinline__ void stream_row(const T* row, int j, int d) {
+    if constexpr (KIND == kEven) stream(row + j);
+    else if constexpr (KIND == kOdd)
+      set(__builtin_nontemporal_load(reinterpret_cast<const any_t*>(row + min(j, d - N))));
+    else load_part(row + j, d - j);
+  }
+  template <int KIND>
+  __device__ __forceinline__ void settle(int j, int d) {
+    if constexpr (KIND == kOdd) {
+      if (j > d - N) shift(j - (d - N));
+    }
+  }
+  // element i becomes element i + by, zeros past the last
+  __device__ __forceinline__ void shift(int by) {
+    if constexpr (!kF32) {
+      if (by & 1) {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) w[i] = (w[i] >> 16) | (i + 1 < NW ? w[i + 1] << 16 : 0u);
+      }
+      by >>= 1;
+    }
+#pragma unroll
+    for (int s = 1; s < NW; s <<= 1) {
+      if (by & s) {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) w[i] = i + s < NW ? w[i + s] : 0u;
+      }
+    }
+  }
+  __device__ __forceinline__ void load_part(const T* p, int left) {
+    T x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = i < left ? p[i] : T(0);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      if constexpr (kF32) w[i] = __float_as_uint(x[i]);
+      else w[i] = (uint32_t)x[2 * i] | ((uint32_t)x[2 * i + 1] << 16);
+    }
+  }
   __device__ __forceinline__ float get(int i) const {
-    return (i & 1) ? bf16w_hi(w[i >> 1]) : bf16w_lo(w[i >> 1]);
+    if constexpr (kF32) return __uint_as_float(w[i]);
+    else return (i & 1) ? bf16w_hi(w[i >> 1]) : bf16w_lo(w[i >> 1]);
   }
   // What get() returned before is not kept in registers for later calls: the packed
-  // words are half as many.
+  // words of bf16 are half as many.
   __device__ __forceinline__ void keep() {
+    if constexpr (!kF32) {
 #pragma unroll
-    for (int i = 0; i < NW; ++i) asm volatile("" : "+v"(w[i]));
-  }
-  static __device__ __forceinline__ void store(uint16_t* p, const float (&x)[N]) {
-    if constexpr (NW == 1) {
-      *reinterpret_cast<uint32_t*>(p) = pack_bf16(x[0], x[1]);
-    } else {
-      raw_t r;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) r[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-      *reinterpret_cast<raw_t*>(p) = r;
+      for (int i = 0; i < NW; ++i) asm volatile("" : "+v"(w[i]));
     }
   }
-  static __device__ __forceinline__ void store_stream(uint16_t* p, const float (&x)[N]) {
-    if constexpr (NW == 1) {
-      __builtin_nontemporal_store(pack_bf16(x[0], x[1]), reinterpret_cast<uint32_t*>(p));
-    } else {
-      raw_t r;
+  template <typename R>
+  static __device__ __forceinline__ R words(const float (&x)[N]) {
+    R r;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) r[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-      __builtin_nontemporal_store(r, reinterpret_cast<raw_t*>(p));
+    for (int i = 0; i < NW; ++i) {
+      if constexpr (kF32) r[i] = __float_as_uint(x[i]);
+      else r[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
     }
+    return r;
   }
-};
-
-template <>
-struct Vec<uint16_t, 1> {
-  uint16_t h;
-  __device__ __forceinline__ void load(const uint16_t* p) { h = *p; }
-  __device__ __forceinline__ void stream(const uint16_t* p) { h = __builtin_nontemporal_load(p); }
-  __device__ __forceinline__ void zero() { h = 0; }
-  __device__ __forceinline__ float get(int) const { return bf16_to_f32(h); }
-  __device__ __forceinline__ void keep() {}
-  static __device__ __forceinline__ void store(uint16_t* p, const float (&x)[1]) {
-    *p = f32_to_bf16(x[0]);
+  static __device__ __forceinline__ void store(T* p, const float (&x)[N]) {
+    *reinterpret_cast<raw_t*>(p) = words<raw_t>(x);
   }
-  static __device__ __forceinline__ void store_stream(uint16_t* p, const float (&x)[1]) {
-    __builtin_nontemporal_store(f32_to_bf16(x[0]), p);
+  static __device__ __forceinline__ void store_stream(T* p, const float (&x)[N]) {
+    __builtin_nontemporal_store(words<raw_t>(x), reinterpret_cast<raw_t*>(p));
+  }
+  template <int KIND>
+  static __device__ __forceinline__ void store_row(T* row, int j, int d, const float (&x)[N]) {
+    if constexpr (KIND == kEven) store(row + j, x);
+    else if (j + N <= d) *reinterpret_cast<any_t*>(row + j) = words<any_t>(x);
+    else store_part(row + j, x, d - j);
+  }
+  template <int KIND>
+  static __device__ __forceinline__ void store_stream_row(T* row, int j, int d,
+                                                          const float (&x)[N]) {
+    if constexpr (KIND == kEven) store_stream(row + j, x);
+    else if (j + N <= d)
+      __builtin_nontemporal_store(words<any_t>(x), reinterpret_cast<any_t*>(row + j));
+    else store_part(row + j, x, d - j);
+  }
+  static __device__ __forceinline__ void store_part(T* p, const float (&x)[N], int left) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i < left) {
+        if constexpr (kF32) p[i] = x[i];
+        else p[i] = f32_to_bf16(x[i]);
+      }
+    }
   }
 };
 

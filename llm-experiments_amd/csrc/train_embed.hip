@@ -20,9 +20,10 @@
 //         range's border leaves its part.
 //   join  adds the parts of each such row, in order.
 //
-// 16384 zipf tokens, table 50304 x 768 fp32 (154 MB written, 50 read): sort 24 us (7
-// without the zeros), sum 22 (17 where HBM is not still writing zeros), join 5; 47 us in
-// all. One bucket per CU and not two: 52.5 against 57 us. Zeros with the nt bit: 51 -> 47.
+// 16384 zipf tokens, table 50304 x 768 fp32 (154 MB written, 50 read): sort 29 us, most of
+// it the zeros (6.5 without them), sum 14, join 5; 46 us in all. One bucket per CU and not
+// two: 52.5 against 57 us. Zeros with the nt bit: 51 -> 47. The sort of 65536 tokens: 14
+// to 19 us, 28 to 36 with every run read twice and its batches' places found unasked.
 #include "train_common.h"
 
 namespace skv {
@@ -32,7 +33,8 @@ using namespace train;
 
 constexpr int kBucket = 256;  // ids of a bucket, at most
 constexpr int kWaves = 16;    // wavefronts of a sorting workgroup
-constexpr int kBatches = 16;  // batches of 64 tokens a sorting wavefront reads at a time
+constexpr int kBatches = 8;   // batches of 64 tokens a sorting wavefront reads at a time
+constexpr int kList = 1280;   // the tokens that it can list
 constexpr int kRange = 16;    // sorted tokens of a summing wavefront
 constexpr int kJoinWaves = 8;
 constexpr int kZeroGroups = 128;  // workgroups that zero the table
@@ -42,7 +44,7 @@ constexpr int kZeroGroups = 128;  // workgroups that zero the table
 // ---------------------------------------------------------------------------
 
 // A workgroup's four wavefronts have a token each; VEC columns a lane and step.
-template <typename TT, typename TO, int VEC>
+template <typename TT, typename TO, int VEC, int KIND>
 __global__ __launch_bounds__(256) void k_embed_rows(TO* __restrict__ out,
                                                     const int32_t* __restrict__ ids,
                                                     const TT* __restrict__ table,
@@ -61,12 +63,14 @@ __global__ __launch_bounds__(256) void k_embed_rows(TO* __restrict__ out,
     Vec<float, VEC> p;
     t.zero();
     p.zero();
-    if (real) t.load(row + j);
-    if (pr) p.load(pr + j);
+    if (real) t.template load_row<KIND>(row, j, d);
+    if (pr) p.template load_row<KIND>(pr, j, d);
+    t.template settle<KIND>(j, d);
+    p.template settle<KIND>(j, d);
     float r[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) r[e] = t.get(e) * scale + p.get(e);
-    Vec<TO, VEC>::store_stream(o + j, r);
+    Vec<TO, VEC>::template store_stream_row<KIND>(o, j, d, r);
   }
 }
 
@@ -82,17 +86,23 @@ struct Sorted {
                    // number of ranges it lies in; or (-1, 0)
 };
 
+// what the wavefront's other lanes wrote to LDS is read behind this
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ int wave_isum(int x) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
   return x;
 }
 
-// width: ids of a bucket. Each wavefront has a run of consecutive tokens in both
-// scans; an id's tokens are placed by wavefront, then by token. Tokens are read 16 x 64
-// at a time and the bucket's own go to a list in LDS, in order: it is short but for a
-// bucket of frequent ids (of 16384 zipf tokens a bucket of 99 ids has 32 on average and
-// 1000 at most, 60 a wavefront), and what finds an id's rank among 64 tokens costs 0.3 us.
+// width: ids of a bucket. Each wavefront has a run of consecutive tokens; an id's tokens
+// are placed by wavefront, then by token. The bucket's own tokens go to a list in LDS, in
+// order: it is short but for a bucket of frequent ids (of 16384 zipf tokens a bucket of 99
+// ids has 32 on average and 1000 at most, 60 a wavefront), and what finds an id's rank
+// among 64 tokens costs 0.3 us. Where the list does not hold them, the run is read again.
 __global__ __launch_bounds__(kWaves * 64, 8) void k_embed_sort(Sorted s,
                                                                const int32_t* __restrict__ ids,
                                                                int T, int V, int width, int buckets,
@@ -111,46 +121,67 @@ __global__ __launch_bounds__(kWaves * 64, 8) void k_embed_sort(Sorted s,
   __shared__ int tot[kBucket];   // tokens of an id
   __shared__ int base[kBucket];  // where they begin in the bucket
   __shared__ int less[kWaves];
-  __shared__ uint16_t list_t[kWaves][kRead];  // the bucket's tokens of those read last
-  __shared__ uint8_t list_l[kWaves][kRead];   // and their ids' places in the bucket
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __shared__ uint16_t list_t[kWaves][kList];  // the bucket's tokens in the run
+  __shared__ uint8_t list_l[kWaves][kList];   // and their ids' places in the bucket
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int lo = blockIdx.x * width, n_ids = min(width, V - lo);
   const int per = ((T + kWaves * 64 - 1) / (kWaves * 64)) * 64;
   const int t0 = min(w * per, T), t1 = min(t0 + per, T);
-  int below = 0;
-  // tokens t .. t + kRead of the wavefront to its list; their number
-  const auto read = [&](int t) {
-    int id[kBatches], n = 0;
+  int upto = 0, n = 0;  // tokens of ids below lo + n_ids; tokens in the list
+  const auto load = [&](int (&id)[kBatches], int t) {
+    if (t + kRead <= t1) {
 #pragma unroll
-    for (int i = 0; i < kBatches; ++i) {
-      const int k = t + i * 64 + lane;
-      id[i] = k < t1 ? ids[k] : -1;
-    }
+      for (int i = 0; i < kBatches; ++i) id[i] = (ids + t)[lane + i * 64];
+    } else {
 #pragma unroll
-    for (int i = 0; i < kBatches; ++i) {
-      const int l = id[i] - lo;
-      const bool in = id[i] >= 0 && (unsigned)l < (unsigned)n_ids;
-      below += id[i] >= 0 && l < 0;
-      const uint64_t mask = __ballot(in);
-      if (in) {
-        const int at = n + __popcll(mask & ((1ull << lane) - 1));
-        list_t[w][at] = (uint16_t)(i * 64 + lane);
-        list_l[w][at] = (uint8_t)l;
+      for (int i = 0; i < kBatches; ++i) {
+        const int k = t + i * 64 + lane, x = ids[min(k, t1 - 1)];
+        id[i] = k < t1 ? x : -1;
       }
-      n += __popcll(mask);
     }
-    __builtin_amdgcn_wave_barrier();
-    return n;
+  };
+  // the bucket's tokens of those read to the list; `at` is the place of the first of them
+  const auto enlist = [&](const int (&id)[kBatches], int at) {
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i) {
+      const unsigned l = (unsigned)id[i] - lo;
+      const bool in = l < (unsigned)n_ids;
+      upto += __popcll(__ballot((unsigned)id[i] < (unsigned)(lo + n_ids)));
+      const uint64_t mask = __ballot(in);
+      if (mask) {  // most batches have none
+        if (in) {
+          const int to = n + __popcll(mask & ((1ull << lane) - 1));
+          list_t[w][to] = (uint16_t)(at + i * 64 + lane);
+          list_l[w][to] = (uint8_t)l;
+        }
+        n += __popcll(mask);
+      }
+    }
+  };
+  const auto count = [&]() {
+    wave_sync();
+    for (int i = lane; i < n; i += 64) atomicAdd(&cnt[w][list_l[w][i]], 1);
   };
   for (int j = lane; j < kBucket; j += 64) cnt[w][j] = 0;  // the wavefront's own
-  __builtin_amdgcn_wave_barrier();
-  int n = 0;
-  for (int t = t0; t < t1; t += kRead) {
-    n = read(t);
-    for (int i = lane; i < n; i += 64) atomicAdd(&cnt[w][list_l[w][i]], 1);
+  bool listed = per <= 1 << 16;
+  if (t0 < t1) {
+    int id[kBatches], next[kBatches];
+    load(next, t0);
+    for (int t = t0; t < t1; t += kRead) {
+#pragma unroll
+      for (int i = 0; i < kBatches; ++i) id[i] = next[i];
+      if (t + kRead < t1) load(next, t + kRead);
+      if (n > kList - kRead) {
+        count();
+        wave_sync();
+        listed = false;
+        n = 0;
+      }
+      enlist(id, t - t0);
+    }
+    count();
   }
-  below = wave_isum(below);
-  if (lane == 0) less[w] = below;
+  if (lane == 0) less[w] = upto;
   __syncthreads();
   if (threadIdx.x < kBucket) {
     int sum = 0;
@@ -164,7 +195,6 @@ __global__ __launch_bounds__(kWaves * 64, 8) void k_embed_sort(Sorted s,
   }
   __syncthreads();
   if (w == 0) {  // exclusive sums over the bucket's ids, four a lane
-    const int first = wave_isum(lane < kWaves ? less[lane] : 0);
     int c[4], sum = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -177,6 +207,8 @@ __global__ __launch_bounds__(kWaves * 64, 8) void k_embed_sort(Sorted s,
       const int up = __shfl_up(incl, o);
       if (lane >= o) incl += up;
     }
+    // where the bucket begins: the tokens of ids up to its last, without its own
+    const int first = wave_isum(lane < kWaves ? less[lane] : 0) - __shfl(incl, 63);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int b = first + incl - sum + c[i];
@@ -186,8 +218,8 @@ __global__ __launch_bounds__(kWaves * 64, 8) void k_embed_sort(Sorted s,
     if ((int)blockIdx.x == buckets - 1 && lane == 63) s.begin[V] = first + incl;
   }
   __syncthreads();
-  for (int t = t0; t < t1; t += kRead) {
-    if (per > kRead) n = read(t);  // else the list of the first scan is still there
+  const auto place = [&](int t) {  // t: the token that the list counts from
+    wave_sync();
     for (int i = 0; i < n; i += 64) {
       const bool in = i + lane < n;
       const int l = in ? list_l[w][i + lane] : 0;
@@ -202,21 +234,33 @@ __global__ __launch_bounds__(kWaves * 64, 8) void k_embed_sort(Sorted s,
         s.pos[to] = t + list_t[w][i + lane];
         s.id[to] = lo + l;
       }
-      __builtin_amdgcn_wave_barrier();
+      wave_sync();
       if (in && (same >> lane) == 1) cnt[w][l] += __popcll(same);  // the last of them
-      __builtin_amdgcn_wave_barrier();
+      wave_sync();
+    }
+  };
+  if (listed) {
+    place(t0);
+  } else {
+    for (int t = t0; t < t1; t += kRead) {
+      int id[kBatches];
+      load(id, t);
+      n = 0;
+      enlist(id, 0);
+      place(t);
     }
   }
 }
 
 // part: [ranges][2][dp]: of a row that began in an earlier range, and of one that
 // goes on in the next.
-template <typename TY, int VEC, bool ACC>
+template <typename TY, int KIND, bool ACC>
 __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
                                                    float* __restrict__ part,
                                                    const TY* __restrict__ dy, Sorted s, int T, int V,
                                                    int d, int dp, float scale, int tiles,
                                                    int ranges) {
+  constexpr int VEC = 4;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int unit = blockIdx.x * 4 + w;
   const int r = unit / tiles, tile = unit - r * tiles, c = tile * 64 * VEC + lane * VEC;
@@ -264,15 +308,17 @@ __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
       v[u].zero();
       was[u].zero();
       if (here && k + u < cnt) {
-        v[u].load(dy + (size_t)p * d + c);
+        v[u].template load_row<KIND>(dy + (size_t)p * d, c, d);
         if (ACC && ((ends >> i) & 1))
-          was[u].load(grad + (size_t)__builtin_amdgcn_readlane(my_id, i) * d + c);
+          was[u].template load_row<KIND>(grad + (size_t)__builtin_amdgcn_readlane(my_id, i) * d, c,
+                                        d);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = k + u;
       if (i < cnt) {
+        v[u].template settle<KIND>(c, d);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] += v[u].get(e);
         if ((ends >> i) & 1) {
@@ -282,10 +328,11 @@ __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
               Vec<float, VEC>::store(part + ((size_t)r * 2 + !head) * dp + c, acc);
             } else {
               float o[VEC];
+              was[u].template settle<KIND>(c, d);
 #pragma unroll
               for (int e = 0; e < VEC; ++e) o[e] = was[u].get(e) + acc[e] * scale;
-              Vec<float, VEC>::store(
-                  grad + (size_t)__builtin_amdgcn_readlane(my_id, i) * d + c, o);
+              Vec<float, VEC>::template store_row<KIND>(
+                  grad + (size_t)__builtin_amdgcn_readlane(my_id, i) * d, c, d, o);
             }
           }
 #pragma unroll
@@ -297,27 +344,28 @@ __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
 }
 
 // grad's row `id`, columns from c on, is (what was there +) scale * sum
-template <int VEC, bool ACC>
+template <int VEC, int KIND, bool ACC>
 __device__ __forceinline__ void put_row(float* __restrict__ grad, int id, int c, int d, float scale,
-                                        const Vec<float, VEC>& was, const float (&sum)[VEC]) {
+                                        Vec<float, VEC> was, const float (&sum)[VEC]) {
+  was.template settle<KIND>(c, d);
   float o[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) o[e] = ACC ? was.get(e) + sum[e] * scale : sum[e] * scale;
-  Vec<float, VEC>::store(grad + (size_t)id * d + c, o);
+  Vec<float, VEC>::template store_row<KIND>(grad + (size_t)id * d, c, d, o);
 }
 
 // A workgroup has kJoinWaves ranges and a column tile: a wavefront the row that begins
 // in its range and goes on, where that is a row of few ranges (most are: about every
 // other range ends inside a row); then, together, those of many, each wavefront a run
 // of consecutive ranges and the wavefronts' sums in order.
-template <int VEC, bool ACC>
+template <int KIND, bool ACC>
 __global__ __launch_bounds__(kJoinWaves * 64) void k_embed_join(float* __restrict__ grad,
                                                                 const float* __restrict__ part,
                                                                 const int2* __restrict__ goes_on,
                                                                 int ranges, int d, int dp,
                                                                 float scale) {
-  __shared__ float sh[kJoinWaves][64 * VEC];
-  constexpr int kFew = 8;
+  constexpr int VEC = 4, kFew = 8;
+  __shared__ __align__(16) float sh[kJoinWaves][64 * VEC];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r0 = blockIdx.x * kJoinWaves;
   const int c = blockIdx.y * 64 * VEC + lane * VEC;
   int2 mine = make_int2(-1, 0);
@@ -331,7 +379,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_embed_join(float* __restric
     if (id >= 0 && n <= kFew && c < d) {
       const float* p = part + (size_t)(r0 + w) * 2 * dp + c;
       Vec<float, VEC> v[kFew];
-      if (ACC) was.load(grad + (size_t)id * d + c);
+      if (ACC) was.template load_row<KIND>(grad + (size_t)id * d, c, d);
 #pragma unroll
       for (int j = 0; j < kFew; ++j) {
         v[j].zero();
@@ -343,7 +391,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_embed_join(float* __restric
 #pragma unroll
         for (int j = 0; j < kFew; ++j) acc[e] += v[j].get(e);
       }
-      put_row<VEC, ACC>(grad, id, c, d, scale, was, acc);
+      put_row<VEC, KIND, ACC>(grad, id, c, d, scale, was, acc);
     }
   }
   while (rows) {
@@ -351,7 +399,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_embed_join(float* __restric
     rows &= rows - 1;
     const int id = __builtin_amdgcn_readlane(mine.x, i), n = __builtin_amdgcn_readlane(mine.y, i);
     const int per = (n + kJoinWaves - 1) / kJoinWaves;
-    if (ACC && w == 0 && c < d) was.load(grad + (size_t)id * d + c);
+    if (ACC && w == 0 && c < d) was.template load_row<KIND>(grad + (size_t)id * d, c, d);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
     if (c < d) {
@@ -373,7 +421,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_embed_join(float* __restric
 #pragma unroll
         for (int q = 0; q < kJoinWaves; ++q) acc[e] += sh[q][lane * VEC + e];
       }
-      put_row<VEC, ACC>(grad, id, c, d, scale, was, acc);
+      put_row<VEC, KIND, ACC>(grad, id, c, d, scale, was, acc);
     }
   }
 }
@@ -406,19 +454,19 @@ extern "C" int skv_embedding_fwd(void* out, const int32_t* ids, const void* tabl
                       {ids, (size_t)T * 4, "tokens"},
                       {pos_table, (size_t)n_pos * d * 4, "pos_table"}}))
     return rc;
-  const dim3 grid((T + 3) / 4);
+  const dim3 grid(((unsigned)T + 3) / 4);
   const auto run = [&](auto* o, auto* t) {
     using TO = std::remove_pointer_t<decltype(o)>;
     using TT = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-    const auto rows = [&](auto VEC) {
-      k_embed_rows<TT, TO, VEC.value><<<grid, 256, 0, (hipStream_t)stream>>>(
+    constexpr int VEC = sizeof(TT) == 2 && sizeof(TO) == 2 ? 8 : 4;
+    const auto rows = [&](auto KIND) {
+      k_embed_rows<TT, TO, VEC, KIND.value><<<grid, 256, 0, (hipStream_t)stream>>>(
           o, ids, t, pos_table, T, V, d, n_pos, scale);
     };
-    if (table_dt == SKV_BF16 && out_dt == SKV_BF16 && d % 8 == 0)
-      rows(std::integral_constant<int, 8>{});
-    else if (d % 4 == 0) rows(std::integral_constant<int, 4>{});
-    else if (d % 2 == 0) rows(std::integral_constant<int, 2>{});
-    else rows(std::integral_constant<int, 1>{});
+    const RowKind kind = row_kind(d, VEC);
+    if (kind == kEven) rows(std::integral_constant<int, kEven>{});
+    else if (kind == kOdd) rows(std::integral_constant<int, kOdd>{});
+    else rows(std::integral_constant<int, kTiny>{});
   };
   if (table_dt == SKV_BF16) {
     if (out_dt == SKV_BF16) run((uint16_t*)out, (const uint16_t*)table);
@@ -461,35 +509,31 @@ extern "C" int skv_embedding_bwd(float* grad, const void* dout, const int32_t* i
   s.id = s.pos + T;
   s.begin = s.id + T;
   float* part = (float*)((int32_t*)ws + ints_of(T, V));
-  // about two buckets to a CU
-  int width = (V + 255) / 256;
-  width = width < 16 ? 16 : width > kBucket ? kBucket : width;
+  const int width = min((V + 255) / 256, kBucket);  // one bucket to a CU
   const int buckets = (V + width - 1) / width;
   const size_t n_zero = accumulate ? 0 : (size_t)V * d;
   const int sort_grid = buckets + (n_zero ? kZeroGroups : 0);
   k_embed_sort<<<sort_grid, kWaves * 64, 0, st>>>(s, ids, T, V, width, buckets, grad, n_zero);
   if (int rc = check_launch("skv_embedding_bwd")) return rc;
-  const auto run = [&](auto* y, auto VEC) {
+  const int tiles = (d + 255) / 256;
+  const unsigned grid = (unsigned)(((size_t)ranges * tiles + 3) / 4);
+  const dim3 join((ranges + kJoinWaves - 1) / kJoinWaves, tiles);
+  const auto run = [&](auto* y, auto KIND, auto ACC) {
     using TY = std::remove_const_t<std::remove_pointer_t<decltype(y)>>;
-    const int tiles = (d + 64 * VEC.value - 1) / (64 * VEC.value);
-    const unsigned grid = (unsigned)(((size_t)ranges * tiles + 3) / 4);
-    const dim3 join((ranges + kJoinWaves - 1) / kJoinWaves, tiles);
-    if (accumulate) {
-      k_embed_sum<TY, VEC.value, true><<<grid, 256, 0, st>>>(grad, part, y, s, T, V, d, dp, scale,
-                                                             tiles, ranges);
-      k_embed_join<VEC.value, true><<<join, kJoinWaves * 64, 0, st>>>(grad, part, s.goes_on, ranges,
-                                                                      d, dp, scale);
-    } else {
-      k_embed_sum<TY, VEC.value, false><<<grid, 256, 0, st>>>(grad, part, y, s, T, V, d, dp, scale,
-                                                              tiles, ranges);
-      k_embed_join<VEC.value, false><<<join, kJoinWaves * 64, 0, st>>>(grad, part, s.goes_on, ranges,
-                                                                       d, dp, scale);
-    }
+    k_embed_sum<TY, KIND.value, ACC.value><<<grid, 256, 0, st>>>(grad, part, y, s, T, V, d, dp, scale,
+                                                                tiles, ranges);
+    k_embed_join<KIND.value, ACC.value><<<join, kJoinWaves * 64, 0, st>>>(grad, part, s.goes_on,
+                                                                         ranges, d, dp, scale);
   };
   const auto with = [&](auto* y) {
-    if (d % 4 == 0) run(y, std::integral_constant<int, 4>{});
-    else if (d % 2 == 0) run(y, std::integral_constant<int, 2>{});
-    else run(y, std::integral_constant<int, 1>{});
+    const auto kind = [&](auto KIND) {
+      if (accumulate) run(y, KIND, std::true_type{});
+      else run(y, KIND, std::false_type{});
+    };
+    const RowKind k = row_kind(d, 4);
+    if (k == kEven) kind(std::integral_constant<int, kEven>{});
+    else if (k == kOdd) kind(std::integral_constant<int, kOdd>{});
+    else kind(std::integral_constant<int, kTiny>{});
   };
   if (dt == SKV_BF16) with((const uint16_t*)dout);
   else with((const float*)dout);

@@ -6,12 +6,14 @@
 //        g = dy gamma, xh = (x - mean) rstd
 //   dgamma = sum over rows of dy xh, dbeta = sum over rows of dy
 //
-// Both directions are bound by HBM: a row is read once into registers, its sums
-// go over the row's wavefronts, and the result is written. A row is on one
-// wavefront up to 1024 columns (no LDS, no barrier), on 4 up to 4096 and on 16 up
-// to 16384. 16384 x 1024 bf16 forward: 11.6 us = 5.8 TB/s (its output with the nt bit;
-// 13.0 without). 16384 x 768 fp32 backward with a residual: 37.9 us = 5.3 TB/s (rows
-// read with the nt bit; 43.5 without), 4 of them for the weight gradients' second pass.
+// Both directions are bound by HBM: a row is read once into registers, its sums go over
+// the row's lanes, and the result is written. A row is on 16 lanes up to 256 columns, on
+// one wavefront up to 1024 (no LDS, no barrier), on 4 up to 4096 and on 16 up to 16384.
+// 16384 x 1024 bf16 forward: 11.6 us = 5.8 TB/s (its output with the nt bit; 13.0
+// without). 16384 x 768 fp32 backward with a residual: 36.3 us = 5.5 TB/s (rows read with
+// the nt bit; 43.5 without), 4 of them for the weight gradients' second pass. Rows that
+// end inside a vector, 8192 x 1001: 8.7 us forward bf16 and 23.4 backward fp32, where
+// 1024 columns take 7.3 and 22.2.
 #include "train_common.h"
 
 namespace skv {
@@ -22,14 +24,30 @@ using namespace train;
 constexpr int kMaxD = 16384;
 constexpr int kLaneCols = 16;  // columns of a row a lane holds
 
-// Sums of a row over its WPR wavefronts: sh [2][WPR][2] (two calls in a row do
-// not share a slot, so one barrier a call is enough).
-template <int WPR>
+constexpr int bwd_threads(int WPR) { return WPR == 16 ? 1024 : 512; }
+
+// A row's place in a workgroup of THREADS lanes: LPR lanes of a wavefront (16 or 64)
+// with WPR = 1, or WPR whole wavefronts.
+template <int LPR, int WPR, int THREADS>
+struct Place {
+  static constexpr int kLanes = LPR * WPR;
+  static constexpr int kRows = THREADS / kLanes;  // rows at a time
+  static __device__ __forceinline__ int row() { return threadIdx.x / kLanes; }
+  static __device__ __forceinline__ int lane() { return threadIdx.x % kLanes; }
+};
+
+// Sums over a row's lanes: sh [2][wavefronts][2] (two calls in a row do not share a
+// slot, so one barrier a call is enough).
+template <int LPR, int WPR, int THREADS>
 __device__ __forceinline__ void row_sums(float& a, float& b, float* sh, int& turn) {
-  a = wave_sum(a);
-  b = wave_sum(b);
+  a = row16_sum(a);
+  b = row16_sum(b);
+  if constexpr (LPR == 64) {
+    a = xor32_sum(xor16_sum(a));
+    b = xor32_sum(xor16_sum(b));
+  }
   if constexpr (WPR > 1) {
-    float* s = sh + turn * 2 * WPR;
+    float* s = sh + turn * 2 * (THREADS / 64);
     turn ^= 1;
     const int w = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) {
@@ -37,6 +55,7 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float* sh, int& tur
       s[2 * w + 1] = b;
     }
     __syncthreads();
+    s += w / WPR * WPR * 2;
     a = b = 0.f;
 #pragma unroll
     for (int i = 0; i < WPR; ++i) {
@@ -46,31 +65,34 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float* sh, int& tur
   }
 }
 
-template <typename T, int VEC, int NCH, int WPR>
+template <typename T, int NCH, int LPR, int WPR, int KIND>
 __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_fwd(
     T* y, float* __restrict__ mean_out, float* __restrict__ rstd_out, const T* x,
     const float* __restrict__ gamma, const float* __restrict__ beta, int M, int d, float eps) {
+  constexpr int kThreads = WPR == 16 ? 1024 : 256, VEC = 16 / sizeof(T);
+  using P = Place<LPR, WPR, kThreads>;
   __shared__ float sh[4 * WPR];
-  constexpr int kRows = WPR == 1 ? 4 : 1;  // rows of a workgroup
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int m = blockIdx.x * kRows + (WPR == 1 ? w : 0);
-  if (m >= M) return;  // WPR = 1: no barrier below
-  const int c0 = ((WPR == 1 ? 0 : w) * 64 + lane) * VEC;
-  constexpr int kStep = WPR * 64 * VEC;
+  const int m = blockIdx.x * P::kRows + P::row();
+  if (m >= M) return;  // only where there are several rows, and then no barrier below
+  const int c0 = P::lane() * VEC;
+  constexpr int kStep = P::kLanes * VEC;
   const T* xr = x + (size_t)m * d;
   Vec<T, VEC> v[NCH];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     v[i].zero();
-    if (c0 + i * kStep < d) v[i].load(xr + c0 + i * kStep);
+    const int j = c0 + i * kStep;
+    if (j < d) v[i].template load_row<KIND>(xr, j, d);
   }
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) v[i].template settle<KIND>(c0 + i * kStep, d);
   float s = 0.f, q = 0.f;
 #pragma unroll
   for (int i = 0; i < NCH; ++i)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) s += v[i].get(e);
   int turn = 0;
-  row_sums<WPR>(s, q, sh, turn);
+  row_sums<LPR, WPR, kThreads>(s, q, sh, turn);
   const float fd = (float)d;
   const float mean = s / fd;
   // deviations from the rounded mean, and their own mean c: what the rounding
@@ -82,15 +104,17 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_fwd(
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float t = v[i].get(e) - mean;
-        s += t;
-        q += t * t;
+        if (KIND == kEven || c0 + i * kStep + e < d) {
+          s += t;
+          q += t * t;
+        }
       }
     }
   }
-  row_sums<WPR>(s, q, sh, turn);
+  row_sums<LPR, WPR, kThreads>(s, q, sh, turn);
   const float c = s / fd;
   const float rstd = 1.f / sqrtf(fmaxf(q / fd - c * c, 0.f) + eps);
-  if (lane == 0 && (WPR == 1 || w == 0)) {
+  if (P::lane() == 0) {
     if (mean_out) mean_out[m] = mean + c;
     if (rstd_out) rstd_out[m] = rstd;
   }
@@ -100,38 +124,42 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_fwd(
     const int j = c0 + i * kStep;
     if (j < d) {
       Vec<float, VEC> g, b;
-      g.load(gamma + j);
-      b.load(beta + j);
+      g.template load_row<KIND>(gamma, j, d);
+      b.template load_row<KIND>(beta, j, d);
+      g.template settle<KIND>(j, d);
+      b.template settle<KIND>(j, d);
       float o[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
         o[e] = ((v[i].get(e) - mean) - c) * rstd * g.get(e) + b.get(e);
-      Vec<T, VEC>::store_stream(yr + j, o);
+      Vec<T, VEC>::template store_stream_row<KIND>(yr, j, d, o);
     }
   }
 }
 
-// Rows m0, m0 + stride, ... of a workgroup (of each of its wavefronts where a
-// row is one wavefront's); a lane holds the same columns of every row, so the
-// sums of dgamma and dbeta stay in its registers until the end. part: the
-// workgroup's sums, [grid][2][dp].
-template <typename T, int VEC, int NCH, int WPR, bool RES>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_bwd(
+// A workgroup's rows, kRows at a time: a lane holds the same columns of every row, so
+// the sums of dgamma and dbeta stay in its registers until the end, and then go over
+// the row places in LDS, in their order. part: the workgroup's sums, [grid][2][dp].
+// (Reading the next row while one is worked on gained nothing: 8 wavefronts a CU hide it.)
+template <typename T, int NCH, int LPR, int WPR, int KIND, bool RES>
+__global__ __launch_bounds__(bwd_threads(WPR)) void k_ln_bwd(
     T* dx, float* __restrict__ part, const T* dy, const T* x, const float* __restrict__ gamma,
     const float* __restrict__ mean, const float* __restrict__ rstd, const T* residual, int M, int d,
     int dp) {
-  __shared__ float sh[4 * WPR];
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  constexpr int kRows = WPR == 1 ? 4 : 1;
-  const int c0 = ((WPR == 1 ? 0 : w) * 64 + lane) * VEC;
-  constexpr int kStep = WPR * 64 * VEC;
+  constexpr int kThreads = bwd_threads(WPR), VEC = 16 / sizeof(T);
+  using P = Place<LPR, WPR, kThreads>;
+  __shared__ float sh[4 * (kThreads / 64)];
+  const int c0 = P::lane() * VEC;
+  constexpr int kStep = P::kLanes * VEC;
   const float inv_d = 1.f / (float)d;
   float ga[NCH][VEC], sg[NCH][VEC], sb[NCH][VEC];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     Vec<float, VEC> g;
     g.zero();
-    if (c0 + i * kStep < d) g.load(gamma + c0 + i * kStep);
+    const int j = c0 + i * kStep;
+    if (j < d) g.template load_row<KIND>(gamma, j, d);
+    g.template settle<KIND>(j, d);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       ga[i][e] = g.get(e);
@@ -139,25 +167,28 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_bwd(
     }
   }
   int turn = 0;
-  for (int m = blockIdx.x * kRows + (WPR == 1 ? w : 0); m < M; m += gridDim.x * kRows) {
-    const T* xr = x + (size_t)m * d;
-    const T* yr = dy + (size_t)m * d;
+  for (int m0 = blockIdx.x * P::kRows; m0 < M; m0 += gridDim.x * P::kRows) {
+    const int m = m0 + P::row();
+    const bool here = m < M;  // a place without a row: zeros, and nothing is stored
+    const size_t at = (size_t)m * d;
     Vec<T, VEC> vx[NCH], vy[NCH], vr[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       vx[i].zero();
       vy[i].zero();
       const int j = c0 + i * kStep;
-      if (j < d) {
-        vx[i].stream(xr + j);
-        vy[i].stream(yr + j);
-        if constexpr (RES) vr[i].stream(residual + (size_t)m * d + j);
+      if (here && j < d) {
+        vx[i].template stream_row<KIND>(x + at, j, d);
+        vy[i].template stream_row<KIND>(dy + at, j, d);
+        if constexpr (RES) vr[i].template stream_row<KIND>(residual + at, j, d);
       }
     }
-    const float mu = mean[m], rs = rstd[m];
+    const float mu = here ? mean[m] : 0.f, rs = here ? rstd[m] : 0.f;
     float a = 0.f, b = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
+      vx[i].template settle<KIND>(c0 + i * kStep, d);
+      vy[i].template settle<KIND>(c0 + i * kStep, d);
       if (c0 + i * kStep < d) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -170,14 +201,14 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_bwd(
         }
       }
     }
-    row_sums<WPR>(a, b, sh, turn);
+    row_sums<LPR, WPR, kThreads>(a, b, sh, turn);
     a *= inv_d;
     b *= inv_d;
-    T* o = dx + (size_t)m * d;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int j = c0 + i * kStep;
-      if (j < d) {
+      if (here && j < d) {
+        if constexpr (RES) vr[i].template settle<KIND>(j, d);
         float r[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -185,37 +216,51 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_bwd(
           r[e] = rs * (vy[i].get(e) * ga[i][e] - a - xh * b);
           if constexpr (RES) r[e] += vr[i].get(e);
         }
-        Vec<T, VEC>::store(o + j, r);
+        Vec<T, VEC>::template store_row<KIND>(dx + at, j, d, r);
       }
     }
   }
   float* out = part + (size_t)blockIdx.x * 2 * dp;
-  if constexpr (WPR == 1) {  // the four wavefronts' sums, in their order
-    __shared__ float acc[2][64 * VEC * NCH];
-    for (int t = 0; t < 4; ++t) {
-      if (w == t) {
+  constexpr int kSlots = kThreads / 64 / WPR;  // sums that come together
+  if constexpr (kSlots > 1) {
+    __shared__ float acc[kSlots][2][P::kLanes * VEC * NCH];
+    const int slot = (threadIdx.x >> 6) / WPR;
+    if constexpr (LPR == 16) {  // a wavefront's four places first
 #pragma unroll
-        for (int i = 0; i < NCH; ++i)
+      for (int i = 0; i < NCH; ++i)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int j = c0 + i * kStep + e;
-            acc[0][j] = t ? acc[0][j] + sg[i][e] : sg[i][e];
-            acc[1][j] = t ? acc[1][j] + sb[i][e] : sb[i][e];
-          }
-      }
-      __syncthreads();
+        for (int e = 0; e < VEC; ++e) {
+          sg[i][e] = xor32_sum(xor16_sum(sg[i][e]));
+          sb[i][e] = xor32_sum(xor16_sum(sb[i][e]));
+        }
     }
-    for (int j = threadIdx.x; j < d; j += 256) {
-      out[j] = acc[0][j];
-      out[dp + j] = acc[1][j];
+    if (LPR == 64 || (threadIdx.x & 63) < 16) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          acc[slot][0][c0 + i * kStep + e] = sg[i][e];
+          acc[slot][1][c0 + i * kStep + e] = sb[i][e];
+        }
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < d; j += kThreads) {
+      float g = 0.f, b = 0.f;
+#pragma unroll
+      for (int q = 0; q < kSlots; ++q) {
+        g += acc[q][0][j];
+        b += acc[q][1][j];
+      }
+      out[j] = g;
+      out[dp + j] = b;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int j = c0 + i * kStep;
       if (j < d) {
-        Vec<float, VEC>::store(out + j, sg[i]);
-        Vec<float, VEC>::store(out + dp + j, sb[i]);
+        Vec<float, VEC>::template store_row<KIND>(out, j, d, sg[i]);
+        Vec<float, VEC>::template store_row<KIND>(out + dp, j, d, sb[i]);
       }
     }
   }
@@ -223,7 +268,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_bwd(
 
 // dgamma and dbeta: the columns' sums over the P workgroups' parts, in a fixed
 // order. A workgroup has 64 columns: 16 lanes of 4 by 64 groups of rows, four to a
-// wavefront; up to 512 parts each group's loads are in flight at once.
+// wavefront; a group's parts, 4 at most, are in flight at once.
 __global__ __launch_bounds__(1024) void k_ln_wgrad(float* __restrict__ dgamma,
                                                    float* __restrict__ dbeta,
                                                    const float* __restrict__ part, int P, int d,
@@ -233,7 +278,7 @@ __global__ __launch_bounds__(1024) void k_ln_wgrad(float* __restrict__ dgamma,
   const int j = blockIdx.x * 64 + c * 4;  // of 2 dp columns
   f32x4_t s = {0.f, 0.f, 0.f, 0.f};
   if (j < 2 * dp) {
-#pragma unroll 8
+#pragma unroll 4
     for (int p = r; p < P; p += 64)
       s += *reinterpret_cast<const f32x4_t*>(part + (size_t)p * 2 * dp + j);
   }
@@ -252,50 +297,47 @@ __global__ __launch_bounds__(1024) void k_ln_wgrad(float* __restrict__ dgamma,
   }
 }
 
-// Vector widths: 16 bytes of a row where every row is aligned to them, else
-// pairs, else single elements.
-int vec_of(int d, int dt) {
-  const int full = dt == SKV_BF16 ? 8 : 4;
-  if (d % full == 0) return full;
-  return d % 2 == 0 ? 2 : 1;
-}
-
+// Up to 256 columns a row has 16 lanes, so that narrow rows leave no lanes idle.
+int lanes_of(int d) { return d <= 16 * kLaneCols ? 16 : 64; }
 int waves_of(int d) { return d <= 64 * kLaneCols ? 1 : d <= 256 * kLaneCols ? 4 : 16; }
+// Rows of a workgroup of `threads` lanes.
+int rows_of(int d, int threads) { return threads / (lanes_of(d) * waves_of(d)); }
+int fwd_rows(int d) { return rows_of(d, waves_of(d) == 16 ? 1024 : 256); }
 
-// f(vector width, vectors a lane, wavefronts a row) as compile-time constants
-template <int FULL, typename F>
-void dispatch(int d, int vec, F f) {
-  const int wpr = waves_of(d);
-  auto with_vec = [&](auto V) {
-    constexpr int v = decltype(V)::value;
-    const int n = (d + 64 * wpr * v - 1) / (64 * wpr * v);  // vectors a lane
-    auto with_n = [&](auto N) {
-      if (wpr == 1) f(V, N, std::integral_constant<int, 1>{});
-      else if (wpr == 4) f(V, N, std::integral_constant<int, 4>{});
-      else f(V, N, std::integral_constant<int, 16>{});
+// f(vectors of VEC elements a lane, lanes and wavefronts of a row, the rows' kind) as
+// compile-time constants
+template <int VEC, typename F>
+void dispatch(int d, F f) {
+  using std::integral_constant;
+  const int wpr = waves_of(d), lpr = lanes_of(d);
+  const int n = (d + lpr * wpr * VEC - 1) / (lpr * wpr * VEC);
+  const auto with_n = [&](auto N) {
+    const auto with_kind = [&](auto KIND) {
+      if (lpr == 16) f(N, integral_constant<int, 16>{}, integral_constant<int, 1>{}, KIND);
+      else if (wpr == 1) f(N, integral_constant<int, 64>{}, integral_constant<int, 1>{}, KIND);
+      else if (wpr == 4) f(N, integral_constant<int, 64>{}, integral_constant<int, 4>{}, KIND);
+      else f(N, integral_constant<int, 64>{}, integral_constant<int, 16>{}, KIND);
     };
-    if constexpr (kLaneCols / v >= 1)
-      if (n <= 1) return with_n(std::integral_constant<int, 1>{});
-    if constexpr (kLaneCols / v >= 4)
-      if (n <= 2) return with_n(std::integral_constant<int, 2>{});
-    if constexpr (kLaneCols / v >= 4 && v >= 4)
-      if (n <= 3) return with_n(std::integral_constant<int, 3>{});
-    if constexpr (kLaneCols / v >= 8)
-      if (n <= 4) return with_n(std::integral_constant<int, 4>{});
-    if constexpr (kLaneCols / v >= 16)
-      if (n <= 8) return with_n(std::integral_constant<int, 8>{});
-    with_n(std::integral_constant<int, kLaneCols / v>{});
+    if (row_kind(d, VEC) == kEven) with_kind(integral_constant<int, kEven>{});
+    else with_kind(integral_constant<int, kOdd>{});
   };
-  if (vec == FULL) with_vec(std::integral_constant<int, FULL>{});
-  else if (vec == 2) with_vec(std::integral_constant<int, 2>{});
-  else with_vec(std::integral_constant<int, 1>{});
+  if (row_kind(d, VEC) == kTiny)
+    return f(integral_constant<int, 1>{}, integral_constant<int, 16>{}, integral_constant<int, 1>{},
+             integral_constant<int, kTiny>{});
+  if (n <= 1) return with_n(integral_constant<int, 1>{});
+  if constexpr (VEC == 4) {
+    if (n <= 2) return with_n(integral_constant<int, 2>{});
+    if (n <= 3) return with_n(integral_constant<int, 3>{});
+  }
+  with_n(integral_constant<int, kLaneCols / VEC>{});
 }
 
-// Workgroups of the backward: two to a CU, no more than there are rows for.
+// Workgroups of the backward: one to a CU (each leaves a part of the weight gradients,
+// to be read again), no more than there are rows for.
 int bwd_groups(int M, int d) {
-  const int rows = waves_of(d) == 1 ? 4 : 1;
+  const int rows = rows_of(d, bwd_threads(waves_of(d)));
   const int need = (M + rows - 1) / rows;
-  return need < 512 ? need : 512;
+  return need < 256 ? need : 256;
 }
 
 int padded(int d) { return (d + 3) / 4 * 4; }
@@ -325,18 +367,17 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
                      {{x, act, "input", 0}, {gamma, (size_t)d * 4, "gamma"},
                       {beta, (size_t)d * 4, "beta"}}))
     return rc;
-  const int rows = waves_of(d) == 1 ? 4 : 1;
-  const dim3 grid((M + rows - 1) / rows);
-  auto run = [&](auto* yt, auto FULL) {
+  const dim3 grid((M + fwd_rows(d) - 1) / fwd_rows(d));
+  const auto run = [&](auto* yt) {
     using T = std::remove_pointer_t<decltype(yt)>;
-    dispatch<decltype(FULL)::value>(d, vec_of(d, dt), [&](auto V, auto N, auto W) {
-      k_ln_fwd<T, V.value, N.value, W.value>
+    dispatch<16 / sizeof(T)>(d, [&](auto N, auto L, auto W, auto KIND) {
+      k_ln_fwd<T, N.value, L.value, W.value, KIND.value>
           <<<grid, W.value == 16 ? 1024 : 256, 0, (hipStream_t)stream>>>(
               yt, mean, rstd, (const T*)x, gamma, beta, M, d, eps);
     });
   };
-  if (dt == SKV_BF16) run((uint16_t*)y, std::integral_constant<int, 8>{});
-  else run((float*)y, std::integral_constant<int, 4>{});
+  if (dt == SKV_BF16) run((uint16_t*)y);
+  else run((float*)y);
   return check_launch("skv_layernorm_fwd");
 }
 
@@ -370,20 +411,21 @@ extern "C" int skv_layernorm_bwd(void* dx, float* dgamma, float* dbeta, const vo
     return rc;
   const int P = bwd_groups(M, d), dp = padded(d);
   float* part = (float*)ws;
-  auto run = [&](auto* xt, auto FULL) {
+  const auto run = [&](auto* xt) {
     using T = std::remove_pointer_t<decltype(xt)>;
-    dispatch<decltype(FULL)::value>(d, vec_of(d, dt), [&](auto V, auto N, auto W) {
-      const int threads = W.value == 16 ? 1024 : 256;
-      if (residual)
-        k_ln_bwd<T, V.value, N.value, W.value, true><<<P, threads, 0, (hipStream_t)stream>>>(
-            xt, part, (const T*)dy, (const T*)x, gamma, mean, rstd, (const T*)residual, M, d, dp);
-      else
-        k_ln_bwd<T, V.value, N.value, W.value, false><<<P, threads, 0, (hipStream_t)stream>>>(
-            xt, part, (const T*)dy, (const T*)x, gamma, mean, rstd, (const T*)nullptr, M, d, dp);
+    dispatch<16 / sizeof(T)>(d, [&](auto N, auto L, auto W, auto KIND) {
+      constexpr int threads = bwd_threads(W.value);
+      const auto go = [&](auto RES) {
+        k_ln_bwd<T, N.value, L.value, W.value, KIND.value, RES.value>
+            <<<P, threads, 0, (hipStream_t)stream>>>(xt, part, (const T*)dy, (const T*)x, gamma, mean,
+                                                     rstd, (const T*)residual, M, d, dp);
+      };
+      if (residual) go(std::true_type{});
+      else go(std::false_type{});
     });
   };
-  if (dt == SKV_BF16) run((uint16_t*)dx, std::integral_constant<int, 8>{});
-  else run((float*)dx, std::integral_constant<int, 4>{});
+  if (dt == SKV_BF16) run((uint16_t*)dx);
+  else run((float*)dx);
   if (int rc = check_launch("skv_layernorm_bwd")) return rc;
   k_ln_wgrad<<<(2 * dp + 63) / 64, 1024, 0, (hipStream_t)stream>>>(dgamma, dbeta, part, P, d, dp,
                                                                    accumulate);

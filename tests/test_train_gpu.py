@@ -270,6 +270,21 @@ def test_embedding_backward_of_one_token(gpu_ctx, n):
     assert torch.equal(grad[ids.long()], dy)
 
 
+@pytest.mark.parametrize("n,vocab,often", [(65536, 256, 0.9), (65536, 50000, 0.3), (100003, 700, 0.5),
+                                           (1048576, 3, 0.2), (1200007, 9000, 0.1)])
+def test_embedding_backward_of_many_tokens(gpu_ctx, n, vocab, often):
+    """Runs whose lists overflow, some only after others did not, and runs past 16-bit places.
+    Small whole numbers: every sum is exact in any order below 2^24."""
+    from simple_llm_amd.gpu import gpu
+    rng = np.random.default_rng(n)
+    ids = ids_of(rng, n, vocab)
+    ids[rng.random(n) < often * np.arange(n) / n] = vocab // 2
+    dy = rng.integers(-4, 5, (n, 3)).astype(np.float64)
+    grad = torch.full((vocab, 3), 7.0, device="cuda")
+    gpu.embedding_backward(gpu_ctx, dev(dy), dev(ids, torch.int32), grad)
+    assert np.array_equal(g64(grad), to.embedding_backward(dy, ids, vocab, 1.0))
+
+
 def test_embedding_backward_keeps_a_bad_row_to_itself(gpu_ctx):
     from simple_llm_amd.gpu import gpu
     rng = np.random.default_rng(5)
