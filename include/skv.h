@@ -801,7 +801,7 @@ typedef struct skv_adamw_tensor {
  * probability of its distance from the lower, by a hash of (seed, t, place in the state);
  * a v above 0 takes no 0. The step itself uses the moments before they are
  * rounded. 128 moments with a NaN or an infinity are stored as scale 255 and codes 0 and
- * read back as NaN. p, g and copy of any alignment (16 bytes: vectors).
+ * read back as NaN. p, g and copy are aligned to their elements.
  */
 int skv_adamw(const skv_adamw_tensor* tensors, const int32_t* chunks, int n_chunks, void* m,
               void* v, uint8_t* m_scale, uint8_t* v_scale, int32_t* count, int bits, int grad_dt,

@@ -10,6 +10,8 @@
 // bf16 gradients and copies: 1101 us = 5.15 TB/s with 256 x 512 lanes, 1129 with 512 x
 // 512, 1170 with 1024 x 256; a copy runs at 4.71 TB/s read and write) and for their
 // arrivals below (3.2 million elements: 16.5, 18.8 and 22.7 us).
+// Vectors lie at any element: 33.5 million elements in tensors that begin 4 bytes behind a
+// 16-byte granule take 215 us, 208 at its begin, and 256 element by element.
 //
 // The step count t is in device memory, so that a captured step counts on when
 // it is replayed: every workgroup reads t before it does anything, and the last
@@ -162,7 +164,7 @@ template <int E>
 __device__ __forceinline__ void load_f32(float (&x)[E], const float* p, bool vec, int left) {
   if (vec) {
     Vec<float, E> v;
-    v.load(p);
+    v.load_any(p);
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = v.get(e);
   } else {
@@ -174,7 +176,7 @@ template <int E>
 __device__ __forceinline__ void load_f32(float (&x)[E], const uint16_t* p, bool vec, int left) {
   if (vec) {
     Vec<uint16_t, E> v;
-    v.load(p);
+    v.load_any(p);
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = v.get(e);
   } else {
@@ -185,7 +187,7 @@ __device__ __forceinline__ void load_f32(float (&x)[E], const uint16_t* p, bool 
 template <int E>
 __device__ __forceinline__ void store_f32(float* p, const float (&x)[E], bool vec, int left) {
   if (vec) {
-    Vec<float, E>::store(p, x);
+    Vec<float, E>::store_any(p, x);
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -195,7 +197,7 @@ __device__ __forceinline__ void store_f32(float* p, const float (&x)[E], bool ve
 template <int E>
 __device__ __forceinline__ void store_bf16(uint16_t* p, const float (&x)[E], bool vec, int left) {
   if (vec) {
-    Vec<uint16_t, E>::store(p, x);
+    Vec<uint16_t, E>::store_any(p, x);
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -206,8 +208,8 @@ __device__ __forceinline__ void store_bf16(uint16_t* p, const float (&x)[E], boo
 // One chunk of a tensor. BITS of a moment; TG: how gradients are stored. A lane has E
 // consecutive elements at a time: 4 of them where the moments are fp32, so that every
 // load of a wavefront is 1 KB in a row, and 8 where they are bytes. FULL: the chunk
-// lies inside the tensor and its vectors are aligned. All loads come before any store:
-// the compiler cannot tell the tensors apart.
+// lies inside the tensor. All loads come before any store: the compiler cannot tell the
+// tensors apart.
 template <typename TG, int BITS, bool FULL>
 __device__ __forceinline__ void step_chunk(const Step& a, const Tensor& x, int chunk, const Coef& c,
                                            uint32_t key) {
@@ -227,9 +229,9 @@ __device__ __forceinline__ void step_chunk(const Step& a, const Tensor& x, int c
     const int64_t i0 = first(part);
     const size_t at = (size_t)(x.at + i0);  // in the state
     const int left = left_of(part);
-    const bool here = FULL || i0 < blocks_end;
-    load_f32<E>(p[part], x.p + i0, FULL, left);
-    load_f32<E>(g[part], (const TG*)x.g + i0, FULL, left);
+    const bool whole = FULL || left == E, here = FULL || i0 < blocks_end;
+    load_f32<E>(p[part], x.p + i0, whole, left);
+    load_f32<E>(g[part], (const TG*)x.g + i0, whole, left);
     if constexpr (BITS == 32) {
       load_f32<E>(m[part], (const float*)a.m + at, here, 0);
       load_f32<E>(v[part], (const float*)a.v + at, here, 0);
@@ -255,17 +257,17 @@ __device__ __forceinline__ void step_chunk(const Step& a, const Tensor& x, int c
     const int64_t i0 = first(part);
     const size_t at = (size_t)(x.at + i0);
     const int left = left_of(part);
-    const bool here = FULL || i0 < blocks_end;
+    const bool whole = FULL || left == E, here = FULL || i0 < blocks_end;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       moments(m[part][e], v[part][e], g[part][e] * c.gs, c);
       p[part][e] = stepped(p[part][e], m[part][e], v[part][e], c, keep);
     }
-    store_f32<E>(x.p + i0, p[part], FULL, left);
-    if (x.copy) store_bf16<E>(x.copy + i0, p[part], FULL, left);
+    store_f32<E>(x.p + i0, p[part], whole, left);
+    if (x.copy) store_bf16<E>(x.copy + i0, p[part], whole, left);
     if constexpr (BITS == 32) {
-      store_f32<E>((float*)a.m + at, m[part], FULL, left);
-      store_f32<E>((float*)a.v + at, v[part], FULL, left);
+      store_f32<E>((float*)a.m + at, m[part], whole, left);
+      store_f32<E>((float*)a.v + at, v[part], whole, left);
     } else {
       uint32_t am = 0, av = 0;
 #pragma unroll
@@ -328,9 +330,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Step a, const Tensor* __rest
     const int after = ch + gridDim.x;
     const int2 next = chunks[min(after, a.n_chunks - 1)];
     const Tensor next_x = tensors[next.x];
-    const bool aligned = ((reinterpret_cast<uintptr_t>(x.p) | reinterpret_cast<uintptr_t>(x.g) |
-                           reinterpret_cast<uintptr_t>(x.copy)) & 15) == 0;
-    if (aligned && (int64_t)(which.y + 1) * kChunk <= x.n)
+    if ((int64_t)(which.y + 1) * kChunk <= x.n)
       step_chunk<TG, BITS, true>(a, x, which.y, c, key);
     else
       step_chunk<TG, BITS, false>(a, x, which.y, c, key);
@@ -387,6 +387,7 @@ extern "C" int skv_adamw(const skv_adamw_tensor* tensors, const int32_t* chunks,
   SKV_REQUIRE(bits == 32 || (m_scale && v_scale), SKV_E_INVALID,
               "skv_adamw: null pointer argument");
   SKV_REQUIRE(n_chunks > 0, SKV_E_INVALID, "skv_adamw: n_chunks must be > 0");
+  SKV_REQUIRE(n_chunks <= kMaxRows, SKV_E_UNSUPPORTED, "skv_adamw: n_chunks=%d > 2^30", n_chunks);
   SKV_REQUIRE(grad_dt == SKV_F32 || grad_dt == SKV_BF16, SKV_E_INVALID, "skv_adamw: bad dtype");
   SKV_REQUIRE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, SKV_E_INVALID,
               "skv_adamw: beta1 and beta2 must lie in [0, 1)");

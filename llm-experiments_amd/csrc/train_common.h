@@ -20,11 +20,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 
 // N consecutive elements of a row as they are stored (T float, or uint16_t for bf16),
-// N elements a power of two of words. load, stream and store take aligned vectors.
+// N elements a power of two of words. load, stream and store take aligned vectors,
+// load_any and store_any those at any element (gfx950 reads and writes them as they are).
 // load_row and stream_row read elements j .. j + N of a row of d, zeros past its end, j a
-// multiple of N below d. Rows that are no multiple of N elements (kOdd): gfx950 reads and
-// writes vectors at any address, so they are read like any other; a vector that would
-// leave its row is the row's last N elements instead, and settle(), called before the
+// multiple of N below d. Where rows are no multiple of N elements (kOdd), a vector that
+// would leave its row is the row's last N elements instead, and settle(), called before the
 // values are used, shifts it to its place: no load waits for another. Rows below N
 // elements (kTiny) are read one by one. stream and store_stream carry the nt bit: what is
 // read or written once does not push other lines out of the caches.
@@ -49,13 +49,14 @@ struct Vec {
     for (int i = 0; i < NW; ++i) w[i] = r[i];
   }
   __device__ __forceinline__ void load(const T* p) { set(*reinterpret_cast<const raw_t*>(p)); }
+  __device__ __forceinline__ void load_any(const T* p) { set(*reinterpret_cast<const any_t*>(p)); }
   __device__ __forceinline__ void stream(const T* p) {
     set(__builtin_nontemporal_load(reinterpret_cast<const raw_t*>(p)));
   }
   template <int KIND>
   __device__ __forceinline__ void load_row(const T* row, int j, int d) {
     if constexpr (KIND == kEven) load(row + j);
-    else if constexpr (KIND == kOdd) set(*reinterpret_cast<const any_t*>(row + min(j, d - N)));
+    else if constexpr (KIND == kOdd) load_any(row + min(j, d - N));
     else load_part(row + j, d - j);
   }
   template <int KIND>
@@ -123,13 +124,16 @@ struct Vec {
   static __device__ __forceinline__ void store(T* p, const float (&x)[N]) {
     *reinterpret_cast<raw_t*>(p) = words<raw_t>(x);
   }
+  static __device__ __forceinline__ void store_any(T* p, const float (&x)[N]) {
+    *reinterpret_cast<any_t*>(p) = words<any_t>(x);
+  }
   static __device__ __forceinline__ void store_stream(T* p, const float (&x)[N]) {
     __builtin_nontemporal_store(words<raw_t>(x), reinterpret_cast<raw_t*>(p));
   }
   template <int KIND>
   static __device__ __forceinline__ void store_row(T* row, int j, int d, const float (&x)[N]) {
     if constexpr (KIND == kEven) store(row + j, x);
-    else if (j + N <= d) *reinterpret_cast<any_t*>(row + j) = words<any_t>(x);
+    else if (j + N <= d) store_any(row + j, x);
     else store_part(row + j, x, d - j);
   }
   template <int KIND>
@@ -164,6 +168,11 @@ __device__ __forceinline__ float xor16_max(float x) {
 }
 __device__ __forceinline__ float wave_sum(float x) { return xor32_sum(xor16_sum(row16_sum(x))); }
 __device__ __forceinline__ float wave_max(float x) { return xor32_max(xor16_max(row16_max(x))); }
+
+// Whether a launch can have so many workgroups: fewer than 2^32 lanes.
+inline bool launchable(size_t groups, int lanes) { return groups * lanes < (size_t)1 << 32; }
+
+constexpr int kMaxRows = 1 << 30;  // rows that a kernel's 32-bit loops pass over
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

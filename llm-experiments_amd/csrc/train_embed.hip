@@ -31,6 +31,7 @@ namespace {
 
 using namespace train;
 
+constexpr int kMaxD = 1 << 22;
 constexpr int kBucket = 256;  // ids of a bucket, at most
 constexpr int kWaves = 16;    // wavefronts of a sorting workgroup
 constexpr int kBatches = 8;   // batches of 64 tokens a sorting wavefront reads at a time
@@ -426,8 +427,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_embed_join(float* __restric
   }
 }
 
-int ranges_of(int T) { return (T + kRange - 1) / kRange; }
-int padded(int d) { return (d + 3) / 4 * 4; }
+int ranges_of(int T) { return (T - 1) / kRange + 1; }
+size_t padded(int d) { return ((size_t)d + 3) / 4 * 4; }
 size_t ints_of(int T, int V) {
   return ((size_t)2 * ranges_of(T) + 2 * (size_t)T + V + 1 + 3) / 4 * 4;
 }
@@ -442,6 +443,8 @@ extern "C" int skv_embedding_fwd(void* out, const int32_t* ids, const void* tabl
                                  float scale, int table_dt, int out_dt, skv_stream_t stream) {
   SKV_REQUIRE(out && ids && table, SKV_E_INVALID, "skv_embedding_fwd: null pointer argument");
   SKV_REQUIRE(T > 0 && V > 0 && d > 0, SKV_E_INVALID, "skv_embedding_fwd: dims must be > 0");
+  SKV_REQUIRE(d <= kMaxD && launchable(((size_t)T + 3) / 4, 256), SKV_E_UNSUPPORTED,
+              "skv_embedding_fwd: T=%d, d=%d: up to 2^26 tokens and 2^22 columns", T, d);
   SKV_REQUIRE(!pos_table || n_pos > 0, SKV_E_INVALID, "skv_embedding_fwd: n_pos must be > 0");
   SKV_REQUIRE((table_dt == SKV_F32 || table_dt == SKV_BF16) &&
                   (out_dt == SKV_F32 || out_dt == SKV_BF16),
@@ -454,7 +457,7 @@ extern "C" int skv_embedding_fwd(void* out, const int32_t* ids, const void* tabl
                       {ids, (size_t)T * 4, "tokens"},
                       {pos_table, (size_t)n_pos * d * 4, "pos_table"}}))
     return rc;
-  const dim3 grid(((unsigned)T + 3) / 4);
+  const unsigned grid = ((unsigned)T + 3) / 4;
   const auto run = [&](auto* o, auto* t) {
     using TO = std::remove_pointer_t<decltype(o)>;
     using TT = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
@@ -489,8 +492,13 @@ extern "C" int skv_embedding_bwd(float* grad, const void* dout, const int32_t* i
   SKV_REQUIRE(grad && dout && ids && ws, SKV_E_INVALID, "skv_embedding_bwd: null pointer argument");
   SKV_REQUIRE(T > 0 && V > 0 && d > 0, SKV_E_INVALID, "skv_embedding_bwd: dims must be > 0");
   SKV_REQUIRE(dt == SKV_F32 || dt == SKV_BF16, SKV_E_INVALID, "skv_embedding_bwd: bad dtype");
-  SKV_REQUIRE(T <= 1 << 30 && V <= 1 << 30, SKV_E_UNSUPPORTED,
-              "skv_embedding_bwd: up to 2^30 tokens and table rows");
+  const int width = V <= 256 * kBucket ? (V + 255) / 256 : kBucket;  // one bucket to a CU
+  const int buckets = (V - 1) / width + 1, tiles = (d - 1) / 256 + 1;
+  SKV_REQUIRE(d <= kMaxD && T <= kMaxRows && launchable((size_t)buckets + kZeroGroups, 1024) &&
+                  launchable(((size_t)ranges_of(T) * tiles + 3) / 4, 256),
+              SKV_E_UNSUPPORTED,
+              "skv_embedding_bwd: T=%d, V=%d, d=%d are too many for a launch (up to 2^22 columns, "
+              "2^29 table rows, 2^30 tokens a 256 columns)", T, V, d);
   SKV_REQUIRE(aligned16(grad) && aligned16(dout) && aligned16(ws), SKV_E_INVALID,
               "skv_embedding_bwd: pointers must be 16-byte aligned");
   SKV_REQUIRE(ws_bytes >= skv_embedding_bwd_workspace_bytes(T, V, d), SKV_E_WORKSPACE,
@@ -509,13 +517,10 @@ extern "C" int skv_embedding_bwd(float* grad, const void* dout, const int32_t* i
   s.id = s.pos + T;
   s.begin = s.id + T;
   float* part = (float*)((int32_t*)ws + ints_of(T, V));
-  const int width = min((V + 255) / 256, kBucket);  // one bucket to a CU
-  const int buckets = (V + width - 1) / width;
   const size_t n_zero = accumulate ? 0 : (size_t)V * d;
   const int sort_grid = buckets + (n_zero ? kZeroGroups : 0);
   k_embed_sort<<<sort_grid, kWaves * 64, 0, st>>>(s, ids, T, V, width, buckets, grad, n_zero);
   if (int rc = check_launch("skv_embedding_bwd")) return rc;
-  const int tiles = (d + 255) / 256;
   const unsigned grid = (unsigned)(((size_t)ranges * tiles + 3) / 4);
   const dim3 join((ranges + kJoinWaves - 1) / kJoinWaves, tiles);
   const auto run = [&](auto* y, auto KIND, auto ACC) {

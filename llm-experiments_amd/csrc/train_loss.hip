@@ -314,9 +314,11 @@ __global__ __launch_bounds__(1024) void k_loss_mean(float* __restrict__ loss,
   }
 }
 
-// By the row's vectors: one wavefront up to 4 vectors a lane (no barrier), then 4 and 8
-// wavefronts up to 8 and 16 up to 16, so that a CU's registers hold many rows in different
-// phases (50304 bf16 logits x 8192: 16 wavefronts of 7 vectors, 290 us, 8 of 13, 295).
+// Wavefronts of a row by its vectors: one up to 4 vectors a lane (no barrier), then 4 and 8
+// up to 8 and 16 up to 16, so that a CU's registers hold many rows in different phases
+// (50304 bf16 logits x 8192: 16 wavefronts of 7 vectors, 290 us, 8 of 13, 295).
+int waves_of(int n) { return n <= 256 ? 1 : n <= 2048 ? 4 : n <= 4096 ? 8 : 16; }
+
 template <typename T, bool GRAD>
 void launch_rows(const LossArgs& a, hipStream_t s) {
   const int n = (a.V + kVec<T> - 1) / kVec<T>;
@@ -335,13 +337,14 @@ void launch_rows(const LossArgs& a, hipStream_t s) {
     else rows(NW, std::integral_constant<int, 16>{});
   };
   using std::integral_constant;
+  const int nw = waves_of(n);
   if (n <= 64) rows(integral_constant<int, 1>{}, integral_constant<int, 1>{});
   else if (n <= 128) rows(integral_constant<int, 1>{}, integral_constant<int, 2>{});
-  else if (n <= 256) rows(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  else if (nw == 1) rows(integral_constant<int, 1>{}, integral_constant<int, 4>{});
   else if (n <= 512) rows(integral_constant<int, 4>{}, integral_constant<int, 2>{});
   else if (n <= 1024) rows(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-  else if (n <= 2048) with(integral_constant<int, 4>{});
-  else if (n <= 4096) with(integral_constant<int, 8>{});
+  else if (nw == 4) with(integral_constant<int, 4>{});
+  else if (nw == 8) with(integral_constant<int, 8>{});
   else if (n <= 16384) with(integral_constant<int, 16>{});
   else k_loss_long<T, GRAD><<<a.M, 1024, 0, s>>>(a);
 }
@@ -362,6 +365,9 @@ extern "C" int skv_cross_entropy(float* loss, float* row_loss, void* dx, const v
   SKV_REQUIRE(M > 0 && V > 0, SKV_E_INVALID, "skv_cross_entropy: dims must be > 0");
   SKV_REQUIRE(dt == SKV_F32 || dt == SKV_BF16, SKV_E_INVALID, "skv_cross_entropy: bad dtype");
   SKV_REQUIRE(V <= 1 << 28, SKV_E_UNSUPPORTED, "skv_cross_entropy: V=%d > 2^28", V);
+  const int n_vec = (V - 1) / (dt == SKV_BF16 ? 8 : 4) + 1, waves = waves_of(n_vec);
+  SKV_REQUIRE(waves == 1 ? launchable(((size_t)M + 3) / 4, 256) : launchable(M, waves * 64),
+              SKV_E_UNSUPPORTED, "skv_cross_entropy: %d rows of %d are too many for a launch", M, V);
   SKV_REQUIRE(aligned16(dx) && aligned16(x) && aligned16(ws), SKV_E_INVALID,
               "skv_cross_entropy: pointers must be 16-byte aligned");
   SKV_REQUIRE(ws_bytes >= skv_cross_entropy_workspace_bytes(M), SKV_E_WORKSPACE,

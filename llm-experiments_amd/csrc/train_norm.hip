@@ -346,6 +346,7 @@ int check(const char* fn, int M, int d, int dt) {
   SKV_REQUIRE(M > 0 && d > 0, SKV_E_INVALID, "%s: dims must be > 0", fn);
   SKV_REQUIRE(dt == SKV_F32 || dt == SKV_BF16, SKV_E_INVALID, "%s: bad dtype", fn);
   SKV_REQUIRE(d <= kMaxD, SKV_E_UNSUPPORTED, "%s: d=%d > %d", fn, d, kMaxD);
+  SKV_REQUIRE(M <= kMaxRows, SKV_E_UNSUPPORTED, "%s: M=%d > 2^30", fn, M);
   return SKV_OK;
 }
 
@@ -359,6 +360,9 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
                                  int dt, skv_stream_t stream) {
   SKV_REQUIRE(y && x && gamma && beta, SKV_E_INVALID, "skv_layernorm_fwd: null pointer argument");
   if (int rc = check("skv_layernorm_fwd", M, d, dt)) return rc;
+  const unsigned grid = (M + fwd_rows(d) - 1) / fwd_rows(d);
+  SKV_REQUIRE(launchable(grid, waves_of(d) == 16 ? 1024 : 256), SKV_E_UNSUPPORTED,
+              "skv_layernorm_fwd: %d rows of %d are too many for a launch", M, d);
   SKV_REQUIRE(aligned16(y) && aligned16(x) && aligned16(gamma) && aligned16(beta), SKV_E_INVALID,
               "skv_layernorm_fwd: pointers must be 16-byte aligned");
   const size_t act = (size_t)M * d * (dt == SKV_BF16 ? 2 : 4), row = (size_t)M * 4;
@@ -367,7 +371,6 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
                      {{x, act, "input", 0}, {gamma, (size_t)d * 4, "gamma"},
                       {beta, (size_t)d * 4, "beta"}}))
     return rc;
-  const dim3 grid((M + fwd_rows(d) - 1) / fwd_rows(d));
   const auto run = [&](auto* yt) {
     using T = std::remove_pointer_t<decltype(yt)>;
     dispatch<16 / sizeof(T)>(d, [&](auto N, auto L, auto W, auto KIND) {
@@ -382,7 +385,7 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
 }
 
 extern "C" size_t skv_layernorm_bwd_workspace_bytes(int M, int d) {
-  if (M <= 0 || d <= 0 || d > kMaxD) return 0;
+  if (M <= 0 || M > kMaxRows || d <= 0 || d > kMaxD) return 0;
   return (size_t)bwd_groups(M, d) * 2 * padded(d) * sizeof(float);
 }
 

@@ -268,3 +268,33 @@ def test_c_entry_points_refuse():
     assert L.skv_adamw_read(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 100, 0, None) == inv
     assert L.skv_adamw_read(FAKE, None, FAKE, FAKE, FAKE, FAKE, 128, 0, None) == inv
     assert L.skv_adamw_read(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 41, 0, None) == uns
+
+
+def test_c_entry_points_refuse_too_many_rows():
+    """More than a launch or a kernel's 32-bit loops can have, on either side of the limits
+    that are refused before memory is looked at."""
+    L = _lib.lib()
+    uns = _lib.SKV_E_UNSUPPORTED
+    big = (1 << 31) - 1
+
+    def fwd(M, d):
+        return L.skv_layernorm_fwd(FAKE, None, None, FAKE, FAKE, FAKE, M, d, 1e-5, 1, None)
+
+    # lanes of a row: 16, 64, 256 and 1024
+    for d, lanes in ((1, 16), (256, 16), (257, 64), (1024, 64), (1025, 256), (4097, 1024)):
+        most = ((1 << 32) - 1) // lanes
+        for M in (min(most + 1, big), big):
+            assert fwd(M, d) == uns, (M, d)
+        assert fwd(most // 1024 * 1024, d) == _lib.SKV_E_INVALID  # gets as far as the overlaps
+    assert L.skv_layernorm_bwd_workspace_bytes(big, 8) == 0
+    assert L.skv_layernorm_bwd(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, big, 8, 0, FAKE,
+                               1 << 40, 0, None) == uns
+    for T, d in (((1 << 26) + 1, 8), (big, 8), (4, (1 << 22) + 1)):
+        assert L.skv_embedding_fwd(FAKE, FAKE, FAKE, None, T, 10, d, 0, 1.0, 0, 0, None) == uns
+    for T, V, d in ((big, 10, 8), (1 << 30, 10, 257), (4, big, 8), (4, 10, big), (1 << 20, 10, 1 << 20)):
+        assert L.skv_embedding_bwd_workspace_bytes(T, V, d) > 0
+        assert L.skv_embedding_bwd(FAKE, FAKE, FAKE, T, V, d, 1.0, 0, FAKE, 1 << 62, 0, None) == uns
+    for M, V in ((big, 1), ((1 << 26) + 1, 2048), (1 << 24, 2049), (1 << 23, 16385), (1 << 22, 40000)):
+        assert L.skv_cross_entropy(FAKE, None, FAKE, FAKE, FAKE, M, V, 1.0, FAKE, 1 << 62, 1, None) == uns
+    assert L.skv_adamw(FAKE, FAKE, big, FAKE, FAKE, None, None, FAKE, 32, 0, 1e-3, None, 0.9, 0.99,
+                       1e-8, 0.1, 1.0, None, 0, None) == uns
