@@ -44,7 +44,7 @@ struct Vec {
     for (int i = 0; i < NW; ++i) w[i] = 0u;
   }
   template <typename R>
-  __device__ __forceinline__ void set(const R& r) {
+  __device__ __forceinline__ void set(R r) {
 #pragma unroll
     for (int i = 0; i < NW; ++i) w[i] = r[i];
   }

@@ -7,8 +7,8 @@
 //   dgamma = sum over rows of dy xh, dbeta = sum over rows of dy
 //
 // Both directions are bound by HBM: a row is read once into registers, its sums go over
-// the row's lanes, and the result is written. A row is on 16 lanes up to 256 columns, on
-// one wavefront up to 1024 (no LDS, no barrier), on 4 up to 4096 and on 16 up to 16384.
+// the row's lanes, and the result is written. A row is on 16, 32 or 64 lanes of a wavefront
+// up to 1024 columns (no LDS, no barrier), on 4 wavefronts up to 4096 and on 16 up to 16384.
 // 16384 x 1024 bf16 forward: 11.6 us = 5.8 TB/s (its output with the nt bit; 13.0
 // without). 16384 x 768 fp32 backward with a residual: 36.3 us = 5.5 TB/s (rows read with
 // the nt bit; 43.5 without), 4 of them for the weight gradients' second pass. Rows that
@@ -26,7 +26,7 @@ constexpr int kLaneCols = 16;  // columns of a row a lane holds
 
 constexpr int bwd_threads(int WPR) { return WPR == 16 ? 1024 : 512; }
 
-// A row's place in a workgroup of THREADS lanes: LPR lanes of a wavefront (16 or 64)
+// A row's place in a workgroup of THREADS lanes: LPR lanes of a wavefront (16, 32 or 64)
 // with WPR = 1, or WPR whole wavefronts.
 template <int LPR, int WPR, int THREADS>
 struct Place {
@@ -42,9 +42,13 @@ template <int LPR, int WPR, int THREADS>
 __device__ __forceinline__ void row_sums(float& a, float& b, float* sh, int& turn) {
   a = row16_sum(a);
   b = row16_sum(b);
+  if constexpr (LPR >= 32) {
+    a = xor16_sum(a);
+    b = xor16_sum(b);
+  }
   if constexpr (LPR == 64) {
-    a = xor32_sum(xor16_sum(a));
-    b = xor32_sum(xor16_sum(b));
+    a = xor32_sum(a);
+    b = xor32_sum(b);
   }
   if constexpr (WPR > 1) {
     float* s = sh + turn * 2 * (THREADS / 64);
@@ -225,16 +229,20 @@ __global__ __launch_bounds__(bwd_threads(WPR)) void k_ln_bwd(
   if constexpr (kSlots > 1) {
     __shared__ float acc[kSlots][2][P::kLanes * VEC * NCH];
     const int slot = (threadIdx.x >> 6) / WPR;
-    if constexpr (LPR == 16) {  // a wavefront's four places first
+    if constexpr (LPR < 64) {  // a wavefront's places first
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          sg[i][e] = xor32_sum(xor16_sum(sg[i][e]));
-          sb[i][e] = xor32_sum(xor16_sum(sb[i][e]));
+          if constexpr (LPR == 16) {
+            sg[i][e] = xor16_sum(sg[i][e]);
+            sb[i][e] = xor16_sum(sb[i][e]);
+          }
+          sg[i][e] = xor32_sum(sg[i][e]);
+          sb[i][e] = xor32_sum(sb[i][e]);
         }
     }
-    if (LPR == 64 || (threadIdx.x & 63) < 16) {
+    if ((threadIdx.x & 63) < LPR) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
@@ -297,34 +305,43 @@ __global__ __launch_bounds__(1024) void k_ln_wgrad(float* __restrict__ dgamma,
   }
 }
 
-// Up to 256 columns a row has 16 lanes, so that narrow rows leave no lanes idle.
-int lanes_of(int d) { return d <= 16 * kLaneCols ? 16 : 64; }
+// Lanes of a row in one wavefront: 16, 32 or 64. Few, so that narrow rows leave few lanes
+// idle: up to kLaneCols columns a lane (32768 x 257 bf16 backward: 28.5 us with 64 lanes,
+// 23.0 with 32). More, down to half as many columns, where there are too few rows for a
+// backward workgroup on every CU (2048 x 390: 7.1 us with 64, 7.9 with 32).
+int lanes_of(int M, int d) {
+  const auto fits = [&](int lanes) {
+    return d <= lanes * (M >= 256 * (512 / lanes) ? kLaneCols : kLaneCols / 2);
+  };
+  return fits(16) ? 16 : fits(32) ? 32 : 64;
+}
 int waves_of(int d) { return d <= 64 * kLaneCols ? 1 : d <= 256 * kLaneCols ? 4 : 16; }
 // Rows of a workgroup of `threads` lanes.
-int rows_of(int d, int threads) { return threads / (lanes_of(d) * waves_of(d)); }
-int fwd_rows(int d) { return rows_of(d, waves_of(d) == 16 ? 1024 : 256); }
+int rows_of(int M, int d, int threads) { return threads / (lanes_of(M, d) * waves_of(d)); }
+int fwd_rows(int M, int d) { return rows_of(M, d, waves_of(d) == 16 ? 1024 : 256); }
 
 // f(vectors of VEC elements a lane, lanes and wavefronts of a row, the rows' kind) as
 // compile-time constants
 template <int VEC, typename F>
-void dispatch(int d, F f) {
+void dispatch(int M, int d, F f) {
   using std::integral_constant;
-  const int wpr = waves_of(d), lpr = lanes_of(d);
+  const int wpr = waves_of(d), lpr = lanes_of(M, d);
   const int n = (d + lpr * wpr * VEC - 1) / (lpr * wpr * VEC);
-  const auto with_n = [&](auto N) {
-    const auto with_kind = [&](auto KIND) {
-      if (lpr == 16) f(N, integral_constant<int, 16>{}, integral_constant<int, 1>{}, KIND);
-      else if (wpr == 1) f(N, integral_constant<int, 64>{}, integral_constant<int, 1>{}, KIND);
-      else if (wpr == 4) f(N, integral_constant<int, 64>{}, integral_constant<int, 4>{}, KIND);
-      else f(N, integral_constant<int, 64>{}, integral_constant<int, 16>{}, KIND);
-    };
-    if (row_kind(d, VEC) == kEven) with_kind(integral_constant<int, kEven>{});
-    else with_kind(integral_constant<int, kOdd>{});
+  const RowKind kind = row_kind(d, VEC);
+  const integral_constant<int, 1> one;
+  const auto with_kind = [&](auto N, auto L, auto W) {
+    if (kind == kEven) f(N, L, W, integral_constant<int, kEven>{});
+    else f(N, L, W, integral_constant<int, kOdd>{});
   };
-  if (row_kind(d, VEC) == kTiny)
-    return f(integral_constant<int, 1>{}, integral_constant<int, 16>{}, integral_constant<int, 1>{},
-             integral_constant<int, kTiny>{});
-  if (n <= 1) return with_n(integral_constant<int, 1>{});
+  const auto with_n = [&](auto N) {
+    if (lpr == 16) with_kind(N, integral_constant<int, 16>{}, one);
+    else if (lpr == 32) with_kind(N, integral_constant<int, 32>{}, one);
+    else if (wpr == 1) with_kind(N, integral_constant<int, 64>{}, one);
+    else if (wpr == 4) with_kind(N, integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    else with_kind(N, integral_constant<int, 64>{}, integral_constant<int, 16>{});
+  };
+  if (kind == kTiny) return f(one, integral_constant<int, 16>{}, one, integral_constant<int, kTiny>{});
+  if (n <= 1) return with_n(one);
   if constexpr (VEC == 4) {
     if (n <= 2) return with_n(integral_constant<int, 2>{});
     if (n <= 3) return with_n(integral_constant<int, 3>{});
@@ -335,7 +352,7 @@ void dispatch(int d, F f) {
 // Workgroups of the backward: one to a CU (each leaves a part of the weight gradients,
 // to be read again), no more than there are rows for.
 int bwd_groups(int M, int d) {
-  const int rows = rows_of(d, bwd_threads(waves_of(d)));
+  const int rows = rows_of(M, d, bwd_threads(waves_of(d)));
   const int need = (M + rows - 1) / rows;
   return need < 256 ? need : 256;
 }
@@ -360,7 +377,7 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
                                  int dt, skv_stream_t stream) {
   SKV_REQUIRE(y && x && gamma && beta, SKV_E_INVALID, "skv_layernorm_fwd: null pointer argument");
   if (int rc = check("skv_layernorm_fwd", M, d, dt)) return rc;
-  const unsigned grid = (M + fwd_rows(d) - 1) / fwd_rows(d);
+  const unsigned grid = (M + fwd_rows(M, d) - 1) / fwd_rows(M, d);
   SKV_REQUIRE(launchable(grid, waves_of(d) == 16 ? 1024 : 256), SKV_E_UNSUPPORTED,
               "skv_layernorm_fwd: %d rows of %d are too many for a launch", M, d);
   SKV_REQUIRE(aligned16(y) && aligned16(x) && aligned16(gamma) && aligned16(beta), SKV_E_INVALID,
@@ -373,7 +390,7 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
     return rc;
   const auto run = [&](auto* yt) {
     using T = std::remove_pointer_t<decltype(yt)>;
-    dispatch<16 / sizeof(T)>(d, [&](auto N, auto L, auto W, auto KIND) {
+    dispatch<16 / sizeof(T)>(M, d, [&](auto N, auto L, auto W, auto KIND) {
       k_ln_fwd<T, N.value, L.value, W.value, KIND.value>
           <<<grid, W.value == 16 ? 1024 : 256, 0, (hipStream_t)stream>>>(
               yt, mean, rstd, (const T*)x, gamma, beta, M, d, eps);
@@ -416,7 +433,7 @@ extern "C" int skv_layernorm_bwd(void* dx, float* dgamma, float* dbeta, const vo
   float* part = (float*)ws;
   const auto run = [&](auto* xt) {
     using T = std::remove_pointer_t<decltype(xt)>;
-    dispatch<16 / sizeof(T)>(d, [&](auto N, auto L, auto W, auto KIND) {
+    dispatch<16 / sizeof(T)>(M, d, [&](auto N, auto L, auto W, auto KIND) {
       constexpr int threads = bwd_threads(W.value);
       const auto go = [&](auto RES) {
         k_ln_bwd<T, N.value, L.value, W.value, KIND.value, RES.value>

@@ -59,6 +59,9 @@ def ids_of(rng, n, vocab, padded=True):
 NORM = [(1, 1), (1, 8), (3, 2), (5, 7), (4, 64), (130, 390), (33, 513), (257, 768), (9, 1000),
         (64, 1024), (17, 1025), (6, 1536), (70, 2048), (5, 4095), (3, 4096), (7, 4098), (2, 5000),
         (600, 8192), (3, 16383), (2, 16384), (2049, 256)]
+# Rows on 16, 32 and 64 lanes, and on both sides of where their number or width changes that.
+MANY = [(5000, 96), (8191, 129), (8193, 200), (8192, 256), (4095, 257), (4097, 300), (4096, 511),
+        (4100, 512), (4100, 513), (9000, 7)]
 
 
 def norm_inputs(rows, d, dtype, offset=0.5):
@@ -83,7 +86,7 @@ def check_norm(x, gamma, beta, y, mean, rstd, what):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
-@pytest.mark.parametrize("rows,d", NORM)
+@pytest.mark.parametrize("rows,d", NORM + MANY)
 def test_layernorm(gpu_ctx, rows, d, dtype):
     from simple_llm_amd.gpu import gpu
     banner(f"layernorm {rows} x {d} {dtype}")
@@ -128,7 +131,7 @@ def test_layernorm_rows_do_not_mix(gpu_ctx, bad):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
-@pytest.mark.parametrize("rows,d", NORM + [(5000, 96)])
+@pytest.mark.parametrize("rows,d", NORM + MANY)
 @pytest.mark.parametrize("residual,accumulate", [(False, True), (True, False)])
 def test_layernorm_backward(gpu_ctx, rows, d, dtype, residual, accumulate):
     from simple_llm_amd.gpu import gpu
