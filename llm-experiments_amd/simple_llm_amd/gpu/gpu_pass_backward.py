@@ -23,8 +23,8 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .gpu_pass_common import (F32, FLOATS, I32, Operand, launch, operand, required, rows_of,
-                              workspace)
+from .gpu_pass_common import (F32, FLOATS, I32, Operand, device_of, launch, operand, required,
+                              rows_of, workspace)
 from .gpu_ops import batch_count, validate_buffer_shape_1d, validate_buffer_shape_2d
 from .gpu_types import GPUBuffer1D, GPUBuffer2D, GPUContext
 
@@ -119,18 +119,19 @@ def layernorm_backward(ctx: GPUContext, grad_output: Operand, input: Operand, ga
     layer), or None. grad_input may be grad_output, input or residual.
     accumulate: grad_gamma and grad_beta are added to (grad_input is not).
     """
-    x, rows, d, dtype = rows_of(ctx, input, "input", FLOATS)
+    dev = device_of(ctx)
+    x, rows, d, dtype = rows_of(dev, input, "input", FLOATS)
     like, shape = (dtype,), (rows, d)
-    dy = required(ctx, grad_output, "grad_output", shape, like)
-    dx = required(ctx, grad_input, "grad_input", shape, like)
-    res = operand(ctx, residual, "residual", shape, like)
-    g = required(ctx, gamma, "gamma", (d,), F32)
-    mu = required(ctx, mean, "mean", (rows,), F32, 4)
-    rs = required(ctx, rstd, "rstd", (rows,), F32, 4)
-    dg = required(ctx, grad_gamma, "grad_gamma", (d,), F32, 4)
-    db = required(ctx, grad_beta, "grad_beta", (d,), F32, 4)
-    ws = workspace(ctx, "skv_layernorm_bwd_workspace_bytes", rows, d)
-    launch(ctx, "skv_layernorm_bwd", dx, dg, db, dy, x, g, mu, rs, res, rows, d,
+    dy = required(dev, grad_output, "grad_output", shape, like)
+    dx = required(dev, grad_input, "grad_input", shape, like)
+    res = operand(dev, residual, "residual", shape, like)
+    g = required(dev, gamma, "gamma", (d,), F32)
+    mu = required(dev, mean, "mean", (rows,), F32, 4)
+    rs = required(dev, rstd, "rstd", (rows,), F32, 4)
+    dg = required(dev, grad_gamma, "grad_gamma", (d,), F32, 4)
+    db = required(dev, grad_beta, "grad_beta", (d,), F32, 4)
+    ws = workspace(dev, "skv_layernorm_bwd_workspace_bytes", rows, d)
+    launch(ctx, dev, "skv_layernorm_bwd", dx, dg, db, dy, x, g, mu, rs, res, rows, d,
            int(bool(accumulate)), ws.data_ptr(), ws.numel(), _lib.dtype_code(dtype))
 
 
@@ -144,11 +145,12 @@ def embedding_backward(ctx: GPUContext, grad_output: Operand, tokens: Operand,
     touched), as where the tied logits have left their part. Tokens outside [0, vocab) are
     padding and add nothing.
     """
-    dy, n, d, dtype = rows_of(ctx, grad_output, "grad_output", FLOATS)
-    ids = required(ctx, tokens, "tokens", (n,), I32, 4)
-    grad, vocab, _, _ = rows_of(ctx, grad_table, "grad_table", F32, d)
-    ws = workspace(ctx, "skv_embedding_bwd_workspace_bytes", n, vocab, d)
-    launch(ctx, "skv_embedding_bwd", grad, dy, ids, n, vocab, d, float(scale),
+    dev = device_of(ctx)
+    dy, n, d, dtype = rows_of(dev, grad_output, "grad_output", FLOATS)
+    ids = required(dev, tokens, "tokens", (n,), I32, 4)
+    grad, vocab, _, _ = rows_of(dev, grad_table, "grad_table", F32, d)
+    ws = workspace(dev, "skv_embedding_bwd_workspace_bytes", n, vocab, d)
+    launch(ctx, dev, "skv_embedding_bwd", grad, dy, ids, n, vocab, d, float(scale),
            int(bool(accumulate)), ws.data_ptr(), ws.numel(), _lib.dtype_code(dtype))
 
 

@@ -24,8 +24,8 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .gpu_pass_common import (F32, FLOATS, I32, Operand, launch, operand, required, rows_of,
-                              tensor_of, workspace)
+from .gpu_pass_common import (F32, FLOATS, I32, Operand, device_of, launch, operand, required,
+                              rows_of, tensor_of, workspace)
 from .gpu_ops import batch_count, validate_buffer_shape_1d, validate_buffer_shape_2d
 from .gpu_types import GPUBuffer1D, GPUBuffer2D, GPUContext
 
@@ -93,17 +93,18 @@ def embedding(ctx: GPUContext, tokens: Operand, table: Operand, output: Operand,
     of exactly `context` tokens). A token outside [0, vocab) is padding: its table row counts
     as zeros.
     """
-    w, vocab, d, w_dtype = rows_of(ctx, table, "table", FLOATS)
-    ids = required(ctx, tokens, "tokens", None, I32, 4)
+    dev = device_of(ctx)
+    w, vocab, d, w_dtype = rows_of(dev, table, "table", FLOATS)
+    ids = required(dev, tokens, "tokens", None, I32, 4)
     shape = tensor_of(tokens).shape
     if len(shape) != 1 or not 0 < shape[0] < 1 << 31:
         raise ValueError(f"tokens must be 1-D and hold elements, got shape {tuple(shape)}")
     n = shape[0]
-    out = required(ctx, output, "output", (n, d), FLOATS)
+    out = required(dev, output, "output", (n, d), FLOATS)
     pos, n_pos = None, 0
     if pos_table is not None:
-        pos, n_pos, _, _ = rows_of(ctx, pos_table, "pos_table", F32, d)
-    launch(ctx, "skv_embedding_fwd", out, ids, w, pos, n, vocab, d, n_pos, float(scale),
+        pos, n_pos, _, _ = rows_of(dev, pos_table, "pos_table", F32, d)
+    launch(ctx, dev, "skv_embedding_fwd", out, ids, w, pos, n, vocab, d, n_pos, float(scale),
            _lib.dtype_code(w_dtype), _lib.dtype_code(tensor_of(output).dtype))
 
 
@@ -116,15 +117,16 @@ def layernorm(ctx: GPUContext, input: Operand, gamma: Operand, beta: Operand, ou
     input. gamma, beta: float32 [d]. mean, rstd: float32 [rows], the rows' statistics for
     layernorm_backward (rstd = 1 / sqrt(var + eps)), or None.
     """
-    x, rows, d, dtype = rows_of(ctx, input, "input", FLOATS)
-    y = required(ctx, output, "output", (rows, d), (dtype,))
-    g = required(ctx, gamma, "gamma", (d,), F32)
-    b = required(ctx, beta, "beta", (d,), F32)
-    mu = operand(ctx, mean, "mean", (rows,), F32, 4)
-    rs = operand(ctx, rstd, "rstd", (rows,), F32, 4)
+    dev = device_of(ctx)
+    x, rows, d, dtype = rows_of(dev, input, "input", FLOATS)
+    y = required(dev, output, "output", (rows, d), (dtype,))
+    g = required(dev, gamma, "gamma", (d,), F32)
+    b = required(dev, beta, "beta", (d,), F32)
+    mu = operand(dev, mean, "mean", (rows,), F32, 4)
+    rs = operand(dev, rstd, "rstd", (rows,), F32, 4)
     if not eps >= 0:
         raise ValueError(f"eps must be >= 0, got {eps}")
-    launch(ctx, "skv_layernorm_fwd", y, mu, rs, x, g, b, rows, d, float(eps),
+    launch(ctx, dev, "skv_layernorm_fwd", y, mu, rs, x, g, b, rows, d, float(eps),
            _lib.dtype_code(dtype))
 
 
@@ -138,13 +140,14 @@ def cross_entropy_loss(ctx: GPUContext, logits: Operand, targets: Operand, loss:
     grad_logits: the loss's gradient times grad_scale, like logits and possibly the same
     buffer, or None. row_losses: float32 [rows], 0 where ignored, or None.
     """
-    x, rows, vocab, dtype = rows_of(ctx, logits, "logits", FLOATS)
-    t = required(ctx, targets, "targets", (rows,), I32, 4)
-    out = required(ctx, loss, "loss", (1,), F32, 4)
-    dx = operand(ctx, grad_logits, "grad_logits", (rows, vocab), (dtype,))
-    row = operand(ctx, row_losses, "row_losses", (rows,), F32, 4)
-    ws = workspace(ctx, "skv_cross_entropy_workspace_bytes", rows)
-    launch(ctx, "skv_cross_entropy", out, row, dx, x, t, rows, vocab, float(grad_scale),
+    dev = device_of(ctx)
+    x, rows, vocab, dtype = rows_of(dev, logits, "logits", FLOATS)
+    t = required(dev, targets, "targets", (rows,), I32, 4)
+    out = required(dev, loss, "loss", (1,), F32, 4)
+    dx = operand(dev, grad_logits, "grad_logits", (rows, vocab), (dtype,))
+    row = operand(dev, row_losses, "row_losses", (rows,), F32, 4)
+    ws = workspace(dev, "skv_cross_entropy_workspace_bytes", rows)
+    launch(ctx, dev, "skv_cross_entropy", out, row, dx, x, t, rows, vocab, float(grad_scale),
            ws.data_ptr(), ws.numel(), _lib.dtype_code(dtype))
 
 

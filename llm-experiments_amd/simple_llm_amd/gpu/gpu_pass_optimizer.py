@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .gpu_pass_common import F32, FLOATS, Operand, launch, required, tensor_of
+from .gpu_pass_common import F32, FLOATS, Operand, device_of, launch, required, tensor_of
 from .gpu_types import GPUContext
 
 _CHUNK = 4096  # elements of a tensor that a workgroup takes at a time
@@ -91,17 +91,18 @@ def adamw_create(ctx: GPUContext, params: Sequence[Operand], grads: Sequence[Ope
                              f"{len(given)}")
     if grads is None:
         raise ValueError("grads must have an entry for each of the params")
+    dev = device_of(ctx)
     ps, gs, cs = [], [], []
     for i in range(n):
-        required(ctx, params[i], f"params[{i}]", None, F32, 4)
+        required(dev, params[i], f"params[{i}]", None, F32, 4)
         p = tensor_of(params[i])
         if p.numel() == 0:
             raise ValueError(f"params[{i}] holds no elements")
         ps.append(p)
-        required(ctx, grads[i], f"grads[{i}]", p.shape, FLOATS if i == 0 else (gs[0].dtype,), 2)
+        required(dev, grads[i], f"grads[{i}]", p.shape, FLOATS if i == 0 else (gs[0].dtype,), 2)
         gs.append(tensor_of(grads[i]))
         if copies is not None:
-            required(ctx, copies[i], f"copies[{i}]", p.shape, (torch.bfloat16,), 2)
+            required(dev, copies[i], f"copies[{i}]", p.shape, (torch.bfloat16,), 2)
             cs.append(tensor_of(copies[i]))
     _disjoint([(p, f"params[{i}]", True) for i, p in enumerate(ps)]
               + [(c, f"copies[{i}]", True) for i, c in enumerate(cs)]
@@ -124,8 +125,6 @@ def adamw_create(ctx: GPUContext, params: Sequence[Operand], grads: Sequence[Ope
     which = np.repeat(np.arange(n), counts)
     inside = np.arange(int(counts.sum())) - np.repeat(np.cumsum(counts) - counts, counts)
     chunks = np.stack([which, inside], -1).astype(np.int32)
-
-    dev = ctx.device
 
     def zeros(size: int, dtype: torch.dtype) -> torch.Tensor:
         return torch.zeros(size, dtype=dtype, device=dev)
@@ -155,13 +154,13 @@ def _disjoint(tensors: Sequence[tuple]) -> None:
             written = (hi, name)
 
 
-def _number(ctx: GPUContext, x: Union[float, Operand], name: str) -> tuple:
+def _number(dev: int, x: Union[float, Operand], name: str) -> tuple:
     """(value, None) of a number, (0, its address) of one in device memory."""
     if isinstance(x, (int, float)):
         if not math.isfinite(x):
             raise ValueError(f"{name} must be finite, got {x}")
         return float(x), None
-    return 0.0, required(ctx, x, name, (1,), F32, 4)
+    return 0.0, required(dev, x, name, (1,), F32, 4)
 
 
 def adamw_update(ctx: GPUContext, state: AdamWState, lr: Union[float, Operand],
@@ -181,10 +180,11 @@ def adamw_update(ctx: GPUContext, state: AdamWState, lr: Union[float, Operand],
     if not (math.isfinite(eps) and eps >= 0 and math.isfinite(weight_decay)):
         raise ValueError(f"eps must be finite and >= 0 and weight_decay finite, got {eps} and "
                          f"{weight_decay}")
-    lr, lr_dev = _number(ctx, lr, "lr")
-    grad_scale, scale_dev = _number(ctx, grad_scale, "grad_scale")
+    dev = device_of(ctx)
+    lr, lr_dev = _number(dev, lr, "lr")
+    grad_scale, scale_dev = _number(dev, grad_scale, "grad_scale")
     _check_state(ctx, state)
-    launch(ctx, "skv_adamw", state._tensors.data_ptr(), state._chunks.data_ptr(),
+    launch(ctx, dev, "skv_adamw", state._tensors.data_ptr(), state._chunks.data_ptr(),
            state._chunks.shape[0], state.m.data_ptr(), state.v.data_ptr(), *state._scales(),
            state._count.data_ptr(), state.bits, _lib.dtype_code(state.grads[0].dtype), lr, lr_dev,
            float(beta1), float(beta2), float(eps), float(weight_decay), grad_scale, scale_dev,
@@ -192,7 +192,7 @@ def adamw_update(ctx: GPUContext, state: AdamWState, lr: Union[float, Operand],
 
 
 def _check_state(ctx: GPUContext, state: AdamWState) -> None:
-    if state.m.get_device() != (ctx.device.index or 0):
+    if state.m.get_device() != device_of(ctx):
         raise ValueError(f"the state lives on {state.m.device}, the context on {ctx.device}")
     if [t.data_ptr() for t in state._held] != state._at:
         raise ValueError("a parameter, gradient or copy is no longer where it was when the state "
@@ -204,12 +204,13 @@ def adamw_read(ctx: GPUContext, state: AdamWState, m: Operand, v: Operand) -> No
     exact in either), of the state's elements in the state's order (AdamWState.offsets)."""
     if state.bits != 8:
         raise ValueError("adamw_read reads 8-bit moments; a 32-bit state holds them in m and v")
+    dev = device_of(ctx)
     n = state.m.numel()
-    mo = required(ctx, m, "m", (n,), FLOATS)
+    mo = required(dev, m, "m", (n,), FLOATS)
     dtype = tensor_of(m).dtype
-    vo = required(ctx, v, "v", (n,), (dtype,))
+    vo = required(dev, v, "v", (n,), (dtype,))
     _check_state(ctx, state)
-    launch(ctx, "skv_adamw_read", mo, vo, state.m.data_ptr(), state.v.data_ptr(),
+    launch(ctx, dev, "skv_adamw_read", mo, vo, state.m.data_ptr(), state.v.data_ptr(),
            *state._scales(), n, _lib.dtype_code(dtype))
 
 
