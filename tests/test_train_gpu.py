@@ -821,3 +821,33 @@ def test_offsets_past_32_bits(gpu_ctx):
     ids = torch.arange(rows, device="cuda").int()
     gpu.embedding(gpu_ctx, ids, x, y)
     assert torch.equal(x[-9:], y[-9:]) and torch.equal(x[:9], y[:9])
+
+
+def test_gradients_and_weights_past_32_bits(gpu_ctx):
+    """A table and a tensor of more than 2^31 elements: rows and weights at both ends."""
+    from simple_llm_amd.gpu import gpu
+    vocab, d, n = (1 << 20) + 300, 2050, 777
+    rng = np.random.default_rng(1)
+    ids = np.concatenate([rng.integers(0, 9, n // 2), vocab - 1 - rng.integers(0, 9, n - n // 2)])
+    dy = dev(rng.integers(-3, 4, (n, d)))  # whole numbers: exact sums
+    grad = torch.full((vocab, d), 7.0, device="cuda")
+    gpu.embedding_backward(gpu_ctx, dy, dev(ids, torch.int32), grad)
+    want = torch.zeros(18, d, device="cuda")
+    want.index_add_(0, dev(np.where(ids < 9, ids, 18 + ids - vocab), torch.int64), dy)
+    assert torch.equal(torch.cat([grad[:9], grad[-9:]]), want)
+    assert int((grad[9:-9] != 0).sum()) == 0
+
+    p = grad.view(-1)
+    p.fill_(0.5)
+    size = p.numel()
+    g = torch.empty(size, dtype=BF, device="cuda").normal_()
+    opt = gpu.adamw_create(gpu_ctx, [p], [g])
+    tail = 5000
+    p2, g2 = torch.full((tail,), 0.5, device="cuda"), g[-tail:].clone()
+    small = gpu.adamw_create(gpu_ctx, [p2], [g2])
+    for _ in range(2):
+        gpu.adamw_update(gpu_ctx, opt, 1e-2)
+        gpu.adamw_update(gpu_ctx, small, 1e-2)
+    assert torch.equal(p[-tail:], p2)
+    assert torch.equal(opt.v[size - tail:size], small.v[:tail])
+    assert not (p == 0.5).any()
