@@ -111,6 +111,11 @@ struct Vec {
       for (int i = 0; i < NW; ++i) asm volatile("" : "+v"(w[i]));
     }
   }
+  // The load of the words has ended.
+  __device__ __forceinline__ void arrive() {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) asm volatile("" ::"v"(w[i]));
+  }
   template <typename R>
   static __device__ __forceinline__ R words(const float (&x)[N]) {
     R r;

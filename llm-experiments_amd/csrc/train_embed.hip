@@ -287,33 +287,35 @@ __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
   const bool opened = before == __builtin_amdgcn_readlane(my_id, 0);
   const bool goes_on = __builtin_amdgcn_readlane(my_id, cnt) ==
                        __builtin_amdgcn_readlane(my_id, cnt - 1);
-  if (tile == 0) {
-    int2 on = make_int2(-1, 0);
-    if (goes_on && !(opened && first_end == cnt - 1)) {
-      on.x = __builtin_amdgcn_readlane(my_id, cnt - 1);
-      on.y = (s.begin[on.x + 1] - 1) / kRange - r + 1;
-    }
-    if (lane == 0) s.goes_on[r] = on;
-  }
+  // the row that begins here and goes on, and where its tokens end: used behind the sums
+  const bool begins = goes_on && !(opened && first_end == cnt - 1);
+  const int on = begins ? __builtin_amdgcn_readlane(my_id, cnt - 1) : -1;
+  const int on_end = s.begin[on + 1];
   float acc[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+  // Every load before any store, and waited for together: the compiler cannot count past the
+  // stores, whose branches are taken or not, and would wait for each of them.
   constexpr int U = 8;
+  const int col = here ? c : 0;
   for (int k = 0; k < cnt; k += U) {
     Vec<TY, VEC> v[U];
     Vec<float, VEC> was[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = min(k + u, cnt - 1);
-      const int p = __builtin_amdgcn_readlane(my_pos, i);
-      v[u].zero();
-      was[u].zero();
-      if (here && k + u < cnt) {
-        v[u].template load_row<KIND>(dy + (size_t)p * d, c, d);
-        if (ACC && ((ends >> i) & 1))
-          was[u].template load_row<KIND>(grad + (size_t)__builtin_amdgcn_readlane(my_id, i) * d, c,
+      v[u].template load_row<KIND>(dy + (size_t)__builtin_amdgcn_readlane(my_pos, i) * d, col, d);
+      if constexpr (ACC) {
+        was[u].zero();
+        if ((ends >> i) & 1)
+          was[u].template load_row<KIND>(grad + (size_t)__builtin_amdgcn_readlane(my_id, i) * d, col,
                                         d);
       }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u].arrive();
+      if constexpr (ACC) was[u].arrive();
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -329,9 +331,9 @@ __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
               Vec<float, VEC>::store(part + ((size_t)r * 2 + !head) * dp + c, acc);
             } else {
               float o[VEC];
-              was[u].template settle<KIND>(c, d);
+              if constexpr (ACC) was[u].template settle<KIND>(c, d);
 #pragma unroll
-              for (int e = 0; e < VEC; ++e) o[e] = was[u].get(e) + acc[e] * scale;
+              for (int e = 0; e < VEC; ++e) o[e] = (ACC ? was[u].get(e) : 0.f) + acc[e] * scale;
               Vec<float, VEC>::template store_row<KIND>(
                   grad + (size_t)__builtin_amdgcn_readlane(my_id, i) * d, c, d, o);
             }
@@ -342,6 +344,8 @@ __global__ __launch_bounds__(256) void k_embed_sum(float* __restrict__ grad,
       }
     }
   }
+  if (lane == 0 && tile == 0)
+    s.goes_on[r] = make_int2(on, begins ? (on_end - 1) / kRange - r + 1 : 0);
 }
 
 // grad's row `id`, columns from c on, is (what was there +) scale * sum
