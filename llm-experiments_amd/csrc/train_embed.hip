@@ -44,14 +44,16 @@ constexpr int kZeroGroups = 128;  // workgroups that zero the table
 // lookup
 // ---------------------------------------------------------------------------
 
-// A workgroup's four wavefronts have a token each; VEC columns a lane and step.
-template <typename TT, typename TO, int VEC, int KIND>
+// A token has LPT lanes, a wavefront or, where that leaves a lane two vectors or fewer, a
+// quarter of one (65536 tokens: 64 columns of fp32 11.2 -> 5.7 us, 256 of bf16 14.3 -> 9.0;
+// 256 of fp32 would be 15.2 -> 16.1); VEC columns a lane and step.
+template <typename TT, typename TO, int VEC, int LPT, int KIND>
 __global__ __launch_bounds__(256) void k_embed_rows(TO* __restrict__ out,
                                                     const int32_t* __restrict__ ids,
                                                     const TT* __restrict__ table,
                                                     const float* __restrict__ pos, int T, int V,
                                                     int d, int n_pos, float scale) {
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int i = blockIdx.x * (256 / LPT) + threadIdx.x / LPT, lane = threadIdx.x % LPT;
   if (i >= T) return;
   const int id = ids[i];
   const bool real = (unsigned)id < (unsigned)V;
@@ -59,7 +61,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(TO* __restrict__ out,
   const float* pr = pos ? pos + (size_t)(i % n_pos) * d : nullptr;
   TO* o = out + (size_t)i * d;
 #pragma unroll 4
-  for (int j = lane * VEC; j < d; j += 64 * VEC) {
+  for (int j = lane * VEC; j < d; j += LPT * VEC) {
     Vec<TT, VEC> t;
     Vec<float, VEC> p;
     t.zero();
@@ -461,19 +463,25 @@ extern "C" int skv_embedding_fwd(void* out, const int32_t* ids, const void* tabl
                       {ids, (size_t)T * 4, "tokens"},
                       {pos_table, (size_t)n_pos * d * 4, "pos_table"}}))
     return rc;
-  const unsigned grid = ((unsigned)T + 3) / 4;
   const auto run = [&](auto* o, auto* t) {
     using TO = std::remove_pointer_t<decltype(o)>;
     using TT = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
     constexpr int VEC = sizeof(TT) == 2 && sizeof(TO) == 2 ? 8 : 4;
-    const auto rows = [&](auto KIND) {
-      k_embed_rows<TT, TO, VEC, KIND.value><<<grid, 256, 0, (hipStream_t)stream>>>(
-          o, ids, t, pos_table, T, V, d, n_pos, scale);
+    const auto rows = [&](auto LPT, auto KIND) {
+      constexpr unsigned tokens = 256 / LPT.value;
+      k_embed_rows<TT, TO, VEC, LPT.value, KIND.value>
+          <<<((unsigned)T + tokens - 1) / tokens, 256, 0, (hipStream_t)stream>>>(
+              o, ids, t, pos_table, T, V, d, n_pos, scale);
     };
+    using std::integral_constant;
     const RowKind kind = row_kind(d, VEC);
-    if (kind == kEven) rows(std::integral_constant<int, kEven>{});
-    else if (kind == kOdd) rows(std::integral_constant<int, kOdd>{});
-    else rows(std::integral_constant<int, kTiny>{});
+    const auto with_kind = [&](auto LPT) {
+      if (kind == kEven) rows(LPT, integral_constant<int, kEven>{});
+      else rows(LPT, integral_constant<int, kOdd>{});
+    };
+    if (kind == kTiny) rows(integral_constant<int, 16>{}, integral_constant<int, kTiny>{});
+    else if (d <= 32 * VEC) with_kind(integral_constant<int, 16>{});
+    else with_kind(integral_constant<int, 64>{});
   };
   if (table_dt == SKV_BF16) {
     if (out_dt == SKV_BF16) run((uint16_t*)out, (const uint16_t*)table);
