@@ -7,12 +7,12 @@
 // gradient of 0, and their logits are not read. Bound by HBM: a row is read once
 // into the registers of its workgroup, which takes the maximum, the sum of
 // exponentials and then writes the gradient from them (each exponential is
-// computed twice, which is cheaper than the registers to keep it in). Rows
-// longer than 65536 logits are read a second time.
+// computed twice, which is cheaper than the registers to keep it in). Rows of more
+// than 16384 vectors (131072 logits in bf16, 65536 in fp32) are read a second time.
 //
-// Rows of any length start anywhere in a 16-byte granule: a lane's vectors are
-// the aligned ones inside the row, and the up to 7 + 7 elements before and after
-// them are one element each of the first lanes.
+// Rows of any length start anywhere: a lane's vectors are the aligned ones inside the
+// row, and the up to 63 + 7 elements before and after them are one element each of the
+// first lanes.
 #include "train_common.h"
 
 namespace skv {
@@ -37,6 +37,12 @@ struct LossArgs {
 // Where the wavefronts count the rows themselves: one launch less (255 x 257 fp32: two
 // launches of 2 us instead of three), and at most 4 MB more from L2.
 constexpr int kCountRows = 1024;
+
+// A gradient that the 256 MB of the last-level cache do not hold goes past the caches, and
+// so do its logits (PAST: the nt bit): 8192 x 50304 bf16, 290 us without, 265 with; and with
+// the three products around the loss, 4096 x 50304: 1201 and 1166 us. One that fits is
+// there for the products that read it: 16384 x 5000 with them, 455 us kept and 474 past.
+constexpr size_t kCached = 256u << 20;
 
 __device__ __forceinline__ float row_scale(const LossArgs& a) {
   if (a.inv) return *a.inv;
@@ -86,16 +92,21 @@ __device__ __forceinline__ Stats group_stats(Stats s, float2* sh) {
   return s;
 }
 
-template <typename T>
+// WIDE: on several wavefronts, whose vectors then begin on a cache line, so that no line is
+// in two wavefronts' loads and stores: 8192 x 50257 bf16, 295 us from a 16-byte granule, 278
+// from a line.
+template <typename T, bool WIDE>
 struct Row {
+  static constexpr int kLine = WIDE ? 128 : 16;  // bytes
+  static constexpr int kHead = WIDE ? 64 : 8;    // lanes for the elements before the vectors
   const T* x;   // the row
-  int head;     // elements before its first aligned vector
-  int n_vec;    // aligned vectors
+  int head;     // elements before its first vector
+  int n_vec;    // whole vectors from there
   int tail_at;  // the first element behind them
   __device__ __forceinline__ Row(const T* base, int m, int V) {
     x = base + (size_t)m * V;
-    const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-    head = min(off ? kVec<T> - off : 0, V);
+    const int off = (int)((reinterpret_cast<uintptr_t>(x) & (kLine - 1)) / sizeof(T));
+    head = min(off ? kLine / (int)sizeof(T) - off : 0, V);
     n_vec = (V - head) / kVec<T>;
     tail_at = head + n_vec * kVec<T>;
   }
@@ -110,7 +121,7 @@ struct Row {
   // the single element of thread t, or -1
   __device__ __forceinline__ int edge(int t, int V) const {
     if (t < head) return t;
-    t -= 8;
+    t -= kHead;
     return t >= 0 && t < V - tail_at ? tail_at + t : -1;
   }
 };
@@ -120,12 +131,13 @@ __device__ __forceinline__ float as_f32(uint16_t x) { return bf16_to_f32(x); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(uint16_t* p, float v) { *p = f32_to_bf16(v); }
 
-// The vectors of a lane that every lane has: all but the last three of NV.
+// The vectors of a lane that every lane has: all but the last three of NV (a row of NV or
+// NV - 1 vectors a lane has at most 9 fewer than its length allows).
 constexpr int sure(int NV) { return NV > 3 ? NV - 3 : 0; }
 
 // A row on NW wavefronts, NV vectors a lane, sure(NV) of them without a test for the
 // row's end; with NW = 1 a workgroup has four.
-template <typename T, int NW, int NV, bool GRAD>
+template <typename T, int NW, int NV, bool GRAD, bool PAST>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs a) {
   __shared__ float2 sh[NW];
   constexpr int N = kVec<T>;
@@ -133,7 +145,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
   const int m = NW == 1 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
                         : blockIdx.x;
   if (m >= a.M) return;
-  const Row<T> row((const T*)a.x, m, a.V);
+  const Row<T, (NW > 1)> row((const T*)a.x, m, a.V);
   T* dx = (T*)a.dx + (size_t)m * a.V;
   const int target = a.targets[m], at = row.edge(t, a.V);
   if ((unsigned)target >= (unsigned)a.V) {
@@ -153,7 +165,10 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const unsigned j = i * NW * 64 + t;
-    if (i < sure(NV) || j < (unsigned)row.n_vec) v[i].load(row.vec(row.x, j));
+    if (i < sure(NV) || j < (unsigned)row.n_vec) {
+      if constexpr (PAST) v[i].stream(row.vec(row.x, j));
+      else v[i].load(row.vec(row.x, j));
+    }
   }
   const float edge = at >= 0 ? as_f32(row.x[at]) : 0.f;
   const float picked = as_f32(row.x[target]);
@@ -195,7 +210,8 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
 #pragma unroll
           for (int e = 0; e < N; ++e) o[e] -= first + e == (unsigned)target ? inv : 0.f;
         }
-        Vec<T, N>::store(row.vec(dx, j), o);
+        if constexpr (PAST) Vec<T, N>::store_stream(row.vec(dx, j), o);
+        else Vec<T, N>::store(row.vec(dx, j), o);
       }
     }
     if (at >= 0) put(dx + at, exp_from(edge, top2) * k - (at == target ? inv : 0.f));
@@ -203,12 +219,12 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
 }
 
 // Any length: the row is read for its statistics and again for its gradient.
-template <typename T, bool GRAD>
+template <typename T, bool GRAD, bool PAST>
 __global__ __launch_bounds__(1024) void k_loss_long(LossArgs a) {
   __shared__ float2 sh[16];
   constexpr int N = kVec<T>;
   const int t = threadIdx.x, m = blockIdx.x;
-  const Row<T> row((const T*)a.x, m, a.V);
+  const Row<T, true> row((const T*)a.x, m, a.V);
   T* dx = (T*)a.dx + (size_t)m * a.V;
   const int target = a.targets[m], at = row.edge(t, a.V);
   const bool counts = (unsigned)target < (unsigned)a.V;
@@ -255,7 +271,8 @@ __global__ __launch_bounds__(1024) void k_loss_long(LossArgs a) {
 #pragma unroll
       for (int e = 0; e < N; ++e)
         o[e] = counts ? exp_from(v.get(e), top2) * k - (first + e == (unsigned)target ? inv : 0.f) : 0.f;
-      Vec<T, N>::store(row.vec(dx, j), o);
+      if constexpr (PAST) Vec<T, N>::store_stream(row.vec(dx, j), o);
+      else Vec<T, N>::store(row.vec(dx, j), o);
     }
     if (at >= 0)
       put(dx + at, counts ? exp_from(edge, top2) * k - (at == target ? inv : 0.f) : 0.f);
@@ -316,15 +333,15 @@ __global__ __launch_bounds__(1024) void k_loss_mean(float* __restrict__ loss,
 
 // Wavefronts of a row by its vectors: one up to 4 vectors a lane (no barrier), then 4 and 8
 // up to 8 and 16 up to 16, so that a CU's registers hold many rows in different phases
-// (50304 bf16 logits x 8192: 16 wavefronts of 7 vectors, 290 us, 8 of 13, 295).
+// (50304 bf16 logits x 8192: 16 wavefronts of 7 vectors 290 us, 8 of 13 295, before PAST).
 int waves_of(int n) { return n <= 256 ? 1 : n <= 2048 ? 4 : n <= 4096 ? 8 : 16; }
 
-template <typename T, bool GRAD>
+template <typename T, bool GRAD, bool PAST>
 void launch_rows(const LossArgs& a, hipStream_t s) {
   const int n = (a.V + kVec<T> - 1) / kVec<T>;
   const auto rows = [&](auto NW, auto NV) {
     constexpr int nw = NW.value;
-    k_loss_rows<T, nw, NV.value, GRAD>
+    k_loss_rows<T, nw, NV.value, GRAD, PAST>
         <<<nw == 1 ? (a.M + 3) / 4 : a.M, nw == 1 ? 256 : nw * 64, 0, s>>>(a);
   };
   const auto with = [&](auto NW) {  // even numbers of vectors
@@ -346,7 +363,7 @@ void launch_rows(const LossArgs& a, hipStream_t s) {
   else if (nw == 4) with(integral_constant<int, 4>{});
   else if (nw == 8) with(integral_constant<int, 8>{});
   else if (n <= 16384) with(integral_constant<int, 16>{});
-  else k_loss_long<T, GRAD><<<a.M, 1024, 0, s>>>(a);
+  else k_loss_long<T, GRAD, PAST><<<a.M, 1024, 0, s>>>(a);
 }
 
 }  // namespace
@@ -384,13 +401,14 @@ extern "C" int skv_cross_entropy(float* loss, float* row_loss, void* dx, const v
   LossArgs a = {x, dx, targets, row_loss ? row_loss : inv + 4, M > kCountRows ? inv : nullptr,
                 grad_scale, M, V};
   if (dx && a.inv) k_loss_count<<<1, 1024, 0, s>>>(inv, targets, M, V, grad_scale);
-  if (dt == SKV_BF16) {
-    if (dx) launch_rows<uint16_t, true>(a, s);
-    else launch_rows<uint16_t, false>(a, s);
-  } else {
-    if (dx) launch_rows<float, true>(a, s);
-    else launch_rows<float, false>(a, s);
-  }
+  const auto with = [&](auto* x) {
+    using T = std::remove_pointer_t<decltype(x)>;
+    if (!dx) launch_rows<T, false, false>(a, s);
+    else if (n <= kCached) launch_rows<T, true, false>(a, s);
+    else launch_rows<T, true, true>(a, s);
+  };
+  if (dt == SKV_BF16) with((uint16_t*)dx);
+  else with((float*)dx);
   k_loss_mean<<<1, 1024, 0, s>>>(loss, a.row, targets, M, V);
   return check_launch("skv_cross_entropy");
 }

@@ -392,6 +392,33 @@ def test_cross_entropy_hard_rows(gpu_ctx, vocab):
         assert loss.item() == 0 and not dx.any() and not row.any()
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [(4096, 50257, BF), (2048, 50304, F32), (65536, 4099, BF),
+                                              (1 << 20, 100, F32), (1 << 17, 1001, BF),
+                                              (16384, 9000, BF), (1024, 200000, BF), (512, 200001, F32)])
+def test_cross_entropy_past_the_caches(gpu_ctx, rows, vocab, dtype):
+    """Gradients of more than 256 MB have loads and stores of their own: 64 rows of them equal a
+    call of those rows, bit by bit (row counts and scales are powers of two, and 64 rows on a
+    row begins at the same place of a cache line, which decides the order of its sum)."""
+    from simple_llm_amd.gpu import gpu
+    banner(f"cross_entropy past the caches {rows} x {vocab} {dtype}")
+    x = torch.empty(rows, vocab, dtype=dtype, device="cuda").normal_()
+    t = torch.randint(0, vocab, (rows,), device="cuda").int()
+    dx, loss, row = torch.empty_like(x), torch.empty(1).cuda(), torch.empty(rows).cuda()
+    gpu.cross_entropy_loss(gpu_ctx, x, t, loss, dx, row)
+    part = torch.empty(64, vocab, dtype=dtype, device="cuda")
+    few, one = torch.empty(64).cuda(), torch.empty(1).cuda()
+    for i in (0, rows // 2, rows - 64):
+        gpu.cross_entropy_loss(gpu_ctx, x[i:i + 64].clone(), t[i:i + 64].clone(), one, part, few,
+                               grad_scale=64 / rows)
+        assert torch.equal(dx[i:i + 64], part) and torch.equal(row[i:i + 64], few)
+    within(loss, row.double().mean().cpu().numpy()[None], 2 * U * abs(loss.item()), "loss")
+    t[::3] = -1  # rows that are ignored, and in place
+    want = torch.empty_like(x)
+    gpu.cross_entropy_loss(gpu_ctx, x, t, loss, want)
+    gpu.cross_entropy_loss(gpu_ctx, x, t, loss, x)
+    assert torch.equal(x, want) and not x[::3].any()
+
+
 # ---- AdamW -----------------------------------------------------------------
 
 SIZES = [(3,), (128,), (127, 5), (1,), (2048,), (64, 100), (4096,), (4097,), (129,), (2, 8191)]
