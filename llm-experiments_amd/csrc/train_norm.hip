@@ -8,7 +8,8 @@
 //
 // Both directions are bound by HBM: a row is read once into registers, its sums go over
 // the row's lanes, and the result is written. A row is on 16, 32 or 64 lanes of a wavefront
-// up to 1024 columns (no LDS, no barrier), on 4 wavefronts up to 4096 and on 16 up to 16384.
+// up to 1024 columns (no LDS, no barrier), on 4 wavefronts up to 4096 and on 16 up to 16384;
+// in a bf16 forward of many rows up to 2048 and 8192.
 // 16384 x 1024 bf16 forward: 11.6 us = 5.8 TB/s (its output with the nt bit; 13.0
 // without). 16384 x 768 fp32 backward with a residual: 36.3 us = 5.5 TB/s (rows read with
 // the nt bit; 43.5 without), 4 of them for the weight gradients' second pass. Rows that
@@ -22,7 +23,7 @@ namespace {
 using namespace train;
 
 constexpr int kMaxD = 16384;
-constexpr int kLaneCols = 16;  // columns of a row a lane holds
+constexpr int kLaneCols = 16;  // columns of a row that a lane has
 
 constexpr int bwd_threads(int WPR) { return WPR == 16 ? 1024 : 512; }
 
@@ -315,17 +316,25 @@ int lanes_of(int M, int d) {
   };
   return fits(16) ? 16 : fits(32) ? 32 : 64;
 }
-int waves_of(int d) { return d <= 64 * kLaneCols ? 1 : d <= 256 * kLaneCols ? 4 : 16; }
+// Wavefronts of a row of up to cols columns a lane.
+int waves_of(int d, int cols) { return d <= 64 * cols ? 1 : d <= 256 * cols ? 4 : 16; }
+// Columns that a lane of the forward has: of bf16 twice as many where the rows are enough for
+// eight wavefronts a CU all the same (65536 x 2048: 116 us with 16, 102 with 32; 1500 columns
+// 114 and 86; 200 x 2048 3.1 and 3.6; fp32 gains nothing: 184 and 187). The backward has
+// kLaneCols: what it sums up takes as many registers again.
+int fwd_cols(int M, int d, int dt) {
+  const bool wide = dt == SKV_BF16 && (size_t)M * waves_of(d, 2 * kLaneCols) >= 2048;
+  return wide ? 2 * kLaneCols : kLaneCols;
+}
 // Rows of a workgroup of `threads` lanes.
-int rows_of(int M, int d, int threads) { return threads / (lanes_of(M, d) * waves_of(d)); }
-int fwd_rows(int M, int d) { return rows_of(M, d, waves_of(d) == 16 ? 1024 : 256); }
+int rows_of(int M, int d, int waves, int threads) { return threads / (lanes_of(M, d) * waves); }
 
 // f(vectors of VEC elements a lane, lanes and wavefronts of a row, the rows' kind) as
-// compile-time constants
-template <int VEC, typename F>
-void dispatch(int M, int d, F f) {
+// compile-time constants; MOST: the most vectors a lane.
+template <int VEC, int MOST, typename F>
+void dispatch(int M, int d, int wpr, F f) {
   using std::integral_constant;
-  const int wpr = waves_of(d), lpr = lanes_of(M, d);
+  const int lpr = lanes_of(M, d);
   const int n = (d + lpr * wpr * VEC - 1) / (lpr * wpr * VEC);
   const RowKind kind = row_kind(d, VEC);
   const integral_constant<int, 1> one;
@@ -342,17 +351,17 @@ void dispatch(int M, int d, F f) {
   };
   if (kind == kTiny) return f(one, integral_constant<int, 16>{}, one, integral_constant<int, kTiny>{});
   if (n <= 1) return with_n(one);
-  if constexpr (VEC == 4) {
+  if constexpr (MOST == 4) {
     if (n <= 2) return with_n(integral_constant<int, 2>{});
     if (n <= 3) return with_n(integral_constant<int, 3>{});
   }
-  with_n(integral_constant<int, kLaneCols / VEC>{});
+  with_n(integral_constant<int, MOST>{});
 }
 
 // Workgroups of the backward: one to a CU (each leaves a part of the weight gradients,
 // to be read again), no more than there are rows for.
 int bwd_groups(int M, int d) {
-  const int rows = rows_of(M, d, bwd_threads(waves_of(d)));
+  const int waves = waves_of(d, kLaneCols), rows = rows_of(M, d, waves, bwd_threads(waves));
   const int need = (M + rows - 1) / rows;
   return need < 256 ? need : 256;
 }
@@ -377,8 +386,10 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
                                  int dt, skv_stream_t stream) {
   SKV_REQUIRE(y && x && gamma && beta, SKV_E_INVALID, "skv_layernorm_fwd: null pointer argument");
   if (int rc = check("skv_layernorm_fwd", M, d, dt)) return rc;
-  const unsigned grid = (M + fwd_rows(M, d) - 1) / fwd_rows(M, d);
-  SKV_REQUIRE(launchable(grid, waves_of(d) == 16 ? 1024 : 256), SKV_E_UNSUPPORTED,
+  const int waves = waves_of(d, fwd_cols(M, d, dt)), threads = waves == 16 ? 1024 : 256;
+  const int rows = rows_of(M, d, waves, threads);
+  const unsigned grid = (M + rows - 1) / rows;
+  SKV_REQUIRE(launchable(grid, threads), SKV_E_UNSUPPORTED,
               "skv_layernorm_fwd: %d rows of %d are too many for a launch", M, d);
   SKV_REQUIRE(aligned16(y) && aligned16(x) && aligned16(gamma) && aligned16(beta), SKV_E_INVALID,
               "skv_layernorm_fwd: pointers must be 16-byte aligned");
@@ -390,9 +401,9 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
     return rc;
   const auto run = [&](auto* yt) {
     using T = std::remove_pointer_t<decltype(yt)>;
-    dispatch<16 / sizeof(T)>(M, d, [&](auto N, auto L, auto W, auto KIND) {
+    dispatch<16 / sizeof(T), 4>(M, d, waves, [&](auto N, auto L, auto W, auto KIND) {
       k_ln_fwd<T, N.value, L.value, W.value, KIND.value>
-          <<<grid, W.value == 16 ? 1024 : 256, 0, (hipStream_t)stream>>>(
+          <<<grid, threads, 0, (hipStream_t)stream>>>(
               yt, mean, rstd, (const T*)x, gamma, beta, M, d, eps);
     });
   };
@@ -433,7 +444,9 @@ extern "C" int skv_layernorm_bwd(void* dx, float* dgamma, float* dbeta, const vo
   float* part = (float*)ws;
   const auto run = [&](auto* xt) {
     using T = std::remove_pointer_t<decltype(xt)>;
-    dispatch<16 / sizeof(T)>(M, d, [&](auto N, auto L, auto W, auto KIND) {
+    constexpr int vec = 16 / sizeof(T);
+    dispatch<vec, kLaneCols / vec>(M, d, waves_of(d, kLaneCols), [&](auto N, auto L, auto W,
+                                                                     auto KIND) {
       constexpr int threads = bwd_threads(W.value);
       const auto go = [&](auto RES) {
         k_ln_bwd<T, N.value, L.value, W.value, KIND.value, RES.value>

@@ -281,8 +281,8 @@ def test_c_entry_points_refuse_too_many_rows():
         return L.skv_layernorm_fwd(FAKE, None, None, FAKE, FAKE, FAKE, M, d, 1e-5, 1, None)
 
     # lanes of a row: 16, 32, 64, 256 and 1024
-    for d, lanes in ((1, 16), (256, 16), (257, 32), (512, 32), (513, 64), (1024, 64), (1025, 256),
-                     (4097, 1024)):
+    for d, lanes in ((1, 16), (256, 16), (257, 32), (512, 32), (513, 64), (2048, 64), (2049, 256),
+                     (8192, 256), (8193, 1024)):
         most = ((1 << 32) - 1) // lanes
         for M in (min(most + 1, big), big):
             assert fwd(M, d) == uns, (M, d)
