@@ -8,8 +8,8 @@
 //
 // Both directions are bound by HBM: a row is read once into registers, its sums go over
 // the row's lanes, and the result is written. A row is on 16, 32 or 64 lanes of a wavefront
-// up to 1024 columns (no LDS, no barrier), on 4 wavefronts up to 4096 and on 16 up to 16384;
-// in a bf16 forward of many rows up to 2048 and 8192.
+// up to 1024 columns or, of many rows, 1280 in fp32 and 2048 in bf16 (no LDS, no barrier), on
+// 4 wavefronts up to 4096 (8192 in a bf16 forward), and on 16 up to 16384.
 // 16384 x 1024 bf16 forward: 11.6 us = 5.8 TB/s (its output with the nt bit; 13.0
 // without). 16384 x 768 fp32 backward with a residual: 36.3 us = 5.5 TB/s (rows read with
 // the nt bit; 43.5 without), 4 of them for the weight gradients' second pass. Rows that
@@ -316,22 +316,23 @@ int lanes_of(int M, int d) {
   };
   return fits(16) ? 16 : fits(32) ? 32 : 64;
 }
-// Wavefronts of a row of up to cols columns a lane.
-int waves_of(int d, int cols) { return d <= 64 * cols ? 1 : d <= 256 * cols ? 4 : 16; }
-// Columns that a lane of the forward has: of bf16 twice as many where the rows are enough for
-// eight wavefronts a CU all the same (65536 x 2048: 116 us with 16, 102 with 32; 1500 columns
-// 114 and 86; 200 x 2048 3.1 and 3.6; fp32 gains nothing: 184 and 187). The backward has
-// kLaneCols: what it sums up takes as many registers again.
-int fwd_cols(int M, int d, int dt) {
-  const bool wide = dt == SKV_BF16 && (size_t)M * waves_of(d, 2 * kLaneCols) >= 2048;
-  return wide ? 2 * kLaneCols : kLaneCols;
+// Wavefronts of a row: 1, 4 or 16, by kLaneCols columns a lane. Where the rows are enough for
+// eight wavefronts a CU all the same, a lane has more of them: on one wavefront 32 columns of
+// bf16 and 20 of fp32 (backward, 65536 rows: 1500 of bf16 198 us on four and 121 on one, 2048
+// of bf16 175 and 132, 1025 of fp32 195 and 141, but 1536 of fp32 224 and 243; forward: 114 and
+// 87, 116 and 102, 139 and 109, 152 and 156), and in the forward 32 of bf16 on four (16384 x
+// 5000: 102 us on sixteen, 72; the backward gains nothing).
+int waves_of(int M, int d, int dt, bool forward) {
+  const bool wide = dt == SKV_BF16;
+  if (d <= (M < 2048 ? 64 * kLaneCols : wide ? 128 * kLaneCols : 80 * kLaneCols)) return 1;
+  return d <= (forward && wide && M >= 512 ? 512 : 256) * kLaneCols ? 4 : 16;
 }
 // Rows of a workgroup of `threads` lanes.
 int rows_of(int M, int d, int waves, int threads) { return threads / (lanes_of(M, d) * waves); }
 
 // f(vectors of VEC elements a lane, lanes and wavefronts of a row, the rows' kind) as
-// compile-time constants; MOST: the most vectors a lane.
-template <int VEC, int MOST, typename F>
+// compile-time constants. MANY: the most vectors a lane of rows on four wavefronts.
+template <int VEC, int MANY, typename F>
 void dispatch(int M, int d, int wpr, F f) {
   using std::integral_constant;
   const int lpr = lanes_of(M, d);
@@ -342,26 +343,42 @@ void dispatch(int M, int d, int wpr, F f) {
     if (kind == kEven) f(N, L, W, integral_constant<int, kEven>{});
     else f(N, L, W, integral_constant<int, kOdd>{});
   };
-  const auto with_n = [&](auto N) {
-    if (lpr == 16) with_kind(N, integral_constant<int, 16>{}, one);
-    else if (lpr == 32) with_kind(N, integral_constant<int, 32>{}, one);
-    else if (wpr == 1) with_kind(N, integral_constant<int, 64>{}, one);
-    else if (wpr == 4) with_kind(N, integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    else with_kind(N, integral_constant<int, 64>{}, integral_constant<int, 16>{});
+  // run(the row's vectors a lane), MOST (2 or 4) or fewer
+  const auto few = [&](auto MOST, auto run) {
+    if (n <= 1) return run(one);
+    if constexpr (MOST.value > 2) {
+      if (n <= 2) return run(integral_constant<int, 2>{});
+      if (n <= 3) return run(integral_constant<int, 3>{});
+    }
+    run(MOST);
   };
+  const integral_constant<int, kLaneCols / VEC> most;
   if (kind == kTiny) return f(one, integral_constant<int, 16>{}, one, integral_constant<int, kTiny>{});
-  if (n <= 1) return with_n(one);
-  if constexpr (MOST == 4) {
-    if (n <= 2) return with_n(integral_constant<int, 2>{});
-    if (n <= 3) return with_n(integral_constant<int, 3>{});
+  if (lpr == 16) {
+    few(most, [&](auto N) { with_kind(N, integral_constant<int, 16>{}, one); });
+  } else if (lpr == 32) {
+    few(most, [&](auto N) { with_kind(N, integral_constant<int, 32>{}, one); });
+  } else if (wpr == 1) {
+    const integral_constant<int, 64> L;
+    if constexpr (VEC == 4) {
+      if (n > 4) return with_kind(integral_constant<int, 5>{}, L, one);
+    }
+    few(integral_constant<int, 4>{}, [&](auto N) { with_kind(N, L, one); });
+  } else if (wpr == 4) {
+    few(integral_constant<int, MANY>{}, [&](auto N) {
+      with_kind(N, integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    });
+  } else {
+    few(most, [&](auto N) {
+      with_kind(N, integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    });
   }
-  with_n(integral_constant<int, MOST>{});
 }
 
 // Workgroups of the backward: one to a CU (each leaves a part of the weight gradients,
 // to be read again), no more than there are rows for.
-int bwd_groups(int M, int d) {
-  const int waves = waves_of(d, kLaneCols), rows = rows_of(M, d, waves, bwd_threads(waves));
+int bwd_groups(int M, int d, int dt) {
+  const int waves = waves_of(M, d, dt, false), rows = rows_of(M, d, waves, bwd_threads(waves));
   const int need = (M + rows - 1) / rows;
   return need < 256 ? need : 256;
 }
@@ -386,7 +403,7 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
                                  int dt, skv_stream_t stream) {
   SKV_REQUIRE(y && x && gamma && beta, SKV_E_INVALID, "skv_layernorm_fwd: null pointer argument");
   if (int rc = check("skv_layernorm_fwd", M, d, dt)) return rc;
-  const int waves = waves_of(d, fwd_cols(M, d, dt)), threads = waves == 16 ? 1024 : 256;
+  const int waves = waves_of(M, d, dt, true), threads = waves == 16 ? 1024 : 256;
   const int rows = rows_of(M, d, waves, threads);
   const unsigned grid = (M + rows - 1) / rows;
   SKV_REQUIRE(launchable(grid, threads), SKV_E_UNSUPPORTED,
@@ -414,7 +431,8 @@ extern "C" int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* 
 
 extern "C" size_t skv_layernorm_bwd_workspace_bytes(int M, int d) {
   if (M <= 0 || M > kMaxRows || d <= 0 || d > kMaxD) return 0;
-  return (size_t)bwd_groups(M, d) * 2 * padded(d) * sizeof(float);
+  // 256 for both types where their wavefronts differ, from 2048 rows on
+  return (size_t)bwd_groups(M, d, SKV_F32) * 2 * padded(d) * sizeof(float);
 }
 
 extern "C" int skv_layernorm_bwd(void* dx, float* dgamma, float* dbeta, const void* dy,
@@ -440,13 +458,13 @@ extern "C" int skv_layernorm_bwd(void* dx, float* dgamma, float* dbeta, const vo
                       {residual, act, "residual", 0}, {gamma, col, "gamma"}, {mean, row, "mean"},
                       {rstd, row, "rstd"}}))
     return rc;
-  const int P = bwd_groups(M, d), dp = padded(d);
+  const int P = bwd_groups(M, d, dt), dp = padded(d);
   float* part = (float*)ws;
   const auto run = [&](auto* xt) {
     using T = std::remove_pointer_t<decltype(xt)>;
     constexpr int vec = 16 / sizeof(T);
-    dispatch<vec, kLaneCols / vec>(M, d, waves_of(d, kLaneCols), [&](auto N, auto L, auto W,
-                                                                     auto KIND) {
+    dispatch<vec, kLaneCols / vec>(M, d, waves_of(M, d, dt, false), [&](auto N, auto L, auto W,
+                                                                       auto KIND) {
       constexpr int threads = bwd_threads(W.value);
       const auto go = [&](auto RES) {
         k_ln_bwd<T, N.value, L.value, W.value, KIND.value, RES.value>

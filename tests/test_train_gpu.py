@@ -62,7 +62,8 @@ NORM = [(1, 1), (1, 8), (3, 2), (5, 7), (4, 64), (130, 390), (33, 513), (257, 76
 # Rows on 16, 32 and 64 lanes, and on both sides of where their number or width changes that.
 MANY = [(5000, 96), (8191, 129), (8193, 200), (8192, 256), (4095, 257), (4097, 300), (4096, 511),
         (4100, 512), (4100, 513), (9000, 7), (2047, 1500), (2048, 1025), (2050, 1500), (2049, 2047),
-        (2048, 2048), (511, 5000), (512, 5003), (513, 8192)]
+        (2048, 2048), (511, 5000), (512, 5003), (513, 8192), (2047, 1280), (2048, 1280), (2060, 1279),
+        (2048, 1281)]
 
 
 def norm_inputs(rows, d, dtype, offset=0.5):
