@@ -711,7 +711,8 @@ int skv_flash_bwd(float* dq, float* dk, float* dv, const float* q, const float* 
  * weights, their gradients and row statistics are fp32. Sums run in a fixed
  * order without atomics: results are bitwise reproducible. Buffers are
  * contiguous and 16-byte aligned unless noted; workspaces need no contents, and
- * calls that share one must be stream ordered.
+ * calls that share one must be stream ordered. More rows than a launch can have
+ * (2^32 lanes; 16 to 1024 lanes a row by its width, and 2^30 rows) are refused.
  * ------------------------------------------------------------------------ */
 
 /* y = (x - mean) rstd gamma + beta of every row, rstd = 1 / sqrt(var + eps),
@@ -753,7 +754,7 @@ size_t skv_embedding_bwd_workspace_bytes(int T, int V, int d);
  * of grad [V, d] fp32; with accumulate != 0 added to the rows that have tokens, and
  * the others are left alone (the reference's embedding_backward and its reduction,
  * gpu_pass_backward.py:183-240, gpu_kernels.py:2946-3068). dout: [T, d] of dt. An
- * id outside [0, V) adds nothing. T, V <= 2^30. */
+ * id outside [0, V) adds nothing. d <= 2^22, V <= 2^29, T ceil(d / 256) <= 2^30. */
 int skv_embedding_bwd(float* grad, const void* dout, const int32_t* ids, int T, int V, int d,
                       float scale, int accumulate, void* ws, size_t ws_bytes, int dt,
                       skv_stream_t stream);
