@@ -54,27 +54,19 @@ __device__ __forceinline__ float row_scale(const LossArgs& a) {
   return a.grad_scale / (float)max(n, 1);
 }
 
-// 2^(x log2(e) - top2), the difference rounded once
-__device__ __forceinline__ float exp_from(float x, float top2) {
-  return fast_exp2(fmaf(x, LOG2E, -top2));
+// e^(x - from). The difference comes first: with finite logits of any size it is 0 at x =
+// from and overflows to -inf only. (The product with log2(e) first, one operation less,
+// leaves up to 2^-25 of itself where it is rounded, which 2^x cannot take from 3e9 on.)
+__device__ __forceinline__ float exp_from(float x, float from) {
+  return fast_exp2((x - from) * LOG2E);
 }
 
-// top + log of the sum of exp(x - top) - picked, from the sum over exp_from: top2
-// is top log2(e) rounded, and what the rounding left is taken out again.
-__device__ __forceinline__ float loss_of(float top, float top2, float sum, float picked) {
-  return (top - picked) + (logf(sum) - fmaf(top, LOG2E, -top2) * LN2);
-}
-
-// A maximum and the sum of 2^(x log2(e) - ref2) of what a wavefront has seen. ref2
-// is top log2(e) rounded, or 0 where top is -inf (nothing seen, or only NaN).
+// A maximum and the sum of e^(x - ref) of what a wavefront has seen. ref is top, or 0
+// where top is -inf (nothing seen, or only NaN).
 struct Stats {
   float top, sum;
 };
-__device__ __forceinline__ float ref2_of(float top) {
-#pragma clang fp contract(off)  // rounded on its own, wherever it is used
-  const float r = top * LOG2E;
-  return top == -INFINITY ? 0.f : r;
-}
+__device__ __forceinline__ float ref_of(float top) { return top == -INFINITY ? 0.f : top; }
 
 // The statistics of the workgroup's NW wavefronts: one barrier, and then a lane has
 // those of wavefront lane % NW (so a row of 16 lanes has each 16 / NW times).
@@ -86,7 +78,7 @@ __device__ __forceinline__ Stats group_stats(Stats s, float2* sh) {
     const float2 o = sh[threadIdx.x % NW];
     s.top = row16_max(o.x);
     // a NaN sum stays one under a factor of 0
-    const float f = o.x == -INFINITY ? 0.f : fast_exp2(ref2_of(o.x) - ref2_of(s.top));
+    const float f = o.x == -INFINITY ? 0.f : exp_from(o.x, s.top);
     s.sum = row16_sum(o.y * f) * (NW / 16.f);
   }
   return s;
@@ -181,19 +173,18 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
       for (int e = 0; e < N; ++e) top = fmaxf(top, v[i].get(e));
     }
   top = wave_max(top);
-  const float ref2 = ref2_of(top);
-  float sum = at >= 0 ? exp_from(edge, ref2) : 0.f;
+  const float ref = ref_of(top);
+  float sum = at >= 0 ? exp_from(edge, ref) : 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     v[i].keep();
     if (i < sure(NV) || i * NW * 64 + t < row.n_vec) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += exp_from(v[i].get(e), ref2);
+      for (int e = 0; e < N; ++e) sum += exp_from(v[i].get(e), ref);
     }
   }
   const Stats s = group_stats<NW>({top, wave_sum(sum)}, sh);
-  const float top2 = s.top == -INFINITY ? -INFINITY : ref2_of(s.top);  // NaN where all is -inf
-  if (t == 0) a.row[m] = loss_of(s.top, top2, s.sum, picked);
+  if (t == 0) a.row[m] = (s.top - picked) + logf(s.sum);  // NaN where all is -inf
   if constexpr (GRAD) {
     const float k = inv / s.sum;
 #pragma unroll
@@ -205,7 +196,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
         const unsigned first = row.head + j * N;
         float o[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = exp_from(v[i].get(e), top2) * k;
+        for (int e = 0; e < N; ++e) o[e] = exp_from(v[i].get(e), s.top) * k;
         if ((unsigned)target - first < (unsigned)N) {
 #pragma unroll
           for (int e = 0; e < N; ++e) o[e] -= first + e == (unsigned)target ? inv : 0.f;
@@ -214,7 +205,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void k_loss_rows(LossArgs 
         else Vec<T, N>::store(row.vec(dx, j), o);
       }
     }
-    if (at >= 0) put(dx + at, exp_from(edge, top2) * k - (at == target ? inv : 0.f));
+    if (at >= 0) put(dx + at, exp_from(edge, s.top) * k - (at == target ? inv : 0.f));
   }
 }
 
@@ -230,12 +221,12 @@ __global__ __launch_bounds__(1024) void k_loss_long(LossArgs a) {
   const bool counts = (unsigned)target < (unsigned)a.V;
   const float inv = GRAD && counts ? row_scale(a) : 0.f;
   const float edge = at >= 0 ? as_f32(row.x[at]) : 0.f;
-  float top2 = 0.f, k = 0.f;
+  float whole = 0.f, k = 0.f;  // the row's maximum, the gradient's factor
   if (counts) {
     const float picked = as_f32(row.x[target]);
     // a lane's sum is taken on to a larger maximum where its vectors have one
-    float top = at >= 0 ? edge : -INFINITY, ref2 = ref2_of(top);
-    float sum = at >= 0 ? exp_from(edge, ref2) : 0.f;
+    float top = at >= 0 ? edge : -INFINITY, ref = ref_of(top);
+    float sum = at >= 0 ? exp_from(edge, ref) : 0.f;
 #pragma unroll 4
     for (unsigned j = t; j < (unsigned)row.n_vec; j += 1024) {
       Vec<T, N> v;
@@ -244,19 +235,17 @@ __global__ __launch_bounds__(1024) void k_loss_long(LossArgs a) {
 #pragma unroll
       for (int e = 0; e < N; ++e) most = fmaxf(most, v.get(e));
       if (most > top) {
-        const float to2 = ref2_of(most);
-        sum *= top == -INFINITY ? 1.f : fast_exp2(ref2 - to2);
-        top = most;
-        ref2 = to2;
+        sum *= top == -INFINITY ? 1.f : exp_from(top, most);
+        top = ref = most;
       }
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += exp_from(v.get(e), ref2);
+      for (int e = 0; e < N; ++e) sum += exp_from(v.get(e), ref);
     }
-    const float wtop = wave_max(top), wref2 = ref2_of(wtop);
-    sum *= top == -INFINITY ? 1.f : fast_exp2(ref2 - wref2);
+    const float wtop = wave_max(top);
+    sum *= top == -INFINITY ? 1.f : exp_from(top, wtop);
     const Stats s = group_stats<16>({wtop, wave_sum(sum)}, sh);
-    top2 = s.top == -INFINITY ? -INFINITY : ref2_of(s.top);
-    if (t == 0) a.row[m] = loss_of(s.top, top2, s.sum, picked);
+    whole = s.top;
+    if (t == 0) a.row[m] = (s.top - picked) + logf(s.sum);
     k = inv / s.sum;
   } else if (t == 0) {
     a.row[m] = 0.f;
@@ -270,12 +259,12 @@ __global__ __launch_bounds__(1024) void k_loss_long(LossArgs a) {
       v.load(row.vec(row.x, j));
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        o[e] = counts ? exp_from(v.get(e), top2) * k - (first + e == (unsigned)target ? inv : 0.f) : 0.f;
+        o[e] = counts ? exp_from(v.get(e), whole) * k - (first + e == (unsigned)target ? inv : 0.f) : 0.f;
       if constexpr (PAST) Vec<T, N>::store_stream(row.vec(dx, j), o);
       else Vec<T, N>::store(row.vec(dx, j), o);
     }
     if (at >= 0)
-      put(dx + at, counts ? exp_from(edge, top2) * k - (at == target ? inv : 0.f) : 0.f);
+      put(dx + at, counts ? exp_from(edge, whole) * k - (at == target ? inv : 0.f) : 0.f);
   }
 }
 

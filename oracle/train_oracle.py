@@ -61,7 +61,8 @@ def cross_entropy(x, targets, grad_scale=1.0):
         top = x.max(-1, keepdims=True)
         e = np.exp(x - top)
         total = e.sum(-1, keepdims=True)
-        row = (top + np.log(total))[:, 0] - x[np.arange(rows), at]
+        # the difference first: 1e30 + log(vocab) is 1e30 in 64 bits too
+        row = (top[:, 0] - x[np.arange(rows), at]) + np.log(total)[:, 0]
         p = e / total
     p[np.arange(rows), at] -= 1
     count = max(1, int(real.sum()))

@@ -1,0 +1,108 @@
+"""The training operators at the ends of their number ranges and sizes, on the MI355X
+against oracle/train_oracle.py (float64). u = 2^-24 is half a step of fp32."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import banner
+from oracle import train_oracle as to
+from test_train_gpu import BF, F32, HYPER, U, dev, g64, half_step, p_tol, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- cross-entropy: large finite logits --------------------------------------
+
+# A vocabulary for every number of wavefronts a row (1, 4, 8, 16), and two that are read
+# twice: of whole vectors, and ending inside one.
+VOCABS = [(v, F32) for v in (1000, 5003, 16001, 50257, 70000, 70001)] + [
+    (v, BF) for v in (2001, 10007, 30001, 100003, 140000, 140001)]
+
+
+def loss_bounds(x, t, scale):
+    """(bound of dx, of the rows' losses, of the loss), absolute.
+
+    An exponential e^-r: the difference from the maximum is rounded, log2(e) is, and their
+    product: 2.3 r u; the instruction 2 u. A logit reaches its row's sum by at most three
+    such factors (to its lane's, its wavefront's and the row's maximum, whose r add up): 6 u
+    and a product's rounding each, 3 u. The sum: at most 129 additions in a lane, or a row's
+    1024th part and a vector and an edge; 6 over a wavefront, 4 over the wavefronts. Then
+    1 / count, 1 / sum and two products: 4 u."""
+    x = g64(x)
+    rows = np.arange(len(x))
+    real = (t >= 0) & (t < x.shape[1])
+    at = np.where(real, t, 0)
+    top = x.max(-1, keepdims=True)
+    r = top - x
+    with np.errstate(under="ignore"):
+        p = np.exp(-r)
+    total = p.sum(-1, keepdims=True)
+    p /= total
+    of_sum = 2.3 * (p * r).sum(-1) + 9 + max(129, x.shape[1] / 1024 + 9) + 10
+    inv = scale / max(1, int(real.sum()))
+    dx = U * inv * p * (2.3 * r + 2 + of_sum[:, None] + 4)
+    dx[rows, at] += U * inv  # p inv - inv: the latter's rounding, and that of the difference
+    dx += U * inv * np.abs(p - (np.arange(x.shape[1]) == at[:, None]))
+    dx[~real] = 0
+    picked = top[:, 0] - x[rows, at]
+    row = U * (picked + of_sum + 2 * np.log(total[:, 0]) + (picked + np.log(total[:, 0])))
+    row[~real] = 0
+    return dx, row, row.sum() / max(1, int(real.sum()))
+
+
+def masked_rows(rng, vocab, mask):
+    """Logits with masked places of one large value, and targets: an allowed part of 300 at
+    either end and inside, an unused end, one allowed place, a masked target, a row of
+    nothing but the mask, one of nothing but its opposite, and an ignored row."""
+    x = 3 * rng.standard_normal((9, vocab))
+    n = min(300, vocab // 3)
+    mid = vocab // 2 + 5
+    x[0, n:] = x[1, :-n] = mask
+    x[2, :mid] = x[2, mid + n:] = mask
+    x[3, -(vocab // 20):] = mask
+    x[4, :] = mask
+    x[4, vocab // 3] = 1.5
+    x[5, ::2] = mask
+    x[6, :] = mask
+    x[7, :] = -mask
+    t = np.array([n - 1, vocab - n, mid, 7, vocab // 3, 2, vocab - 1, 3, -100], np.int32)
+    return x, t
+
+
+@pytest.mark.parametrize("vocab,dtype", VOCABS)
+def test_cross_entropy_of_finite_masks(gpu_ctx, vocab, dtype):
+    from simple_llm_amd.gpu import gpu
+    rng = np.random.default_rng(vocab)
+    most = torch.finfo(dtype).max
+    for mask in (-1e9, -1e10, -2e10, -1e30, -0.7 * most, -most):
+        banner(f"cross_entropy {vocab} {dtype} mask {mask:.3g}")
+        x, t = masked_rows(rng, vocab, mask)
+        x, td = dev(x, dtype), dev(t, torch.int32)
+        loss, row, dx = torch.empty(1).cuda(), torch.empty(9).cuda(), torch.empty_like(x)
+        gpu.cross_entropy_loss(gpu_ctx, x, td, loss, dx, row, grad_scale=0.5)
+        wl, wr, wx = to.cross_entropy(g64(x), t, 0.5)
+        assert np.isfinite(wx).all() and np.isfinite(wr).all()
+        tx, tr, tl = loss_bounds(x, t, 0.5)
+        within(dx, wx, tx + half_step(dtype) * (np.abs(wx) + tx), f"mask {mask:.3g} dx")
+        within(row, wr, tr, f"mask {mask:.3g} rows")
+        within(loss, np.array([wl]), tl + U * abs(wl), f"mask {mask:.3g} loss")
+        only, into = torch.empty(1).cuda(), x.clone()
+        gpu.cross_entropy_loss(gpu_ctx, x, td, only)
+        gpu.cross_entropy_loss(gpu_ctx, into, td, loss, into, grad_scale=0.5)
+        assert torch.equal(only, loss) and torch.equal(into, dx)
+
+
+def test_cross_entropy_of_finite_masks_past_the_caches(gpu_ctx):
+    """More than 256 MB of gradients: the rows of a small call, bit by bit."""
+    from simple_llm_amd.gpu import gpu
+    rng = np.random.default_rng(0)
+    x, t = masked_rows(rng, 50304, torch.finfo(F32).min)
+    x, t = dev(x[:8]).repeat(256, 1), dev(t[:8], torch.int32).repeat(256)
+    dx, part = torch.empty_like(x), torch.empty(8, 50304, device="cuda")
+    loss, one = torch.empty(1).cuda(), torch.empty(1).cuda()
+    gpu.cross_entropy_loss(gpu_ctx, x, t, loss, dx)
+    gpu.cross_entropy_loss(gpu_ctx, x[:8].clone(), t[:8].clone(), one, part, grad_scale=8 / 2048)
+    assert part.isfinite().all() and torch.equal(loss, one)
+    assert torch.equal(dx, part.repeat(256, 1))
