@@ -86,7 +86,9 @@ __device__ __forceinline__ Stats group_stats(Stats s, float2* sh) {
 
 // WIDE: on several wavefronts, whose vectors then begin on a cache line, so that no line is
 // in two wavefronts' loads and stores: 8192 x 50257 bf16, 295 us from a 16-byte granule, 278
-// from a line.
+// from a line. Lines are counted from the first row, not from address 0: which elements are
+// summed together, and so the result's bits, depend on sizes alone. (Where the logits
+// themselves begin inside a line, the vectors do too.)
 template <typename T, bool WIDE>
 struct Row {
   static constexpr int kLine = WIDE ? 128 : 16;  // bytes
@@ -97,7 +99,8 @@ struct Row {
   int tail_at;  // the first element behind them
   __device__ __forceinline__ Row(const T* base, int m, int V) {
     x = base + (size_t)m * V;
-    const int off = (int)((reinterpret_cast<uintptr_t>(x) & (kLine - 1)) / sizeof(T));
+    const size_t from = WIDE ? (size_t)m * V * sizeof(T) : reinterpret_cast<uintptr_t>(x);
+    const int off = (int)((from & (kLine - 1)) / sizeof(T));
     head = min(off ? kLine / (int)sizeof(T) - off : 0, V);
     n_vec = (V - head) / kVec<T>;
     tail_at = head + n_vec * kVec<T>;

@@ -106,3 +106,22 @@ def test_cross_entropy_of_finite_masks_past_the_caches(gpu_ctx):
     gpu.cross_entropy_loss(gpu_ctx, x[:8].clone(), t[:8].clone(), one, part, grad_scale=8 / 2048)
     assert part.isfinite().all() and torch.equal(loss, one)
     assert torch.equal(dx, part.repeat(256, 1))
+
+
+@pytest.mark.parametrize("vocab,dtype", VOCABS)
+def test_cross_entropy_bits_do_not_depend_on_addresses(gpu_ctx, vocab, dtype):
+    """The same logits at every 16-byte granule of a cache line."""
+    from simple_llm_amd.gpu import gpu
+    x = torch.randn(9, vocab, device="cuda").to(dtype)
+    t = torch.arange(9, device="cuda").int()
+    want = None
+    for k in range(8):
+        banner(f"cross_entropy {vocab} {dtype} {16 * k} bytes on")
+        at = 16 * k // x.element_size()
+        here = torch.empty(9 * vocab + at, dtype=dtype, device="cuda")[at:].view(9, vocab).copy_(x)
+        loss, row, dx = torch.empty(1).cuda(), torch.empty(9).cuda(), torch.empty_like(x)
+        gpu.cross_entropy_loss(gpu_ctx, here, t, loss, dx, row)
+        gpu.cross_entropy_loss(gpu_ctx, here, t, loss, here)
+        got = (loss, row, dx, here.clone())
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
