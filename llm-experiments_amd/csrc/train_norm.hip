@@ -118,7 +118,8 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_fwd(
   }
   row_sums<LPR, WPR, kThreads>(s, q, sh, turn);
   const float c = s / fd;
-  const float rstd = 1.f / sqrtf(fmaxf(q / fd - c * c, 0.f) + eps);
+  const float var = q / fd - c * c;
+  const float rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);  // a NaN stays one
   if (P::lane() == 0) {
     if (mean_out) mean_out[m] = mean + c;
     if (rstd_out) rstd_out[m] = rstd;

@@ -8,7 +8,7 @@ import torch
 
 from conftest import banner
 from oracle import train_oracle as to
-from test_train_gpu import BF, F32, HYPER, U, dev, g64, half_step, p_tol, within
+from test_train_gpu import BF, F32, U, dev, g64, half_step, norm_inputs, within
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +125,23 @@ def test_cross_entropy_bits_do_not_depend_on_addresses(gpu_ctx, vocab, dtype):
         got = (loss, row, dx, here.clone())
         want = want or got
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- LayerNorm: bad rows, rows that end inside a vector ------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_layernorm_of_a_bad_row(gpu_ctx, bad, dtype):
+    """One NaN or infinity: the row's output and rstd are NaN, and no other row changes."""
+    from simple_llm_amd.gpu import gpu
+    for d in (3, 300, 2000, 6000, 16384):
+        banner(f"layernorm 9 x {d} {dtype} with {bad}")
+        _, x, gamma, beta = norm_inputs(9, d, dtype)
+        (y, mean, rstd), clean = ((torch.empty_like(x), torch.empty(9).cuda(), torch.empty(9).cuda())
+                                  for _ in range(2))
+        gpu.layernorm(gpu_ctx, x, gamma, beta, *clean)
+        x[4, d // 2] = bad
+        gpu.layernorm(gpu_ctx, x, gamma, beta, y, mean, rstd)
+        assert y[4].isnan().all() and rstd[4].isnan()
+        keep = torch.arange(9) != 4
+        assert all(torch.equal(a[keep], b[keep]) for a, b in zip((y, mean, rstd), clean))
