@@ -121,7 +121,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void k_ln_fwd(
   const float var = q / fd - c * c;
   const float rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);  // a NaN stays one
   if (P::lane() == 0) {
-    if (mean_out) mean_out[m] = mean + c;
+    if (mean_out) mean_out[m] = c == c ? mean + c : mean;  // an infinite mean has no deviations
     if (rstd_out) rstd_out[m] = rstd;
   }
   T* yr = y + (size_t)m * d;

@@ -145,3 +145,19 @@ def test_layernorm_of_a_bad_row(gpu_ctx, bad, dtype):
         assert y[4].isnan().all() and rstd[4].isnan()
         keep = torch.arange(9) != 4
         assert all(torch.equal(a[keep], b[keep]) for a, b in zip((y, mean, rstd), clean))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_layernorm_mean_of_a_bad_row(gpu_ctx, dtype):
+    """The mean of a row with an infinity is that infinity, of one with a NaN, or with
+    infinities of both signs, NaN."""
+    from simple_llm_amd.gpu import gpu
+    inf, nan = float("inf"), float("nan")
+    for d in (3, 300, 2000, 6000):
+        _, x, gamma, beta = norm_inputs(4, d, dtype)
+        x[0, d - 1], x[1, 0], x[2, d // 2] = inf, -inf, nan
+        x[3, 0], x[3, 1] = inf, -inf
+        y, mean, rstd = torch.empty_like(x), torch.empty(4).cuda(), torch.empty(4).cuda()
+        gpu.layernorm(gpu_ctx, x, gamma, beta, y, mean, rstd)
+        np.testing.assert_array_equal(g64(mean), [inf, -inf, nan, nan])
+        assert rstd.isnan().all() and y.isnan().all()
