@@ -201,7 +201,8 @@ __global__ __launch_bounds__(bwd_threads(WPR)) void k_ln_bwd(
           const float xh = (vx[i].get(e) - mu) * rs, t = vy[i].get(e);
           const float g = t * ga[i][e];
           a += g;
-          b += g * xh;
+          // past the row's end, in its last vectors, g is 0 but xh may be infinite
+          if (KIND == kEven || i < NCH - 1 || c0 + i * kStep + e < d) b += g * xh;
           sg[i][e] += t * xh;
           sb[i][e] += t;
         }
@@ -331,7 +332,7 @@ int waves_of(int M, int d, int dt, bool forward) {
 // Rows of a workgroup of `threads` lanes.
 int rows_of(int M, int d, int waves, int threads) { return threads / (lanes_of(M, d) * waves); }
 
-// f(vectors of VEC elements a lane, lanes and wavefronts of a row, the rows' kind) as
+// f(vectors of VEC elements a lane, exactly, lanes and wavefronts of a row, the rows' kind) as
 // compile-time constants. MANY: the most vectors a lane of rows on four wavefronts.
 template <int VEC, int MANY, typename F>
 void dispatch(int M, int d, int wpr, F f) {

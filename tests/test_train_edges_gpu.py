@@ -161,3 +161,29 @@ def test_layernorm_mean_of_a_bad_row(gpu_ctx, dtype):
         gpu.layernorm(gpu_ctx, x, gamma, beta, y, mean, rstd)
         np.testing.assert_array_equal(g64(mean), [inf, -inf, nan, nan])
         assert rstd.isnan().all() and y.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("d", [2, 7, 30, 257, 1027, 4099])
+def test_layernorm_backward_of_constant_rows_far_out(gpu_ctx, d, dtype):
+    """Rows of one value whose product with rstd overflows: xh is 0 in every column, so dx =
+    rstd (g - mean(g)), and dgamma gets nothing from them; also where rows end inside a
+    vector."""
+    from simple_llm_amd.gpu import gpu
+    banner(f"layernorm_backward of constant rows, {d} {dtype}")
+    rng = np.random.default_rng(d)
+    x = torch.full((5, d), 2.0 ** 121, dtype=dtype, device="cuda")
+    gamma = dev(1 + 0.3 * rng.standard_normal(d))
+    dy = dev(rng.standard_normal((5, d)), dtype)
+    mean, rstd = torch.full((5,), 2.0 ** 121).cuda(), torch.full((5,), 256.0).cuda()
+    dx, dg, db = torch.empty_like(x), torch.empty(d).cuda(), torch.empty(d).cuda()
+    gpu.layernorm_backward(gpu_ctx, dy, x, gamma, mean, rstd, dx, dg, db)
+    g = g64(dy) * g64(gamma)
+    want = 256 * (g - g.mean(-1, keepdims=True))
+    # g is rounded; its mean has a path of at most 16 + 10 + 17 additions and 2 more; then two
+    # differences and a product
+    tol = 256 * U * (3 * np.abs(g) + 47 * np.abs(g).mean(-1, keepdims=True)) + U * 2 * np.abs(want)
+    within(dx, want, tol + half_step(dtype) * (np.abs(want) + tol), "dx")
+    assert not dg.any()
+    # five rows on up to 32 places: at most 1 + 10, 4 + 2 + 16 additions, none of them long
+    within(db, g64(dy).sum(0), 33 * U * np.abs(g64(dy)).sum(0), "dbeta")
