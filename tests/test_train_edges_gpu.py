@@ -8,7 +8,7 @@ import torch
 
 from conftest import banner
 from oracle import train_oracle as to
-from test_train_gpu import BF, F32, U, dev, g64, half_step, norm_inputs, within
+from test_train_gpu import BF, F32, HYPER, U, dev, g64, half_step, norm_inputs, p_tol, within
 
 pytestmark = pytest.mark.gpu
 
@@ -187,3 +187,33 @@ def test_layernorm_backward_of_constant_rows_far_out(gpu_ctx, d, dtype):
     assert not dg.any()
     # five rows on up to 32 places: at most 1 + 10, 4 + 2 + 16 additions, none of them long
     within(db, g64(dy).sum(0), 33 * U * np.abs(g64(dy)).sum(0), "dbeta")
+
+
+# ---- AdamW: the smallest moments -----------------------------------------------
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-30])
+def test_adamw_of_subnormal_moments(gpu_ctx, eps, bits):
+    """Gradients whose v is below 2^-126, with an eps that does not hide it."""
+    from simple_llm_amd.gpu import gpu
+    banner(f"adamw subnormal v, eps {eps} bits {bits}")
+    rng = np.random.default_rng(0)
+    n = 1152
+    g = np.exp(rng.uniform(np.log(1e-21), np.log(1e-16), n)) * rng.choice([-1, 1], n)
+    g = g.astype(np.float32)
+    pd, gd = dev(rng.standard_normal(n)), dev(g)
+    opt = gpu.adamw_create(gpu_ctx, [pd], [gd], bits=bits, seed=5)
+    h = {**HYPER, "eps": eps}
+    m, v = np.zeros(n, np.float32), np.zeros(n, np.float32)
+    for t in (1, 2):
+        old = g64(pd)
+        gpu.adamw_update(gpu_ctx, opt, **h)
+        m, v = to.moments(m, v, g, h["beta1"], h["beta2"])
+        assert (v > 0).all() and (t == 2 or (v < 2.0 ** -126).sum() > n // 2)
+        want = to.stepped(old, m, v, t, **h)
+        within(pd, want, p_tol(old, m.astype(float), v.astype(float), t, h, want), f"step {t}")
+        if bits == 32:
+            np.testing.assert_array_equal(opt.v.cpu().numpy(), v)
+        else:
+            m = to.values(opt.m.cpu().numpy(), opt.m_scale.cpu().numpy(), False).astype(np.float32)
+            v = to.values(opt.v.cpu().numpy(), opt.v_scale.cpu().numpy(), True).astype(np.float32)
