@@ -793,7 +793,7 @@ typedef struct skv_adamw_tensor {
  * c) for its elements [4096 c, 4096 c + 4096), each chunk of each tensor once. count:
  * two int32, t (advanced by the call, on the device, so that a captured step counts on)
  * and 0. lr_dev, grad_scale_dev: where not NULL, fp32 in device memory in place of
- * lr and grad_scale.
+ * lr and grad_scale. eps: 0 or at least 2^-126.
  * bits = 32: m, v fp32, by element of the state (the places between tensors are not
  * touched). bits = 8: a byte an element and m_scale, v_scale a byte k + 127 for 128
  * elements, k the exponent of their largest magnitude in [-90, 126]: m as sign and

@@ -405,6 +405,9 @@ extern "C" int skv_adamw(const skv_adamw_tensor* tensors, const int32_t* chunks,
   SKV_REQUIRE(grad_dt == SKV_F32 || grad_dt == SKV_BF16, SKV_E_INVALID, "skv_adamw: bad dtype");
   SKV_REQUIRE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, SKV_E_INVALID,
               "skv_adamw: beta1 and beta2 must lie in [0, 1)");
+  // a subnormal one would be taken for 0: 0 / eps a NaN
+  SKV_REQUIRE(eps == 0 || eps >= 0x1p-126, SKV_E_INVALID,
+              "skv_adamw: eps must be 0 or at least 2^-126");
   SKV_REQUIRE(aligned16(m) && aligned16(v), SKV_E_INVALID,
               "skv_adamw: the state must be 16-byte aligned");
   Step a;

@@ -19,6 +19,7 @@ from .gpu_types import GPUContext
 _CHUNK = 4096  # elements of a tensor that a workgroup takes at a time
 _BLOCK = 128  # moments that share a scale; a tensor's begin a block
 _ZERO_SCALE = 127 - 90  # the scale byte of a block of zeros
+_LEAST = 2.0 ** -126  # the least normal float32
 
 
 class AdamWState:
@@ -173,13 +174,14 @@ def adamw_update(ctx: GPUContext, state: AdamWState, lr: Union[float, Operand],
         p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
 
     lr, grad_scale: numbers, or float32 device tensors [1], which a captured step reads anew
-    when it is replayed. With 8-bit moments the step uses them before they are rounded.
+    when it is replayed. eps: 0 or at least 2^-126. With 8-bit moments the step uses them before
+    they are rounded.
     """
     if not (0 <= beta1 < 1 and 0 <= beta2 < 1):
         raise ValueError(f"beta1 and beta2 must lie in [0, 1), got {beta1} and {beta2}")
-    if not (math.isfinite(eps) and eps >= 0 and math.isfinite(weight_decay)):
-        raise ValueError(f"eps must be finite and >= 0 and weight_decay finite, got {eps} and "
-                         f"{weight_decay}")
+    if not ((eps == 0 or _LEAST <= eps < math.inf) and math.isfinite(weight_decay)):
+        raise ValueError(f"eps must be 0, or at least 2^-126 and finite, and weight_decay finite, "
+                         f"got {eps} and {weight_decay}")
     dev = device_of(ctx)
     lr, lr_dev = _number(dev, lr, "lr")
     grad_scale, scale_dev = _number(dev, grad_scale, "grad_scale")

@@ -217,3 +217,12 @@ def test_adamw_of_subnormal_moments(gpu_ctx, eps, bits):
         else:
             m = to.values(opt.m.cpu().numpy(), opt.m_scale.cpu().numpy(), False).astype(np.float32)
             v = to.values(opt.v.cpu().numpy(), opt.v_scale.cpu().numpy(), True).astype(np.float32)
+
+
+def test_adamw_of_the_least_eps(gpu_ctx):
+    """Weights without gradients stay where they are, up to their decay."""
+    from simple_llm_amd.gpu import gpu
+    p, g = torch.ones(300, device="cuda"), torch.zeros(300, device="cuda")
+    opt = gpu.adamw_create(gpu_ctx, [p], [g])
+    gpu.adamw_update(gpu_ctx, opt, 2.0 ** -10, eps=2.0 ** -126, weight_decay=0.5)
+    assert (p == 1 - 2.0 ** -11).all()
