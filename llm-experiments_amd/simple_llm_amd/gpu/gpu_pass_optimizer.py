@@ -29,11 +29,13 @@ class AdamWState:
     multiple of 128; the places in between hold zeros): float32, or uint8 codes with
     m_scale, v_scale, a byte for 128 moments (include/skv.h has the formats).
     step: int32 device tensor [1], the steps taken, advanced on the device by every
-    adamw_update, also when a captured one is replayed. m, v, the scales and step are all
-    there is to save; a program that resumes copies them back in.
+    adamw_update, also when a captured one is replayed.
+    seed: of the 8-bit moments' rounding; a number, read by adamw_update.
 
-    The parameters, gradients and copies are held, and used where they were when the
-    state was made.
+    m, v, the scales, step and seed are all there is to save. A program that resumes copies
+    the saved tensors into those of a new state (state.m.copy_(saved), ...): the attributes
+    themselves cannot be replaced. The parameters, gradients and copies are held, and used
+    where they were when the state was made.
     """
 
     def __init__(self, params: List[torch.Tensor], grads: List[torch.Tensor],
@@ -44,19 +46,42 @@ class AdamWState:
         self.params = params
         self.grads = grads
         self.copies = copies
-        self.bits = bits
         self.offsets = offsets
         self.seed = seed
-        self.m = m
-        self.v = v
-        self.m_scale = m_scale
-        self.v_scale = v_scale
-        self.step = count[:1]
+        self._bits = bits
+        self._m = m
+        self._v = v
+        self._m_scale = m_scale
+        self._v_scale = v_scale
+        self._step = count[:1]
         self._count = count
         self._tensors = tensors
         self._chunks = chunks
-        self._held = [*params, *grads, *(copies or [])]
+        self._grad_dtype = grads[0].dtype
+        # Every tensor that the kernel reaches by its address: it has to be there still, and
+        # a second reference keeps the memory from being given away in any case.
+        self._held = [*params, *grads, *(copies or []), m, v, self._step]
+        if bits == 8:
+            self._held += [m_scale, v_scale]
         self._at = [t.data_ptr() for t in self._held]
+        self._memory = [t.detach() for t in self._held]
+
+    bits = property(lambda self: self._bits)
+    m = property(lambda self: self._m)
+    v = property(lambda self: self._v)
+    m_scale = property(lambda self: self._m_scale)
+    v_scale = property(lambda self: self._v_scale)
+    step = property(lambda self: self._step)
+
+    @property
+    def seed(self) -> int:
+        return self._seed
+
+    @seed.setter
+    def seed(self, seed: int) -> None:
+        if not 0 <= int(seed) < 1 << 32:
+            raise ValueError(f"seed must lie in [0, 2^32), got {seed}")
+        self._seed = int(seed)
 
     def _scales(self) -> tuple:
         if self.bits == 32:
@@ -188,17 +213,17 @@ def adamw_update(ctx: GPUContext, state: AdamWState, lr: Union[float, Operand],
     _check_state(ctx, state)
     launch(ctx, dev, "skv_adamw", state._tensors.data_ptr(), state._chunks.data_ptr(),
            state._chunks.shape[0], state.m.data_ptr(), state.v.data_ptr(), *state._scales(),
-           state._count.data_ptr(), state.bits, _lib.dtype_code(state.grads[0].dtype), lr, lr_dev,
+           state._count.data_ptr(), state.bits, _lib.dtype_code(state._grad_dtype), lr, lr_dev,
            float(beta1), float(beta2), float(eps), float(weight_decay), grad_scale, scale_dev,
            state.seed)
 
 
 def _check_state(ctx: GPUContext, state: AdamWState) -> None:
+    if [t.data_ptr() for t in state._held] != state._at:
+        raise ValueError("a parameter, gradient, copy or tensor of the state is no longer where it "
+                         "was when the state was made: write into their buffers, or make a new state")
     if state.m.get_device() != device_of(ctx):
         raise ValueError(f"the state lives on {state.m.device}, the context on {ctx.device}")
-    if [t.data_ptr() for t in state._held] != state._at:
-        raise ValueError("a parameter, gradient or copy is no longer where it was when the state "
-                         "was made: write into their buffers, or make a new state")
 
 
 def adamw_read(ctx: GPUContext, state: AdamWState, m: Operand, v: Operand) -> None:

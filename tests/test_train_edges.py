@@ -3,9 +3,11 @@ here reaches a launch."""
 from __future__ import annotations
 
 import pytest
+import torch
 
 from simple_llm_amd import _lib
 from simple_llm_amd.gpu import gpu
+from simple_llm_amd.gpu.gpu_pass_optimizer import _check_state
 from test_train import FAKE, _ctx
 
 
@@ -18,3 +20,54 @@ def test_adamw_refuses_a_subnormal_eps(eps):
     rc = L.skv_adamw(FAKE, FAKE, 3, FAKE, FAKE, None, None, FAKE, 32, 0, 1e-3, None, 0.9, 0.999, eps,
                      0.1, 1.0, None, 0, None)
     assert rc == _lib.SKV_E_INVALID and b"eps" in L.skv_last_error()
+
+
+def _state(bits):
+    kind = torch.float32 if bits == 32 else torch.uint8
+    m, v = torch.zeros(256, dtype=kind), torch.zeros(256, dtype=kind)
+    scales = [torch.zeros(2, dtype=torch.uint8) for _ in "mv"] if bits == 8 else [None, None]
+    return gpu.AdamWState([torch.zeros(200)], [torch.zeros(200)], [torch.zeros(200).bfloat16()], bits,
+                          [0], 3, m, v, *scales, torch.zeros(2, dtype=torch.int32),
+                          torch.zeros(1, 6, dtype=torch.int64), torch.zeros(1, 2, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_state_cannot_be_replaced(bits):
+    """What the kernel reaches by its address, by assignment: a tensor of another type, size
+    or device, or a count that the kernel would not see."""
+    s = _state(bits)
+    for name, other in (("m", torch.zeros(5)), ("v", torch.zeros(256, dtype=torch.float64)),
+                        ("m_scale", torch.zeros(1)), ("v_scale", None), ("bits", 40 - bits),
+                        ("step", torch.ones(1, dtype=torch.int32))):
+        with pytest.raises(AttributeError):
+            setattr(s, name, other)
+    for seed in (-1, 1 << 32):
+        with pytest.raises(ValueError, match="seed must"):
+            s.seed = seed
+    s.seed = 7
+    assert s.seed == 7 and s.step.item() == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_state_cannot_move(bits):
+    """The same through a tensor's data, for every tensor that is held."""
+    names = ["m", "v", "step"] + (["m_scale", "v_scale"] if bits == 8 else [])
+    held = [lambda s, n=n: getattr(s, n) for n in names] + [
+        lambda s, n=n: getattr(s, n)[0] for n in ("params", "grads", "copies")]
+    for get in held:
+        s = _state(bits)
+        with pytest.raises(ValueError, match="the state lives on cpu"):  # the check behind it
+            _check_state(_ctx(), s)
+        at = get(s).data_ptr()
+        get(s).data = torch.zeros(5)
+        with pytest.raises(ValueError, match="no longer where it was"):
+            _check_state(_ctx(), s)
+        # and the memory is still the state's, whatever is allocated next
+        assert at in [t.data_ptr() for t in s._memory]
+
+
+def test_adamw_gradients_keep_their_type():
+    """The lists are the program's own; the kernel's types are those of the making."""
+    s = _state(32)
+    s.grads[0] = torch.zeros(200).bfloat16()
+    assert s._grad_dtype == torch.float32

@@ -226,3 +226,35 @@ def test_adamw_of_the_least_eps(gpu_ctx):
     opt = gpu.adamw_create(gpu_ctx, [p], [g])
     gpu.adamw_update(gpu_ctx, opt, 2.0 ** -10, eps=2.0 ** -126, weight_decay=0.5)
     assert (p == 1 - 2.0 ** -11).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_resumes(gpu_ctx, bits):
+    """A saved state copied into a new one goes on bit by bit; one that was replaced is refused
+    before anything is launched."""
+    from simple_llm_amd.gpu import gpu
+    torch.manual_seed(bits)
+    p, g = torch.randn(5000, device="cuda"), torch.randn(5000, device="cuda")
+    opt = gpu.adamw_create(gpu_ctx, [p], [g], bits=bits, seed=11)
+    for _ in range(3):
+        gpu.adamw_update(gpu_ctx, opt, 1e-2)
+    names = ["m", "v", "step"] + (["m_scale", "v_scale"] if bits == 8 else [])
+    saved = {n: getattr(opt, n).cpu() for n in names}
+    q = p.clone()
+    new = gpu.adamw_create(gpu_ctx, [q], [g], bits=bits, seed=opt.seed)
+    for n in names:
+        getattr(new, n).copy_(saved[n])
+    for _ in range(2):
+        gpu.adamw_update(gpu_ctx, opt, 1e-2)
+        gpu.adamw_update(gpu_ctx, new, 1e-2)
+    assert torch.equal(p, q) and all(torch.equal(getattr(opt, n), getattr(new, n)) for n in names)
+    before = p.clone()
+    for n in names:
+        at = getattr(opt, n).data
+        getattr(opt, n).data = saved[n].cuda()
+        with pytest.raises(ValueError, match="no longer where it was"):
+            gpu.adamw_update(gpu_ctx, opt, 1e-2)
+        getattr(opt, n).data = at
+    assert torch.equal(p, before) and opt.step.item() == 5
+    gpu.adamw_update(gpu_ctx, opt, 1e-2)
+    assert opt.step.item() == 6 and not torch.equal(p, before)
