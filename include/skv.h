@@ -810,8 +810,8 @@ int skv_adamw(const skv_adamw_tensor* tensors, const int32_t* chunks, int n_chun
               double weight_decay, double grad_scale, const float* grad_scale_dev, uint32_t seed,
               skv_stream_t stream);
 
-/* The 8-bit moments of a state of n elements (a multiple of 128) as values, exact in
- * either out_dt. */
+/* The 8-bit moments of a state of n elements (a multiple of 128, up to 2^35 - 2048) as
+ * values, exact in either out_dt. */
 int skv_adamw_read(void* m_out, void* v_out, const uint8_t* m, const uint8_t* v,
                    const uint8_t* m_scale, const uint8_t* v_scale, long long n, int out_dt,
                    skv_stream_t stream);

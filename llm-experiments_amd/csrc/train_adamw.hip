@@ -451,7 +451,9 @@ extern "C" int skv_adamw_read(void* m_out, void* v_out, const uint8_t* m, const 
               "skv_adamw_read: null pointer argument");
   SKV_REQUIRE(n > 0 && n % kBlock == 0, SKV_E_INVALID,
               "skv_adamw_read: n must be a positive multiple of %d", kBlock);
-  SKV_REQUIRE(n < (1ll << 40), SKV_E_UNSUPPORTED, "skv_adamw_read: n=%lld is too large", n);
+  const size_t groups = ((size_t)n / 8 + 255) / 256;
+  SKV_REQUIRE(launchable(groups, 256), SKV_E_UNSUPPORTED,
+              "skv_adamw_read: n=%lld is too large for a launch", n);
   SKV_REQUIRE(out_dt == SKV_F32 || out_dt == SKV_BF16, SKV_E_INVALID, "skv_adamw_read: bad dtype");
   SKV_REQUIRE(aligned16(m_out) && aligned16(v_out) && aligned16(m) && aligned16(v), SKV_E_INVALID,
               "skv_adamw_read: pointers must be 16-byte aligned");
@@ -461,7 +463,7 @@ extern "C" int skv_adamw_read(void* m_out, void* v_out, const uint8_t* m, const 
                       {m_scale, (size_t)n / kBlock, "the state's m_scale"},
                       {v_scale, (size_t)n / kBlock, "the state's v_scale"}}))
     return rc;
-  const unsigned grid = (unsigned)((n / 8 + 255) / 256);
+  const unsigned grid = (unsigned)groups;
   hipStream_t s = (hipStream_t)stream;
   if (out_dt == SKV_BF16)
     k_adamw_read<<<grid, 256, 0, s>>>((uint16_t*)m_out, (uint16_t*)v_out, m, v, m_scale, v_scale,

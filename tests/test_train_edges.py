@@ -71,3 +71,14 @@ def test_adamw_gradients_keep_their_type():
     s = _state(32)
     s.grads[0] = torch.zeros(200).bfloat16()
     assert s._grad_dtype == torch.float32
+
+
+def test_adamw_read_refuses_more_than_a_launch():
+    """A lane for 8 elements, 256 a workgroup, fewer than 2^32 lanes: the last size that gets
+    as far as the overlaps, and the next ones."""
+    L = _lib.lib()
+    most = 8 * ((1 << 32) - 256)
+    for n, rc in ((most, _lib.SKV_E_INVALID), (most + 128, _lib.SKV_E_UNSUPPORTED),
+                  (1 << 35, _lib.SKV_E_UNSUPPORTED), ((1 << 40) - 128, _lib.SKV_E_UNSUPPORTED),
+                  ((1 << 63) - 128, _lib.SKV_E_UNSUPPORTED)):
+        assert L.skv_adamw_read(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, n, 0, None) == rc, n
