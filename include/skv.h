@@ -754,7 +754,8 @@ size_t skv_embedding_bwd_workspace_bytes(int T, int V, int d);
  * of grad [V, d] fp32; with accumulate != 0 added to the rows that have tokens, and
  * the others are left alone (the reference's embedding_backward and its reduction,
  * gpu_pass_backward.py:183-240, gpu_kernels.py:2946-3068). dout: [T, d] of dt. An
- * id outside [0, V) adds nothing. d <= 2^22, V <= 2^29, T ceil(d / 256) <= 2^30. */
+ * id outside [0, V) adds nothing. d <= 2^22, V <= 2^29, ceil(T / 16) ceil(d / 256) <=
+ * 2^26 - 8. */
 int skv_embedding_bwd(float* grad, const void* dout, const int32_t* ids, int T, int V, int d,
                       float scale, int accumulate, void* ws, size_t ws_bytes, int dt,
                       skv_stream_t stream);

@@ -506,11 +506,13 @@ extern "C" int skv_embedding_bwd(float* grad, const void* dout, const int32_t* i
   SKV_REQUIRE(dt == SKV_F32 || dt == SKV_BF16, SKV_E_INVALID, "skv_embedding_bwd: bad dtype");
   const int width = V <= 256 * kBucket ? (V + 255) / 256 : kBucket;  // one bucket to a CU
   const int buckets = (V - 1) / width + 1, tiles = (d - 1) / 256 + 1;
+  const size_t units = (size_t)ranges_of(T) * tiles;
   SKV_REQUIRE(d <= kMaxD && T <= kMaxRows && launchable((size_t)buckets + kZeroGroups, 1024) &&
-                  launchable(((size_t)ranges_of(T) * tiles + 3) / 4, 256),
+                  launchable((units + 3) / 4, 256) &&
+                  launchable((units + kJoinWaves - 1) / kJoinWaves, kJoinWaves * 64),
               SKV_E_UNSUPPORTED,
               "skv_embedding_bwd: T=%d, V=%d, d=%d are too many for a launch (up to 2^22 columns, "
-              "2^29 table rows, 2^30 tokens a 256 columns)", T, V, d);
+              "2^29 table rows, nearly 2^30 tokens a 256 columns)", T, V, d);
   SKV_REQUIRE(aligned16(grad) && aligned16(dout) && aligned16(ws), SKV_E_INVALID,
               "skv_embedding_bwd: pointers must be 16-byte aligned");
   SKV_REQUIRE(ws_bytes >= skv_embedding_bwd_workspace_bytes(T, V, d), SKV_E_WORKSPACE,
@@ -533,7 +535,7 @@ extern "C" int skv_embedding_bwd(float* grad, const void* dout, const int32_t* i
   const int sort_grid = buckets + (n_zero ? kZeroGroups : 0);
   k_embed_sort<<<sort_grid, kWaves * 64, 0, st>>>(s, ids, T, V, width, buckets, grad, n_zero);
   if (int rc = check_launch("skv_embedding_bwd")) return rc;
-  const unsigned grid = (unsigned)(((size_t)ranges * tiles + 3) / 4);
+  const unsigned grid = (unsigned)((units + 3) / 4);
   const dim3 join((ranges + kJoinWaves - 1) / kJoinWaves, tiles);
   const auto run = [&](auto* y, auto KIND, auto ACC) {
     using TY = std::remove_const_t<std::remove_pointer_t<decltype(y)>>;

@@ -82,3 +82,18 @@ def test_adamw_read_refuses_more_than_a_launch():
                   (1 << 35, _lib.SKV_E_UNSUPPORTED), ((1 << 40) - 128, _lib.SKV_E_UNSUPPORTED),
                   ((1 << 63) - 128, _lib.SKV_E_UNSUPPORTED)):
         assert L.skv_adamw_read(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, n, 0, None) == rc, n
+
+
+def test_embedding_backward_refuses_more_than_its_last_launch():
+    """The third launch has 512 lanes for 8 ranges of 16 tokens: it reaches 2^32 lanes before
+    the second one does. The workspace's size is the last check before the overlaps."""
+    L = _lib.lib()
+    for T, d in ((1 << 30) - 128, 8), ((1 << 29) - 64, 257), (1 << 20, 250 * 256):
+        units = -(-T // 16) * -(-d // 256)
+        assert units <= (1 << 26) - 8
+        need = L.skv_embedding_bwd_workspace_bytes(T, 10, d)
+        assert L.skv_embedding_bwd(FAKE, FAKE, FAKE, T, 10, d, 1.0, 0, FAKE, need - 1, 0,
+                                   None) == _lib.SKV_E_WORKSPACE
+    for T, d in ((1 << 30) - 127, 8), ((1 << 30) - 64, 8), ((1 << 30) - 48, 8), (1 << 20, 1 << 18):
+        assert L.skv_embedding_bwd(FAKE, FAKE, FAKE, T, 10, d, 1.0, 0, FAKE, 1 << 62, 0,
+                                   None) == _lib.SKV_E_UNSUPPORTED, (T, d)
