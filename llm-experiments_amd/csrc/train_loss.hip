@@ -336,14 +336,16 @@ void launch_rows(const LossArgs& a, hipStream_t s) {
     k_loss_rows<T, nw, NV.value, GRAD, PAST>
         <<<nw == 1 ? (a.M + 3) / 4 : a.M, nw == 1 ? 256 : nw * 64, 0, s>>>(a);
   };
-  const auto with = [&](auto NW) {  // even numbers of vectors
+  const auto with = [&](auto NW) {  // even numbers of vectors: 5 to 8 a lane, or 16
     const int nv = (n + NW.value * 64 - 1) / (NW.value * 64);
-    if (nv <= 6) rows(NW, std::integral_constant<int, 6>{});
-    else if (nv <= 8) rows(NW, std::integral_constant<int, 8>{});
-    else if (nv <= 10) rows(NW, std::integral_constant<int, 10>{});
-    else if (nv <= 12) rows(NW, std::integral_constant<int, 12>{});
-    else if (nv <= 14) rows(NW, std::integral_constant<int, 14>{});
-    else rows(NW, std::integral_constant<int, 16>{});
+    if constexpr (NW.value == 16) {
+      if (nv > 14) return rows(NW, std::integral_constant<int, 16>{});
+      if (nv > 12) return rows(NW, std::integral_constant<int, 14>{});
+      if (nv > 10) return rows(NW, std::integral_constant<int, 12>{});
+      if (nv > 8) return rows(NW, std::integral_constant<int, 10>{});
+    }
+    if (nv > 6) rows(NW, std::integral_constant<int, 8>{});
+    else rows(NW, std::integral_constant<int, 6>{});
   };
   using std::integral_constant;
   const int nw = waves_of(n);
