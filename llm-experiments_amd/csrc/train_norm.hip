@@ -345,9 +345,12 @@ void dispatch(int M, int d, int wpr, F f) {
     if (kind == kEven) f(N, L, W, integral_constant<int, kEven>{});
     else f(N, L, W, integral_constant<int, kOdd>{});
   };
-  // run(the row's vectors a lane), MOST (2 or 4) or fewer
-  const auto few = [&](auto MOST, auto run) {
-    if (n <= 1) return run(one);
+  // run(the row's vectors a lane), MOST (2 or 4) or fewer. On 32 lanes and more a row has over
+  // kLaneCols / 4 columns a lane: two vectors of fp32 at least.
+  const auto few = [&](auto LANES, auto MOST, auto run) {
+    if constexpr (LANES.value == 16 || VEC > kLaneCols / 4) {
+      if (n <= 1) return run(one);
+    }
     if constexpr (MOST.value > 2) {
       if (n <= 2) return run(integral_constant<int, 2>{});
       if (n <= 3) return run(integral_constant<int, 3>{});
@@ -357,23 +360,24 @@ void dispatch(int M, int d, int wpr, F f) {
   const integral_constant<int, kLaneCols / VEC> most;
   if (kind == kTiny) return f(one, integral_constant<int, 16>{}, one, integral_constant<int, kTiny>{});
   if (lpr == 16) {
-    few(most, [&](auto N) { with_kind(N, integral_constant<int, 16>{}, one); });
+    const integral_constant<int, 16> L;
+    few(L, most, [&](auto N) { with_kind(N, L, one); });
   } else if (lpr == 32) {
-    few(most, [&](auto N) { with_kind(N, integral_constant<int, 32>{}, one); });
+    const integral_constant<int, 32> L;
+    few(L, most, [&](auto N) { with_kind(N, L, one); });
   } else if (wpr == 1) {
     const integral_constant<int, 64> L;
     if constexpr (VEC == 4) {
       if (n > 4) return with_kind(integral_constant<int, 5>{}, L, one);
     }
-    few(integral_constant<int, 4>{}, [&](auto N) { with_kind(N, L, one); });
+    few(L, integral_constant<int, 4>{}, [&](auto N) { with_kind(N, L, one); });
   } else if (wpr == 4) {
-    few(integral_constant<int, MANY>{}, [&](auto N) {
-      with_kind(N, integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    });
+    const integral_constant<int, 64> L;
+    few(L, integral_constant<int, MANY>{},
+        [&](auto N) { with_kind(N, L, integral_constant<int, 4>{}); });
   } else {
-    few(most, [&](auto N) {
-      with_kind(N, integral_constant<int, 64>{}, integral_constant<int, 16>{});
-    });
+    const integral_constant<int, 64> L;
+    few(L, most, [&](auto N) { with_kind(N, L, integral_constant<int, 16>{}); });
   }
 }
 
