@@ -258,3 +258,124 @@ def test_adamw_resumes(gpu_ctx, bits):
     assert torch.equal(p, before) and opt.step.item() == 5
     gpu.adamw_update(gpu_ctx, opt, 1e-2)
     assert opt.step.item() == 6 and not torch.equal(p, before)
+
+
+# ---- bounds from the kernels' longest sums ---------------------------------------
+
+# Rows on 16, 32 and 64 lanes, 4 and 16 wavefronts; many rows a place.
+SUMS = [(70000, 64), (40000, 300), (20000, 1500), (2048, 2048), (3000, 5000), (513, 8192), (3, 16384),
+        (300, 16381)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,d", SUMS)
+def test_layernorm_sums(gpu_ctx, rows, d, dtype):
+    """A row's sum: at most 32 columns in a lane, 6 additions over a wavefront and 4 over
+    wavefronts, or 16 + 6 + 16: 42. A column's: the rows of a place, then at most 2 and 8
+    over a workgroup's places, 4 + 2 + 16 over the workgroups."""
+    from simple_llm_amd.gpu import gpu
+    banner(f"layernorm sums {rows} x {d} {dtype}")
+    rng, x, gamma, beta = norm_inputs(rows, d, dtype)
+    y, mean, rstd = torch.empty_like(x), torch.empty(rows).cuda(), torch.empty(rows).cuda()
+    gpu.layernorm(gpu_ctx, x, gamma, beta, y, mean, rstd)
+    want, mu, rs = to.layernorm(g64(x), g64(gamma), g64(beta))
+    # the deviations' mean: its sum, the deviations' roundings and a quotient, 44 u of a deviation
+    within(mean, mu, U * (np.abs(mu) + 44 / rs), "mean")
+    # squares of rounded deviations, 3 u each, their sum, a quotient, eps; half of it, and 2 more
+    within(rstd, rs, 26 * U * rs, "rstd")
+    xh = (g64(x) - mu[:, None]) * rs[:, None]
+    tol = U * (np.abs(g64(gamma)) * (30 * np.abs(xh) + 44) + np.abs(g64(beta)) + np.abs(want))
+    within(y, want, tol + half_step(dtype) * (np.abs(want) + tol), "y")
+
+    dy = dev(rng.standard_normal((rows, d)), dtype)
+    dx, dg, db = torch.empty_like(x), torch.empty(d).cuda(), torch.empty(d).cuda()
+    gpu.layernorm_backward(gpu_ctx, dy, x, gamma, mean, rstd, dx, dg, db)
+    want, wg, wb = to.layernorm_backward(g64(dy), g64(x), g64(gamma), g64(mean), g64(rstd))
+    mu, rs = g64(mean)[:, None], g64(rstd)[:, None]
+    xh = np.abs((g64(x) - mu) * rs)
+    g = np.abs(g64(dy) * g64(gamma))
+    # xh: two roundings; g: one; the means: 42 and 2, their terms 4; then six more
+    tol = U * rs * (8 * g + 50 * g.mean(-1, keepdims=True)
+                    + 54 * xh * (g * xh).mean(-1, keepdims=True)) + 2 * U * np.abs(want)
+    within(dx, want, tol + half_step(dtype) * (np.abs(want) + tol), "dx")
+    at_once = 256 * (32 if d <= 128 else 8 if d <= 1024 else 1)  # rows, at the least
+    path = -(-rows // at_once) + 10 + 22
+    s = np.abs(g64(dy))
+    within(dg, wg, U * ((path + 3) * (s * xh).sum(0) + np.abs(wg)), "dgamma")
+    within(db, wb, U * (path * s.sum(0) + np.abs(wb)), "dbeta")
+
+
+@pytest.mark.parametrize("before", [0, 1, 9, 16])
+@pytest.mark.parametrize("count", [15, 16, 17, 111, 112, 113, 127, 128, 129, 145, 6000, 30000])
+def test_embedding_backward_sums(gpu_ctx, count, before):
+    """A row of so many tokens behind `before` others in the sorted order, so that it lies in
+    one range of 16, in up to 8 and in more. A range's tokens are added one after the other;
+    then up to 8 ranges' parts, or, of more ranges, an eighth of them and 8 sums."""
+    from simple_llm_amd.gpu import gpu
+    banner(f"embedding_backward of {count} tokens behind {before}")
+    rng = np.random.default_rng(count + before)
+    n, d = count + before + 40, 65
+    ids = np.concatenate([np.zeros(before), np.full(count, 1), rng.integers(2, 9, 40)])
+    ids = rng.permutation(ids).astype(np.int32)
+    dy = dev(rng.standard_normal((n, d)))
+    want = to.embedding_backward(g64(dy), ids, 9, 3.0)
+    size = to.embedding_backward(np.abs(g64(dy)), ids, 9, 3.0)
+    ranges = count // 16 + 2
+    path = 16 + max(8, -(-ranges // 8) + 8) + 2
+    for accumulate in (False, True):
+        grad = dev(rng.standard_normal((9, d)))
+        was = g64(grad) * accumulate
+        gpu.embedding_backward(gpu_ctx, dy, dev(ids, torch.int32), grad, 3.0, accumulate)
+        within(grad, want + was, U * (path * size + 2 * np.abs(want + was)), f"{accumulate}")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("grads", [F32, BF])
+def test_adamw_of_many_chunks(gpu_ctx, bits, grads):
+    """More chunks of 4096 than workgroups, over tensors of unlike sizes, alignments and
+    decay, with copies: moments bit by bit, the codes of two steps too."""
+    from simple_llm_amd.gpu import gpu
+    banner(f"adamw of many chunks bits={bits} grads={grads}")
+    rng = np.random.default_rng(bits)
+    shapes = [(700, 1500), (1,), (4097,), (300, 4096), (129,), (511, 1000), (77,), (8192,)]
+
+    def tensors(dtype, scale):
+        out = []
+        for i, s in enumerate(shapes):
+            n = int(np.prod(s))
+            flat = torch.zeros(n + i % 2, dtype=dtype, device="cuda")
+            flat[i % 2:] = dev(scale * rng.standard_normal(n) * np.exp(2 * rng.standard_normal(n)),
+                               dtype)
+            out.append(flat[i % 2:].view(s))
+        return out
+
+    ps, gs, cs = tensors(F32, 1.0), tensors(grads, 1e-2), tensors(BF, 1.0)
+    decay = [i % 3 == 0 for i in range(len(shapes))]
+    opt = gpu.adamw_create(gpu_ctx, ps, gs, bits=bits, copies=cs, decay=decay, seed=77)
+    assert opt._chunks.shape[0] > 2 * 256
+    n = opt.m.numel()
+    place = np.concatenate([o + np.arange(p.numel()) for o, p in zip(opt.offsets, ps)])
+    dec = np.concatenate([np.full(p.numel(), d) for p, d in zip(ps, decay)])
+    flat = lambda ts: np.concatenate([g64(x).ravel() for x in ts])
+    m, v, g = (np.zeros(n, np.float32) for _ in range(3))
+    g[place] = flat(gs)
+    for t in (1, 2):
+        old = flat(ps)
+        gpu.adamw_update(gpu_ctx, opt, **HYPER)
+        m, v = to.moments(m, v, g, HYPER["beta1"], HYPER["beta2"])
+        want = np.where(dec, to.stepped(old, m[place], v[place], t, **HYPER),
+                        to.stepped(old, m[place], v[place], t, **{**HYPER, "weight_decay": 0}))
+        within(flat(ps), want, p_tol(old, m[place].astype(float), v[place].astype(float), t, HYPER,
+                                     want), f"step {t}")
+        assert all(torch.equal(c, p.bfloat16()) for p, c in zip(ps, cs))
+        if bits == 32:
+            np.testing.assert_array_equal(opt.m.cpu().numpy(), m)
+            np.testing.assert_array_equal(opt.v.cpu().numpy(), v)
+            continue
+        r, back = to.hashed(77, t, n), []
+        for x, name, shift, uns in ((m, "m", 0, False), (v, "v", 16, True)):
+            code, byte = to.store(x, (r >> shift) & 0xffff, uns)
+            np.testing.assert_array_equal(getattr(opt, name).cpu().numpy(), code)
+            np.testing.assert_array_equal(getattr(opt, name + "_scale").cpu().numpy(), byte)
+            back.append(to.values(code, byte, uns).astype(np.float32))
+        m, v = back
