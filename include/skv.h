@@ -719,7 +719,9 @@ int skv_flash_bwd(float* dq, float* dk, float* dv, const float* q, const float* 
  * population variance: the reference's layernorm (simple-llm/src/gpu/
  * gpu_pass_forward.py:140-176, kernel gpu_kernels.py:137-249) with the rows'
  * statistics kept for the backward. x, y: [M, d] of dt, y may be x; gamma, beta:
- * [d]; mean, rstd: [M] or NULL. d <= 16384. */
+ * [d]; mean, rstd: [M] or NULL. d <= 16384. A row with a NaN or an infinity has NaN for
+ * y and rstd. Deviations from the mean have to be below 2^56: their squares are summed in
+ * fp32, and where the sum overflows rstd is 0 or NaN. */
 int skv_layernorm_fwd(void* y, float* mean, float* rstd, const void* x, const float* gamma,
                       const float* beta, int M, int d, float eps, int dt, skv_stream_t stream);
 
@@ -770,7 +772,8 @@ size_t skv_cross_entropy_workspace_bytes(int M);
  * A row counts if its target lies in [0, V); the others have a loss and a gradient
  * of 0 and their logits are not read; if none counts the loss is 0. x, dx: [M, V]
  * of dt, dx may be x, or NULL; row_loss: [M] or NULL. Logits of -inf have
- * probability 0; a row with a NaN or +inf, or of -inf only, has NaN results. */
+ * probability 0; a row with a NaN or +inf, or of -inf only, has NaN results. Finite logits
+ * of any size have finite probabilities. */
 int skv_cross_entropy(float* loss, float* row_loss, void* dx, const void* x,
                       const int32_t* targets, int M, int V, float grad_scale, void* ws,
                       size_t ws_bytes, int dt, skv_stream_t stream);

@@ -103,9 +103,9 @@ __device__ __forceinline__ int wave_isum(int x) {
 
 // width: ids of a bucket. Each wavefront has a run of consecutive tokens; an id's tokens
 // are placed by wavefront, then by token. The bucket's own tokens go to a list in LDS, in
-// order: it is short but for a bucket of frequent ids (of 16384 zipf tokens a bucket of 99
-// ids has 32 on average and 1000 at most, 60 a wavefront), and what finds an id's rank
-// among 64 tokens costs 0.3 us. Where the list does not hold them, the run is read again.
+// order: it is short but for a bucket of frequent ids (of 16384 zipf tokens a bucket of 197
+// ids has 64 on average, the largest some 700, 50 to 100 in a wavefront), and what finds an
+// id's rank among 64 tokens costs 0.3 us. Where the list does not hold them, the run is read again.
 __global__ __launch_bounds__(kWaves * 64, 8) void k_embed_sort(Sorted s,
                                                                const int32_t* __restrict__ ids,
                                                                int T, int V, int width, int buckets,
